@@ -73,6 +73,10 @@ EXPORTED_SYMBOLS = (
     "qlin_qat_codes",
     "qlin_qat_split",
     "qlin_qat_product",
+    "qlin_qk_rope",
+    "qlin_paged_attention",
+    "qlin_paged_attention_workspace_bytes",
+    "qlin_prompt_attention",
 )
 
 
@@ -299,6 +303,34 @@ class PeerBarrierArgs(C.Structure):
     ]
 
 
+class QkRopeArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_out", "q_weight", "k_weight", "cos", "sin", "positions", "k_pages", "v_pages", "slots",
+                                    "k_scale", "v_scale", "status")),
+        *((n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "page_stride", "head_stride", "slot_stride", "num_slots")),
+        *((n, C.c_int32) for n in ("tokens", "q_heads", "kv_heads", "head_dim", "rotary", "table_rows", "page_size", "dtype", "weight_dtype", "cache_dtype")),
+        ("eps", C.c_float),
+    ]  # fmt: skip
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("q", "k_pages", "v_pages", "block_table", "lens", "k_scale", "v_scale", "out", "workspace", "status")),
+        *((n, C.c_int64) for n in ("q_batch", "q_head", "page_stride", "head_stride", "slot_stride", "table_stride")),
+        *((n, C.c_int32) for n in ("batch", "q_heads", "kv_heads", "head_dim", "page_size", "num_pages", "max_pages", "window", "sinks", "dtype", "cache_dtype")),
+        ("scale", C.c_float),
+    ]  # fmt: skip
+
+
+class PromptAttentionArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("q", "k", "v", "out", "cu_q", "cu_k", "status")),
+        *((n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head")),
+        *((n, C.c_int32) for n in ("tokens_q", "tokens_k", "batch", "max_q", "q_heads", "kv_heads", "head_dim", "window", "sinks", "dtype")),
+        ("scale", C.c_float),
+    ]  # fmt: skip
+
+
 _host = None
 
 
@@ -351,6 +383,9 @@ def load() -> C.CDLL:
         ("qlin_peer_barrier", PeerBarrierArgs),
         ("qlin_col_absmax", ColAbsmaxArgs),
         ("qlin_shard_reduce", ShardReduceArgs),
+        ("qlin_qk_rope", QkRopeArgs),
+        ("qlin_paged_attention", PagedAttentionArgs),
+        ("qlin_prompt_attention", PromptAttentionArgs),
     ):
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(struct), C.c_void_p]
@@ -372,6 +407,8 @@ def load() -> C.CDLL:
     lib.qlin_ipc_close.restype = C.c_int
     lib.qlin_tensor_fq_workspace_bytes.argtypes = [C.c_int64]
     lib.qlin_tensor_fq_workspace_bytes.restype = C.c_int64
+    lib.qlin_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedAttentionArgs)]
+    lib.qlin_paged_attention_workspace_bytes.restype = C.c_int64
     _lib = lib
     return lib
 

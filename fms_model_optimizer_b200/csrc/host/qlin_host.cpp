@@ -18,10 +18,13 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <variant>
 #include <vector>
 
@@ -671,6 +674,230 @@ Tensor qat_linear(const Tensor& x, const Tensor& w, const OptTensor& bias, const
   return QatProduct::apply(x, w, bias, clip_x.detach(), clipn_x ? OptTensor(clipn_x->detach()) : std::nullopt, clip_w, bits_x, bits_w, variant);
 }
 
+// ------------------------------------------------------------------------------------------------ attention of a generating decoder
+// These calls have no gradient; one that autograd would have to record is refused rather than cut off silently.
+void refuse_grad(const char* what, std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : tensors)
+    if (t != nullptr && t->defined() && t->requires_grad()) raise(std::string(what) + " has no gradient: call it under torch.no_grad(), or detach its inputs");
+}
+
+// The stride of a dimension; 0 where a single entry makes it meaningless.
+int64_t step(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+bool on16(const Tensor& t, int64_t stride) { return stride * static_cast<int64_t>(t.element_size()) % 16 == 0; }
+
+// [rows, heads, head_dim] with contiguous heads whose rows start on 16 bytes: the tensor itself, or a dense copy.
+Tensor head_rows(const Tensor& t, const char* what) {
+  if (t.dim() != 3) raise(std::string(what) + " must be [tokens, heads, head_dim]");
+  const bool fits = t.stride(2) == 1 && on16(t, step(t, 0)) && on16(t, step(t, 1)) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  if (fits && !t.is_neg()) return t;
+  return t.resolve_neg().clone(at::MemoryFormat::Contiguous);
+}
+
+void check_index(const Tensor& t, at::ScalarType type, int64_t n, const char* what) {
+  if (t.scalar_type() != type || t.dim() != 1 || t.size(0) != n || !t.is_contiguous())
+    raise(std::string(what) + " must be a contiguous " + std::string(at::toString(type)) + " vector of " + std::to_string(n) + " elements");
+}
+
+// k_pages and v_pages [pages, kv heads, page size, head_dim] of one layout; with e4m3 their scales.
+void check_cache(const Tensor& k, const Tensor& v, int64_t kv_heads, int64_t head_dim, at::ScalarType model, const Tensor& ks, const Tensor& vs) {
+  if (k.dim() != 4 || k.sizes() != v.sizes() || k.size(1) != kv_heads || k.size(3) != head_dim) raise("k_pages and v_pages must both be [pages, kv heads, page size, head_dim]");
+  if (k.scalar_type() != v.scalar_type() || (k.scalar_type() != model && k.scalar_type() != at::kFloat8_e4m3fn))
+    raise("k_pages and v_pages must have the type of the model's tensors, or float8_e4m3fn");
+  if (step(k, 0) != step(v, 0) || step(k, 1) != step(v, 1) || step(k, 2) != step(v, 2) || k.stride(3) != 1 || v.stride(3) != 1)
+    raise("k_pages and v_pages must have the same strides and contiguous heads");
+  if (k.scalar_type() == at::kFloat8_e4m3fn) {
+    if (!ks.defined() || !vs.defined()) raise("a float8_e4m3fn cache needs k_scale and v_scale");
+    if (ks.numel() != kv_heads || vs.numel() != kv_heads) raise("k_scale and v_scale must have one entry per kv head");
+  } else if (ks.defined() || vs.defined()) {
+    raise("k_scale and v_scale belong to a float8_e4m3fn cache");
+  }
+}
+
+std::tuple<Tensor, OptTensor> qk_rope(const Tensor& q_in, const Tensor& k_in, const Tensor& cos, const Tensor& sin, const Tensor& positions, const OptTensor& q_weight,
+                                      const OptTensor& k_weight, double eps, const OptTensor& v_in, const OptTensor& k_pages, const OptTensor& v_pages,
+                                      const OptTensor& slots, const OptTensor& k_scale, const OptTensor& v_scale, bool want_k) {
+  const at::Device dev = require_cuda({&q_in, &k_in, &cos, &sin, &positions, ptr_of(q_weight), ptr_of(k_weight), ptr_of(v_in), ptr_of(k_pages), ptr_of(v_pages),
+                                       ptr_of(slots), ptr_of(k_scale), ptr_of(v_scale)});
+  refuse_grad("qk_norm_rope", {&q_in, &k_in, ptr_of(q_weight), ptr_of(k_weight), ptr_of(v_in)});
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k");
+  const int64_t t = q.size(0), d = q.size(2);
+  const at::ScalarType type = q.scalar_type();
+  if (!is_float(type) || k.scalar_type() != type) raise("q and k must both be float32, float16 or bfloat16");
+  if (k.size(0) != t || k.size(2) != d) raise("q and k must have the same tokens and head_dim");
+  if (t > 0x7fffffff) raise("too many tokens");
+  if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat || cos.dim() != 2 || cos.sizes() != sin.sizes() || !cos.is_contiguous() || !sin.is_contiguous())
+    raise("cos / sin must be contiguous fp32 [positions, rotary / 2]");
+  check_index(positions, at::kInt, t, "positions");
+  at::ScalarType weight_type = type;
+  for (const OptTensor* w : {&q_weight, &k_weight}) {
+    if (!*w) continue;
+    if ((*w)->dim() != 1 || (*w)->size(0) != d || !(*w)->is_contiguous()) raise("the norm's weights must be contiguous [head_dim]");
+    weight_type = (*w)->scalar_type();
+  }
+  if (q_weight && k_weight && q_weight->scalar_type() != k_weight->scalar_type()) raise("q_weight and k_weight must have the same type");
+  if (weight_type != type && weight_type != at::kFloat) raise("the norm's weights must have the type of q and k, or float32");
+  qlin_qk_rope_args a = {};
+  Tensor v, ks, vs;
+  if (k_pages) {
+    if (!v_in || !v_pages || !slots) raise("a cache needs v, k_pages, v_pages and slots");
+    v = head_rows(*v_in, "v");
+    if (v.scalar_type() != type || v.sizes() != k.sizes()) raise("v must have the shape and type of k");
+    ks = f32(k_scale);
+    vs = f32(v_scale);
+    check_cache(*k_pages, *v_pages, k.size(1), d, type, ks, vs);
+    check_index(*slots, at::kLong, t, "slots");
+    a.v = data(v);
+    a.v_token = step(v, 0);
+    a.v_head = step(v, 1);
+    a.k_pages = data(*k_pages);
+    a.v_pages = data(*v_pages);
+    a.slots = static_cast<const int64_t*>(data(*slots));
+    a.k_scale = static_cast<const float*>(data(ks));
+    a.v_scale = static_cast<const float*>(data(vs));
+    a.page_stride = step(*k_pages, 0);
+    a.head_stride = step(*k_pages, 1);
+    a.slot_stride = step(*k_pages, 2);
+    a.page_size = static_cast<int32_t>(k_pages->size(2));
+    a.num_slots = k_pages->size(0) * k_pages->size(2);
+    a.cache_dtype = dtype_code(k_pages->scalar_type());
+  } else if (v_in || v_pages || slots || k_scale || v_scale) {
+    raise("v, v_pages, slots and scales belong to a cache: k_pages is missing");
+  }
+  Tensor q_out = empty(q.sizes(), type, dev), k_out;
+  if (want_k) k_out = empty(k.sizes(), type, dev);
+  a.q = data(q);
+  a.k = data(k);
+  a.q_out = data(q_out);
+  a.k_out = data(k_out);
+  a.q_weight = q_weight ? data(*q_weight) : nullptr;
+  a.k_weight = k_weight ? data(*k_weight) : nullptr;
+  a.cos = static_cast<const float*>(data(cos));
+  a.sin = static_cast<const float*>(data(sin));
+  a.positions = static_cast<const int32_t*>(data(positions));
+  a.status = static_cast<int32_t*>(status_word(dev.index()).data_ptr());
+  a.q_token = step(q, 0);
+  a.q_head = step(q, 1);
+  a.k_token = step(k, 0);
+  a.k_head = step(k, 1);
+  a.tokens = static_cast<int32_t>(t);
+  a.q_heads = static_cast<int32_t>(q.size(1));
+  a.kv_heads = static_cast<int32_t>(k.size(1));
+  a.head_dim = static_cast<int32_t>(d);
+  a.rotary = static_cast<int32_t>(2 * cos.size(1));
+  a.table_rows = static_cast<int32_t>(std::min<int64_t>(cos.size(0), 0x7fffffff));
+  a.dtype = dtype_code(type);
+  a.weight_dtype = dtype_code(weight_type);
+  a.eps = static_cast<float>(eps);
+  check(qlin_qk_rope(&a, stream_of(dev)), "qlin_qk_rope");
+  return {q_out, want_k ? OptTensor(k_out) : std::nullopt};
+}
+
+// `out`: given or fresh, dense and of q's shape and type.
+Tensor attention_out(const OptTensor& out, const Tensor& q, at::Device dev) {
+  if (!out) return empty(q.sizes(), q.scalar_type(), dev);
+  if (out->scalar_type() != q.scalar_type() || out->sizes() != q.sizes() || !out->is_contiguous()) raise("out must be contiguous, with the shape and type of q");
+  return *out;
+}
+
+Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& lens, const std::optional<double>& scale,
+                       int64_t window, int64_t sinks, const OptTensor& k_scale, const OptTensor& v_scale, const OptTensor& out_in) {
+  const at::Device dev = require_cuda({&q_in, &k_pages, &v_pages, &block_table, &lens, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
+  refuse_grad("paged_attention", {&q_in, &k_pages, &v_pages});
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor q = head_rows(q_in, "q");
+  const int64_t b = q.size(0), d = q.size(2);
+  if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) raise("q must be float16 or bfloat16");
+  if (k_pages.dim() != 4) raise("k_pages and v_pages must both be [pages, kv heads, page size, head_dim]");
+  const Tensor ks = f32(k_scale), vs = f32(v_scale);
+  check_cache(k_pages, v_pages, k_pages.size(1), d, q.scalar_type(), ks, vs);
+  if (block_table.scalar_type() != at::kInt || block_table.dim() != 2 || block_table.size(0) != b || (block_table.size(1) > 1 && block_table.stride(1) != 1))
+    raise("block_table must be int32 [batch, pages of a sequence] with contiguous rows");
+  check_index(lens, at::kInt, b, "lens");
+  if (b > 0x7fffffff || k_pages.size(0) > 0x7fffffff || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff) raise("batch, pages, window or sinks out of range");
+  const Tensor out = attention_out(out_in, q, dev);
+  qlin_paged_attention_args a = {};
+  a.q = data(q);
+  a.k_pages = data(k_pages);
+  a.v_pages = data(v_pages);
+  a.block_table = static_cast<const int32_t*>(data(block_table));
+  a.lens = static_cast<const int32_t*>(data(lens));
+  a.k_scale = static_cast<const float*>(data(ks));
+  a.v_scale = static_cast<const float*>(data(vs));
+  a.out = data(out);
+  a.status = static_cast<int32_t*>(status_word(dev.index()).data_ptr());
+  a.q_batch = step(q, 0);
+  a.q_head = step(q, 1);
+  a.page_stride = step(k_pages, 0);
+  a.head_stride = step(k_pages, 1);
+  a.slot_stride = step(k_pages, 2);
+  a.table_stride = step(block_table, 0);
+  a.batch = static_cast<int32_t>(b);
+  a.q_heads = static_cast<int32_t>(q.size(1));
+  a.kv_heads = static_cast<int32_t>(k_pages.size(1));
+  a.head_dim = static_cast<int32_t>(d);
+  a.page_size = static_cast<int32_t>(k_pages.size(2));
+  a.num_pages = static_cast<int32_t>(k_pages.size(0));
+  a.max_pages = static_cast<int32_t>(block_table.size(1));
+  a.window = static_cast<int32_t>(std::max<int64_t>(window, 0));
+  a.sinks = static_cast<int32_t>(sinks);
+  a.dtype = dtype_code(q.scalar_type());
+  a.cache_dtype = dtype_code(k_pages.scalar_type());
+  a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d)));
+  const int64_t bytes = qlin_paged_attention_workspace_bytes(&a);
+  if (bytes < 0) check(static_cast<int>(bytes), "qlin_paged_attention");
+  Tensor ws;
+  if (bytes > 0) ws = empty({bytes}, at::kByte, dev);
+  a.workspace = data(ws);
+  check(qlin_paged_attention(&a, stream_of(dev)), "qlin_paged_attention");
+  return out;
+}
+
+Tensor prompt_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& cu_q, const Tensor& cu_k, int64_t max_q, const std::optional<double>& scale,
+                        int64_t window, int64_t sinks, const OptTensor& out_in) {
+  const at::Device dev = require_cuda({&q_in, &k_in, &v_in, &cu_q, &cu_k, ptr_of(out_in)});
+  refuse_grad("prompt_attention", {&q_in, &k_in, &v_in});
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k"), v = head_rows(v_in, "v");
+  const at::ScalarType type = q.scalar_type();
+  if ((type != at::kHalf && type != at::kBFloat16) || k.scalar_type() != type || v.scalar_type() != type) raise("q, k and v must all be float16 or bfloat16");
+  if (k.sizes() != v.sizes() || k.size(2) != q.size(2)) raise("k and v must have the same shape, and the head_dim of q");
+  if (cu_q.dim() != 1 || cu_q.size(0) < 1) raise("cu_q must hold the first row of every sequence and the end");
+  check_index(cu_q, at::kInt, cu_q.size(0), "cu_q");
+  check_index(cu_k, at::kInt, cu_q.size(0), "cu_k");
+  if (q.size(0) > 0x7fffff00 || k.size(0) > 0x7fffff00 || max_q < 0 || max_q > q.size(0) || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff)
+    raise("tokens, max_q, window or sinks out of range");
+  const Tensor out = attention_out(out_in, q, dev);
+  qlin_prompt_attention_args a = {};
+  a.q = data(q);
+  a.k = data(k);
+  a.v = data(v);
+  a.out = data(out);
+  a.cu_q = static_cast<const int32_t*>(data(cu_q));
+  a.cu_k = static_cast<const int32_t*>(data(cu_k));
+  a.status = static_cast<int32_t*>(status_word(dev.index()).data_ptr());
+  a.q_token = step(q, 0);
+  a.q_head = step(q, 1);
+  a.k_token = step(k, 0);
+  a.k_head = step(k, 1);
+  a.v_token = step(v, 0);
+  a.v_head = step(v, 1);
+  a.tokens_q = static_cast<int32_t>(q.size(0));
+  a.tokens_k = static_cast<int32_t>(k.size(0));
+  a.batch = static_cast<int32_t>(cu_q.size(0) - 1);
+  a.max_q = static_cast<int32_t>(max_q);
+  a.q_heads = static_cast<int32_t>(q.size(1));
+  a.kv_heads = static_cast<int32_t>(k.size(1));
+  a.head_dim = static_cast<int32_t>(q.size(2));
+  a.window = static_cast<int32_t>(std::max<int64_t>(window, 0));
+  a.sinks = static_cast<int32_t>(sinks);
+  a.dtype = dtype_code(type);
+  a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2))));
+  check(qlin_prompt_attention(&a, stream_of(dev)), "qlin_prompt_attention");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_qlin_host, m) {
@@ -686,4 +913,7 @@ PYBIND11_MODULE(_qlin_host, m) {
   m.def("pact2_bwd", &pact2_bwd, rel());
   m.def("qat_takes", &qat_takes, rel());
   m.def("qat_linear", &qat_linear, rel());
+  m.def("qk_rope", &qk_rope, rel());
+  m.def("paged_attention", &paged_attention, rel());
+  m.def("prompt_attention", &prompt_attention, rel());
 }

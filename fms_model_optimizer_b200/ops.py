@@ -614,6 +614,81 @@ def shard_reduce_(x: torch.Tensor, src_multicast: int, max_ctas: int = 0) -> tor
 
 
 # --------------------------------------------------------------------------------------------------
+# Attention of a decoder that generates
+# --------------------------------------------------------------------------------------------------
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: torch.Tensor,
+    *,
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    v: Optional[torch.Tensor] = None,
+    k_pages: Optional[torch.Tensor] = None,
+    v_pages: Optional[torch.Tensor] = None,
+    slots: Optional[torch.Tensor] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    want_k: bool = True,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Per-head RMS norm of queries and keys (where weights are given), rotary embedding, and the write of k and v into a paged
+    cache, in one pass (``qlin_qk_rope``).  ``q [tokens, q heads, head_dim]``, ``k`` and ``v [tokens, kv heads, head_dim]``;
+    ``cos`` / ``sin`` fp32 ``[positions, rotary / 2]`` (``rotary`` <= head_dim, halves rotated as in ``rope_``), ``positions``
+    int32 ``[tokens]``.  With ``k_pages`` / ``v_pages [pages, kv heads, page size, head_dim]`` given, token t goes to slot
+    ``slots[t] = page * page size + offset`` (int64, negative: not written), in the model's type or as e4m3 codes of
+    ``x / k_scale[kv head]``.  Returns new ``(q, k)``; ``k`` is None without ``want_k``.  No gradient."""
+    dev = q.device
+    work = 2.0 * (q.numel() + k.numel()) * q.element_size()
+    return _call("qk_rope", work, dev, L.host().qk_rope, q, k, cos, sin, positions, q_weight, k_weight, eps, v, k_pages, v_pages, slots, k_scale, v_scale, want_k)
+
+
+def paged_attention(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    scale: Optional[float] = None,
+    window: int = 0,
+    sinks: int = 0,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of one new token of every sequence over its keys in a paged cache (``qlin_paged_attention``).  ``q [batch, q
+    heads, head_dim]`` stands at position ``lens[b] - 1``; key i of sequence b lies in page ``block_table[b, i // page size]``.
+    ``block_table`` int32 ``[batch, pages of a sequence]``, ``lens`` int32 ``[batch]``, both on the device.  ``window`` > 0: only
+    the last ``window`` keys and the first ``sinks`` are visible.  ``scale`` defaults to ``head_dim ** -0.5``.  A sequence of
+    length 0 gives zeros.  The width of ``block_table`` bounds the lengths and with them how finely the keys are split, so pass
+    no more columns than the longest sequence needs.  No gradient."""
+    return _call("paged_attention", 0.0, q.device, L.host().paged_attention, q, k_pages, v_pages, block_table, lens, scale, window, sinks, k_scale, v_scale, out)
+
+
+def prompt_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_q: torch.Tensor,
+    cu_k: torch.Tensor,
+    max_q: int,
+    *,
+    scale: Optional[float] = None,
+    window: int = 0,
+    sinks: int = 0,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Causal attention of packed prompts (``qlin_prompt_attention``).  Sequence b has the rows ``cu_q[b] : cu_q[b + 1]`` of ``q
+    [tokens, q heads, head_dim]`` and ``cu_k[b] : cu_k[b + 1]`` of ``k`` and ``v [keys, kv heads, head_dim]`` (int32 on the device); with n
+    queries and m keys, query i stands at position ``i + m - n``.  ``max_q``: the most queries of a sequence.  ``window`` and
+    ``sinks`` as in ``paged_attention``; a query that sees no key gives zeros.  No gradient."""
+    return _call("prompt_attention", 0.0, q.device, L.host().prompt_attention, q, k, v, cu_q, cu_k, max_q, scale, window, sinks, out)
+
+
+# --------------------------------------------------------------------------------------------------
 # Calibration statistics
 # --------------------------------------------------------------------------------------------------
 def col_absmax(x: torch.Tensor, running: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -634,6 +634,104 @@ int qlin_qat_split(const qlin_qat_args* args, void* stream);
 /* which: 0 out = x w^T + bias, 1 gx = g w, 2 gw = g^T x */
 int qlin_qat_product(const qlin_qat_args* args, int32_t which, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Attention of a decoder that generates: the rotation that fills a paged key-value cache, attention of whole prompts, attention of
+ * one new token over the cache.  No counterpart in the reference, whose quantized models leave generation to a serving stack.
+ *
+ * The cache is a pool of pages: k_pages and v_pages are [num_pages, kv_heads, page_size, head_dim] with the same strides (elements,
+ * head_dim contiguous), in the model's type or in e4m3 with one scale per kv head (value = code * scale).  A slot is
+ * page * page_size + offset.  Sequence b keeps its key i in page block_table[b, i / page_size], offset i % page_size.
+ *
+ * Mask of both attentions: a query at position p sees the keys j <= p with window <= 0 or j > p - window or j < sinks.  A query
+ * that sees no key, or whose visible logits are all minus infinity, gives zeros; what is not visible is not part of the result, NaN
+ * and infinities included.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* qlin_qk_rope -- norm, rotation and cache write of the queries and keys of `tokens` tokens in one pass.  Per head x of q and k:
+ *   y = x * rsqrt(mean x^2 + eps) * weight   (weight NULL: y = x)
+ *   z[i] = y[i] cos[i] - y[i + r/2] sin[i],  z[i + r/2] = y[i + r/2] cos[i] + y[i] sin[i]   for i < r/2, r = rotary;  z = y behind
+ * in fp32, rounded once; cos / sin are rows positions[t] of [table_rows, r/2] fp32 tables.  q_out and k_out (optional) are dense
+ * [tokens, heads, head_dim]; with k_pages given, z of the keys and v go to slot slots[t] of the cache (negative: not written),
+ * e4m3 as the code of x * (1 / scale) clamped to +-448.  A position or slot out of range writes QLIN_ERR_BAD_SHAPE to *status;
+ * a token with such a position gets NaN in q_out and k_out and stays out of the cache.
+ * head_dim and rotary are multiples of 16, head_dim <= 512; rows of every tensor start on 16 bytes. */
+typedef struct qlin_qk_rope_args {
+  const void* q;
+  const void* k;
+  const void* v;           /* with k_pages */
+  void* q_out;
+  void* k_out;             /* optional */
+  const void* q_weight;    /* optional [head_dim], weight_dtype */
+  const void* k_weight;    /* optional */
+  const float* cos;
+  const float* sin;
+  const int32_t* positions; /* [tokens] */
+  void* k_pages;           /* optional */
+  void* v_pages;
+  const int64_t* slots;    /* [tokens] */
+  const float* k_scale;    /* [kv_heads], e4m3 cache */
+  const float* v_scale;
+  int32_t* status;         /* optional device status word, written only on failure */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides in elements */
+  int64_t page_stride, head_stride, slot_stride;             /* of the cache, in elements */
+  int64_t num_slots;
+  int32_t tokens, q_heads, kv_heads, head_dim, rotary, table_rows, page_size;
+  int32_t dtype;           /* qlin_dtype of q, k, v, q_out, k_out: F32, F16 or BF16 */
+  int32_t weight_dtype;    /* the same, or F32 */
+  int32_t cache_dtype;     /* the same, or F8E4M3 */
+  float eps;
+} qlin_qk_rope_args;
+
+int qlin_qk_rope(const qlin_qk_rope_args* args, void* stream);
+
+/* qlin_paged_attention -- one new token of every sequence against its keys in the cache, the new token's own key included:
+ * sequence b has lens[b] keys and its query stands at position lens[b] - 1.  The keys of a sequence are split over several blocks
+ * and joined in order, so results do not depend on timing.  out is dense [batch, q_heads, head_dim].  q_heads is a multiple of
+ * kv_heads; head_dim a multiple of 8 (16 with an e4m3 cache) up to 128.  lens above max_pages * page_size or a page that does not
+ * exist write QLIN_ERR_BAD_SHAPE to *status; such a length is cut, such a page read as page 0. */
+typedef struct qlin_paged_attention_args {
+  const void* q;              /* [batch, q_heads, head_dim] */
+  const void* k_pages;
+  const void* v_pages;
+  const int32_t* block_table; /* [batch, max_pages], row stride table_stride */
+  const int32_t* lens;        /* [batch] */
+  const float* k_scale;       /* [kv_heads], e4m3 cache */
+  const float* v_scale;
+  void* out;
+  void* workspace;            /* qlin_paged_attention_workspace_bytes, 16-byte aligned */
+  int32_t* status;            /* optional device status word, written only on failure */
+  int64_t q_batch, q_head;    /* strides in elements */
+  int64_t page_stride, head_stride, slot_stride, table_stride;
+  int32_t batch, q_heads, kv_heads, head_dim, page_size, num_pages, max_pages, window, sinks;
+  int32_t dtype;              /* qlin_dtype of q and out: F16 or BF16 */
+  int32_t cache_dtype;        /* the same, or F8E4M3 */
+  float scale;                /* of the logits */
+} qlin_paged_attention_args;
+
+int64_t qlin_paged_attention_workspace_bytes(const qlin_paged_attention_args* args);
+int qlin_paged_attention(const qlin_paged_attention_args* args, void* stream);
+
+/* qlin_prompt_attention -- attention of packed sequences: sequence b has the queries cu_q[b] .. cu_q[b + 1] of q [tokens_q, q_heads,
+ * head_dim] and the keys cu_k[b] .. cu_k[b + 1] of k, v [tokens_k, kv_heads, head_dim]; query i of n stands at position i + m - n
+ * where m is the number of keys.  out is dense [tokens_q, q_heads, head_dim].  F16 or BF16; q_heads a multiple of kv_heads, at
+ * most 128 query heads a kv head; head_dim a multiple of 8 up to 128.  cu_q and cu_k start at 0, end at tokens_q and tokens_k and
+ * do not fall, and no sequence has more than max_q queries; otherwise QLIN_ERR_BAD_SHAPE in *status and rows left unwritten. */
+typedef struct qlin_prompt_attention_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const int32_t* cu_q;        /* [batch + 1] */
+  const int32_t* cu_k;
+  int32_t* status;            /* optional device status word, written only on failure */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides in elements */
+  int32_t tokens_q, tokens_k, batch, max_q, q_heads, kv_heads, head_dim, window, sinks;
+  int32_t dtype;
+  float scale;                /* of the logits */
+} qlin_prompt_attention_args;
+
+int qlin_prompt_attention(const qlin_prompt_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
