@@ -690,7 +690,8 @@ bool on16(const Tensor& t, int64_t stride) { return stride * static_cast<int64_t
 Tensor head_rows(const Tensor& t, const char* what) {
   if (t.dim() != 3) raise(std::string(what) + " must be [tokens, heads, head_dim]");
   const bool fits = t.stride(2) == 1 && on16(t, step(t, 0)) && on16(t, step(t, 1)) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  if (fits && !t.is_neg()) return t;
+  const bool spread = (t.size(0) <= 1 || t.stride(0) > 0) && (t.size(1) <= 1 || t.stride(1) > 0);  // an expanded tensor has strides of 0
+  if (fits && spread && !t.is_neg()) return t;
   return t.resolve_neg().clone(at::MemoryFormat::Contiguous);
 }
 
@@ -868,6 +869,7 @@ Tensor prompt_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_
   check_index(cu_k, at::kInt, cu_q.size(0), "cu_k");
   if (q.size(0) > 0x7fffff00 || k.size(0) > 0x7fffff00 || max_q < 0 || max_q > q.size(0) || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff)
     raise("tokens, max_q, window or sinks out of range");
+  if (q.size(0) > 0 && (cu_q.size(0) < 2 || max_q < 1)) raise("q has rows, but cu_q no sequence or max_q no row");
   const Tensor out = attention_out(out_in, q, dev);
   qlin_prompt_attention_args a = {};
   a.q = data(q);

@@ -459,6 +459,7 @@ static int check_paged(const qlin_paged_attention_args* a) {
   if (a->batch < 0 || a->q_heads < 1 || a->kv_heads < 1 || a->q_heads % a->kv_heads != 0)
     return fail(QLIN_ERR_BAD_SHAPE, "qlin_paged_attention: q_heads must be a multiple of kv_heads");
   if (a->page_size < 1 || a->num_pages < 0 || a->max_pages < 0) return fail(QLIN_ERR_BAD_SHAPE, "qlin_paged_attention: bad cache dimensions");
+  if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return fail(QLIN_ERR_UNSUPPORTED, "qlin_paged_attention: scale must be positive and finite");
   if (static_cast<int64_t>(a->max_pages) * a->page_size > (1 << 30)) return fail(QLIN_ERR_TOO_LARGE, "qlin_paged_attention: at most 2^30 keys a sequence");
   if (a->dtype != QLIN_DT_F16 && a->dtype != QLIN_DT_BF16) return fail(QLIN_ERR_BAD_DTYPE, "qlin_paged_attention: q must be fp16 or bf16");
   if (a->cache_dtype != a->dtype && a->cache_dtype != QLIN_DT_F8E4M3) return fail(QLIN_ERR_BAD_DTYPE, "qlin_paged_attention: the cache must have the type of q, or e4m3");

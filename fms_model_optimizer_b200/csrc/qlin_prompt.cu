@@ -3,16 +3,20 @@
 //   o_i = sum_j w_j v_j / sum_j w_j,   w_j = 2^(x_j - max x),   x_j = q_i.k_j scale log2(e),   j over the keys that i sees
 #include <type_traits>
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "qlin_internal.h"
+#include "qlin_ptx.cuh"
 
 namespace qlin {
 
 struct PromptParams {
   qlin_prompt_attention_args a;
   int32_t group;  // query heads per kv head
+  int32_t tq;     // queries of a tile: its rows are tq queries times the group's heads
+  int32_t units;  // pairs of tiles of the longest sequence
   float cl2;      // scale * log2(e)
 };
 
@@ -113,16 +117,495 @@ __device__ __noinline__ void attend_row(const PromptParams& p, const Sequence& s
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(128) prompt_rows_kernel(const __grid_constant__ PromptParams p) {
-  const int b = blockIdx.z, head = blockIdx.y;
-  const Sequence s = sequence_of(p, b);
-  if (s.bad) {
-    if (threadIdx.x == 0 && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
+// ------------------------------------------------------------------------------------------------ tensor cores
+constexpr int kRows = 128;        // rows of a tile of queries
+constexpr int kKeys = 128;        // keys of a tile
+constexpr int kSoftmaxWarps = 8;  // four a tile of queries, a thread a row
+constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;
+constexpr int kPromptThreads = (kSoftmaxWarps + 4) * 32;  // whole warpgroups: registers are handed over between them
+// A block starts with 168 registers a thread (64,512 in all); the softmax warps take 208 each once the others have gone down to 80
+// (63,488): a row of 128 logits stays in registers.
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
+constexpr int kChunkBytes = 128 * 128;  // 128 rows of 64 elements, 128-byte swizzle
+constexpr float kSlack = 8.0f;
+
+struct PromptAux {
+  uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], p_full[2], o_full[2], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <typename T, int DP>
+struct PromptCfg {
+  static constexpr int CHUNKS = DP / 64;
+  static constexpr int TILE_BYTES = CHUNKS * kChunkBytes;  // a tile of queries, keys or values
+  static constexpr int STAGES = DP == 128 ? 4 : 8;         // tiles of keys or values in flight
+  static constexpr int KV_OFFSET = 2 * TILE_BYTES;
+  static constexpr int AUX_OFFSET = KV_OFFSET + STAGES * TILE_BYTES;
+  static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(PromptAux));
+  static constexpr float SHIFT = std::is_same<T, __half>::value ? 6.0f : 0.0f;
+  static constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
+  static constexpr uint32_t IDESC_S = make_idesc(1u, FMT, kRows, kKeys);
+  static constexpr uint32_t IDESC_O = make_idesc(1u, FMT, kRows, DP) | (1u << 16);  // V is read with its head dimension contiguous
+};
+
+__device__ __forceinline__ void prompt_load(uint64_t* bar, void* dst, const void* tmap, int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred pe;\n\t"
+      "elect.sync _|pe, 0xffffffff;\n\t"
+      "@pe cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%3, %4, %5}], [%0];\n\t"
+      "}" ::"r"(smem_u32(bar)),
+      "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void prompt_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred pe;\n\t"
+      "elect.sync _|pe, 0xffffffff;\n\t"
+      "@pe mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t"
+      "}" ::"r"(smem_u32(bar)),
+      "r"(bytes)
+      : "memory");
+}
+// Four K = 16 steps; A from shared memory (descriptor, two units of 16 bytes a step) and B likewise.
+__device__ __forceinline__ void mma4_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred pe, pa, pt;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "elect.sync _|pe, 0xffffffff;\n\t"
+      "setp.ne.b32 pa, %4, 0;\n\t"
+      "setp.ne.b32 pt, %3, 0;\n\t"
+      "add.s64 a1, %1, 2;\n\t"
+      "add.s64 b1, %2, 2;\n\t"
+      "add.s64 a2, %1, 4;\n\t"
+      "add.s64 b2, %2, 4;\n\t"
+      "add.s64 a3, %1, 6;\n\t"
+      "add.s64 b3, %2, 6;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pa;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, pt;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, pt;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, pt;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Four K = 16 steps; A from tensor memory (8 columns a step), B an MN-major tile (128 units of 16 bytes a step).
+__device__ __forceinline__ void mma4_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred pe, pa, pt;\n\t"
+      ".reg .b32 a1, a2, a3;\n\t"
+      ".reg .b64 b1, b2, b3;\n\t"
+      "elect.sync _|pe, 0xffffffff;\n\t"
+      "setp.ne.b32 pa, %4, 0;\n\t"
+      "setp.ne.b32 pt, %3, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\t"
+      "add.s64 b1, %2, 128;\n\t"
+      "add.u32 a2, %1, 16;\n\t"
+      "add.s64 b2, %2, 256;\n\t"
+      "add.u32 a3, %1, 24;\n\t"
+      "add.s64 b3, %2, 384;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pa;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, pt;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, pt;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, pt;\n\t"
+      "}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of a tile of values, [128 keys][64 elements] pieces 16 KB apart: the head dimension is contiguous, groups of eight
+// keys are 1024 bytes apart.
+__device__ __forceinline__ uint64_t values_desc(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(kChunkBytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+#define QLIN_R32(v, o)                                                                                                                                       \
+  "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7]), "r"(v[o + 8]), "r"(v[o + 9]),          \
+      "r"(v[o + 10]), "r"(v[o + 11]), "r"(v[o + 12]), "r"(v[o + 13]), "r"(v[o + 14]), "r"(v[o + 15]), "r"(v[o + 16]), "r"(v[o + 17]), "r"(v[o + 18]),        \
+      "r"(v[o + 19]), "r"(v[o + 20]), "r"(v[o + 21]), "r"(v[o + 22]), "r"(v[o + 23]), "r"(v[o + 24]), "r"(v[o + 25]), "r"(v[o + 26]), "r"(v[o + 27]),        \
+      "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]), "r"(v[o + 31])
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::QLIN_R32(r, 0),
+      "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Two tiles of queries of one kv head and the tiles of keys that any of their rows sees.
+struct Unit {
+  int t0, kvh;     // first query
+  int shift;       // position of query 0
+  int sink_tiles, win_tile, tiles;
+  bool second;     // the second tile has rows
+  __device__ __forceinline__ int key0(int t) const { return (t < sink_tiles ? t : win_tile + (t - sink_tiles)) * kKeys; }
+};
+__device__ __forceinline__ Unit unit_of(const PromptParams& p, const Sequence& s, int t0, int kvh) {
+  Unit u;
+  u.t0 = t0;
+  u.kvh = kvh;
+  u.shift = s.m - s.n;
+  const int lo = t0 + u.shift, hi = min(t0 + 2 * p.tq, s.n) - 1 + u.shift;
+  const int end = hi < 0 ? 0 : hi / kKeys + 1;
+  u.win_tile = p.a.window > 0 ? min(max(lo - p.a.window + 1, 0) / kKeys, end) : 0;
+  u.sink_tiles = min((p.a.sinks + kKeys - 1) / kKeys, u.win_tile);
+  u.tiles = u.sink_tiles + end - u.win_tile;
+  u.second = t0 + p.tq < s.n;
+  return u;
+}
+
+// One tile of logits to weights: the row's 128 logits x are in registers; the weights go to tensor memory over them.
+template <typename T, int DP, bool MASKED>
+__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, float cl2, int hi, int lo, int sinks, bool first, float& m, float& l) {
+  using C = PromptCfg<T, DP>;
+  uint32_t x[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, x[c]);
+  if constexpr (MASKED) {
+    // column j is seen when j <= hi and (j > lo or j < sinks)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const int col = 32 * c + j;
+        if (col > hi || (col <= lo && col >= sinks)) x[c][j] = 0xff800000u;
+      }
+  }
+  float top[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    top[c] = __uint_as_float(x[c][0]);
+#pragma unroll
+    for (int j = 1; j < 32; ++j) top[c] = fmaxf(top[c], __uint_as_float(x[c][j]));
+  }
+  const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cl2;
+  // The reference that the weights are relative to follows the maximum only when that has outgrown it by 2^kSlack: the sums are the
+  // same up to rounding, and the accumulator is seldom rewritten.
+  const bool grow = most > m + kSlack || (m == -INFINITY && most > -INFINITY);
+  if (__any_sync(0xffffffffu, grow)) {
+    const float next = grow ? most : m;
+    if (!first) {
+      const float keep = grow ? exp2f(m - next) : 1.0f;
+      l *= keep;
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(o_addr + 32 * c, o);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+        tmem_st32(o_addr + 32 * c, o);
+      }
+    }
+    m = next;
+  }
+  const float ref = C::SHIFT - (m == -INFINITY ? 0.0f : m);
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float a = exp2_fast(__uint_as_float(x[2 * half + i / 16][2 * i % 32]) * cl2 + ref);
+      const float b = exp2_fast(__uint_as_float(x[2 * half + i / 16][2 * i % 32 + 1]) * cl2 + ref);
+      sum[i & 3] += a + b;
+      w[i] = pack2<T>(a, b);
+    }
+    tmem_st32(s_addr + 32 * half, w);
+  }
+  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  tmem_wait_st();
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+              const __grid_constant__ PromptParams p) {
+  using C = PromptCfg<T, DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  PromptAux* aux = reinterpret_cast<PromptAux*>(smem + C::AUX_OFFSET);
+  volatile int* abort_flag = &aux->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the longest units first: the last queries of every sequence and head
+  const int heads_all = p.a.kv_heads * p.a.batch;
+  const int unit = p.units - 1 - static_cast<int>(blockIdx.x / heads_all), rest = static_cast<int>(blockIdx.x % heads_all);
+  const int b = rest / p.a.kv_heads, kvh = rest % p.a.kv_heads;
+  const Sequence seq = sequence_of(p, b);
+  if (seq.bad || (smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0 && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(seq.bad ? QLIN_ERR_BAD_SHAPE : QLIN_ERR_BAD_ALIGN));
     return;
   }
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (i < s.n) attend_row<T>(p, s, i, head);
+  if (unit * 2 * p.tq >= seq.n) return;
+  const Unit u = unit_of(p, seq, unit * 2 * p.tq, kvh);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&aux->q_full, 1);
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&aux->kv_full[i], 1);
+      mbar_init(&aux->kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&aux->s_full[i], 1);
+      mbar_init(&aux->p_full[i], 128);
+      mbar_init(&aux->o_full[i], 1);
+    }
+    mbar_init(&aux->drain, 1);
+    aux->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&aux->tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = aux->tmem_base;  // S 0, S 1 (128 columns each), O 0, O 1 (DP columns each)
+  bool ok = true, timed_out = false;
+
+  if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kLoadWarp) {
+      // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ...
+      if (u.tiles > 0) {
+        const int q_tiles = u.second ? 2 : 1;
+        prompt_expect(&aux->q_full, static_cast<uint32_t>(q_tiles * C::CHUNKS * p.tq * p.group * 128));
+        for (int i = 0; i < q_tiles; ++i)
+          for (int c = 0; c < C::CHUNKS; ++c)
+            prompt_load(&aux->q_full, smem + i * C::TILE_BYTES + c * kChunkBytes, &tmap_q, c * 64, kvh * p.group, seq.q0 + u.t0 + i * p.tq);
+      }
+      uint32_t s = 0, ph = 1;
+      int issued = 0;
+      for (int t = 0; t < u.tiles && ok; ++t) {
+        const int row = seq.k0 + u.key0(t);
+        for (int kv = 0; kv < 2; ++kv) {
+          ok = warp_mbar_wait(&aux->kv_empty[s], ph, abort_flag);
+          if (!ok) break;
+          ++issued;
+          prompt_expect(&aux->kv_full[s], C::TILE_BYTES);
+          for (int c = 0; c < C::CHUNKS; ++c)
+            prompt_load(&aux->kv_full[s], smem + C::KV_OFFSET + s * C::TILE_BYTES + c * kChunkBytes, kv ? &tmap_v : &tmap_k, c * 64, kvh, row);
+          if (++s == C::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (!ok) {  // copies in flight land before the block retires
+        if (lane == 0) {
+          timed_out = !*abort_flag;
+          *abort_flag = 1;
+        }
+        mbar_wait_drain(&aux->q_full, 0);
+        for (int n = max(0, issued - C::STAGES); n < issued; ++n) mbar_wait_drain(&aux->kv_full[n % C::STAGES], (n / C::STAGES) & 1);
+      }
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------------ products
+      const uint32_t base = smem_u32(smem);
+      uint32_t s = 0, ph = 0;
+      const auto logits = [&](int i, uint32_t stage) {
+  #pragma unroll
+        for (int c = 0; c < C::CHUNKS; ++c)
+          mma4_ss(tmem + i * kKeys, make_smem_desc_sw128(base + i * C::TILE_BYTES + c * kChunkBytes),
+                  make_smem_desc_sw128(base + C::KV_OFFSET + stage * C::TILE_BYTES + c * kChunkBytes), C::IDESC_S, c > 0);
+        tc_commit_elect(&aux->s_full[i]);
+      };
+      const auto outputs = [&](int i, uint32_t stage, bool first) {
+        const uint64_t v = values_desc(base + C::KV_OFFSET + stage * C::TILE_BYTES);
+        mma4_ts(tmem + 2 * kKeys + i * DP, tmem + i * kKeys, v, C::IDESC_O, !first);
+        mma4_ts(tmem + 2 * kKeys + i * DP, tmem + i * kKeys + 32, v + 512, C::IDESC_O, 1);
+      };
+      const auto next_stage = [&]() {
+        if (++s == C::STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
+      };
+      if (u.tiles > 0) {
+        ok = warp_mbar_wait(&aux->q_full, 0, abort_flag) && warp_mbar_wait(&aux->kv_full[0], 0, abort_flag);
+        if (ok) {
+          tc_fence_after();
+          logits(0, 0);
+          if (u.second) logits(1, 0);
+          tc_commit_elect(&aux->kv_empty[0]);
+          next_stage();
+        }
+        for (int t = 0; t < u.tiles && ok; ++t) {
+          const uint32_t sv = s;
+          ok = warp_mbar_wait(&aux->kv_full[sv], ph, abort_flag);
+          if (!ok) break;
+          next_stage();
+          const bool more = t + 1 < u.tiles;
+          const uint32_t sk = s;
+          if (more) {
+            ok = warp_mbar_wait(&aux->kv_full[sk], ph, abort_flag);
+            if (!ok) break;
+            next_stage();
+          }
+          for (int i = 0; i < (u.second ? 2 : 1) && ok; ++i) {
+            ok = warp_mbar_wait(&aux->p_full[i], t & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            outputs(i, sv, t == 0);
+            if (i == (u.second ? 1 : 0)) tc_commit_elect(&aux->kv_empty[sv]);
+            if (more) {
+              logits(i, sk);
+            } else {
+              tc_commit_elect(&aux->o_full[i]);
+            }
+          }
+          if (ok && more) tc_commit_elect(&aux->kv_empty[sk]);
+        }
+      }
+      if (!ok && lane == 0) {
+        timed_out = !*abort_flag;
+        *abort_flag = 1;
+      }
+      __syncwarp();
+      // nothing may still be reading shared memory or writing tensor memory when the block retires
+      tc_commit_elect(&aux->drain);
+      mbar_wait_drain(&aux->drain, 0);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax: a thread a row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int i = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int token = u.t0 + i * p.tq + r / p.group, head = kvh * p.group + r % p.group;
+    const bool row_ok = r < p.tq * p.group && token < seq.n;
+    const int pos = token + u.shift;
+    const int tile_lo = u.t0 + i * p.tq + u.shift, tile_hi = tile_lo + p.tq - 1;  // positions of this tile of queries
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + i * kKeys, o_addr = tmem + lanes + 2 * kKeys + i * DP;
+    float m = -INFINITY, l = 0.0f;
+    if (i == 0 || u.second) {
+      for (int t = 0; t < u.tiles && ok; ++t) {
+        ok = warp_mbar_wait(&aux->s_full[i], t & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const int k0 = u.key0(t);
+        const bool full = k0 + kKeys - 1 <= tile_lo && (p.a.window <= 0 || k0 > tile_hi - p.a.window || k0 + kKeys <= p.a.sinks);
+        if (full) {
+          softmax_tile<T, DP, false>(s_addr, o_addr, p.cl2, 0, 0, 0, t == 0, m, l);
+        } else {
+          softmax_tile<T, DP, true>(s_addr, o_addr, p.cl2, pos - k0, p.a.window > 0 ? pos - p.a.window - k0 : -1, p.a.sinks - k0, t == 0, m, l);
+        }
+        tc_fence_before();
+        mbar_arrive(&aux->p_full[i]);
+      }
+      if (ok && u.tiles > 0) ok = warp_mbar_wait(&aux->o_full[i], 0, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+        T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(seq.q0 + token) * p.a.q_heads + head) * p.a.head_dim;
+        bool again = false;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          if (u.tiles > 0) {
+            tmem_ld32(o_addr + 32 * c, o);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) again |= __uint_as_float(o[j]) != __uint_as_float(o[j]);
+          if (row_ok) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (32 * c + j < p.a.head_dim) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = pack2<T>(__uint_as_float(o[j + 2 * e]) * scale, __uint_as_float(o[j + 2 * e + 1]) * scale);
+                *reinterpret_cast<uint4*>(out + 32 * c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+          }
+        }
+        // A weight of zero times NaN or infinity is NaN: a value that the row does not see may have got into its sums, so rows that
+        // come out as NaN are computed again from what they do see.
+        uint32_t redo = __ballot_sync(0xffffffffu, row_ok && again);
+        __syncwarp();  // the rows are written before they are written again
+        while (redo != 0) {
+          const int r2 = (warp & 3) * 32 + __ffs(redo) - 1;
+          redo &= redo - 1;
+          attend_row<T>(p, seq, u.t0 + i * p.tq + r2 / p.group, kvh * p.group + r2 % p.group);
+        }
+      } else if (lane == 0) {
+        timed_out = !*abort_flag;
+        *abort_flag = 1;
+      }
+    }
+    __syncwarp();
+  }
+  if (timed_out && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_TIMEOUT));
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// [tokens, heads, head_dim] read in boxes of box_tokens x box_heads x 64 elements; head dimensions past the end are zeros.
+static int head_map(CUtensorMap* tm, const void* base, int dtype, int64_t tokens, int64_t heads, int64_t dim, int64_t token_stride, int64_t head_stride, int box_tokens,
+                    int box_heads) {
+  using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                          CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  const Fn enc = reinterpret_cast<Fn>(tensor_map_encoder());
+  if (enc == nullptr) return fail(QLIN_ERR_DEVICE, "cuTensorMapEncodeTiled is not available from this driver");
+  const int64_t row = (dim * 2 + 15) / 16 * 16;  // stands in for the stride of a dimension with one entry
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? head_stride * 2 : row), static_cast<cuuint64_t>(tokens > 1 ? token_stride * 2 : row)};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(tm, dtype == QLIN_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(QLIN_ERR_BAD_ALIGN, "qlin_prompt_attention: cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+  return QLIN_OK;
+}
+
+template <typename T, int DP>
+static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
+  using C = PromptCfg<T, DP>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return fail(QLIN_ERR_DEVICE, "device ordinal %d out of range", dev);
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    if (e != cudaSuccess) return fail(QLIN_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    configured[dev] = true;
+  }
+  CUtensorMap tq, tk, tv;
+  int rc = head_map(&tq, p.a.q, p.a.dtype, p.a.tokens_q, p.a.q_heads, p.a.head_dim, p.a.q_token, p.a.q_head, p.tq, p.group);
+  if (rc == QLIN_OK) rc = head_map(&tk, p.a.k, p.a.dtype, p.a.tokens_k, p.a.kv_heads, p.a.head_dim, p.a.k_token, p.a.k_head, kKeys, 1);
+  if (rc == QLIN_OK) rc = head_map(&tv, p.a.v, p.a.dtype, p.a.tokens_k, p.a.kv_heads, p.a.head_dim, p.a.v_token, p.a.v_head, kKeys, 1);
+  if (rc != QLIN_OK) return rc;
+  const int64_t blocks = static_cast<int64_t>(p.units) * p.a.kv_heads * p.a.batch;
+  if (blocks > 0x7fffffff) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: too many queries, heads and sequences");
+  prompt_kernel<T, DP><<<static_cast<unsigned>(blocks), kPromptThreads, C::SMEM_BYTES, stream>>>(tq, tk, tv, p);
+  QLIN_CHECK_LAUNCH("qlin_prompt_attention");
+  return QLIN_OK;
 }
 
 }  // namespace qlin
@@ -138,7 +621,12 @@ extern "C" int qlin_prompt_attention(const qlin_prompt_attention_args* a, void* 
   if (a->batch == 0 || a->tokens_q == 0 || a->max_q == 0) return QLIN_OK;
   if (a->q == nullptr || a->out == nullptr || a->cu_q == nullptr || a->cu_k == nullptr) return fail(QLIN_ERR_NULL, "qlin_prompt_attention: q, out, cu_q or cu_k is NULL");
   if (a->tokens_k > 0 && (a->k == nullptr || a->v == nullptr)) return fail(QLIN_ERR_NULL, "qlin_prompt_attention: k or v is NULL");
-  if (a->q_heads > 65535 || a->batch > 65535) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: at most 65535 heads and sequences");
+  if (static_cast<int64_t>(a->kv_heads) * a->batch > (1 << 24)) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: too many heads and sequences");
+  if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return fail(QLIN_ERR_UNSUPPORTED, "qlin_prompt_attention: scale must be positive and finite");
+  const auto pitch = [](int64_t entries, int64_t stride) { return entries > 1 && (stride <= 0 || stride >= (int64_t{1} << 38)); };
+  if (pitch(a->tokens_q, a->q_token) || pitch(a->q_heads, a->q_head) || pitch(a->tokens_k, a->k_token) || pitch(a->kv_heads, a->k_head) ||
+      pitch(a->tokens_k, a->v_token) || pitch(a->kv_heads, a->v_head))
+    return fail(QLIN_ERR_BAD_SHAPE, "qlin_prompt_attention: strides must be positive");
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) || a->q_token % 8 != 0 || a->q_head % 8 != 0 || a->k_token % 8 != 0 ||
       a->k_head % 8 != 0 || a->v_token % 8 != 0 || a->v_head % 8 != 0)
     return fail(QLIN_ERR_BAD_ALIGN, "qlin_prompt_attention: every row must start on 16 bytes");
@@ -146,13 +634,13 @@ extern "C" int qlin_prompt_attention(const qlin_prompt_attention_args* a, void* 
   p.a = *a;
   p.group = a->q_heads / a->kv_heads;
   p.cl2 = a->scale * 1.4426950408889634f;
-  const dim3 grid(static_cast<unsigned>((a->max_q + 3) / 4), static_cast<unsigned>(a->q_heads), static_cast<unsigned>(a->batch));
-  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (a->dtype == QLIN_DT_BF16) {
-    prompt_rows_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
-  } else {
-    prompt_rows_kernel<__half><<<grid, 128, 0, s>>>(p);
+  p.tq = kRows / p.group;
+  p.units = static_cast<int32_t>((static_cast<int64_t>(a->max_q) + 2 * p.tq - 1) / (2 * p.tq));
+  if (a->tokens_k == 0) {  // nothing to see: the tensor maps have no memory to describe
+    const cudaError_t e = cudaMemsetAsync(a->out, 0, static_cast<size_t>(a->tokens_q) * a->q_heads * a->head_dim * 2, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? QLIN_OK : fail(QLIN_ERR_LAUNCH, "qlin_prompt_attention: %s", cudaGetErrorString(e));
   }
-  QLIN_CHECK_LAUNCH("qlin_prompt_attention");
-  return QLIN_OK;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->dtype == QLIN_DT_BF16) return a->head_dim <= 64 ? launch_prompt<__nv_bfloat16, 64>(p, s) : launch_prompt<__nv_bfloat16, 128>(p, s);
+  return a->head_dim <= 64 ? launch_prompt<__half, 64>(p, s) : launch_prompt<__half, 128>(p, s);
 }

@@ -705,7 +705,7 @@ typedef struct qlin_paged_attention_args {
   int32_t batch, q_heads, kv_heads, head_dim, page_size, num_pages, max_pages, window, sinks;
   int32_t dtype;              /* qlin_dtype of q and out: F16 or BF16 */
   int32_t cache_dtype;        /* the same, or F8E4M3 */
-  float scale;                /* of the logits */
+  float scale;                /* of the logits, positive */
 } qlin_paged_attention_args;
 
 int64_t qlin_paged_attention_workspace_bytes(const qlin_paged_attention_args* args);
@@ -714,7 +714,7 @@ int qlin_paged_attention(const qlin_paged_attention_args* args, void* stream);
 /* qlin_prompt_attention -- attention of packed sequences: sequence b has the queries cu_q[b] .. cu_q[b + 1] of q [tokens_q, q_heads,
  * head_dim] and the keys cu_k[b] .. cu_k[b + 1] of k, v [tokens_k, kv_heads, head_dim]; query i of n stands at position i + m - n
  * where m is the number of keys.  out is dense [tokens_q, q_heads, head_dim].  F16 or BF16; q_heads a multiple of kv_heads, at
- * most 128 query heads a kv head; head_dim a multiple of 8 up to 128.  cu_q and cu_k start at 0, end at tokens_q and tokens_k and
+ * most 128 query heads a kv head; head_dim a multiple of 8 up to 128; strides positive.  cu_q and cu_k start at 0, end at tokens_q and tokens_k and
  * do not fall, and no sequence has more than max_q queries; otherwise QLIN_ERR_BAD_SHAPE in *status and rows left unwritten. */
 typedef struct qlin_prompt_attention_args {
   const void* q;
@@ -727,7 +727,7 @@ typedef struct qlin_prompt_attention_args {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides in elements */
   int32_t tokens_q, tokens_k, batch, max_q, q_heads, kv_heads, head_dim, window, sinks;
   int32_t dtype;
-  float scale;                /* of the logits */
+  float scale;                /* of the logits, positive */
 } qlin_prompt_attention_args;
 
 int qlin_prompt_attention(const qlin_prompt_attention_args* args, void* stream);
