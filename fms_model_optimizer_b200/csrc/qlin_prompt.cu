@@ -130,7 +130,7 @@ constexpr int kChunkBytes = 128 * 128;  // 128 rows of 64 elements, 128-byte swi
 constexpr float kSlack = 8.0f;
 
 struct PromptAux {
-  uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], p_full[2], o_full[2], drain;
+  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], p_full[2][2], o_full[2], drain;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -250,56 +250,124 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 // Two tiles of queries of one kv head and the tiles of keys that any of their rows sees.
 struct Unit {
-  int t0, kvh;     // first query
+  Sequence seq;
+  int b, kvh, t0;  // sequence, kv head, first query
   int shift;       // position of query 0
   int sink_tiles, win_tile, tiles;
   bool second;     // the second tile has rows
   __device__ __forceinline__ int key0(int t) const { return (t < sink_tiles ? t : win_tile + (t - sink_tiles)) * kKeys; }
 };
-__device__ __forceinline__ Unit unit_of(const PromptParams& p, const Sequence& s, int t0, int kvh) {
-  Unit u;
-  u.t0 = t0;
-  u.kvh = kvh;
-  u.shift = s.m - s.n;
-  const int lo = t0 + u.shift, hi = min(t0 + 2 * p.tq, s.n) - 1 + u.shift;
-  const int end = hi < 0 ? 0 : hi / kKeys + 1;
-  u.win_tile = p.a.window > 0 ? min(max(lo - p.a.window + 1, 0) / kKeys, end) : 0;
-  u.sink_tiles = min((p.a.sinks + kKeys - 1) / kKeys, u.win_tile);
-  u.tiles = u.sink_tiles + end - u.win_tile;
-  u.second = t0 + p.tq < s.n;
-  return u;
+// The units of a block, every gridDim.x-th one of the list that begins with the last queries of every sequence and head, which see
+// the most keys.  `busy`: units without keys are passed over.
+struct Units {
+  int64_t id, step, total;
+  __device__ __forceinline__ explicit Units(const PromptParams& p)
+      : id(blockIdx.x), step(gridDim.x), total(static_cast<int64_t>(p.units) * p.a.kv_heads * p.a.batch) {}
+  __device__ __forceinline__ bool next(const PromptParams& p, bool busy, Unit& u) {
+    const int lanes = p.a.kv_heads * p.a.batch;
+    for (; id < total; id += step) {
+      const int rest = static_cast<int>(id % lanes);
+      u.b = rest / p.a.kv_heads;
+      u.kvh = rest % p.a.kv_heads;
+      u.t0 = (p.units - 1 - static_cast<int>(id / lanes)) * 2 * p.tq;
+      u.seq = sequence_of(p, u.b);
+      if (u.seq.bad || u.t0 >= u.seq.n) continue;
+      u.shift = u.seq.m - u.seq.n;
+      const int lo = u.t0 + u.shift, hi = min(u.t0 + 2 * p.tq, u.seq.n) - 1 + u.shift;
+      const int end = hi < 0 ? 0 : hi / kKeys + 1;
+      u.win_tile = p.a.window > 0 ? min(max(lo - p.a.window + 1, 0) / kKeys, end) : 0;
+      u.sink_tiles = min((p.a.sinks + kKeys - 1) / kKeys, u.win_tile);
+      u.tiles = u.sink_tiles + end - u.win_tile;
+      u.second = u.t0 + p.tq < u.seq.n;
+      if (busy && u.tiles == 0) continue;
+      id += step;
+      return true;
+    }
+    return false;
+  }
+};
+
+__device__ __forceinline__ void tmem_issue32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+        "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// Waits for every load issued so far; the registers pass through so that no use of them can move above it.
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+// The larger of three, NaN if one is NaN.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair64(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair64(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
-// One tile of logits to weights: the row's 128 logits x are in registers; the weights go to tensor memory over them.
+// One tile of logits to weights: the row's 128 logits come from tensor memory and the weights go there over them, half by half;
+// each half is handed to the product when it is there.
 template <typename T, int DP, bool MASKED>
-__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, float cl2, int hi, int lo, int sinks, bool first, float& m, float& l) {
+__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, float cl2, int hi, int lo, int sinks, bool first, bool live, uint64_t* p_full, float& m, float& l) {
   using C = PromptCfg<T, DP>;
   uint32_t x[4][32];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, x[c]);
+  for (int c = 0; c < 4; ++c) tmem_issue32(s_addr + 32 * c, x[c]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_wait32(x[c]);
   if constexpr (MASKED) {
     // column j is seen when j <= hi and (j > lo or j < sinks)
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < 4; ++c) {
+      const auto below = [&](int n) { return n <= 32 * c ? 0u : (n >= 32 * c + 32 ? 0xffffffffu : (1u << (n - 32 * c)) - 1u); };  // columns under n
+      const uint32_t seen = below(hi + 1) & (~below(lo + 1) | below(sinks));
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const int col = 32 * c + j;
-        if (col > hi || (col <= lo && col >= sinks)) x[c][j] = 0xff800000u;
-      }
+      for (int j = 0; j < 32; ++j)
+        if (!((seen >> j) & 1u)) x[c][j] = 0xff800000u;
+    }
   }
   float top[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    top[c] = __uint_as_float(x[c][0]);
+    top[c] = max3_nan(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
 #pragma unroll
-    for (int j = 1; j < 32; ++j) top[c] = fmaxf(top[c], __uint_as_float(x[c][j]));
+    for (int j = 3; j < 31; j += 2) top[c] = max3_nan(top[c], __uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1]));
   }
-  const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cl2;
+  top[0] = max3_nan(top[0], top[1], __uint_as_float(x[0][31]));
+  top[2] = max3_nan(top[2], top[3], __uint_as_float(x[1][31]));
+  top[0] = max3_nan(top[0], __uint_as_float(x[2][31]), __uint_as_float(x[3][31]));
+  const float most = max3_nan(top[0], top[2], top[2]) * cl2;
   // The reference that the weights are relative to follows the maximum only when that has outgrown it by 2^kSlack: the sums are the
-  // same up to rounding, and the accumulator is seldom rewritten.
-  const bool grow = most > m + kSlack || (m == -INFINITY && most > -INFINITY);
+  // same up to rounding, and the accumulator is seldom rewritten.  A NaN or an infinity among the logits makes it NaN, and with it the row.
+  // Rows that are no query's hold anything and are left alone.
+  const bool grow = live && (!(most <= m + kSlack) || (m == -INFINITY && most > -INFINITY));
   if (__any_sync(0xffffffffu, grow)) {
-    const float next = grow ? most : m;
+    const float next = !grow ? m : (most == INFINITY ? __int_as_float(0x7fc00000) : most);
     if (!first) {
       const float keep = grow ? exp2f(m - next) : 1.0f;
       l *= keep;
@@ -315,21 +383,29 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, f
     m = next;
   }
   const float ref = C::SHIFT - (m == -INFINITY ? 0.0f : m);
-  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const uint64_t ref2 = pair64(ref, ref), cl22 = pair64(cl2, cl2);
+  uint64_t sum[2] = {0, 0};
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     uint32_t w[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const float a = exp2_fast(__uint_as_float(x[2 * half + i / 16][2 * i % 32]) * cl2 + ref);
-      const float b = exp2_fast(__uint_as_float(x[2 * half + i / 16][2 * i % 32 + 1]) * cl2 + ref);
-      sum[i & 3] += a + b;
+      const int c = 2 * half + i / 16, j = 2 * i % 32;
+      float a, b;
+      unpair64(fma2(pair64(__uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1])), cl22, ref2), a, b);
+      a = exp2_fast(a);
+      b = exp2_fast(b);
+      sum[i & 1] = add2(sum[i & 1], pair64(a, b));
       w[i] = pack2<T>(a, b);
     }
     tmem_st32(s_addr + 32 * half, w);
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(p_full + half);
   }
-  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-  tmem_wait_st();
+  float a, b;
+  unpair64(add2(sum[0], sum[1]), a, b);
+  l += a + b;
 }
 
 template <typename T, int DP>
@@ -341,27 +417,25 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   PromptAux* aux = reinterpret_cast<PromptAux*>(smem + C::AUX_OFFSET);
   volatile int* abort_flag = &aux->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the longest units first: the last queries of every sequence and head
-  const int heads_all = p.a.kv_heads * p.a.batch;
-  const int unit = p.units - 1 - static_cast<int>(blockIdx.x / heads_all), rest = static_cast<int>(blockIdx.x % heads_all);
-  const int b = rest / p.a.kv_heads, kvh = rest % p.a.kv_heads;
-  const Sequence seq = sequence_of(p, b);
-  if (seq.bad || (smem_u32(smem) & 1023u) != 0) {
-    if (threadIdx.x == 0 && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(seq.bad ? QLIN_ERR_BAD_SHAPE : QLIN_ERR_BAD_ALIGN));
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0 && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_ALIGN));
     return;
   }
-  if (unit * 2 * p.tq >= seq.n) return;
-  const Unit u = unit_of(p, seq, unit * 2 * p.tq, kvh);
+  if (blockIdx.x == 0 && p.a.status != nullptr)
+    for (int b = threadIdx.x; b < p.a.batch; b += kPromptThreads)
+      if (sequence_of(p, b).bad) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
 
   if (threadIdx.x == 0) {
-    mbar_init(&aux->q_full, 1);
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&aux->kv_full[i], 1);
       mbar_init(&aux->kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&aux->q_full[i], 1);
+      mbar_init(&aux->q_empty[i], 1);
       mbar_init(&aux->s_full[i], 1);
-      mbar_init(&aux->p_full[i], 128);
+      mbar_init(&aux->p_full[i][0], 128);
+      mbar_init(&aux->p_full[i][1], 128);
       mbar_init(&aux->o_full[i], 1);
     }
     mbar_init(&aux->drain, 1);
@@ -386,28 +460,34 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   if (warp >= kSoftmaxWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kLoadWarp) {
-      // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ...
-      if (u.tiles > 0) {
-        const int q_tiles = u.second ? 2 : 1;
-        prompt_expect(&aux->q_full, static_cast<uint32_t>(q_tiles * C::CHUNKS * p.tq * p.group * 128));
-        for (int i = 0; i < q_tiles; ++i)
-          for (int c = 0; c < C::CHUNKS; ++c)
-            prompt_load(&aux->q_full, smem + i * C::TILE_BYTES + c * kChunkBytes, &tmap_q, c * 64, kvh * p.group, seq.q0 + u.t0 + i * p.tq);
-      }
-      uint32_t s = 0, ph = 1;
+      // ------------------------------------------------------------------ loads: per unit Q 0, K 0, Q 1, V 0, K 1, V 1, K 2, ...
+      uint32_t s = 0, ph = 1, uses[2] = {0, 0};
       int issued = 0;
-      for (int t = 0; t < u.tiles && ok; ++t) {
-        const int row = seq.k0 + u.key0(t);
-        for (int kv = 0; kv < 2; ++kv) {
-          ok = warp_mbar_wait(&aux->kv_empty[s], ph, abort_flag);
-          if (!ok) break;
-          ++issued;
-          prompt_expect(&aux->kv_full[s], C::TILE_BYTES);
+      Unit u;
+      for (Units walk(p); ok && walk.next(p, true, u);) {
+        const auto load_q = [&](int i) {
+          ok = warp_mbar_wait(&aux->q_empty[i], (uses[i] & 1) ^ 1, abort_flag);
+          if (!ok) return;
+          ++uses[i];
+          prompt_expect(&aux->q_full[i], static_cast<uint32_t>(C::CHUNKS * p.tq * p.group * 128));
           for (int c = 0; c < C::CHUNKS; ++c)
-            prompt_load(&aux->kv_full[s], smem + C::KV_OFFSET + s * C::TILE_BYTES + c * kChunkBytes, kv ? &tmap_v : &tmap_k, c * 64, kvh, row);
-          if (++s == C::STAGES) {
-            s = 0;
-            ph ^= 1u;
+            prompt_load(&aux->q_full[i], smem + i * C::TILE_BYTES + c * kChunkBytes, &tmap_q, c * 64, u.kvh * p.group, u.seq.q0 + u.t0 + i * p.tq);
+        };
+        load_q(0);
+        for (int t = 0; t < u.tiles && ok; ++t) {
+          const int row = u.seq.k0 + u.key0(t);
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            ok = warp_mbar_wait(&aux->kv_empty[s], ph, abort_flag);
+            if (!ok) break;
+            ++issued;
+            prompt_expect(&aux->kv_full[s], C::TILE_BYTES);
+            for (int c = 0; c < C::CHUNKS; ++c)
+              prompt_load(&aux->kv_full[s], smem + C::KV_OFFSET + s * C::TILE_BYTES + c * kChunkBytes, kv ? &tmap_v : &tmap_k, c * 64, u.kvh, row);
+            if (++s == C::STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
+            if (t == 0 && kv == 0 && u.second) load_q(1);
           }
         }
       }
@@ -416,67 +496,97 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
           timed_out = !*abort_flag;
           *abort_flag = 1;
         }
-        mbar_wait_drain(&aux->q_full, 0);
+        for (int i = 0; i < 2; ++i)
+          if (uses[i] > 0) mbar_wait_drain(&aux->q_full[i], (uses[i] - 1) & 1);
         for (int n = max(0, issued - C::STAGES); n < issued; ++n) mbar_wait_drain(&aux->kv_full[n % C::STAGES], (n / C::STAGES) & 1);
       }
       __syncwarp();
     } else if (warp == kMmaWarp) {
       // ------------------------------------------------------------------ products
       const uint32_t base = smem_u32(smem);
-      uint32_t s = 0, ph = 0;
+      uint32_t s = 0, ph = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
       const auto logits = [&](int i, uint32_t stage) {
-  #pragma unroll
+#pragma unroll
         for (int c = 0; c < C::CHUNKS; ++c)
           mma4_ss(tmem + i * kKeys, make_smem_desc_sw128(base + i * C::TILE_BYTES + c * kChunkBytes),
                   make_smem_desc_sw128(base + C::KV_OFFSET + stage * C::TILE_BYTES + c * kChunkBytes), C::IDESC_S, c > 0);
         tc_commit_elect(&aux->s_full[i]);
       };
+      // The weights' product waits for either half of them, then takes its half of the values.
       const auto outputs = [&](int i, uint32_t stage, bool first) {
         const uint64_t v = values_desc(base + C::KV_OFFSET + stage * C::TILE_BYTES);
-        mma4_ts(tmem + 2 * kKeys + i * DP, tmem + i * kKeys, v, C::IDESC_O, !first);
-        mma4_ts(tmem + 2 * kKeys + i * DP, tmem + i * kKeys + 32, v + 512, C::IDESC_O, 1);
+        for (int half = 0; half < 2; ++half) {
+          ok = warp_mbar_wait(&aux->p_full[i][half], p_uses[i] & 1, abort_flag);
+          if (!ok) return;
+          tc_fence_after();
+          mma4_ts(tmem + 2 * kKeys + i * DP, tmem + i * kKeys + 32 * half, v + 512 * half, C::IDESC_O, !first || half);
+        }
+        ++p_uses[i];
       };
-      const auto next_stage = [&]() {
+      const auto wait_stage = [&]() -> uint32_t {
+        const uint32_t now = s;
+        ok = warp_mbar_wait(&aux->kv_full[now], ph, abort_flag);
         if (++s == C::STAGES) {
           s = 0;
           ph ^= 1u;
         }
+        return now;
       };
-      if (u.tiles > 0) {
-        ok = warp_mbar_wait(&aux->q_full, 0, abort_flag) && warp_mbar_wait(&aux->kv_full[0], 0, abort_flag);
+      // The first logits of a unit come right behind the last outputs of the one before, tile by tile.
+      const auto first_logits = [&](int i, uint32_t stage) {
+        ok = warp_mbar_wait(&aux->q_full[i], q_uses[i] & 1, abort_flag);
+        if (!ok) return;
+        ++q_uses[i];
+        tc_fence_after();
+        logits(i, stage);
+      };
+      Unit u, v;
+      Units walk(p);
+      bool have = walk.next(p, true, u);
+      if (have) {
+        const uint32_t sk = wait_stage();
+        if (ok) first_logits(0, sk);
+        if (ok && u.second) first_logits(1, sk);
         if (ok) {
-          tc_fence_after();
-          logits(0, 0);
-          if (u.second) logits(1, 0);
-          tc_commit_elect(&aux->kv_empty[0]);
-          next_stage();
-        }
-        for (int t = 0; t < u.tiles && ok; ++t) {
-          const uint32_t sv = s;
-          ok = warp_mbar_wait(&aux->kv_full[sv], ph, abort_flag);
-          if (!ok) break;
-          next_stage();
-          const bool more = t + 1 < u.tiles;
-          const uint32_t sk = s;
-          if (more) {
-            ok = warp_mbar_wait(&aux->kv_full[sk], ph, abort_flag);
-            if (!ok) break;
-            next_stage();
+          tc_commit_elect(&aux->kv_empty[sk]);
+          if (u.tiles == 1) {
+            tc_commit_elect(&aux->q_empty[0]);
+            if (u.second) tc_commit_elect(&aux->q_empty[1]);
           }
-          for (int i = 0; i < (u.second ? 2 : 1) && ok; ++i) {
-            ok = warp_mbar_wait(&aux->p_full[i], t & 1, abort_flag);
+        }
+      }
+      while (have && ok) {
+        const bool next = walk.next(p, true, v);
+        for (int t = 0; t < u.tiles && ok; ++t) {
+          const bool more = t + 1 < u.tiles;
+          const uint32_t sv = wait_stage();
+          if (!ok) break;
+          uint32_t sk = 0;
+          if (more || next) {
+            sk = wait_stage();
             if (!ok) break;
-            tc_fence_after();
-            outputs(i, sv, t == 0);
+          }
+          for (int i = 0; i < 2 && ok; ++i) {
+            if (i == 0 || u.second) {
+              outputs(i, sv, t == 0);
+              if (!ok) break;
+              if (!more) tc_commit_elect(&aux->o_full[i]);
+            }
             if (i == (u.second ? 1 : 0)) tc_commit_elect(&aux->kv_empty[sv]);
             if (more) {
-              logits(i, sk);
-            } else {
-              tc_commit_elect(&aux->o_full[i]);
+              if (i == 0 || u.second) {
+                logits(i, sk);
+                if (t + 2 == u.tiles) tc_commit_elect(&aux->q_empty[i]);
+              }
+            } else if (next && (i == 0 || v.second)) {
+              first_logits(i, sk);
+              if (ok && v.tiles == 1) tc_commit_elect(&aux->q_empty[i]);
             }
           }
-          if (ok && more) tc_commit_elect(&aux->kv_empty[sk]);
+          if (ok && (more || next)) tc_commit_elect(&aux->kv_empty[sk]);
         }
+        u = v;
+        have = next;
       }
       if (!ok && lane == 0) {
         timed_out = !*abort_flag;
@@ -491,69 +601,76 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     // ------------------------------------------------------------------ softmax: a thread a row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int i = warp >> 2, r = (warp & 3) * 32 + lane;
-    const int token = u.t0 + i * p.tq + r / p.group, head = kvh * p.group + r % p.group;
-    const bool row_ok = r < p.tq * p.group && token < seq.n;
-    const int pos = token + u.shift;
-    const int tile_lo = u.t0 + i * p.tq + u.shift, tile_hi = tile_lo + p.tq - 1;  // positions of this tile of queries
+    const int row_token = r / p.group, row_head = r % p.group;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + i * kKeys, o_addr = tmem + lanes + 2 * kKeys + i * DP;
-    float m = -INFINITY, l = 0.0f;
-    if (i == 0 || u.second) {
+    uint32_t s_uses = 0, o_uses = 0;
+    Unit u;
+    for (Units walk(p); ok && walk.next(p, false, u);) {
+      if (i == 1 && !u.second) continue;
+      const int token = u.t0 + i * p.tq + row_token, head = u.kvh * p.group + row_head;
+      const bool row_ok = row_token < p.tq && token < u.seq.n;
+      const int pos = token + u.shift;
+      const int tile_lo = u.t0 + i * p.tq + u.shift, tile_hi = tile_lo + p.tq - 1;  // positions of this tile of queries
+      float m = -INFINITY, l = 0.0f;
       for (int t = 0; t < u.tiles && ok; ++t) {
-        ok = warp_mbar_wait(&aux->s_full[i], t & 1, abort_flag);
+        ok = warp_mbar_wait(&aux->s_full[i], s_uses & 1, abort_flag);
         if (!ok) break;
+        ++s_uses;
         tc_fence_after();
         const int k0 = u.key0(t);
         const bool full = k0 + kKeys - 1 <= tile_lo && (p.a.window <= 0 || k0 > tile_hi - p.a.window || k0 + kKeys <= p.a.sinks);
         if (full) {
-          softmax_tile<T, DP, false>(s_addr, o_addr, p.cl2, 0, 0, 0, t == 0, m, l);
+          softmax_tile<T, DP, false>(s_addr, o_addr, p.cl2, 0, 0, 0, t == 0, row_ok, aux->p_full[i], m, l);
         } else {
-          softmax_tile<T, DP, true>(s_addr, o_addr, p.cl2, pos - k0, p.a.window > 0 ? pos - p.a.window - k0 : -1, p.a.sinks - k0, t == 0, m, l);
+          softmax_tile<T, DP, true>(s_addr, o_addr, p.cl2, pos - k0, p.a.window > 0 ? pos - p.a.window - k0 : -1, p.a.sinks - k0, t == 0, row_ok, aux->p_full[i], m, l);
         }
-        tc_fence_before();
-        mbar_arrive(&aux->p_full[i]);
       }
-      if (ok && u.tiles > 0) ok = warp_mbar_wait(&aux->o_full[i], 0, abort_flag);
-      if (ok) {
-        tc_fence_after();
-        const float scale = l == 0.0f ? 0.0f : 1.0f / l;
-        T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(seq.q0 + token) * p.a.q_heads + head) * p.a.head_dim;
-        bool again = false;
-#pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          if (u.tiles > 0) {
-            tmem_ld32(o_addr + 32 * c, o);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0u;
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) again |= __uint_as_float(o[j]) != __uint_as_float(o[j]);
-          if (row_ok) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (32 * c + j < p.a.head_dim) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = pack2<T>(__uint_as_float(o[j + 2 * e]) * scale, __uint_as_float(o[j + 2 * e + 1]) * scale);
-                *reinterpret_cast<uint4*>(out + 32 * c + j) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-          }
-        }
-        // A weight of zero times NaN or infinity is NaN: a value that the row does not see may have got into its sums, so rows that
-        // come out as NaN are computed again from what they do see.
-        uint32_t redo = __ballot_sync(0xffffffffu, row_ok && again);
-        __syncwarp();  // the rows are written before they are written again
-        while (redo != 0) {
-          const int r2 = (warp & 3) * 32 + __ffs(redo) - 1;
-          redo &= redo - 1;
-          attend_row<T>(p, seq, u.t0 + i * p.tq + r2 / p.group, kvh * p.group + r2 % p.group);
-        }
-      } else if (lane == 0) {
-        timed_out = !*abort_flag;
-        *abort_flag = 1;
+      if (ok && u.tiles > 0) {
+        ok = warp_mbar_wait(&aux->o_full[i], o_uses & 1, abort_flag);
+        ++o_uses;
       }
+      if (!ok) break;
+      tc_fence_after();
+      const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+      T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(u.seq.q0 + token) * p.a.q_heads + head) * p.a.head_dim;
+      bool again = false;
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        if (u.tiles > 0) {
+          tmem_ld32(o_addr + 32 * c, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) again |= __uint_as_float(o[j]) != __uint_as_float(o[j]);
+        if (row_ok) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+            if (32 * c + j < p.a.head_dim) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack2<T>(__uint_as_float(o[j + 2 * e]) * scale, __uint_as_float(o[j + 2 * e + 1]) * scale);
+              *reinterpret_cast<uint4*>(out + 32 * c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+      }
+      tc_fence_before();  // the next unit's weights are announced behind these reads of the accumulator
+      // A weight of zero times NaN or infinity is NaN: a value that the row does not see may have got into its sums, so rows that
+      // come out as NaN are computed again from what they do see.
+      uint32_t redo = __ballot_sync(0xffffffffu, row_ok && again);
+      __syncwarp();  // the rows are written before they are written again
+      while (redo != 0) {
+        const int r2 = (warp & 3) * 32 + __ffs(redo) - 1;
+        redo &= redo - 1;
+        attend_row<T>(p, u.seq, u.t0 + i * p.tq + r2 / p.group, u.kvh * p.group + r2 % p.group);
+      }
+    }
+    if (!ok && lane == 0) {
+      timed_out = !*abort_flag;
+      *abort_flag = 1;
     }
     __syncwarp();
   }
@@ -602,8 +719,8 @@ static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
   if (rc == QLIN_OK) rc = head_map(&tv, p.a.v, p.a.dtype, p.a.tokens_k, p.a.kv_heads, p.a.head_dim, p.a.v_token, p.a.v_head, kKeys, 1);
   if (rc != QLIN_OK) return rc;
   const int64_t blocks = static_cast<int64_t>(p.units) * p.a.kv_heads * p.a.batch;
-  if (blocks > 0x7fffffff) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: too many queries, heads and sequences");
-  prompt_kernel<T, DP><<<static_cast<unsigned>(blocks), kPromptThreads, C::SMEM_BYTES, stream>>>(tq, tk, tv, p);
+  const unsigned grid = static_cast<unsigned>(blocks < sm_count() ? blocks : sm_count());
+  prompt_kernel<T, DP><<<grid, kPromptThreads, C::SMEM_BYTES, stream>>>(tq, tk, tv, p);
   QLIN_CHECK_LAUNCH("qlin_prompt_attention");
   return QLIN_OK;
 }
