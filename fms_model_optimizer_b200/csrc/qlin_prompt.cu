@@ -123,9 +123,9 @@ constexpr int kKeys = 128;        // keys of a tile
 constexpr int kSoftmaxWarps = 8;  // four a tile of queries, a thread a row
 constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;
 constexpr int kPromptThreads = (kSoftmaxWarps + 4) * 32;  // whole warpgroups: registers are handed over between them
-// A block starts with 168 registers a thread (64,512 in all); the softmax warps take 208 each once the others have gone down to 80
-// (63,488): a row of 128 logits stays in registers.
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
+// A block starts with 168 registers a thread (64,512 in all); the softmax warps take 216 each once the others have gone down to 72
+// (64,512): a row of 128 logits stays in registers.
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kChunkBytes = 128 * 128;  // 128 rows of 64 elements, 128-byte swizzle
 constexpr float kSlack = 8.0f;
 
@@ -169,75 +169,110 @@ __device__ __forceinline__ void prompt_expect(uint64_t* bar, uint32_t bytes) {
       "r"(bytes)
       : "memory");
 }
-// Four K = 16 steps; A from shared memory (descriptor, two units of 16 bytes a step) and B likewise.
-__device__ __forceinline__ void mma4_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// A value that is the same in every lane, in a form that the compiler knows to be: with it in the loops' bounds the products are issued
+// from uniform registers (32 instructions a turn; from ordinary ones the issue alone takes longer than the tensor core).
+__device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
+// A bounded wait of a whole warp by one elected lane, whose loop and answer are uniform too.  (Lanes that poll one barrier are
+// served one after the other: a poll by all of them takes about 350 cycles even where the phase is long over.)
+__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred pe, p;\n\t"
+      "elect.sync _|pe, 0xffffffff;\n\t"
+      "setp.ne.u32 p, 0, 0;\n\t"
+      "@pe mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __any_sync(0xffffffffu, done != 0);
+}
+__device__ __forceinline__ bool uniform_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  uint64_t began = 0;
+#pragma unroll 1
+  for (uint32_t n = 0;; ++n) {
+    if (poll(bar, parity)) return true;
+    if (n < kSpinFast) continue;
+    const uint64_t now = global_timer_ns();
+    if (began == 0) began = now;
+    if (__any_sync(0xffffffffu, *abort_flag != 0 || now - began > kWaitBudgetNs)) return false;
+    __nanosleep(64);
+  }
+}
+// Descriptors are built from their low words: start address in units of 16 bytes and leading offset.  The high words: 1024 bytes
+// between groups of eight rows, version, 128-byte swizzle.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+// Low word of a tile of values, [128 keys][64 elements] pieces 16 KB apart, the head dimension contiguous.
+constexpr uint32_t kValuesLow = static_cast<uint32_t>(kChunkBytes >> 4) << 16;
+constexpr uint32_t kRowsLow = 1u << 16;
+// Four K = 16 steps; A from shared memory (two units of 16 bytes a step) and B likewise.  One elected lane issues.
+__device__ __forceinline__ void mma4_ss(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
       ".reg .pred pe, pa, pt;\n\t"
-      ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      ".reg .b32 l;\n\t"
+      ".reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t"
       "elect.sync _|pe, 0xffffffff;\n\t"
       "setp.ne.b32 pa, %4, 0;\n\t"
       "setp.ne.b32 pt, %3, 0;\n\t"
-      "add.s64 a1, %1, 2;\n\t"
-      "add.s64 b1, %2, 2;\n\t"
-      "add.s64 a2, %1, 4;\n\t"
-      "add.s64 b2, %2, 4;\n\t"
-      "add.s64 a3, %1, 6;\n\t"
-      "add.s64 b3, %2, 6;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pa;\n\t"
+      "mov.b64 a0, {%1, %5};\n\t"
+      "mov.b64 b0, {%2, %5};\n\t"
+      "add.u32 l, %1, 2;\n\t"
+      "mov.b64 a1, {l, %5};\n\t"
+      "add.u32 l, %2, 2;\n\t"
+      "mov.b64 b1, {l, %5};\n\t"
+      "add.u32 l, %1, 4;\n\t"
+      "mov.b64 a2, {l, %5};\n\t"
+      "add.u32 l, %2, 4;\n\t"
+      "mov.b64 b2, {l, %5};\n\t"
+      "add.u32 l, %1, 6;\n\t"
+      "mov.b64 a3, {l, %5};\n\t"
+      "add.u32 l, %2, 6;\n\t"
+      "mov.b64 b3, {l, %5};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %3, pa;\n\t"
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, pt;\n\t"
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, pt;\n\t"
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, pt;\n\t"
       "}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
-// Four K = 16 steps; A from tensor memory (8 columns a step), B an MN-major tile (128 units of 16 bytes a step).
-__device__ __forceinline__ void mma4_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Four K = 16 steps; A from tensor memory (8 columns a step), B a tile of values (128 units of 16 bytes a step).
+__device__ __forceinline__ void mma4_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
       ".reg .pred pe, pa, pt;\n\t"
-      ".reg .b32 a1, a2, a3;\n\t"
-      ".reg .b64 b1, b2, b3;\n\t"
+      ".reg .b32 l, a1, a2, a3;\n\t"
+      ".reg .b64 b0, b1, b2, b3;\n\t"
       "elect.sync _|pe, 0xffffffff;\n\t"
       "setp.ne.b32 pa, %4, 0;\n\t"
       "setp.ne.b32 pt, %3, 0;\n\t"
+      "mov.b64 b0, {%2, %5};\n\t"
       "add.u32 a1, %1, 8;\n\t"
-      "add.s64 b1, %2, 128;\n\t"
+      "add.u32 l, %2, 128;\n\t"
+      "mov.b64 b1, {l, %5};\n\t"
       "add.u32 a2, %1, 16;\n\t"
-      "add.s64 b2, %2, 256;\n\t"
+      "add.u32 l, %2, 256;\n\t"
+      "mov.b64 b2, {l, %5};\n\t"
       "add.u32 a3, %1, 24;\n\t"
-      "add.s64 b3, %2, 384;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pa;\n\t"
+      "add.u32 l, %2, 384;\n\t"
+      "mov.b64 b3, {l, %5};\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b0, %3, pa;\n\t"
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, pt;\n\t"
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, pt;\n\t"
       "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, pt;\n\t"
       "}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
-// Descriptor of a tile of values, [128 keys][64 elements] pieces 16 KB apart: the head dimension is contiguous, groups of eight
-// keys are 1024 bytes apart.
-__device__ __forceinline__ uint64_t values_desc(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(kChunkBytes >> 4) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-#define QLIN_R32(v, o)                                                                                                                                       \
-  "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7]), "r"(v[o + 8]), "r"(v[o + 9]),          \
-      "r"(v[o + 10]), "r"(v[o + 11]), "r"(v[o + 12]), "r"(v[o + 13]), "r"(v[o + 14]), "r"(v[o + 15]), "r"(v[o + 16]), "r"(v[o + 17]), "r"(v[o + 18]),        \
-      "r"(v[o + 19]), "r"(v[o + 20]), "r"(v[o + 21]), "r"(v[o + 22]), "r"(v[o + 23]), "r"(v[o + 24]), "r"(v[o + 25]), "r"(v[o + 26]), "r"(v[o + 27]),        \
-      "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]), "r"(v[o + 31])
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::QLIN_R32(r, 0),
-      "r"(taddr)
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]), "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -260,11 +295,12 @@ struct Unit {
 // The units of a block, every gridDim.x-th one of the list that begins with the last queries of every sequence and head, which see
 // the most keys.  `busy`: units without keys are passed over.
 struct Units {
-  int64_t id, step, total;
+  uint32_t id, step, total;
   __device__ __forceinline__ explicit Units(const PromptParams& p)
-      : id(blockIdx.x), step(gridDim.x), total(static_cast<int64_t>(p.units) * p.a.kv_heads * p.a.batch) {}
+      : id(blockIdx.x), step(gridDim.x), total(static_cast<uint32_t>(p.units) * p.a.kv_heads * p.a.batch) {}
   __device__ __forceinline__ bool next(const PromptParams& p, bool busy, Unit& u) {
-    const int lanes = p.a.kv_heads * p.a.batch;
+    const uint32_t lanes = p.a.kv_heads * p.a.batch;
+#pragma unroll 1
     for (; id < total; id += step) {
       const int rest = static_cast<int>(id % lanes);
       u.b = rest / p.a.kv_heads;
@@ -330,81 +366,116 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// The largest of a row's 128 logits, NaN if one is NaN.
+__device__ __forceinline__ float largest(const uint32_t (&x)[4][32]) {
+  float top[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) top[c] = max3_nan(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
+#pragma unroll
+  for (int j = 3; j < 31; j += 2)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) top[c] = max3_nan(top[c], __uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1]));
+  top[0] = max3_nan(top[0], top[1], __uint_as_float(x[0][31]));
+  top[2] = max3_nan(top[2], top[3], __uint_as_float(x[1][31]));
+  top[0] = max3_nan(top[0], __uint_as_float(x[2][31]), __uint_as_float(x[3][31]));
+  return max3_nan(top[0], top[2], top[2]);
+}
+// Weights 2^(x cl2 + ref) of 32 columns, as pairs of 16 bits in w, and their sum.
+template <typename T>
+__device__ __forceinline__ void weights_of(const uint32_t (&x)[32], uint32_t (&w)[16], uint64_t cl2, uint64_t ref, uint64_t& sum) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float a, b;
+    unpair64(fma2(pair64(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), cl2, ref), a, b);
+    a = exp2_fast(a);
+    b = exp2_fast(b);
+    sum = add2(sum, pair64(a, b));
+    w[i] = pack2<T>(a, b);
+  }
+}
+// Columns under n of the 32 that begin at `from`.
+__device__ __forceinline__ uint32_t columns_under(int n, int from) { return n <= from ? 0u : (n >= from + 32 ? 0xffffffffu : (1u << (n - from)) - 1u); }
+
 // One tile of logits to weights: the row's 128 logits come from tensor memory and the weights go there over them, half by half;
-// each half is handed to the product when it is there.
+// each half is handed to the product when it is there.  The first quarter is made relative to the reference of the tiles before
+// while the maximum is still being looked for, and made again where that has outgrown the reference.
 template <typename T, int DP, bool MASKED>
 __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, float cl2, int hi, int lo, int sinks, bool first, bool live, uint64_t* p_full, float& m, float& l) {
   using C = PromptCfg<T, DP>;
-  uint32_t x[4][32];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_issue32(s_addr + 32 * c, x[c]);
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_wait32(x[c]);
-  if constexpr (MASKED) {
-    // column j is seen when j <= hi and (j > lo or j < sinks)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const auto below = [&](int n) { return n <= 32 * c ? 0u : (n >= 32 * c + 32 ? 0xffffffffu : (1u << (n - 32 * c)) - 1u); };  // columns under n
-      const uint32_t seen = below(hi + 1) & (~below(lo + 1) | below(sinks));
+  uint32_t x[4][32], w[16];
+  // column j is seen when j <= hi and (j > lo or j < sinks)
+  const auto mask = [&](int c) {
+    if constexpr (MASKED) {
+      const uint32_t seen = columns_under(hi + 1, 32 * c) & (~columns_under(lo + 1, 32 * c) | columns_under(sinks, 32 * c));
 #pragma unroll
       for (int j = 0; j < 32; ++j)
         if (!((seen >> j) & 1u)) x[c][j] = 0xff800000u;
     }
-  }
-  float top[4];
+  };
+  const uint64_t cl22 = pair64(cl2, cl2);
+  const auto reference = [&]() {
+    const float ref = C::SHIFT - (m == -INFINITY ? 0.0f : m);
+    return pair64(ref, ref);
+  };
+  uint64_t sum = 0;
+  tmem_issue32(s_addr, x[0]);
+  tmem_wait32(x[0]);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    top[c] = max3_nan(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
+  for (int c = 1; c < 4; ++c) tmem_issue32(s_addr + 32 * c, x[c]);
+  mask(0);
+  float most;
+  if (first) {
 #pragma unroll
-    for (int j = 3; j < 31; j += 2) top[c] = max3_nan(top[c], __uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1]));
+    for (int c = 1; c < 4; ++c) tmem_wait32(x[c]);
+#pragma unroll
+    for (int c = 1; c < 4; ++c) mask(c);
+    most = largest(x) * cl2;
+  } else {
+    const uint64_t ref = reference();
+    weights_of<T>(x[0], w, cl22, ref, sum);
+#pragma unroll
+    for (int c = 1; c < 4; ++c) tmem_wait32(x[c]);
+#pragma unroll
+    for (int c = 1; c < 4; ++c) mask(c);
+    most = largest(x) * cl2;
   }
-  top[0] = max3_nan(top[0], top[1], __uint_as_float(x[0][31]));
-  top[2] = max3_nan(top[2], top[3], __uint_as_float(x[1][31]));
-  top[0] = max3_nan(top[0], __uint_as_float(x[2][31]), __uint_as_float(x[3][31]));
-  const float most = max3_nan(top[0], top[2], top[2]) * cl2;
   // The reference that the weights are relative to follows the maximum only when that has outgrown it by 2^kSlack: the sums are the
   // same up to rounding, and the accumulator is seldom rewritten.  A NaN or an infinity among the logits makes it NaN, and with it the row.
   // Rows that are no query's hold anything and are left alone.
   const bool grow = live && (!(most <= m + kSlack) || (m == -INFINITY && most > -INFINITY));
-  if (__any_sync(0xffffffffu, grow)) {
+  if (first || __any_sync(0xffffffffu, grow)) {
     const float next = !grow ? m : (most == INFINITY ? __int_as_float(0x7fc00000) : most);
     if (!first) {
       const float keep = grow ? exp2f(m - next) : 1.0f;
       l *= keep;
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(o_addr + 32 * c, o);
+      for (int c = 0; c < DP / 16; ++c) {
+        uint32_t o[16];
+        tmem_issue16(o_addr + 16 * c, o);
+        tmem_wait16(o);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-        tmem_st32(o_addr + 32 * c, o);
+        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+        tmem_st16(o_addr + 16 * c, o);
       }
     }
     m = next;
+    sum = 0;
+    weights_of<T>(x[0], w, cl22, reference(), sum);
   }
-  const float ref = C::SHIFT - (m == -INFINITY ? 0.0f : m);
-  const uint64_t ref2 = pair64(ref, ref), cl22 = pair64(cl2, cl2);
-  uint64_t sum[2] = {0, 0};
+  const uint64_t ref = reference();
+  tmem_st16(s_addr, w);
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint32_t w[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int c = 2 * half + i / 16, j = 2 * i % 32;
-      float a, b;
-      unpair64(fma2(pair64(__uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1])), cl22, ref2), a, b);
-      a = exp2_fast(a);
-      b = exp2_fast(b);
-      sum[i & 1] = add2(sum[i & 1], pair64(a, b));
-      w[i] = pack2<T>(a, b);
+  for (int c = 1; c < 4; ++c) {
+    weights_of<T>(x[c], w, cl22, ref, sum);
+    tmem_st16(s_addr + 16 * c, w);
+    if (c & 1) {
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(p_full + c / 2);
     }
-    tmem_st32(s_addr + 32 * half, w);
-    tmem_wait_st();
-    tc_fence_before();
-    mbar_arrive(p_full + half);
   }
   float a, b;
-  unpair64(add2(sum[0], sum[1]), a, b);
+  unpair64(sum, a, b);
   l += a + b;
 }
 
@@ -466,7 +537,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       Unit u;
       for (Units walk(p); ok && walk.next(p, true, u);) {
         const auto load_q = [&](int i) {
-          ok = warp_mbar_wait(&aux->q_empty[i], (uses[i] & 1) ^ 1, abort_flag);
+          ok = uniform_wait(&aux->q_empty[i], (uses[i] & 1) ^ 1, abort_flag);
           if (!ok) return;
           ++uses[i];
           prompt_expect(&aux->q_full[i], static_cast<uint32_t>(C::CHUNKS * p.tq * p.group * 128));
@@ -477,7 +548,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         for (int t = 0; t < u.tiles && ok; ++t) {
           const int row = u.seq.k0 + u.key0(t);
           for (int kv = 0; kv < 2 && ok; ++kv) {
-            ok = warp_mbar_wait(&aux->kv_empty[s], ph, abort_flag);
+            ok = uniform_wait(&aux->kv_empty[s], ph, abort_flag);
             if (!ok) break;
             ++issued;
             prompt_expect(&aux->kv_full[s], C::TILE_BYTES);
@@ -503,62 +574,66 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       __syncwarp();
     } else if (warp == kMmaWarp) {
       // ------------------------------------------------------------------ products
-      const uint32_t base = smem_u32(smem);
-      uint32_t s = 0, ph = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
-      const auto logits = [&](int i, uint32_t stage) {
-#pragma unroll
-        for (int c = 0; c < C::CHUNKS; ++c)
-          mma4_ss(tmem + i * kKeys, make_smem_desc_sw128(base + i * C::TILE_BYTES + c * kChunkBytes),
-                  make_smem_desc_sw128(base + C::KV_OFFSET + stage * C::TILE_BYTES + c * kChunkBytes), C::IDESC_S, c > 0);
-        tc_commit_elect(&aux->s_full[i]);
-      };
-      // The weights' product waits for either half of them, then takes its half of the values.
-      const auto outputs = [&](int i, uint32_t stage, bool first) {
-        const uint64_t v = values_desc(base + C::KV_OFFSET + stage * C::TILE_BYTES);
-        for (int half = 0; half < 2; ++half) {
-          ok = warp_mbar_wait(&aux->p_full[i][half], p_uses[i] & 1, abort_flag);
-          if (!ok) return;
-          tc_fence_after();
-          mma4_ts(tmem + 2 * kKeys + i * DP, tmem + i * kKeys + 32 * half, v + 512 * half, C::IDESC_O, !first || half);
-        }
-        ++p_uses[i];
-      };
+      // The tiles of queries take turns, so that one is in the softmax while the other is in the tensor core.
+      const uint32_t base = smem_u32(smem) >> 4, d0 = uniform(tmem);
+      uint32_t s = 0, ph = 0, q_ph = 0, p_ph = 0;  // bit i of the last two: tile i
       const auto wait_stage = [&]() -> uint32_t {
         const uint32_t now = s;
-        ok = warp_mbar_wait(&aux->kv_full[now], ph, abort_flag);
+        ok = uniform_wait(&aux->kv_full[now], ph, abort_flag);
         if (++s == C::STAGES) {
           s = 0;
           ph ^= 1u;
         }
         return now;
       };
-      // The first logits of a unit come right behind the last outputs of the one before, tile by tile.
-      const auto first_logits = [&](int i, uint32_t stage) {
-        ok = warp_mbar_wait(&aux->q_full[i], q_uses[i] & 1, abort_flag);
+      const auto logits = [&](int i, uint32_t stage) {
+#pragma unroll
+        for (int c = 0; c < C::CHUNKS; ++c)
+          mma4_ss(d0 + i * kKeys, (base + ((i * C::TILE_BYTES + c * kChunkBytes) >> 4)) | kRowsLow,
+                  (base + ((C::KV_OFFSET + c * kChunkBytes) >> 4) + stage * (C::TILE_BYTES >> 4)) | kRowsLow, C::IDESC_S, c > 0);
+        tc_commit_elect(&aux->s_full[i]);
+      };
+      const auto first_logits = [&](int i, uint32_t stage, bool only) {
+        ok = uniform_wait(&aux->q_full[i], (q_ph >> i) & 1, abort_flag);
         if (!ok) return;
-        ++q_uses[i];
+        q_ph ^= 1u << i;
         tc_fence_after();
         logits(i, stage);
+        if (only) tc_commit_elect(&aux->q_empty[i]);
       };
-      Unit u, v;
+      // The weights' product waits for either half of them, then takes its half of the values.
+      const auto outputs = [&](int i, uint32_t stage, bool first) {
+        const uint32_t values = (base + (C::KV_OFFSET >> 4) + stage * (C::TILE_BYTES >> 4)) | kValuesLow;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          ok = uniform_wait(&aux->p_full[i][half], (p_ph >> i) & 1, abort_flag);
+          if (!ok) return;
+          tc_fence_after();
+          mma4_ts(d0 + 2 * kKeys + i * DP, d0 + i * kKeys + 32 * half, values + 512 * half, C::IDESC_O, !first || half);
+        }
+        p_ph ^= 1u << i;
+      };
+      Unit unit;
       Units walk(p);
-      bool have = walk.next(p, true, u);
+      const auto advance = [&](int& tiles, bool& second) {
+        const bool have = uniform(walk.next(p, true, unit)) != 0;
+        tiles = uniform(have ? unit.tiles : 0);
+        second = uniform(have && unit.second) != 0;
+        return have;
+      };
+      int tiles, next_tiles;
+      bool second, next_second;
+      bool have = advance(tiles, second);
       if (have) {
         const uint32_t sk = wait_stage();
-        if (ok) first_logits(0, sk);
-        if (ok && u.second) first_logits(1, sk);
-        if (ok) {
-          tc_commit_elect(&aux->kv_empty[sk]);
-          if (u.tiles == 1) {
-            tc_commit_elect(&aux->q_empty[0]);
-            if (u.second) tc_commit_elect(&aux->q_empty[1]);
-          }
-        }
+        if (ok) first_logits(0, sk, tiles == 1);
+        if (ok && second) first_logits(1, sk, tiles == 1);
+        if (ok) tc_commit_elect(&aux->kv_empty[sk]);
       }
       while (have && ok) {
-        const bool next = walk.next(p, true, v);
-        for (int t = 0; t < u.tiles && ok; ++t) {
-          const bool more = t + 1 < u.tiles;
+        const bool next = advance(next_tiles, next_second);
+        for (int t = 0; t < tiles && ok; ++t) {
+          const bool more = t + 1 < tiles;
           const uint32_t sv = wait_stage();
           if (!ok) break;
           uint32_t sk = 0;
@@ -566,26 +641,25 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             sk = wait_stage();
             if (!ok) break;
           }
-          for (int i = 0; i < 2 && ok; ++i) {
-            if (i == 0 || u.second) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const bool mine = i == 0 || second;
+            if (mine && ok) {
               outputs(i, sv, t == 0);
-              if (!ok) break;
-              if (!more) tc_commit_elect(&aux->o_full[i]);
+              if (ok && !more) tc_commit_elect(&aux->o_full[i]);
             }
-            if (i == (u.second ? 1 : 0)) tc_commit_elect(&aux->kv_empty[sv]);
-            if (more) {
-              if (i == 0 || u.second) {
-                logits(i, sk);
-                if (t + 2 == u.tiles) tc_commit_elect(&aux->q_empty[i]);
-              }
-            } else if (next && (i == 0 || v.second)) {
-              first_logits(i, sk);
-              if (ok && v.tiles == 1) tc_commit_elect(&aux->q_empty[i]);
+            if (ok && i == (second ? 1 : 0)) tc_commit_elect(&aux->kv_empty[sv]);
+            if (ok && more && mine) {
+              logits(i, sk);
+              if (t + 2 == tiles) tc_commit_elect(&aux->q_empty[i]);
+            } else if (ok && !more && next && (i == 0 || next_second)) {
+              first_logits(i, sk, next_tiles == 1);  // right behind the last outputs of the unit before
             }
           }
           if (ok && (more || next)) tc_commit_elect(&aux->kv_empty[sk]);
         }
-        u = v;
+        tiles = next_tiles;
+        second = next_second;
         have = next;
       }
       if (!ok && lane == 0) {
@@ -614,7 +688,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       const int tile_lo = u.t0 + i * p.tq + u.shift, tile_hi = tile_lo + p.tq - 1;  // positions of this tile of queries
       float m = -INFINITY, l = 0.0f;
       for (int t = 0; t < u.tiles && ok; ++t) {
-        ok = warp_mbar_wait(&aux->s_full[i], s_uses & 1, abort_flag);
+        ok = uniform_wait(&aux->s_full[i], s_uses & 1, abort_flag);
         if (!ok) break;
         ++s_uses;
         tc_fence_after();
@@ -627,7 +701,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         }
       }
       if (ok && u.tiles > 0) {
-        ok = warp_mbar_wait(&aux->o_full[i], o_uses & 1, abort_flag);
+        ok = uniform_wait(&aux->o_full[i], o_uses & 1, abort_flag);
         ++o_uses;
       }
       if (!ok) break;
@@ -719,6 +793,7 @@ static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
   if (rc == QLIN_OK) rc = head_map(&tv, p.a.v, p.a.dtype, p.a.tokens_k, p.a.kv_heads, p.a.head_dim, p.a.v_token, p.a.v_head, kKeys, 1);
   if (rc != QLIN_OK) return rc;
   const int64_t blocks = static_cast<int64_t>(p.units) * p.a.kv_heads * p.a.batch;
+  if (blocks > 0x7fffffff) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: too many queries, heads and sequences");
   const unsigned grid = static_cast<unsigned>(blocks < sm_count() ? blocks : sm_count());
   prompt_kernel<T, DP><<<grid, kPromptThreads, C::SMEM_BYTES, stream>>>(tq, tk, tv, p);
   QLIN_CHECK_LAUNCH("qlin_prompt_attention");
