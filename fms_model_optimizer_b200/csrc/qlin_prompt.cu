@@ -139,7 +139,7 @@ template <typename T, int DP>
 struct PromptCfg {
   static constexpr int CHUNKS = DP / 64;
   static constexpr int TILE_BYTES = CHUNKS * kChunkBytes;  // a tile of queries, keys or values
-  static constexpr int STAGES = DP == 128 ? 4 : 8;         // tiles of keys or values in flight
+  static constexpr int STAGES = DP == 128 ? 5 : 8;         // tiles of keys or values in flight
   static constexpr int KV_OFFSET = 2 * TILE_BYTES;
   static constexpr int AUX_OFFSET = KV_OFFSET + STAGES * TILE_BYTES;
   static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(PromptAux));
@@ -172,28 +172,14 @@ __device__ __forceinline__ void prompt_expect(uint64_t* bar, uint32_t bytes) {
 // A value that is the same in every lane, in a form that the compiler knows to be: with it in the loops' bounds the products are issued
 // from uniform registers (32 instructions a turn; from ordinary ones the issue alone takes longer than the tensor core).
 __device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
-// A bounded wait of a whole warp by one elected lane, whose loop and answer are uniform too.  (Lanes that poll one barrier are
-// served one after the other: a poll by all of them takes about 350 cycles even where the phase is long over.)
-__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred pe, p;\n\t"
-      "elect.sync _|pe, 0xffffffff;\n\t"
-      "setp.ne.u32 p, 0, 0;\n\t"
-      "@pe mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return __any_sync(0xffffffffu, done != 0);
-}
-__device__ __forceinline__ bool uniform_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+// A bounded wait of a whole warp for one barrier, or two, whose loop and answer are uniform too.
+__device__ __forceinline__ bool uniform_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t* other = nullptr, uint32_t other_parity = 0) {
   uint64_t began = 0;
 #pragma unroll 1
   for (uint32_t n = 0;; ++n) {
-    if (poll(bar, parity)) return true;
+    bool done = mbar_try_wait(bar, parity);
+    if (other != nullptr) done &= mbar_try_wait(other, other_parity);
+    if (__all_sync(0xffffffffu, done)) return true;
     if (n < kSpinFast) continue;
     const uint64_t now = global_timer_ns();
     if (began == 0) began = now;
@@ -279,7 +265,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
@@ -357,40 +343,69 @@ __device__ __forceinline__ uint64_t pair64(float a, float b) {
 __device__ __forceinline__ void unpair64(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_in_order(float a, float b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) {
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  } else {
+    asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  }
   return r;
 }
 
-// The largest of a row's 128 logits, NaN if one is NaN.
-__device__ __forceinline__ float largest(const uint32_t (&x)[4][32]) {
+// The largest of a row's 128 logits, in pieces that fit between other work.  NaN if one is NaN.
+struct Largest {
   float top[4];
+  __device__ __forceinline__ explicit Largest(const uint32_t (&x)[4][32]) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) top[c] = max3_nan(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
+    for (int c = 0; c < 4; ++c) top[c] = max3_nan(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][31]));
+  }
+  __device__ __forceinline__ explicit Largest(const float (&t)[4]) : top{t[0], t[1], t[2], t[3]} {}
+  // one of 15 steps
+  __device__ __forceinline__ void step(const uint32_t (&x)[4][32], int n) {
+    if (n < 0 || n > 14) return;
+    const int j = n == 14 ? 30 : 2 + 2 * n;
 #pragma unroll
-  for (int j = 3; j < 31; j += 2)
+    for (int c = 0; c < 4; ++c) top[c] = max3_nan(top[c], __uint_as_float(x[c][j]), __uint_as_float(x[c][n == 14 ? 30 : j + 1]));
+  }
+  __device__ __forceinline__ float result() const { return max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]); }
+};
+
+// Weights 2^(x cl2 + ref) of the pairs of columns FIRST to LAST.  The exponentials keep their unit (8 cycles a warp's instruction)
+// busy only if the work around them is done between them, so the multiplications run two pairs ahead of them, the sums and the
+// roundings two pairs behind; `beside(i)` is more work to be done in between, `done(k, words)` takes 16 words of two weights each.
+template <typename T, int FIRST, int LAST, typename Beside, typename Done>
+__device__ __forceinline__ void weigh(const uint32_t (&x)[4][32], uint64_t cl2, uint64_t ref, uint64_t (&sum)[2], Beside beside, Done done) {
+  uint64_t y[LAST - FIRST];
+  float a[LAST - FIRST], b[LAST - FIRST];
+  uint32_t w[16];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) top[c] = max3_nan(top[c], __uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1]));
-  top[0] = max3_nan(top[0], top[1], __uint_as_float(x[0][31]));
-  top[2] = max3_nan(top[2], top[3], __uint_as_float(x[1][31]));
-  top[0] = max3_nan(top[0], __uint_as_float(x[2][31]), __uint_as_float(x[3][31]));
-  return max3_nan(top[0], top[2], top[2]);
-}
-// Weights 2^(x cl2 + ref) of 32 columns, as pairs of 16 bits in w, and their sum.
-template <typename T>
-__device__ __forceinline__ void weights_of(const uint32_t (&x)[32], uint32_t (&w)[16], uint64_t cl2, uint64_t ref, uint64_t& sum) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float a, b;
-    unpair64(fma2(pair64(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), cl2, ref), a, b);
-    a = exp2_fast(a);
-    b = exp2_fast(b);
-    sum = add2(sum, pair64(a, b));
-    w[i] = pack2<T>(a, b);
+  for (int i = 0; i < LAST - FIRST + 4; ++i) {
+    if (i < LAST - FIRST) {
+      const int c = (FIRST + i) / 16, j = 2 * (FIRST + i) % 32;
+      y[i] = fma2(pair64(__uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1])), cl2, ref);
+    }
+    if (i >= 2 && i - 2 < LAST - FIRST) {
+      unpair64(y[i - 2], a[i - 2], b[i - 2]);
+      a[i - 2] = exp2_fast(a[i - 2]);
+      b[i - 2] = exp2_fast(b[i - 2]);
+    }
+    beside(i);
+    if (i >= 4) {
+      const int k = i - 4;
+      sum[k & 1] = add2(sum[k & 1], pair64(a[k], b[k]));
+      w[k % 16] = pack2_in_order<T>(a[k], b[k]);
+      if (k % 16 == 15) done((FIRST + k) / 16, w);
+    }
   }
 }
 // Columns under n of the 32 that begin at `from`.
@@ -417,7 +432,18 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, f
     const float ref = C::SHIFT - (m == -INFINITY ? 0.0f : m);
     return pair64(ref, ref);
   };
-  uint64_t sum = 0;
+  const auto rest = [&]() {
+#pragma unroll
+    for (int c = 1; c < 4; ++c) tmem_wait32(x[c]);
+#pragma unroll
+    for (int c = 1; c < 4; ++c) mask(c);
+  };
+  const auto nothing = [](int) {};
+  const auto keep_words = [&](int, const uint32_t(&words)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = words[j];
+  };
+  uint64_t sum[2] = {0, 0};
   tmem_issue32(s_addr, x[0]);
   tmem_wait32(x[0]);
 #pragma unroll
@@ -425,19 +451,31 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, f
   mask(0);
   float most;
   if (first) {
+    rest();
+    Largest top(x);
 #pragma unroll
-    for (int c = 1; c < 4; ++c) tmem_wait32(x[c]);
-#pragma unroll
-    for (int c = 1; c < 4; ++c) mask(c);
-    most = largest(x) * cl2;
+    for (int n = 0; n < 15; ++n) top.step(x, n);
+    most = top.result() * cl2;
   } else {
-    const uint64_t ref = reference();
-    weights_of<T>(x[0], w, cl22, ref, sum);
+    if constexpr (MASKED) rest();
+    float top[4];
+    weigh<T, 0, 16>(x, cl22, reference(), sum,
+                    [&](int i) {
+                      if (i == 4) {
+                        if constexpr (!MASKED) rest();
+                        const Largest l0(x);
 #pragma unroll
-    for (int c = 1; c < 4; ++c) tmem_wait32(x[c]);
+                        for (int c = 0; c < 4; ++c) top[c] = l0.top[c];
+                      }
+                      if (i > 4) {
+                        Largest li(top);
+                        li.step(x, i - 5);
 #pragma unroll
-    for (int c = 1; c < 4; ++c) mask(c);
-    most = largest(x) * cl2;
+                        for (int c = 0; c < 4; ++c) top[c] = li.top[c];
+                      }
+                    },
+                    keep_words);
+    most = Largest(top).result() * cl2;
   }
   // The reference that the weights are relative to follows the maximum only when that has outgrown it by 2^kSlack: the sums are the
   // same up to rounding, and the accumulator is seldom rewritten.  A NaN or an infinity among the logits makes it NaN, and with it the row.
@@ -459,23 +497,20 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, f
       }
     }
     m = next;
-    sum = 0;
-    weights_of<T>(x[0], w, cl22, reference(), sum);
+    sum[0] = sum[1] = 0;
+    weigh<T, 0, 16>(x, cl22, reference(), sum, nothing, keep_words);
   }
-  const uint64_t ref = reference();
   tmem_st16(s_addr, w);
-#pragma unroll
-  for (int c = 1; c < 4; ++c) {
-    weights_of<T>(x[c], w, cl22, ref, sum);
-    tmem_st16(s_addr + 16 * c, w);
+  weigh<T, 16, 64>(x, cl22, reference(), sum, nothing, [&](int c, const uint32_t(&words)[16]) {
+    tmem_st16(s_addr + 16 * c, words);
     if (c & 1) {
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(p_full + c / 2);
     }
-  }
+  });
   float a, b;
-  unpair64(sum, a, b);
+  unpair64(add2(sum[0], sum[1]), a, b);
   l += a + b;
 }
 
@@ -577,14 +612,11 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       // The tiles of queries take turns, so that one is in the softmax while the other is in the tensor core.
       const uint32_t base = smem_u32(smem) >> 4, d0 = uniform(tmem);
       uint32_t s = 0, ph = 0, q_ph = 0, p_ph = 0;  // bit i of the last two: tile i
-      const auto wait_stage = [&]() -> uint32_t {
-        const uint32_t now = s;
-        ok = uniform_wait(&aux->kv_full[now], ph, abort_flag);
+      const auto step = [&]() {
         if (++s == C::STAGES) {
           s = 0;
           ph ^= 1u;
         }
-        return now;
       };
       const auto logits = [&](int i, uint32_t stage) {
 #pragma unroll
@@ -625,7 +657,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       bool second, next_second;
       bool have = advance(tiles, second);
       if (have) {
-        const uint32_t sk = wait_stage();
+        const uint32_t sk = s;
+        ok = uniform_wait(&aux->kv_full[sk], ph, abort_flag);
+        step();
         if (ok) first_logits(0, sk, tiles == 1);
         if (ok && second) first_logits(1, sk, tiles == 1);
         if (ok) tc_commit_elect(&aux->kv_empty[sk]);
@@ -634,13 +668,13 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         const bool next = advance(next_tiles, next_second);
         for (int t = 0; t < tiles && ok; ++t) {
           const bool more = t + 1 < tiles;
-          const uint32_t sv = wait_stage();
+          // the values of this tile and the keys of the next one, in one wait
+          const uint32_t sv = s, v_ph = ph;
+          step();
+          const uint32_t sk = s, k_ph = ph;
+          if (more || next) step();
+          ok = uniform_wait(&aux->kv_full[sv], v_ph, abort_flag, more || next ? &aux->kv_full[sk] : nullptr, k_ph);
           if (!ok) break;
-          uint32_t sk = 0;
-          if (more || next) {
-            sk = wait_stage();
-            if (!ok) break;
-          }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const bool mine = i == 0 || second;
