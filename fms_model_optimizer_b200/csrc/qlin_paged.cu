@@ -34,10 +34,12 @@ constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kTileKeys = 16;
 constexpr int kRingBytes = 24576;  // stages of a warp: two blocks an SM keep about 190 KB between them
 constexpr int kMinTiles = 8;       // tiles of a block at least, two a warp
+constexpr int kWaves = 1;
 
 struct PagedParams {
   qlin_paged_attention_args a;
   int32_t splits, head_blocks, group;  // blocks of query heads per kv head, query heads per kv head
+  int32_t cluster;                     // the splits of a head are a cluster of blocks and join in shared memory
   float* part_o;                       // [batch * q_heads, splits, head_dim]
   float2* part_ml;                     // [batch * q_heads, splits]: maximum and sum
 };
@@ -114,6 +116,22 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
+// A value at this offset in the shared memory of another block of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t offset, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(offset), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t offset, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_block(offset, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t offset, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(in_block(offset, rank)) : "memory");
+  return v;
+}
 __device__ __forceinline__ float max_of_rows(float v) {  // over the eight lanes that hold one column
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
@@ -133,7 +151,7 @@ struct PagedCfg {
   static constexpr int OROW = DP + 4;                  // floats of a row of the joined outputs
   static constexpr int SMEM = kPagedWarps * STAGES * STAGE;
   static constexpr float SHIFT = BF16 ? 0.0f : 12.0f;
-  static_assert(kPagedWarps * HEADS * (OROW + 2) * 4 <= SMEM, "the join reuses the stages");
+  static_assert((kPagedWarps + 1) * HEADS * (OROW + 2) * 4 <= SMEM, "the join reuses the stages");
 };
 
 template <int RB>
@@ -157,7 +175,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
   const Visible vis = visible_keys(len, p.a.window, p.a.sinks);
   const int tiles = (vis.n + kTileKeys - 1) / kTileKeys;
   const int per = tiles_per_split(tiles, p.splits), used = splits_used(tiles, per);
-  if (split >= used) return;
+  if (split >= used && !p.cluster) return;
   const int first = split * per + warp, last = min(tiles, (split + 1) * per);
 
   // ---------------------------------------------------------------- loads
@@ -379,6 +397,14 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
     }
   __syncthreads();
   const float v_scale = F8 ? p.a.v_scale[kvh] : 1.0f;
+  float* block_o = reinterpret_cast<float*>(warp_ml + kPagedWarps * C::HEADS);  // [heads][OROW]
+  float2* block_ml = reinterpret_cast<float2*>(block_o + C::HEADS * C::OROW);   // [heads]
+  const auto store_out = [&](int h, int d, const float (&acc)[4], float sum) {
+    constexpr bool bf16 = std::is_same<QT, __nv_bfloat16>::value;
+    const float r = sum == 0.0f ? 0.0f : v_scale / sum;
+    QT* out = static_cast<QT*>(p.a.out) + (static_cast<int64_t>(b) * p.a.q_heads + kvh * p.group + head0 + h) * D + d;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack16<bf16>(acc[0] * r, acc[1] * r), pack16<bf16>(acc[2] * r, acc[3] * r));
+  };
   for (int i = threadIdx.x; i < heads * (DP / 4); i += kPagedThreads) {
     const int h = i / (DP / 4), d = i % (DP / 4) * 4;
     float top = -INFINITY;
@@ -398,14 +424,47 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
     }
     if (d >= D) continue;
     const int64_t row = static_cast<int64_t>(b) * p.a.q_heads + kvh * p.group + head0 + h;
-    if (used == 1) {
-      const float r = sum == 0.0f ? 0.0f : v_scale / sum;
-      *reinterpret_cast<uint2*>(static_cast<QT*>(p.a.out) + row * D + d) =
-          make_uint2(pack16<std::is_same<QT, __nv_bfloat16>::value>(acc[0] * r, acc[1] * r), pack16<std::is_same<QT, __nv_bfloat16>::value>(acc[2] * r, acc[3] * r));
+    if (p.cluster) {
+      *reinterpret_cast<float4*>(block_o + h * C::OROW + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (d == 0) block_ml[h] = make_float2(top, sum);
+    } else if (used == 1) {
+      store_out(h, d, acc, sum);
     } else {
       *reinterpret_cast<float4*>(p.part_o + (row * p.splits + split) * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (d == 0) p.part_ml[row * p.splits + split] = make_float2(top, sum);
     }
+  }
+  if (p.cluster) {
+    // the blocks of the cluster share out the outputs and read each other's sums, in the order of the splits
+    cluster_arrive_wait();
+    const uint32_t o_base = smem_u32(block_o), ml_base = smem_u32(block_ml);
+    for (int i = static_cast<int>(cluster_cta_rank()) * kPagedThreads + threadIdx.x; i < heads * (DP / 4); i += p.splits * kPagedThreads) {
+      const int h = i / (DP / 4), d = i % (DP / 4) * 4;
+      if (d >= D) continue;
+      float2 ml[8];
+      float4 v[8];
+      float top = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < used) {
+          ml[r] = ld_cluster_f2(ml_base + h * 8, r);
+          v[r] = ld_cluster_f4(o_base + (h * C::OROW + d) * 4, r);
+          top = fmaxf(top, ml[r].x);
+        }
+      float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < used) {
+          const float f = ml[r].x == top ? 1.0f : exp2f(ml[r].x - top);
+          sum += ml[r].y * f;
+          acc[0] += v[r].x * f;
+          acc[1] += v[r].y * f;
+          acc[2] += v[r].z * f;
+          acc[3] += v[r].w * f;
+        }
+      store_out(h, d, acc, sum);
+    }
+    cluster_arrive_wait();  // nobody leaves while its sums are read
   }
 }
 
@@ -442,15 +501,25 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   }
 }
 
-// Splits of the keys: as many blocks as run at once, none with fewer than kMinTiles tiles.
-static int choose_splits(const qlin_paged_attention_args& a, int head_blocks) {
+// Splits of the keys: as many blocks as run at once, none with fewer than kMinTiles tiles where the page table is as wide as its longest
+// sequence.  Up to kClusterSplits of them (a power of two) are a cluster of blocks, which joins without a second launch and without
+// a workspace; only few heads with long tables take more.
+constexpr int kClusterSplits = 8;
+struct Splits {
+  int32_t n, cluster;
+};
+static Splits choose_splits(const qlin_paged_attention_args& a, int head_blocks) {
   int64_t most = static_cast<int64_t>(a.max_pages) * a.page_size;
   if (a.window > 0 && most > static_cast<int64_t>(a.window) + a.sinks) most = static_cast<int64_t>(a.window) + (a.sinks > 0 ? a.sinks : 0);
   const int64_t tiles = (most + kTileKeys - 1) / kTileKeys, rows = static_cast<int64_t>(a.batch) * a.kv_heads * head_blocks;
-  int64_t want = 2 * sm_count() / rows;
-  const int64_t cap = (tiles + kMinTiles - 1) / kMinTiles;
-  if (want > cap) want = cap;
-  return want < 1 ? 1 : static_cast<int>(want);
+  const int64_t want = (kWaves * 2 * sm_count() + rows - 1) / rows, cap = (tiles + kMinTiles - 1) / kMinTiles;
+  if (want > 2 * kClusterSplits && cap > 4 * kClusterSplits) {
+    const int64_t n = 2 * sm_count() / rows;
+    return Splits{static_cast<int32_t>(n < cap ? n : cap), 0};
+  }
+  int32_t n = 1;
+  while (n < kClusterSplits && n < want && n < cap) n *= 2;
+  return Splits{n, n > 1};
 }
 static int heads_per_block(int group) { return group <= 8 ? 8 : 16; }
 
@@ -486,9 +555,23 @@ static int launch_paged(const PagedParams& p, cudaStream_t stream) {
     configured[dev] = true;
   }
   const unsigned blocks = static_cast<unsigned>(p.a.batch) * p.a.kv_heads * p.head_blocks * p.splits;
-  kernel<<<blocks, kPagedThreads, C::SMEM, stream>>>(p);
-  QLIN_CHECK_LAUNCH("qlin_paged_attention");
-  if (p.splits > 1) {
+  cudaLaunchConfig_t main = {};
+  main.gridDim = dim3(blocks, 1, 1);
+  main.blockDim = dim3(kPagedThreads, 1, 1);
+  main.dynamicSmemBytes = C::SMEM;
+  main.stream = stream;
+  cudaLaunchAttribute size[1];
+  size[0].id = cudaLaunchAttributeClusterDimension;
+  size[0].val.clusterDim.x = static_cast<unsigned>(p.cluster ? p.splits : 1);
+  size[0].val.clusterDim.y = size[0].val.clusterDim.z = 1;
+  main.attrs = size;
+  main.numAttrs = p.cluster ? 1 : 0;
+  const cudaError_t launched = cudaLaunchKernelEx(&main, kernel, p);
+  if (launched != cudaSuccess) {
+    cudaGetLastError();
+    return fail(QLIN_ERR_LAUNCH, "qlin_paged_attention: %s", cudaGetErrorString(launched));
+  }
+  if (p.splits > 1 && !p.cluster) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.a.batch) * p.a.q_heads, 1, 1);
     cfg.blockDim = dim3(128, 1, 1);
@@ -521,9 +604,9 @@ extern "C" int64_t qlin_paged_attention_workspace_bytes(const qlin_paged_attenti
   if (rc != QLIN_OK) return rc;
   if (a->batch == 0) return 0;
   const int group = a->q_heads / a->kv_heads;
-  const int64_t splits = choose_splits(*a, (group + heads_per_block(group) - 1) / heads_per_block(group));
-  if (splits == 1) return 0;
-  const int64_t rows = static_cast<int64_t>(a->batch) * a->q_heads * splits;
+  const Splits splits = choose_splits(*a, (group + heads_per_block(group) - 1) / heads_per_block(group));
+  if (splits.n == 1 || splits.cluster) return 0;
+  const int64_t rows = static_cast<int64_t>(a->batch) * a->q_heads * splits.n;
   return rows * a->head_dim * 4 + rows * 8;
 }
 
@@ -545,10 +628,12 @@ extern "C" int qlin_paged_attention(const qlin_paged_attention_args* a, void* st
   p.a = *a;
   p.group = a->q_heads / a->kv_heads;
   p.head_blocks = (p.group + heads_per_block(p.group) - 1) / heads_per_block(p.group);
-  p.splits = choose_splits(*a, p.head_blocks);
+  const Splits splits = choose_splits(*a, p.head_blocks);
+  p.splits = splits.n;
+  p.cluster = splits.cluster;
   p.part_o = nullptr;
   p.part_ml = nullptr;
-  if (p.splits > 1) {
+  if (p.splits > 1 && !p.cluster) {
     if (a->workspace == nullptr) return fail(QLIN_ERR_NULL, "qlin_paged_attention: workspace is NULL");
     if (!aligned16(a->workspace)) return fail(QLIN_ERR_BAD_ALIGN, "qlin_paged_attention: workspace must start on 16 bytes");
     p.part_o = static_cast<float*>(a->workspace);

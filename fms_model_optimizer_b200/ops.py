@@ -640,9 +640,7 @@ def qk_norm_rope(
     int32 ``[tokens]``.  With ``k_pages`` / ``v_pages [pages, kv heads, page size, head_dim]`` given, token t goes to slot
     ``slots[t] = page * page size + offset`` (int64, negative: not written), in the model's type or as e4m3 codes of
     ``x / k_scale[kv head]``.  Returns new ``(q, k)``; ``k`` is None without ``want_k``.  No gradient."""
-    dev = q.device
-    work = 2.0 * (q.numel() + k.numel()) * q.element_size()
-    return _call("qk_rope", work, dev, L.host().qk_rope, q, k, cos, sin, positions, q_weight, k_weight, eps, v, k_pages, v_pages, slots, k_scale, v_scale, want_k)
+    return _call("qk_rope", 0.0, q.device, L.host().qk_rope, q, k, cos, sin, positions, q_weight, k_weight, eps, v, k_pages, v_pages, slots, k_scale, v_scale, want_k)
 
 
 def paged_attention(
