@@ -9,6 +9,10 @@ SwiGLU are plumbing; the seven Linears of every layer run ``QLinearINT8Deploy``'
 * ``surface="modules"``: the drop-in route a user of the reference takes: ``QLinear`` modules lowered with
   ``lower_qmodel_b200`` to ``QLinearINT8Deploy`` (fms_mo/dq.py:262-272 does the same with ``lower_qmodel_triton``),
   norms and activations as PyTorch ops.  One GPU only.
+* ``generate``: greedy generation on one GPU with the fused surface.  A prompt's keys and values go into a paged cache on their way out
+  of the rotation, later tokens attend over it (``kvcache.PagedKVCache``, ``ops.qk_norm_rope``, ``ops.prompt_attention``,
+  ``ops.paged_attention``).  ``cfg`` may ask for per-head norms of queries and keys (``qk_norm``) and a sliding window with first
+  tokens that stay visible (``window``, ``sinks``); ``forward`` follows them too.
 * sharded (``world > 1``): weights split column-parallel (q, k, v, gate, up) and row-parallel (o, down) following the
   reference's tables (fms_mo/aiu_addons/i8i8/i8i8_aiu_linear.py:304-389), one process per GPU.  ``exchange`` picks how
   the shard boundary is crossed:
@@ -32,6 +36,7 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from . import ops, tp
+from .kvcache import PagedKVCache, Step
 
 LLAMA3_8B = dict(layers=32, hidden=4096, q_heads=32, kv_heads=8, head_dim=128, ffn=14336, vocab=128256, rope_theta=500000.0,
                  batch=8, seq=2048)  # fmt: skip
@@ -168,6 +173,9 @@ class W8A8Decoder:
         nl = layers if layers is not None else cfg["layers"]
         if surface == "modules" and world != 1:
             raise RuntimeError("the module surface runs on one GPU")
+        self.own_attention = bool(cfg.get("qk_norm", False) or cfg.get("window", 0))
+        if self.own_attention and (surface != "fused" or world != 1):
+            raise RuntimeError("qk_norm and window run on one GPU with the fused surface")
         self.layers = []
         for li in range(nl):
             lin = {}
@@ -185,6 +193,11 @@ class W8A8Decoder:
                 del w
             lin["ln1"] = torch.ones(H, device=dev, dtype=torch.bfloat16)
             lin["ln2"] = torch.ones(H, device=dev, dtype=torch.bfloat16)
+            lin["q_norm"] = lin["k_norm"] = None
+            if cfg.get("qk_norm", False):
+                g = torch.Generator(device=dev).manual_seed(1000 * li + 100)
+                for name in ("q_norm", "k_norm"):
+                    lin[name] = (1 + 0.1 * torch.randn(cfg["head_dim"], generator=g, device=dev)).bfloat16()
             self.layers.append(lin)
         g = torch.Generator(device=dev).manual_seed(4)
         self.embed = (torch.randn(cfg["vocab"], H, generator=g, device=dev) * 0.02).bfloat16()
@@ -240,12 +253,57 @@ class W8A8Decoder:
         return (last @ self.lm_head.t()).argmax(-1), last
 
     # ------------------------------------------------------------------------------------------------ one GPU / NCCL
-    def _forward_steps(self, ids):
+    def _rotate(self, lin, q, k, positions, **cache):
+        return ops.qk_norm_rope(q, k, self.cos, self.sin, positions, q_weight=lin["q_norm"], k_weight=lin["k_norm"], eps=1e-6, **cache)
+
+    def _mask(self):
+        return dict(window=self.cfg.get("window", 0), sinks=self.cfg.get("sinks", 0))
+
+    def _attend_whole(self, B, S):
+        """Rotation and attention of B whole sequences of S tokens: (layer, its Linears, q, k, v) -> (q, k, output)."""
+        if not self.own_attention:
+
+            def attend(li, lin, q, k, v):
+                q, k = ops.rope_(q, self.cos, self.sin, S), ops.rope_(k, self.cos, self.sin, S)
+                return q, k, self._attention(q, k, v, B, S)
+
+            return attend
+        positions = torch.arange(S, dtype=torch.int32, device=self.dev).repeat(B)
+        cu = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=self.dev)
+
+        def attend(li, lin, q, k, v):
+            q, k = self._rotate(lin, q, k, positions)
+            a = ops.prompt_attention(q, k, v.view(k.shape), cu, cu, S, **self._mask())
+            return q, k, a.view(B * S, -1)
+
+        return attend
+
+    def _attend_cached(self, cache, step: Step):
+        """Rotation into the cache and attention: of prompts among themselves, of single tokens over the cache."""
+
+        def attend(li, lin, q, k, v):
+            pages = cache.layer(li)
+            v = v.view(k.shape)
+            q, k = self._rotate(lin, q, k, step.positions, v=v, slots=step.slots, want_k=not step.single, **pages)
+            if step.single:
+                a = ops.paged_attention(q, block_table=cache.table, lens=cache.lens, **pages, **self._mask())
+            else:
+                a = ops.prompt_attention(q, k, v, step.cu, step.cu, step.max_q, **self._mask())
+            return q, k, a.view(a.shape[0], -1)
+
+        return attend
+
+    def _forward_steps(self, ids, attend=None, last=None):
         """The forward pass of one group of sequences as a generator: it yields after every row-parallel Linear
         (whose all-reduce, if any, has just been queued), so that a driver can advance another group on another
-        stream meanwhile.  Returns the next-token ids through StopIteration."""
+        stream meanwhile.  Returns the next-token ids through StopIteration.  ``ids`` [batch, seq], or with ``attend`` (what
+        ``_attend_cached`` returns) [tokens] packed, ``last`` the rows that reach the head."""
         cfg = self.cfg
-        B, S = ids.shape
+        if attend is None:
+            B, S = ids.shape
+            attend = self._attend_whole(B, S)
+        else:
+            B, S = ids.numel(), 1
         hd, bf = cfg["head_dim"], torch.bfloat16
         x = F.embedding(ids, self.embed).view(B * S, -1)
         pending = None  # output of the last row-parallel Linear, added to the stream by the next fused kernel
@@ -264,10 +322,8 @@ class W8A8Decoder:
                 for name, c_, s_ in zip("qkv", cs, ss):
                     self._note("codes_" + name, li, c_)
                     self._note("scale_" + name, li, s_)
-            q = ops.rope_(q.view(B * S, self.nq, hd), self.cos, self.sin, S)
-            k = ops.rope_(k.view(B * S, self.nkv, hd), self.cos, self.sin, S)
             del cs, ss
-            a = self._attention(q, k, v, B, S)
+            q, k, a = attend(li, lin, q.view(B * S, self.nq, hd), k.view(B * S, self.nkv, hd), v)
             qa = lin["o"].quantise_fused(a)
             pending = lin["o"](None, qa, bf)
             if tr:
@@ -289,7 +345,10 @@ class W8A8Decoder:
             del cs, ss
             yield
         # only the last token of every sequence reaches the head
-        x_last, p_last = x.view(B, S, -1)[:, -1].contiguous(), pending.view(B, S, -1)[:, -1].contiguous()
+        if last is None:
+            x_last, p_last = x.view(B, S, -1)[:, -1].contiguous(), pending.view(B, S, -1)[:, -1].contiguous()
+        else:
+            x_last, p_last = x[last], pending[last]
         _, _, x_last, h = ops.block_quant(x_last, prologue=L.BLOCK_NORM, r=p_last, norm_w=self.norm, store_sum=True, smooth_rcps=[], want_h=True)
         self._note("x_final_last", len(self.layers), x_last)
         return self._head(h)
@@ -482,6 +541,31 @@ class W8A8Decoder:
             gens = [self._forward_steps(p) for p in parts]
         out, self.last_hidden = self._drive(gens)
         return out
+
+    @torch.no_grad()
+    def generate(self, prompts, new_tokens, cache: Optional[PagedKVCache] = None, cache_dtype=torch.bfloat16, page_size=64):
+        """Greedy generation: ``new_tokens`` ids [batch, new_tokens] behind each of ``prompts`` (1-D id tensors, lengths as they come).
+        ``cache``: an empty ``PagedKVCache`` for as many sequences; by default one of ``cache_dtype`` (bfloat16, or float8_e4m3fn
+        codes) is made.  ``self.last_hidden`` keeps the last step's final hidden states."""
+        if self.surface != "fused" or self.world != 1:
+            raise RuntimeError("generate runs on one GPU with the fused surface")
+        lengths = [int(p.numel()) for p in prompts]
+        if not lengths or min(lengths) < 1 or new_tokens < 1:
+            raise RuntimeError("generate takes prompts of at least one token and produces at least one")
+        longest = max(lengths) + new_tokens - 1  # the last id is produced, not read
+        if longest > self.cos.shape[0]:
+            raise RuntimeError(f"{longest} tokens are more than the {self.cos.shape[0]} positions of cfg['seq']")
+        if cache is None:
+            cache = PagedKVCache(len(self.layers), len(lengths), longest, self.nkv, self.cfg["head_dim"], self.dev, cache_dtype, page_size)
+        if cache.batch != len(lengths) or len(cache.k) != len(self.layers):
+            raise RuntimeError("the cache is for another number of sequences or layers")
+        ids, step, out = torch.cat([p.reshape(-1) for p in prompts]).to(self.dev), cache.prompts(lengths), []
+        while True:
+            ids, self.last_hidden = self._drive([self._forward_steps(ids, self._attend_cached(cache, step), step.last)])
+            out.append(ids)
+            if len(out) == new_tokens:
+                return torch.stack(out, 1)
+            step = cache.token()
 
     def _drive(self, gens):
         """Advances the groups round-robin, one segment at a time, each on its own stream."""

@@ -1,0 +1,108 @@
+"""A paged key-value cache for a decoder that generates: the pool of pages, the page table and the lengths that
+``ops.qk_norm_rope`` writes with and ``ops.paged_attention`` reads with.
+
+Every layer has its own pool ``[pages, kv heads, page size, head_dim]`` of keys and of values; all layers share one page table
+``[batch, pages of a sequence]`` and one length for each sequence.  Pages are handed out as sequences grow and come back with
+``release``.  Tables, lengths, positions and slots live on the device; the host keeps a copy of the lengths to hand out pages by, so
+that a step needs no synchronisation.  No counterpart in the reference, which leaves generation to a serving stack.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import List, Optional, Sequence
+
+import torch
+
+
+@dataclass
+class Step:
+    """The tokens of one forward pass, packed sequence behind sequence."""
+
+    positions: torch.Tensor  # int32 [tokens]
+    slots: torch.Tensor  # int64 [tokens]
+    last: torch.Tensor  # int64 [batch]: row of every sequence's last token
+    single: bool  # one new token for every sequence
+    cu: Optional[torch.Tensor] = None  # int32 [batch + 1], prompts only
+    max_q: int = 1
+
+
+class PagedKVCache:
+    def __init__(self, layers: int, batch: int, max_len: int, kv_heads: int, head_dim: int, dev, dtype: torch.dtype = torch.bfloat16, page_size: int = 64,
+                 pages: Optional[int] = None):  # fmt: skip
+        """``max_len``: the most tokens of a sequence.  ``pages``: size of the pool, by default enough for all sequences at full
+        length.  ``dtype`` float8_e4m3fn holds codes with one fp32 scale per layer and kv head (``k_scale`` / ``v_scale``, 1 at first)."""
+        if min(layers, batch, max_len, page_size) < 1:
+            raise RuntimeError("layers, batch, max_len and page_size must be positive")
+        if dtype not in (torch.bfloat16, torch.float16, torch.float8_e4m3fn):
+            raise RuntimeError("the cache holds bfloat16, float16 or float8_e4m3fn")
+        per = -(-max_len // page_size)
+        pages = batch * per if pages is None else pages
+        shape = (pages, kv_heads, page_size, head_dim)
+        self.k = [torch.zeros(shape, dtype=dtype, device=dev) for _ in range(layers)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=dev) for _ in range(layers)]
+        f8 = dtype == torch.float8_e4m3fn
+        self.k_scale = [torch.ones(kv_heads, device=dev) for _ in range(layers)] if f8 else [None] * layers
+        self.v_scale = [torch.ones(kv_heads, device=dev) for _ in range(layers)] if f8 else [None] * layers
+        self.dev, self.batch, self.max_len, self.page_size = dev, batch, max_len, page_size
+        self.table = torch.zeros(batch, per, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.host_lens = [0] * batch
+        self._owned: List[List[int]] = [[] for _ in range(batch)]
+        self._free = list(range(pages - 1, -1, -1))
+
+    def layer(self, i: int) -> dict:
+        """The keyword arguments of layer ``i`` for ``ops.qk_norm_rope`` (and, without the slots, ``ops.paged_attention``)."""
+        return dict(k_pages=self.k[i], v_pages=self.v[i], k_scale=self.k_scale[i], v_scale=self.v_scale[i])
+
+    def reserve(self, lengths: Sequence[int]) -> None:
+        """Hands out the pages for sequences of these lengths.  Refused as a whole where the pool does not hold them."""
+        need = [max(0, -(-int(n) // self.page_size) - len(own)) for n, own in zip(lengths, self._owned)]
+        if any(n > self.max_len for n in lengths):
+            raise RuntimeError(f"a sequence of {max(lengths)} tokens does not fit a cache of {self.max_len}")
+        if sum(need) > len(self._free):
+            raise RuntimeError(f"the cache is out of pages: {sum(need)} wanted, {len(self._free)} free")
+        for b, n in enumerate(need):
+            if n:
+                new = [self._free.pop() for _ in range(n)]
+                first = len(self._owned[b])
+                self._owned[b] += new
+                self.table[b, first : first + n] = torch.tensor(new, dtype=torch.int32).to(self.dev)
+
+    def release(self, b: int) -> None:
+        """Sequence ``b`` is over: its pages go back to the pool and its length to 0."""
+        self._free += reversed(self._owned[b])
+        self._owned[b] = []
+        self.host_lens[b] = 0
+        self.lens[b] = 0
+
+    def _slots(self, which: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        page = self.table[which, positions // self.page_size].long()
+        return page * self.page_size + positions % self.page_size
+
+    def prompts(self, lengths: Sequence[int]) -> Step:
+        """Room for the prompts of all (empty) sequences, ``lengths[b]`` >= 1 tokens each."""
+        if len(lengths) != self.batch or min(lengths) < 1:
+            raise RuntimeError("one prompt of at least one token for every sequence is wanted")
+        if any(self.host_lens):
+            raise RuntimeError("prompts start empty sequences: release them first")
+        self.reserve(lengths)
+        n = torch.tensor(lengths)
+        cu = torch.zeros(self.batch + 1, dtype=torch.int64)
+        cu[1:] = n.cumsum(0)
+        which = torch.repeat_interleave(torch.arange(self.batch), n)
+        positions = (torch.arange(int(cu[-1])) - cu[which]).to(self.dev)
+        self.host_lens = [int(x) for x in lengths]
+        self.lens.copy_(n.to(torch.int32))
+        slots = self._slots(which.to(self.dev), positions)
+        return Step(positions.to(torch.int32), slots, (cu[1:] - 1).to(self.dev), False, cu.to(torch.int32).to(self.dev), max(self.host_lens))
+
+    def token(self) -> Step:
+        """Room for one more token of every sequence."""
+        self.reserve([n + 1 for n in self.host_lens])
+        positions = self.lens.clone()
+        every = torch.arange(self.batch, device=self.dev)
+        slots = self._slots(every, positions.long())
+        self.lens += 1
+        self.host_lens = [n + 1 for n in self.host_lens]
+        return Step(positions, slots, every, True)
