@@ -139,9 +139,10 @@ template <typename T, int DP>
 struct PromptCfg {
   static constexpr int CHUNKS = DP / 64;
   static constexpr int TILE_BYTES = CHUNKS * kChunkBytes;  // a tile of queries, keys or values
-  static constexpr int STAGES = DP == 128 ? 5 : 8;         // tiles of keys or values in flight
+  static constexpr int STAGES = DP == 128 ? 4 : 8;         // tiles of keys or values in flight
   static constexpr int KV_OFFSET = 2 * TILE_BYTES;
-  static constexpr int AUX_OFFSET = KV_OFFSET + STAGES * TILE_BYTES;
+  static constexpr int OUT_OFFSET = KV_OFFSET + STAGES * TILE_BYTES;  // 32 rows of 64 outputs for each softmax warp
+  static constexpr int AUX_OFFSET = OUT_OFFSET + kSoftmaxWarps * 4096;
   static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(PromptAux));
   static constexpr float SHIFT = std::is_same<T, __half>::value ? 6.0f : 0.0f;
   static constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
@@ -422,9 +423,11 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, f
   const auto mask = [&](int c) {
     if constexpr (MASKED) {
       const uint32_t seen = columns_under(hi + 1, 32 * c) & (~columns_under(lo + 1, 32 * c) | columns_under(sinks, 32 * c));
+      if (__any_sync(0xffffffffu, seen != 0xffffffffu)) {  // most quarters of a tile at the edge are seen by all rows of a warp
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (!((seen >> j) & 1u)) x[c][j] = 0xff800000u;
+        for (int j = 0; j < 32; ++j)
+          if (!((seen >> j) & 1u)) x[c][j] = 0xff800000u;
+      }
     }
   };
   const uint64_t cl22 = pair64(cl2, cl2);
@@ -741,7 +744,11 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       if (!ok) break;
       tc_fence_after();
       const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+      // Rows go through shared memory, 64 outputs at a time, so that eight lanes write the 128 bytes of a row together (a lane for
+      // each row touches 32 lines with every store: 8 x 2048 @@ us).
       T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(u.seq.q0 + token) * p.a.q_heads + head) * p.a.head_dim;
+      const uint64_t out_row = row_ok ? reinterpret_cast<uint64_t>(out) : 0;
+      uint8_t* stage = smem + C::OUT_OFFSET + warp * 4096;
       bool again = false;
 #pragma unroll
       for (int c = 0; c < DP / 32; ++c) {
@@ -754,15 +761,23 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         }
 #pragma unroll
         for (int j = 0; j < 32; ++j) again |= __uint_as_float(o[j]) != __uint_as_float(o[j]);
-        if (row_ok) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8)
-            if (32 * c + j < p.a.head_dim) {
-              uint32_t w[4];
+        for (int j = 0; j < 32; j += 8) {
+          uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = pack2<T>(__uint_as_float(o[j + 2 * e]) * scale, __uint_as_float(o[j + 2 * e + 1]) * scale);
-              *reinterpret_cast<uint4*>(out + 32 * c + j) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+          for (int e = 0; e < 4; ++e) w[e] = pack2<T>(__uint_as_float(o[j + 2 * e]) * scale, __uint_as_float(o[j + 2 * e + 1]) * scale);
+          *reinterpret_cast<uint4*>(stage + lane * 128 + (((c & 1) * 4 + j / 8) ^ (lane & 7)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (c & 1) {
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int rr = 4 * k + (lane >> 3), piece = lane & 7;
+            const uint64_t dst = __shfl_sync(0xffffffffu, out_row, rr);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((piece ^ (rr & 7)) * 16));
+            if (dst != 0 && 32 * (c - 1) + piece * 8 < p.a.head_dim) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(dst) + 32 * (c - 1) + piece * 8) = v;
+          }
+          __syncwarp();
         }
       }
       tc_fence_before();  // the next unit's weights are announced behind these reads of the accumulator
