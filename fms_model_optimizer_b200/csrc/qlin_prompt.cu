@@ -275,9 +275,16 @@ struct Unit {
   Sequence seq;
   int b, kvh, t0;  // sequence, kv head, first query
   int shift;       // position of query 0
-  int sink_tiles, win_tile, tiles;
+  int win_tile, win_tiles, tiles;
   bool second;     // the second tile has rows
-  __device__ __forceinline__ int key0(int t) const { return (t < sink_tiles ? t : win_tile + (t - sink_tiles)) * kKeys; }
+  // Tiles of the window, then those of the first keys.  Under a window the tile at its edge comes last of the former: a row that sees few
+  // keys of its first tile has a low reference, and the next tile would rewrite its accumulator (1 x 8191 under a window of 2048
+  // with four first keys in front: a rewrite for every 13th tile of a warp, 277 us; @@ so).
+  __device__ __forceinline__ int key0(int t) const {
+    if (t >= win_tiles) return (t - win_tiles) * kKeys;
+    if (win_tile == 0) return t * kKeys;
+    return (win_tile + (t + 1 == win_tiles ? 0 : t + 1)) * kKeys;
+  }
 };
 // The units of a block, every gridDim.x-th one of the list that begins with the last queries of every sequence and head, which see
 // the most keys.  `busy`: units without keys are passed over.
@@ -299,8 +306,8 @@ struct Units {
       const int lo = u.t0 + u.shift, hi = min(u.t0 + 2 * p.tq, u.seq.n) - 1 + u.shift;
       const int end = hi < 0 ? 0 : hi / kKeys + 1;
       u.win_tile = p.a.window > 0 ? min(max(lo - p.a.window + 1, 0) / kKeys, end) : 0;
-      u.sink_tiles = min((p.a.sinks + kKeys - 1) / kKeys, u.win_tile);
-      u.tiles = u.sink_tiles + end - u.win_tile;
+      u.win_tiles = end - u.win_tile;
+      u.tiles = u.win_tiles + min((p.a.sinks + kKeys - 1) / kKeys, u.win_tile);
       u.second = u.t0 + p.tq < u.seq.n;
       if (busy && u.tiles == 0) continue;
       id += step;
