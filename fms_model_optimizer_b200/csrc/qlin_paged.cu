@@ -17,6 +17,10 @@
 // order of the 16 head dimensions of a step is permuted, the same way in Q (keys) and in the rows of O^T (values).  A bf16 query
 // meets them as fp16 times a power of two that brings its largest element to 2^13..2^14: no digit of it is lost above 2^-27 of the largest.
 //
+// Measured (device time): 1 x 131072 keys of 8 heads of 128 in bf16 87 us, 6.1 TB/s; 61 x 2050 78.5 us, 6.5 TB/s; 61 x up to 4099 in e4m3
+// 52 us, 5.0 TB/s, where the chain of conversions, products and shuffles of a tile is as long as its loads; 1 x 2048 6.7 us, which is
+// the latency of the length, the page table, the keys and the join behind one another.
+//
 // Statistics, sums and the join are fp32.  Weights are rounded to the cache's 16-bit type (fp16 with an e4m3 cache) as operands of
 // the product; fp16 weights carry a factor of 2^12, so that weights down to 2^-26 of the largest keep 11 bits.
 #include <type_traits>
@@ -32,13 +36,12 @@ namespace qlin {
 constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kTileKeys = 16;
-constexpr int kRingBytes = 24576;  // stages of a warp: two blocks an SM keep about 190 KB between them
-constexpr int kMinTiles = 8;       // tiles of a block at least, two a warp
-constexpr int kWaves = 1;
+constexpr int kMinTiles = 4;       // tiles of a block at least, one a warp (1 x 2048 keys 6.7 us; with eight 7.6)
 
 struct PagedParams {
   qlin_paged_attention_args a;
   int32_t splits, head_blocks, group;  // blocks of query heads per kv head, query heads per kv head
+  int32_t page_shift;                  // log2 of the page size, or -1
   int32_t cluster;                     // the splits of a head are a cluster of blocks and join in shared memory
   float* part_o;                       // [batch * q_heads, splits, head_dim]
   float2* part_ml;                     // [batch * q_heads, splits]: maximum and sum
@@ -145,7 +148,12 @@ struct PagedCfg {
   static constexpr int RB = DP * ES;                   // bytes of a row
   static constexpr int CH = RB / 16;                   // 16-byte pieces of a row
   static constexpr int STAGE = 2 * kTileKeys * RB;     // keys, then values
-  static constexpr int STAGES = kRingBytes / STAGE < 8 ? kRingBytes / STAGE : 8;
+  // Three stages at least; where they are small, 16 KB a warp, so that a third block fits the SM: its warps cover the latency of the
+  // chain from a tile's keys to its outputs (3 x up to 30000 keys in e4m3 32 us, 37 with two).  16-bit rows of 128 run as fast as
+  // memory does with two blocks of three stages (61 x 2050 keys 78.5 us, three blocks of two stages 95).
+  static constexpr int RING = STAGE >= 8192 ? 24576 : 16384;
+  static constexpr int STAGES = RING / STAGE;
+  static constexpr int BLOCKS = NT == 1 && RING == 16384 ? 3 : 2;  // an SM
   static constexpr int LOADS = kTileKeys * CH / 32;    // pieces of K a lane copies, and as many of V
   static constexpr int HEADS = 8 * NT;
   static constexpr int OROW = DP + 4;                  // floats of a row of the joined outputs
@@ -160,7 +168,7 @@ __device__ __forceinline__ uint32_t piece(int row, int c) {
 }
 
 template <typename QT, bool F8, int DP, int NT>
-__global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOCKS)) paged_kernel(const __grid_constant__ PagedParams p) {
   using C = PagedCfg<QT, F8, DP, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   griddep_launch();
@@ -187,28 +195,29 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
   const int lrow = lane / C::CH, lc = lane % C::CH;  // of the first piece this lane copies
   const bool piece_real = lc * 16 < D * C::ES;
   bool bad_page = false;
-  // lane r < 16 finds row r of a tile: the page of the next tile to load is read one tile ahead
-  int page_next = 0, off_next = 0;
+  // lane r < 16 finds row r of a tile: its page is read one turn ahead of its copies
+  struct Place {
+    int page, offset;
+  };
   const auto look_up = [&](int tile) {
     const int u = tile * kTileKeys + (lane & 15);
+    Place at{0, 0};
     if (tile < last && u < vis.n) {
-      const int key = vis.key(u), pg = key / p.a.page_size;
-      off_next = key - pg * p.a.page_size;
-      page_next = table[pg];
+      const int key = vis.key(u), pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.a.page_size;
+      at.offset = key - pg * p.a.page_size;
+      at.page = table[pg];
     }
+    return at;
   };
-  const auto load_tile = [&](int tile, int stage) {
+  const auto load_tile = [&](int tile, int stage, Place where) {
     if (tile < last) {
-      const int u = tile * kTileKeys + (lane & 15);
-      const bool real = u < vis.n;
-      int pg = page_next;
-      if (real && (pg < 0 || pg >= p.a.num_pages)) {
+      const bool real = tile * kTileKeys + (lane & 15) < vis.n;
+      if (real && (where.page < 0 || where.page >= p.a.num_pages)) {
         bad_page = true;
-        pg = 0;
+        where.page = 0;
       }
-      const int64_t off = real ? (pg * p.a.page_stride + off_next * p.a.slot_stride + head_off) * C::ES : 0;
+      const int64_t off = real ? (where.page * p.a.page_stride + where.offset * p.a.slot_stride + head_off) * C::ES : 0;
       const uint32_t reals = __ballot_sync(0xffffffffu, real);
-      look_up(tile + kPagedWarps);
       const uint32_t dst = ring + stage * C::STAGE;
 #pragma unroll
       for (int i = 0; i < C::LOADS; ++i) {
@@ -221,9 +230,14 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  look_up(first);
+  {
+    Place ahead[C::STAGES - 1];  // all of them are read together
 #pragma unroll
-  for (int s = 0; s < C::STAGES - 1; ++s) load_tile(first + s * kPagedWarps, s);
+    for (int s = 0; s < C::STAGES - 1; ++s) ahead[s] = look_up(first + s * kPagedWarps);
+#pragma unroll
+    for (int s = 0; s < C::STAGES - 1; ++s) load_tile(first + s * kPagedWarps, s, ahead[s]);
+  }
+  Place place = look_up(first + (C::STAGES - 1) * kPagedWarps);
 
   // ---------------------------------------------------------------- queries, as columns g of the product's second operand
   uint32_t qf[DP / 16][NT][2];
@@ -285,7 +299,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
   for (int tile = first; tile < last; tile += kPagedWarps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
     __syncwarp();
-    load_tile(tile + (C::STAGES - 1) * kPagedWarps, stage_in);  // into the stage of the tile before this one
+    load_tile(tile + (C::STAGES - 1) * kPagedWarps, stage_in, place);  // into the stage of the tile before this one
+    place = look_up(tile + C::STAGES * kPagedWarps);
     const uint32_t ks = ring + stage * C::STAGE, vs = ks + kTileKeys * C::RB;
     float s[NT][4];
 #pragma unroll
@@ -468,42 +483,66 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
   }
 }
 
-// The splits of one query head, in order.  One block a head, a thread for each output.
+// The splits of one query head, in order.  One block a head: its warps take every kJoinWarps-th split, a lane four outputs, and are
+// added up in turn.
+constexpr int kJoinWarps = 8;
 template <typename QT>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedParams p, bool f8) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedParams p, bool f8) {
+  __shared__ float warp_top[kJoinWarps], warp_sum[kJoinWarps];
+  __shared__ float4 warp_o[kJoinWarps][32];
   const int64_t row = blockIdx.x;
-  const int b = static_cast<int>(row / p.a.q_heads), h = static_cast<int>(row % p.a.q_heads), d = threadIdx.x;
+  const int b = static_cast<int>(row / p.a.q_heads), h = static_cast<int>(row % p.a.q_heads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane * 4, D = p.a.head_dim;
   const Visible vis = visible_keys(sequence_length(p, b, false), p.a.window, p.a.sinks);
   const int tiles = (vis.n + kTileKeys - 1) / kTileKeys;
   const int used = splits_used(tiles, tiles_per_split(tiles, p.splits));
   griddep_wait();
   if (used == 1) return;
   const float2* ml = p.part_ml + row * p.splits;
-  const float* part = p.part_o + row * p.splits * p.a.head_dim + d;
+  const float* part = p.part_o + row * p.splits * D;
   float top = -INFINITY;
-  for (int s = 0; s < used; ++s) top = fmaxf(top, ml[s].x);
-  float sum = 0.0f, acc = 0.0f;
-  if (d < p.a.head_dim) {
-#pragma unroll 8
-    for (int s = 0; s < used; ++s) {
-      const float2 v = ml[s];
-      const float f = v.x == top ? 1.0f : exp2f(v.x - top);
-      sum += v.y * f;
-      acc += part[static_cast<int64_t>(s) * p.a.head_dim] * f;
-    }
-    const float r = sum == 0.0f ? 0.0f : (f8 ? p.a.v_scale[h / p.group] : 1.0f) / sum;
-    QT* out = static_cast<QT*>(p.a.out) + row * p.a.head_dim + d;
-    if constexpr (std::is_same<QT, __nv_bfloat16>::value) {
-      *out = __float2bfloat16_rn(acc * r);
-    } else {
-      *out = __float2half_rn(acc * r);
-    }
+  for (int s = threadIdx.x; s < used; s += kJoinWarps * 32) top = fmaxf(top, ml[s].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) warp_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, warp_top[w]);
+  float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = warp; s < used; s += kJoinWarps) {
+    const float2 v = ml[s];
+    const float4 o = d < D ? *reinterpret_cast<const float4*>(part + static_cast<int64_t>(s) * D + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float f = v.x == top ? 1.0f : exp2f(v.x - top);
+    sum += v.y * f;
+    acc[0] += o.x * f;
+    acc[1] += o.y * f;
+    acc[2] += o.z * f;
+    acc[3] += o.w * f;
   }
+  warp_o[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  if (lane == 0) warp_sum[warp] = sum;
+  __syncthreads();
+  if (warp != 0 || d >= D) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w) {
+    sum += warp_sum[w];
+    const float4 o = warp_o[w][lane];
+    acc[0] += o.x;
+    acc[1] += o.y;
+    acc[2] += o.z;
+    acc[3] += o.w;
+  }
+  const float r = sum == 0.0f ? 0.0f : (f8 ? p.a.v_scale[h / p.group] : 1.0f) / sum;
+  constexpr bool bf16 = std::is_same<QT, __nv_bfloat16>::value;
+  *reinterpret_cast<uint2*>(static_cast<QT*>(p.a.out) + row * D + d) = make_uint2(pack16<bf16>(acc[0] * r, acc[1] * r), pack16<bf16>(acc[2] * r, acc[3] * r));
 }
 
-// Splits of the keys: as many blocks as run at once, none with fewer than kMinTiles tiles where the page table is as wide as its longest
+// Splits of the keys: blocks for every SM, none with fewer than kMinTiles tiles where the page table is as wide as its longest
 // sequence.  Up to kClusterSplits of them (a power of two) are a cluster of blocks, which joins without a second launch and without
-// a workspace; only few heads with long tables take more.
+// a workspace; few heads with long tables take more.  Blocks an SM, device time: 16-bit caches two (1 x 131072 keys 83 us, with
+// three 100, with six 90); e4m3 three, and up to nine where they join in a cluster, which evens out ragged batches (61 x up to 4099
+// keys 59 us unsplit, 52 in pairs, 68 in fours; 3 x up to 30000 keys with two blocks 37, three 32, six 32).
 constexpr int kClusterSplits = 8;
 struct Splits {
   int32_t n, cluster;
@@ -512,11 +551,11 @@ static Splits choose_splits(const qlin_paged_attention_args& a, int head_blocks)
   int64_t most = static_cast<int64_t>(a.max_pages) * a.page_size;
   if (a.window > 0 && most > static_cast<int64_t>(a.window) + a.sinks) most = static_cast<int64_t>(a.window) + (a.sinks > 0 ? a.sinks : 0);
   const int64_t tiles = (most + kTileKeys - 1) / kTileKeys, rows = static_cast<int64_t>(a.batch) * a.kv_heads * head_blocks;
-  const int64_t want = (kWaves * 2 * sm_count() + rows - 1) / rows, cap = (tiles + kMinTiles - 1) / kMinTiles;
-  if (want > 2 * kClusterSplits && cap > 4 * kClusterSplits) {
-    const int64_t n = 2 * sm_count() / rows;
-    return Splits{static_cast<int32_t>(n < cap ? n : cap), 0};
-  }
+  const bool f8 = a.cache_dtype == QLIN_DT_F8E4M3;
+  const int64_t cap = (tiles + kMinTiles - 1) / kMinTiles, blocks = (f8 ? 3 : 2) * sm_count();
+  int64_t want = (blocks + rows - 1) / rows;
+  if (want > kClusterSplits && cap > 2 * kClusterSplits) return Splits{static_cast<int32_t>(want < cap ? want : cap), 0};
+  if (f8) want = (3 * blocks / 2 + rows - 1) / rows;
   int32_t n = 1;
   while (n < kClusterSplits && n < want && n < cap) n *= 2;
   return Splits{n, n > 1};
@@ -574,7 +613,7 @@ static int launch_paged(const PagedParams& p, cudaStream_t stream) {
   if (p.splits > 1 && !p.cluster) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.a.batch) * p.a.q_heads, 1, 1);
-    cfg.blockDim = dim3(128, 1, 1);
+    cfg.blockDim = dim3(kJoinWarps * 32, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -630,6 +669,9 @@ extern "C" int qlin_paged_attention(const qlin_paged_attention_args* a, void* st
   p.head_blocks = (p.group + heads_per_block(p.group) - 1) / heads_per_block(p.group);
   const Splits splits = choose_splits(*a, p.head_blocks);
   p.splits = splits.n;
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (a->page_size == 1 << i) p.page_shift = i;
   p.cluster = splits.cluster;
   p.part_o = nullptr;
   p.part_ml = nullptr;
