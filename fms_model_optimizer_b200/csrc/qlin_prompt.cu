@@ -12,6 +12,8 @@
 
 namespace qlin {
 
+constexpr int kMostTokens = 1 << 30;
+
 struct PromptParams {
   qlin_prompt_attention_args a;
   int32_t group;  // query heads per kv head
@@ -789,8 +791,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       }
       tc_fence_before();  // the next unit's weights are announced behind these reads of the accumulator
       // A weight of zero times NaN or infinity is NaN: a value that the row does not see may have got into its sums, so rows that
-      // come out as NaN are computed again from what they do see.
-      uint32_t redo = __ballot_sync(0xffffffffu, row_ok && again);
+      // come out as NaN are computed again from what they do see.  (A NaN or an infinity among the logits that a row sees makes its sum
+      // NaN, and with that every output, rightly.)
+      uint32_t redo = __ballot_sync(0xffffffffu, row_ok && again && l == l);
       __syncwarp();  // the rows are written before they are written again
       while (redo != 0) {
         const int r2 = (warp & 3) * 32 + __ffs(redo) - 1;
@@ -869,6 +872,7 @@ extern "C" int qlin_prompt_attention(const qlin_prompt_attention_args* a, void* 
   if (a->batch == 0 || a->tokens_q == 0 || a->max_q == 0) return QLIN_OK;
   if (a->q == nullptr || a->out == nullptr || a->cu_q == nullptr || a->cu_k == nullptr) return fail(QLIN_ERR_NULL, "qlin_prompt_attention: q, out, cu_q or cu_k is NULL");
   if (a->tokens_k > 0 && (a->k == nullptr || a->v == nullptr)) return fail(QLIN_ERR_NULL, "qlin_prompt_attention: k or v is NULL");
+  if (a->tokens_q > kMostTokens || a->tokens_k > kMostTokens) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: at most 2^30 tokens");
   if (static_cast<int64_t>(a->kv_heads) * a->batch > (1 << 24)) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: too many heads and sequences");
   if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return fail(QLIN_ERR_UNSUPPORTED, "qlin_prompt_attention: scale must be positive and finite");
   const auto pitch = [](int64_t entries, int64_t stride) { return entries > 1 && (stride <= 0 || stride >= (int64_t{1} << 38)); };
@@ -882,6 +886,9 @@ extern "C" int qlin_prompt_attention(const qlin_prompt_attention_args* a, void* 
   p.a = *a;
   p.group = a->q_heads / a->kv_heads;
   p.cl2 = a->scale * 1.4426950408889634f;
+  if (p.a.window > kMostTokens) p.a.window = kMostTokens;  // as far as any sequence reaches, and sums with positions stay in 32 bits
+  if (p.a.sinks > kMostTokens) p.a.sinks = kMostTokens;
+  if (p.a.sinks < 0) p.a.sinks = 0;
   p.tq = kRows / p.group;
   p.units = static_cast<int32_t>((static_cast<int64_t>(a->max_q) + 2 * p.tq - 1) / (2 * p.tq));
   if (a->tokens_k == 0) {  // nothing to see: the tensor maps have no memory to describe

@@ -290,6 +290,25 @@ def test_rows_of_minus_infinity_are_zeros(cuda_dev):
     assert not got[0].any() and got[1, 0].isnan().all() and not got[1, 1].any()
 
 
+def test_windows_and_first_tokens_beyond_every_sequence(cuda_dev):
+    """The largest 32-bit window or number of first tokens is no window, and both attentions refuse a scale that is not positive."""
+    g = torch.Generator().manual_seed(12)
+    q, k, v = (_randn(g, 300, h, 64).to(cuda_dev) for h in (4, 2, 2))
+    cu = torch.tensor([0, 300], dtype=torch.int32, device=cuda_dev)
+    pages = [t.transpose(0, 1)[None].contiguous() for t in (k, v)]
+    table = torch.zeros(1, 1, dtype=torch.int32, device=cuda_dev)
+    prompt = lambda **kw: ops.prompt_attention(q, k, v, cu, cu, 300, **kw)  # noqa: E731
+    token = lambda **kw: ops.paged_attention(q[-1:], *pages, table, cu[1:], **kw)  # noqa: E731
+    big = 2**31 - 1
+    for run in (prompt, token):
+        want = run()
+        assert torch.equal(run(window=big), want) and torch.equal(run(window=big, sinks=big), want)
+        assert torch.allclose(run(window=7, sinks=big).float(), want.float(), atol=2.0**-6)
+        for scale in (0.0, -1.0, math.nan, math.inf):
+            with pytest.raises(RuntimeError, match="scale"):
+                run(scale=scale)
+
+
 def test_large_logits_and_scales(cuda_dev):
     """Logits of several thousand: the running maximum has to be followed upwards and the sums must not overflow."""
     g = torch.Generator().manual_seed(8)
