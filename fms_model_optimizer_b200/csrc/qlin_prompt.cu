@@ -1,6 +1,23 @@
 // qlin_prompt_attention: attention of packed prompts under a causal mask, a sliding window and first tokens that stay visible.
 //
-//   o_i = sum_j w_j v_j / sum_j w_j,   w_j = 2^(x_j - max x),   x_j = q_i.k_j scale log2(e),   j over the keys that i sees
+//   o_i = sum_j w_j v_j / sum_j w_j,   w_j = 2^(x_j - r),   x_j = q_i.k_j scale log2(e),   j over the keys that i sees
+//
+// for any r; r follows the running maximum.  A persistent block has two tiles of 128 rows of one kv head and goes over tiles of 128
+// keys.  A tile's rows are 128 / G queries times the G query heads that share the kv head, so grouped heads share each load and a
+// tile spans few positions, which keeps what the mask throws away small.  S = Q K^T on tcgen05 with both operands in shared memory, one
+// thread for each row of 128 logits in tensor memory, the weights back to tensor memory over their logits in 16 bits, O += P V
+// with the weights as the operand from there.  Tensor memory is full: two S of 128 columns, two O of head_dim.  The tiles take turns, one in the softmax
+// while the other is in the tensor core.
+//
+// What bounds it: that chain.  A turn (two tiles against 128 keys) is 2048 cycles of tensor core and 2048 of exponentials (two
+// tiles x 128 a thread x 8 cycles), and takes about 4200: the exponentials of a tile and its products follow one another, and the
+// third pair of buffers that would let a tile's next logits be made meanwhile does not fit.  Measured (device time): 8 x 2048, 32 + 8 heads
+// of 128 in bf16 280 us, 980 TFLOP/s = 0.60 of the measured rate; 1 x 8191 under a window of 2048 with four first keys 243 us,
+// 990; 5 x up to 333 after 77, 12 heads of 64 in fp16 13 us, four turns behind a cold start.  With exponentials, maxima and masks left
+// out the first two would take 252 and 204: what else is in a turn is loads and stores of tensor memory, conversions and hand-overs.
+// Tried and slower, 8 x 2048 in us at the time: a warp for each tile's products 340 against 290 (both tiles fall into step and wait
+// together), the same with the tensor core handed from one to the other 299, all of a tile's weights in one hand-over 307, logits read
+// twice instead of held in registers 317, half of a tile's weights ahead of its maximum instead of a quarter 304.
 #include <type_traits>
 
 #include <cuda.h>
@@ -129,6 +146,8 @@ constexpr int kPromptThreads = (kSoftmaxWarps + 4) * 32;  // whole warpgroups: r
 // (64,512): a row of 128 logits stays in registers.
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kChunkBytes = 128 * 128;  // 128 rows of 64 elements, 128-byte swizzle
+// The reference may lie this far (in powers of two) below the maximum.  Weights up to 2^8 are as exact in 16 bits as those up to 1;
+// fp16 ones carry a factor of 2^6 on top, so that they stay below 2^14 and lose bits only under 2^-20 of the largest.
 constexpr float kSlack = 8.0f;
 
 struct PromptAux {
@@ -173,7 +192,7 @@ __device__ __forceinline__ void prompt_expect(uint64_t* bar, uint32_t bytes) {
       : "memory");
 }
 // A value that is the same in every lane, in a form that the compiler knows to be: with it in the loops' bounds the products are issued
-// from uniform registers (32 instructions a turn; from ordinary ones the issue alone takes longer than the tensor core).
+// from uniform registers (8 x 2048: 304 us; by a single lane from ordinary ones 377).
 __device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
 // A bounded wait of a whole warp for one barrier, or two, whose loop and answer are uniform too.
 __device__ __forceinline__ bool uniform_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t* other = nullptr, uint32_t other_parity = 0) {
@@ -281,7 +300,7 @@ struct Unit {
   bool second;     // the second tile has rows
   // Tiles of the window, then those of the first keys.  Under a window the tile at its edge comes last of the former: a row that sees few
   // keys of its first tile has a low reference, and the next tile would rewrite its accumulator (1 x 8191 under a window of 2048
-  // with four first keys in front: a rewrite for every 13th tile of a warp, 277 us; @@ so).
+  // with four first keys in front: a rewrite for every 13th tile of a warp, 277 us; 243 so).
   __device__ __forceinline__ int key0(int t) const {
     if (t >= win_tiles) return (t - win_tiles) * kKeys;
     if (win_tile == 0) return t * kKeys;
@@ -754,7 +773,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       tc_fence_after();
       const float scale = l == 0.0f ? 0.0f : 1.0f / l;
       // Rows go through shared memory, 64 outputs at a time, so that eight lanes write the 128 bytes of a row together (a lane for
-      // each row touches 32 lines with every store: 8 x 2048 @@ us).
+      // each row touches 32 lines with every store: 8 x 2048 290 us, 282 so).
       T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(u.seq.q0 + token) * p.a.q_heads + head) * p.a.head_dim;
       const uint64_t out_row = row_ok ? reinterpret_cast<uint64_t>(out) : 0;
       uint8_t* stage = smem + C::OUT_OFFSET + warp * 4096;
@@ -844,6 +863,12 @@ static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
   if (!configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     if (e != cudaSuccess) return fail(QLIN_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    cudaFuncAttributes attr;
+    const cudaError_t f = cudaFuncGetAttributes(&attr, prompt_kernel<T, DP>);
+    if (f != cudaSuccess) return fail(QLIN_ERR_LAUNCH, "cudaFuncGetAttributes: %s", cudaGetErrorString(f));
+    // what the softmax warps ask for must be there, or they would wait for it for good
+    if (attr.numRegs * kPromptThreads < 32 * (kSoftmaxWarps * kSoftmaxRegs + 4 * kOtherRegs))
+      return fail(QLIN_ERR_LAUNCH, "qlin_prompt_attention: built with %d registers a thread, too few for its split", attr.numRegs);
     configured[dev] = true;
   }
   CUtensorMap tq, tk, tv;
