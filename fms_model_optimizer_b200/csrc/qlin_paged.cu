@@ -119,22 +119,6 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
-// A value at this offset in the shared memory of another block of the cluster.
-__device__ __forceinline__ uint32_t in_block(uint32_t offset, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(offset), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float2 ld_cluster_f2(uint32_t offset, uint32_t rank) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_block(offset, rank)) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t offset, uint32_t rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(in_block(offset, rank)) : "memory");
-  return v;
-}
 __device__ __forceinline__ float max_of_rows(float v) {  // over the eight lanes that hold one column
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));

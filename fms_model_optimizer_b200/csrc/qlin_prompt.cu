@@ -149,6 +149,7 @@ constexpr int kChunkBytes = 128 * 128;  // 128 rows of 64 elements, 128-byte swi
 // The reference may lie this far (in powers of two) below the maximum.  Weights up to 2^8 are as exact in 16 bits as those up to 1;
 // fp16 ones carry a factor of 2^6 on top, so that they stay below 2^14 and lose bits only under 2^-20 of the largest.
 constexpr float kSlack = 8.0f;
+constexpr int kSplitTiles = 10;
 
 struct PromptAux {
   uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], p_full[2][2], o_full[2], drain;
@@ -164,6 +165,10 @@ struct PromptCfg {
   static constexpr int KV_OFFSET = 2 * TILE_BYTES;
   static constexpr int OUT_OFFSET = KV_OFFSET + STAGES * TILE_BYTES;  // 32 rows of 64 outputs for each softmax warp
   static constexpr int AUX_OFFSET = OUT_OFFSET + kSoftmaxWarps * 4096;
+  // with a unit split over a cluster: a block's accumulators and (maximum, sum), over the tiles that are no longer needed
+  static constexpr int PART_ML = 2 * kRows * DP * 4;
+  static_assert(PART_ML + 2 * kRows * 8 <= OUT_OFFSET, "the sums fit the tiles' place");
+  static __device__ __forceinline__ uint32_t part_o(int row, int piece) { return static_cast<uint32_t>(row * DP * 4 + ((piece ^ (row & 7)) << 4)); }
   static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(PromptAux));
   static constexpr float SHIFT = std::is_same<T, __half>::value ? 6.0f : 0.0f;
   static constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
@@ -297,22 +302,25 @@ struct Unit {
   int b, kvh, t0;  // sequence, kv head, first query
   int shift;       // position of query 0
   int win_tile, win_tiles, tiles;
+  int from, every; // of the unit's tiles, this block has every `every`-th one from `from` on
   bool second;     // the second tile has rows
   // Tiles of the window, then those of the first keys.  Under a window the tile at its edge comes last of the former: a row that sees few
   // keys of its first tile has a low reference, and the next tile would rewrite its accumulator (1 x 8191 under a window of 2048
   // with four first keys in front: a rewrite for every 13th tile of a warp, 277 us; 243 so).
-  __device__ __forceinline__ int key0(int t) const {
+  __device__ __forceinline__ int key0(int n) const {
+    const int t = n * every + from;
     if (t >= win_tiles) return (t - win_tiles) * kKeys;
     if (win_tile == 0) return t * kKeys;
     return (win_tile + (t + 1 == win_tiles ? 0 : t + 1)) * kKeys;
   }
 };
 // The units of a block, every gridDim.x-th one of the list that begins with the last queries of every sequence and head, which see
-// the most keys.  `busy`: units without keys are passed over.
+// the most keys.  `busy`: units without keys are passed over.  SPLIT: one unit for the two blocks of a cluster, which share out its keys.
+template <bool SPLIT>
 struct Units {
   uint32_t id, step, total;
   __device__ __forceinline__ explicit Units(const PromptParams& p)
-      : id(blockIdx.x), step(gridDim.x), total(static_cast<uint32_t>(p.units) * p.a.kv_heads * p.a.batch) {}
+      : id(SPLIT ? blockIdx.x / 2 : blockIdx.x), step(SPLIT ? 0x7fffffff : gridDim.x), total(static_cast<uint32_t>(p.units) * p.a.kv_heads * p.a.batch) {}
   __device__ __forceinline__ bool next(const PromptParams& p, bool busy, Unit& u) {
     const uint32_t lanes = p.a.kv_heads * p.a.batch;
 #pragma unroll 1
@@ -329,6 +337,9 @@ struct Units {
       u.win_tile = p.a.window > 0 ? min(max(lo - p.a.window + 1, 0) / kKeys, end) : 0;
       u.win_tiles = end - u.win_tile;
       u.tiles = u.win_tiles + min((p.a.sinks + kKeys - 1) / kKeys, u.win_tile);
+      u.from = SPLIT ? static_cast<int>(blockIdx.x % 2) : 0;
+      u.every = SPLIT ? 2 : 1;
+      if constexpr (SPLIT) u.tiles = (u.tiles - u.from + 1) / 2;
       u.second = u.t0 + p.tq < u.seq.n;
       if (busy && u.tiles == 0) continue;
       id += step;
@@ -545,7 +556,9 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, f
   l += a + b;
 }
 
-template <typename T, int DP>
+// SPLIT: where units are few, the two blocks of a cluster share one, every second tile of its keys each, and the first joins their
+// sums over distributed shared memory.
+template <typename T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(kPromptThreads, 1)
 prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
               const __grid_constant__ PromptParams p) {
@@ -601,7 +614,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       uint32_t s = 0, ph = 1, uses[2] = {0, 0};
       int issued = 0;
       Unit u;
-      for (Units walk(p); ok && walk.next(p, true, u);) {
+      for (Units<SPLIT> walk(p); ok && walk.next(p, true, u);) {
         const auto load_q = [&](int i) {
           ok = uniform_wait(&aux->q_empty[i], (uses[i] & 1) ^ 1, abort_flag);
           if (!ok) return;
@@ -641,7 +654,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     } else if (warp == kMmaWarp) {
       // ------------------------------------------------------------------ products
       // The tiles of queries take turns, so that one is in the softmax while the other is in the tensor core.
-      const uint32_t base = smem_u32(smem) >> 4, d0 = uniform(tmem);
+      // in a cluster the address also names the block, which is no part of a descriptor
+      const uint32_t base = (smem_u32(smem) & 0x3FFFFu) >> 4, d0 = uniform(tmem);
       uint32_t s = 0, ph = 0, q_ph = 0, p_ph = 0;  // bit i of the last two: tile i
       const auto step = [&]() {
         if (++s == C::STAGES) {
@@ -677,7 +691,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         p_ph ^= 1u << i;
       };
       Unit unit;
-      Units walk(p);
+      Units<SPLIT> walk(p);
       const auto advance = [&](int& tiles, bool& second) {
         const bool have = uniform(walk.next(p, true, unit)) != 0;
         tiles = uniform(have ? unit.tiles : 0);
@@ -744,33 +758,18 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + i * kKeys, o_addr = tmem + lanes + 2 * kKeys + i * DP;
     uint32_t s_uses = 0, o_uses = 0;
-    Unit u;
-    for (Units walk(p); ok && walk.next(p, false, u);) {
-      if (i == 1 && !u.second) continue;
+    // The outputs of a tile of queries, from its accumulator and sum (with SPLIT, and those of the cluster's other block).
+    const auto finish = [&](const Unit& u, float m, float l) {
       const int token = u.t0 + i * p.tq + row_token, head = u.kvh * p.group + row_head;
       const bool row_ok = row_token < p.tq && token < u.seq.n;
-      const int pos = token + u.shift;
-      const int tile_lo = u.t0 + i * p.tq + u.shift, tile_hi = tile_lo + p.tq - 1;  // positions of this tile of queries
-      float m = -INFINITY, l = 0.0f;
-      for (int t = 0; t < u.tiles && ok; ++t) {
-        ok = uniform_wait(&aux->s_full[i], s_uses & 1, abort_flag);
-        if (!ok) break;
-        ++s_uses;
-        tc_fence_after();
-        const int k0 = u.key0(t);
-        const bool full = k0 + kKeys - 1 <= tile_lo && (p.a.window <= 0 || k0 > tile_hi - p.a.window || k0 + kKeys <= p.a.sinks);
-        if (full) {
-          softmax_tile<T, DP, false>(s_addr, o_addr, p.cl2, 0, 0, 0, t == 0, row_ok, aux->p_full[i], m, l);
-        } else {
-          softmax_tile<T, DP, true>(s_addr, o_addr, p.cl2, pos - k0, p.a.window > 0 ? pos - p.a.window - k0 : -1, p.a.sinks - k0, t == 0, row_ok, aux->p_full[i], m, l);
-        }
+      float own = 1.0f, other = 0.0f;  // factors of the two blocks' sums
+      if constexpr (SPLIT) {
+        const float2 ml = ld_cluster_f2(smem_u32(smem) + C::PART_ML + (i * kRows + r) * 8, 1);
+        const float top = max3_nan(m, ml.x, ml.x);
+        own = m == top ? 1.0f : exp2f(m - top);
+        other = ml.x == top ? 1.0f : exp2f(ml.x - top);
+        l = l * own + ml.y * other;
       }
-      if (ok && u.tiles > 0) {
-        ok = uniform_wait(&aux->o_full[i], o_uses & 1, abort_flag);
-        ++o_uses;
-      }
-      if (!ok) break;
-      tc_fence_after();
       const float scale = l == 0.0f ? 0.0f : 1.0f / l;
       // Rows go through shared memory, 64 outputs at a time, so that eight lanes write the 128 bytes of a row together (a lane for
       // each row touches 32 lines with every store: 8 x 2048 290 us, 282 so).
@@ -786,6 +785,16 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0u;
+        }
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 v = ld_cluster_f4(smem_u32(smem) + C::part_o(i * kRows + r, 8 * c + j / 4), 1);
+            o[j] = __float_as_uint(__uint_as_float(o[j]) * own + v.x * other);
+            o[j + 1] = __float_as_uint(__uint_as_float(o[j + 1]) * own + v.y * other);
+            o[j + 2] = __float_as_uint(__uint_as_float(o[j + 2]) * own + v.z * other);
+            o[j + 3] = __float_as_uint(__uint_as_float(o[j + 3]) * own + v.w * other);
+          }
         }
 #pragma unroll
         for (int j = 0; j < 32; ++j) again |= __uint_as_float(o[j]) != __uint_as_float(o[j]);
@@ -819,12 +828,74 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         redo &= redo - 1;
         attend_row<T>(p, u.seq, u.t0 + i * p.tq + r2 / p.group, u.kvh * p.group + r2 % p.group);
       }
+    };
+    Unit u;
+    bool mine = false;
+    float m, l;
+    for (Units<SPLIT> walk(p); ok && walk.next(p, false, u);) {
+      if (i == 1 && !u.second) continue;
+      mine = true;
+      const int token = u.t0 + i * p.tq + row_token;
+      const bool row_ok = row_token < p.tq && token < u.seq.n;
+      const int pos = token + u.shift;
+      const int tile_lo = u.t0 + i * p.tq + u.shift, tile_hi = tile_lo + p.tq - 1;  // positions of this tile of queries
+      m = -INFINITY;
+      l = 0.0f;
+      for (int t = 0; t < u.tiles && ok; ++t) {
+        ok = uniform_wait(&aux->s_full[i], s_uses & 1, abort_flag);
+        if (!ok) break;
+        ++s_uses;
+        tc_fence_after();
+        const int k0 = u.key0(t);
+        const bool full = k0 + kKeys - 1 <= tile_lo && (p.a.window <= 0 || k0 > tile_hi - p.a.window || k0 + kKeys <= p.a.sinks);
+        if (full) {
+          softmax_tile<T, DP, false>(s_addr, o_addr, p.cl2, 0, 0, 0, t == 0, row_ok, aux->p_full[i], m, l);
+        } else {
+          softmax_tile<T, DP, true>(s_addr, o_addr, p.cl2, pos - k0, p.a.window > 0 ? pos - p.a.window - k0 : -1, p.a.sinks - k0, t == 0, row_ok, aux->p_full[i], m, l);
+        }
+      }
+      if (ok && u.tiles > 0) {
+        ok = uniform_wait(&aux->o_full[i], o_uses & 1, abort_flag);
+        ++o_uses;
+      }
+      if (!ok) break;
+      tc_fence_after();
+      if constexpr (!SPLIT) {
+        finish(u, m, l);
+      } else {
+        // the other tile's products may still read what the sums go over
+        if (u.second && u.tiles > 0) ok = uniform_wait(&aux->o_full[1 - i], 0, abort_flag);
+        if (!ok) break;
+        if (u.from > 0) {
+#pragma unroll 1
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t o[16] = {};
+            if (u.tiles > 0) {
+              tmem_issue16(o_addr + 16 * c, o);
+              tmem_wait16(o);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(smem + C::part_o(i * kRows + r, 4 * c + j / 4)) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+          *reinterpret_cast<float2*>(smem + C::PART_ML + (i * kRows + r) * 8) = make_float2(m, l);
+        }
+      }
     }
     if (!ok && lane == 0) {
       timed_out = !*abort_flag;
       *abort_flag = 1;
     }
     __syncwarp();
+    if constexpr (SPLIT) {
+      cluster_arrive_wait();
+      if (mine && ok && u.from == 0) finish(u, m, l);
+      __syncwarp();
+    }
+  }
+  if constexpr (SPLIT) {
+    __syncwarp();  // the barriers of a cluster are taken by whole warps
+    if (warp >= kSoftmaxWarps) cluster_arrive_wait();
+    cluster_arrive_wait();  // nobody leaves while its sums are read
   }
   if (timed_out && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_TIMEOUT));
   tc_fence_before();
@@ -853,24 +924,46 @@ static int head_map(CUtensorMap* tm, const void* base, int dtype, int64_t tokens
   return QLIN_OK;
 }
 
-template <typename T, int DP>
-static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
+template <typename T, int DP, bool SPLIT>
+static int launch_prompt_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PromptParams& p, unsigned grid, cudaStream_t stream) {
   using C = PromptCfg<T, DP>;
+  const auto kernel = prompt_kernel<T, DP, SPLIT>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(QLIN_ERR_DEVICE, "device ordinal %d out of range", dev);
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     if (e != cudaSuccess) return fail(QLIN_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     cudaFuncAttributes attr;
-    const cudaError_t f = cudaFuncGetAttributes(&attr, prompt_kernel<T, DP>);
+    const cudaError_t f = cudaFuncGetAttributes(&attr, kernel);
     if (f != cudaSuccess) return fail(QLIN_ERR_LAUNCH, "cudaFuncGetAttributes: %s", cudaGetErrorString(f));
     // what the softmax warps ask for must be there, or they would wait for it for good
     if (attr.numRegs * kPromptThreads < 32 * (kSoftmaxWarps * kSoftmaxRegs + 4 * kOtherRegs))
       return fail(QLIN_ERR_LAUNCH, "qlin_prompt_attention: built with %d registers a thread, too few for its split", attr.numRegs);
     configured[dev] = true;
   }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(kPromptThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = SPLIT ? 2 : 1;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = SPLIT ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tq, tk, tv, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(QLIN_ERR_LAUNCH, "qlin_prompt_attention: %s", cudaGetErrorString(e));
+  }
+  return QLIN_OK;
+}
+
+template <typename T, int DP>
+static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
   CUtensorMap tq, tk, tv;
   int rc = head_map(&tq, p.a.q, p.a.dtype, p.a.tokens_q, p.a.q_heads, p.a.head_dim, p.a.q_token, p.a.q_head, p.tq, p.group);
   if (rc == QLIN_OK) rc = head_map(&tk, p.a.k, p.a.dtype, p.a.tokens_k, p.a.kv_heads, p.a.head_dim, p.a.k_token, p.a.k_head, kKeys, 1);
@@ -878,10 +971,15 @@ static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
   if (rc != QLIN_OK) return rc;
   const int64_t blocks = static_cast<int64_t>(p.units) * p.a.kv_heads * p.a.batch;
   if (blocks > 0x7fffffff) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: too many queries, heads and sequences");
-  const unsigned grid = static_cast<unsigned>(blocks < sm_count() ? blocks : sm_count());
-  prompt_kernel<T, DP><<<grid, kPromptThreads, C::SMEM_BYTES, stream>>>(tq, tk, tv, p);
-  QLIN_CHECK_LAUNCH("qlin_prompt_attention");
-  return QLIN_OK;
+  // Units that leave half of the SMs idle are split over two blocks where the longest has kSplitTiles tiles of keys (as far as the host
+  // knows: the earlier keys are taken as evenly spread).  Device time without and with: 1200 queries of 12 heads of 64 (10 tiles) 23.7 and 19.7 us,
+  // 2000 of 8 + 1 heads of 96 35.7 and 30.4, 16 after 2900 of 32 + 8 heads of 128 41.0 and 26.3; 40 after 900 (8 tiles) 20.8 and 22.4.
+  // Four blocks lose more in the join than they save (64 after 2900 of 8 + 2 heads 39 in two, 59 in four).
+  int64_t keys = p.a.max_q + (p.a.tokens_k > p.a.tokens_q ? (p.a.tokens_k - p.a.tokens_q) / p.a.batch : 0);
+  const int64_t seen = static_cast<int64_t>(p.a.window) + p.a.sinks + 2 * p.tq;
+  if (p.a.window > 0 && keys > seen) keys = seen;
+  if (2 * blocks <= sm_count() && (keys + kKeys - 1) / kKeys >= kSplitTiles) return launch_prompt_as<T, DP, true>(tq, tk, tv, p, static_cast<unsigned>(2 * blocks), stream);
+  return launch_prompt_as<T, DP, false>(tq, tk, tv, p, static_cast<unsigned>(blocks < sm_count() ? blocks : sm_count()), stream);
 }
 
 }  // namespace qlin

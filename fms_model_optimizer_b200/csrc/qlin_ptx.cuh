@@ -397,6 +397,22 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
   return v;
 }
+// A value at this offset in the shared memory of another block of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t offset, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(offset), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t offset, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_block(offset, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t offset, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(in_block(offset, rank)) : "memory");
+  return v;
+}
 // Release at CTA scope, the default: what the arrival hands over are TMEM reads, ordered by tcgen05.fence.  With a cluster-scope
 // release it waited for every store of the warp:
 // 4096 x 768 x 3072 with fp32 output 21.5 -> 18.7 us, the deployed Linear around it 26.7 -> 24.1.

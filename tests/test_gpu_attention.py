@@ -140,7 +140,9 @@ def _check_rows(got, q, k, v, pos, window, sinks, scale, dtype, what, weights=No
 @pytest.mark.parametrize("lens,hq,hkv,dim,window,sinks", [
     ([(1, 1)], 1, 1, 64, 0, 0), ([(2, 2), (129, 129), (1, 1), (0, 0), (64, 64)], 8, 2, 128, 0, 0), ([(300, 300), (5, 300)], 5, 1, 96, 0, 0),
     ([(260, 400), (7, 7)], 4, 4, 64, 100, 3), ([(513, 513)], 32, 8, 128, 128, 130), ([(200, 200)], 2, 1, 40, 1, 0), ([(40, 7), (3, 0)], 4, 2, 128, 0, 0),
-    ([(150, 500)], 12, 12, 64, 33, 1), ([(31, 31), (90, 90)], 24, 1, 128, 0, 0), ([(70, 70)], 128, 1, 64, 20, 5), ([(257, 1025)], 6, 2, 8, 0, 0)])  # fmt: skip
+    ([(150, 500)], 12, 12, 64, 33, 1), ([(31, 31), (90, 90)], 24, 1, 128, 0, 0), ([(70, 70)], 128, 1, 64, 20, 5), ([(257, 1025)], 6, 2, 8, 0, 0),
+    ([(400, 400), (390, 500)] * 4, 12, 12, 64, 0, 0), ([(280, 600), (3, 600), (290, 290)] * 3, 16, 16, 128, 130, 5), ([(40, 3000)], 8, 1, 128, 0, 0),
+    ([(700, 700), (0, 5), (1, 900)], 8, 1, 64, 0, 0), ([(300, 2500)], 4, 1, 96, 1000, 200)])  # fmt: skip
 def test_prompt_attention(cuda_dev, dtype, lens, hq, hkv, dim, window, sinks):
     g = torch.Generator().manual_seed(dim + hq)
     nq, nk = sum(n for n, _ in lens), sum(m for _, m in lens)
