@@ -3,7 +3,7 @@
 
 Every layer has its own pool ``[pages, kv heads, page size, head_dim]`` of keys and of values; all layers share one page table
 ``[batch, pages of a sequence]`` and one length for each sequence.  Pages are handed out as sequences grow and come back with
-``release``.  Tables, lengths, positions and slots live on the device; the host keeps a copy of the lengths to hand out pages by, so
+``release``; a released place stays out of the steps until ``prompts`` fills it again.  Tables, lengths, positions and slots live on the device; the host keeps a copy of the lengths to hand out pages by, so
 that a step needs no synchronisation.  No counterpart in the reference, which leaves generation to a serving stack.
 """
 
@@ -20,10 +20,10 @@ class Step:
     """The tokens of one forward pass, packed sequence behind sequence."""
 
     positions: torch.Tensor  # int32 [tokens]
-    slots: torch.Tensor  # int64 [tokens]
-    last: torch.Tensor  # int64 [batch]: row of every sequence's last token
-    single: bool  # one new token for every sequence
-    cu: Optional[torch.Tensor] = None  # int32 [batch + 1], prompts only
+    slots: torch.Tensor  # int64 [tokens]; -1: the row of a sequence that does not run, which is not written
+    last: torch.Tensor  # int64 [sequences]: row of every sequence's last token
+    single: bool  # a row for every sequence of the cache, one new token for those that run
+    cu: Optional[torch.Tensor] = None  # int32 [sequences + 1], prompts only
     max_q: int = 1
 
 
@@ -48,6 +48,8 @@ class PagedKVCache:
         self.table = torch.zeros(batch, per, dtype=torch.int32, device=dev)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.host_lens = [0] * batch
+        self._runs = [True] * batch
+        self._runs_dev = torch.ones(batch, dtype=torch.int32, device=dev)
         self._owned: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(pages - 1, -1, -1))
 
@@ -70,39 +72,49 @@ class PagedKVCache:
                 self.table[b, first : first + n] = torch.tensor(new, dtype=torch.int32).to(self.dev)
 
     def release(self, b: int) -> None:
-        """Sequence ``b`` is over: its pages go back to the pool and its length to 0."""
+        """Sequence ``b`` is over: its pages go back to the pool, its length to 0, and ``token`` passes it over."""
         self._free += reversed(self._owned[b])
         self._owned[b] = []
         self.host_lens[b] = 0
         self.lens[b] = 0
+        self._runs[b] = False
+        self._runs_dev[b] = 0
 
     def _slots(self, which: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         page = self.table[which, positions // self.page_size].long()
         return page * self.page_size + positions % self.page_size
 
-    def prompts(self, lengths: Sequence[int]) -> Step:
-        """Room for the prompts of all (empty) sequences, ``lengths[b]`` >= 1 tokens each."""
-        if len(lengths) != self.batch or min(lengths) < 1:
+    def prompts(self, lengths: Sequence[int], which: Optional[Sequence[int]] = None) -> Step:
+        """Room for prompts of ``lengths[i]`` >= 1 tokens in the empty sequences ``which[i]``, by default in all of them.  From then on
+        ``token`` goes on with these and with those that have tokens already; other empty ones wait for a prompt of their own."""
+        which = list(range(self.batch)) if which is None else [int(b) for b in which]
+        if len(lengths) != len(which) or not which or min(lengths) < 1:
             raise RuntimeError("one prompt of at least one token for every sequence is wanted")
-        if any(self.host_lens):
+        if len(set(which)) != len(which) or min(which) < 0 or max(which) >= self.batch:
+            raise RuntimeError(f"prompts go to different sequences of the {self.batch}")
+        if any(self.host_lens[b] for b in which):
             raise RuntimeError("prompts start empty sequences: release them first")
-        self.reserve(lengths)
-        n = torch.tensor(lengths)
-        cu = torch.zeros(self.batch + 1, dtype=torch.int64)
+        new = dict(zip(which, (int(n) for n in lengths)))
+        self.reserve([new.get(b, 0) for b in range(self.batch)])
+        n, rows = torch.tensor(lengths), torch.tensor(which)
+        cu = torch.zeros(len(which) + 1, dtype=torch.int64)
         cu[1:] = n.cumsum(0)
-        which = torch.repeat_interleave(torch.arange(self.batch), n)
-        positions = (torch.arange(int(cu[-1])) - cu[which]).to(self.dev)
-        self.host_lens = [int(x) for x in lengths]
-        self.lens.copy_(n.to(torch.int32))
-        slots = self._slots(which.to(self.dev), positions)
-        return Step(positions.to(torch.int32), slots, (cu[1:] - 1).to(self.dev), False, cu.to(torch.int32).to(self.dev), max(self.host_lens))
+        of = torch.repeat_interleave(torch.arange(len(which)), n)
+        positions = (torch.arange(int(cu[-1])) - cu[of]).to(self.dev)
+        self.host_lens = [new.get(b, have) for b, have in enumerate(self.host_lens)]
+        self._runs = [have > 0 for have in self.host_lens]
+        self.lens.copy_(torch.tensor(self.host_lens, dtype=torch.int32))
+        self._runs_dev.copy_(torch.tensor(self._runs, dtype=torch.int32))
+        slots = self._slots(rows[of].to(self.dev), positions)
+        return Step(positions.to(torch.int32), slots, (cu[1:] - 1).to(self.dev), False, cu.to(torch.int32).to(self.dev), int(n.max()))
 
     def token(self) -> Step:
-        """Room for one more token of every sequence."""
-        self.reserve([n + 1 for n in self.host_lens])
+        """Room for one more token of every sequence that runs."""
+        grown = [n + 1 if runs else n for n, runs in zip(self.host_lens, self._runs)]
+        self.reserve(grown)
         positions = self.lens.clone()
         every = torch.arange(self.batch, device=self.dev)
-        slots = self._slots(every, positions.long())
-        self.lens += 1
-        self.host_lens = [n + 1 for n in self.host_lens]
+        slots = torch.where(self._runs_dev > 0, self._slots(every, positions.long()), -1)
+        self.lens += self._runs_dev
+        self.host_lens = grown
         return Step(positions, slots, every, True)

@@ -1,0 +1,70 @@
+"""The paged cache in a running batch: the kernels on what ``PagedKVCache`` hands out, against every sequence's own history."""
+
+import pytest
+import torch
+
+from fms_model_optimizer_b200 import ops
+from fms_model_optimizer_b200.kvcache import PagedKVCache
+from oracle import attention as OA
+
+pytestmark = pytest.mark.gpu
+
+HQ, HKV, DIM = 4, 2, 64
+
+
+class _Batch:
+    """A cache and, on the host, the keys and values of each of its sequences."""
+
+    def __init__(self, dev, batch, pages):
+        self.dev, self.g = dev, torch.Generator().manual_seed(21)
+        self.cache = PagedKVCache(1, batch, 64, HKV, DIM, dev, page_size=8, pages=pages)
+        self.k, self.v = ([torch.zeros(0, HKV, DIM, dtype=torch.bfloat16) for _ in range(batch)] for _ in range(2))
+        self.cos, self.sin = torch.ones(64, DIM // 2, device=dev), torch.zeros(64, DIM // 2, device=dev)  # keys reach the cache as they are
+
+    def write(self, step, of):
+        """Random queries, keys and values into the step's slots; ``of[t]``: the sequence of row t, None where it does not run."""
+        q, k, v = (torch.randn(len(of), h, DIM, generator=self.g).bfloat16() for h in (HQ, HKV, HKV))
+        for t, b in enumerate(of):
+            if b is not None:
+                self.k[b], self.v[b] = torch.cat([self.k[b], k[t : t + 1]]), torch.cat([self.v[b], v[t : t + 1]])
+        ops.qk_norm_rope(*(x.to(self.dev) for x in (q, k)), self.cos, self.sin, step.positions, v=v.to(self.dev), slots=step.slots, want_k=False, **self.cache.layer(0))
+        return q
+
+    def token(self):
+        q = self.write(self.cache.token(), [b if self.k[b].shape[0] else None for b in range(self.cache.batch)])
+        got = ops.paged_attention(q.to(self.dev), block_table=self.cache.table, lens=self.cache.lens, **self.cache.layer(0)).cpu()
+        ops.check_status(self.dev)
+        for b in range(self.cache.batch):
+            for h in range(HKV):
+                heads = slice(h * HQ // HKV, (h + 1) * HQ // HKV)
+                # weights rounded to 16 bits, then the output; logits off by a few fp32 roundings
+                want, weighted, size = OA.attend(q[b, heads], self.k[b][:, h], self.v[b][:, h], self.k[b].shape[0] - 1, 0, 0, DIM**-0.5)
+                tol = (2 * 2.0**-8 + 2 * (DIM + 16) * 2.0**-23 * size[:, None] + 2.0**-20) * weighted + 1e-30
+                assert bool(((got[b, heads].double() - want).abs() <= tol).all()), (b, h)
+
+    def prompts(self, lengths, which):
+        self.write(self.cache.prompts(lengths, which), [b for b, n in zip(which, lengths) for _ in range(n)])
+
+    def release(self, b):
+        self.cache.release(b)
+        self.k[b], self.v[b] = self.k[b][:0], self.v[b][:0]
+
+
+def test_sequences_end_and_others_take_their_place(cuda_dev):
+    batch = _Batch(cuda_dev, 3, 9)
+    batch.prompts([5, 17, 1], [0, 1, 2])
+    for _ in range(4):
+        batch.token()
+    batch.release(1)
+    for _ in range(3):
+        batch.token()  # the released row gives zeros
+    batch.prompts([20], [1])
+    for _ in range(5):
+        batch.token()
+    batch.release(0)
+    batch.release(2)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        batch.cache.prompts([9, 30], [2, 0])  # four pages are held, six would be wanted
+    batch.prompts([9, 12], [2, 0])
+    for _ in range(3):
+        batch.token()
