@@ -3,8 +3,9 @@
 
 Every layer has its own pool ``[pages, kv heads, page size, head_dim]`` of keys and of values; all layers share one page table
 ``[batch, pages of a sequence]`` and one length for each sequence.  Pages are handed out as sequences grow and come back with
-``release``; a released place stays out of the steps until ``prompts`` fills it again.  Tables, lengths, positions and slots live on the device; the host keeps a copy of the lengths to hand out pages by, so
-that a step needs no synchronisation.  No counterpart in the reference, which leaves generation to a serving stack.
+``release``; a released place stays out of the steps until ``prompts`` fills it again.  Tables, lengths, positions and slots live on
+the device; the host keeps a copy of the lengths to hand out pages by, and what it sends goes through pinned memory, so that a step
+waits for nothing.  No counterpart in the reference, which leaves generation to a serving stack.
 """
 
 from __future__ import annotations
@@ -44,7 +45,7 @@ class PagedKVCache:
         f8 = dtype == torch.float8_e4m3fn
         self.k_scale = [torch.ones(kv_heads, device=dev) for _ in range(layers)] if f8 else [None] * layers
         self.v_scale = [torch.ones(kv_heads, device=dev) for _ in range(layers)] if f8 else [None] * layers
-        self.dev, self.batch, self.max_len, self.page_size = dev, batch, max_len, page_size
+        self.dev, self.batch, self.max_len, self.page_size = torch.device(dev), batch, max_len, page_size
         self.table = torch.zeros(batch, per, dtype=torch.int32, device=dev)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.host_lens = [0] * batch
@@ -64,21 +65,33 @@ class PagedKVCache:
             raise RuntimeError(f"a sequence of {max(lengths)} tokens does not fit a cache of {self.max_len}")
         if sum(need) > len(self._free):
             raise RuntimeError(f"the cache is out of pages: {sum(need)} wanted, {len(self._free)} free")
+        rows, columns, pages = [], [], []
         for b, n in enumerate(need):
-            if n:
-                new = [self._free.pop() for _ in range(n)]
-                first = len(self._owned[b])
-                self._owned[b] += new
-                self.table[b, first : first + n] = torch.tensor(new, dtype=torch.int32).to(self.dev)
+            rows += [b] * n
+            columns += range(len(self._owned[b]), len(self._owned[b]) + n)
+            self._owned[b] += [self._free.pop() for _ in range(n)]
+            pages += self._owned[b][len(self._owned[b]) - n :]
+        if rows:
+            rows, columns, pages = self._send(rows, columns, pages)
+            self.table[rows, columns] = pages.to(torch.int32)
+
+    def _send(self, *parts) -> List[torch.Tensor]:
+        """Integers to the device as int64 tensors, in one copy that the host does not wait for.  PyTorch keeps the pinned memory until
+        the copy has run."""
+        parts = [torch.as_tensor(p, dtype=torch.int64) for p in parts]
+        whole = torch.cat(parts)
+        if self.dev.type == "cuda":
+            whole = whole.pin_memory().to(self.dev, non_blocking=True)
+        return list(whole.split([p.numel() for p in parts]))
 
     def release(self, b: int) -> None:
         """Sequence ``b`` is over: its pages go back to the pool, its length to 0, and ``token`` passes it over."""
         self._free += reversed(self._owned[b])
         self._owned[b] = []
         self.host_lens[b] = 0
-        self.lens[b] = 0
+        self.lens[b].zero_()
         self._runs[b] = False
-        self._runs_dev[b] = 0
+        self._runs_dev[b].zero_()
 
     def _slots(self, which: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         page = self.table[which, positions // self.page_size].long()
@@ -100,13 +113,12 @@ class PagedKVCache:
         cu = torch.zeros(len(which) + 1, dtype=torch.int64)
         cu[1:] = n.cumsum(0)
         of = torch.repeat_interleave(torch.arange(len(which)), n)
-        positions = (torch.arange(int(cu[-1])) - cu[of]).to(self.dev)
         self.host_lens = [new.get(b, have) for b, have in enumerate(self.host_lens)]
         self._runs = [have > 0 for have in self.host_lens]
-        self.lens.copy_(torch.tensor(self.host_lens, dtype=torch.int32))
-        self._runs_dev.copy_(torch.tensor(self._runs, dtype=torch.int32))
-        slots = self._slots(rows[of].to(self.dev), positions)
-        return Step(positions.to(torch.int32), slots, (cu[1:] - 1).to(self.dev), False, cu.to(torch.int32).to(self.dev), int(n.max()))
+        positions, of, last, cu, lens, runs = self._send(torch.arange(int(cu[-1])) - cu[of], rows[of], cu[1:] - 1, cu, self.host_lens, self._runs)
+        self.lens.copy_(lens)
+        self._runs_dev.copy_(runs)
+        return Step(positions.to(torch.int32), self._slots(of, positions), last, False, cu.to(torch.int32), int(n.max()))
 
     def token(self) -> Step:
         """Room for one more token of every sequence that runs."""

@@ -68,3 +68,38 @@ def test_sequences_end_and_others_take_their_place(cuda_dev):
     batch.prompts([9, 12], [2, 0])
     for _ in range(3):
         batch.token()
+
+
+def test_a_step_waits_for_nothing(cuda_dev):
+    """Handing out pages, prompts and releases included, never blocks the host on the device's work."""
+    cache = PagedKVCache(1, 3, 64, HKV, DIM, cuda_dev, page_size=4)
+    cache.token()  # a first use of each operation may load its code
+    torch.cuda.synchronize()
+    for b in range(3):
+        cache.release(b)
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        cache.prompts([3, 9, 4])
+        for _ in range(6):  # a page starts in most of the steps, in two sequences at once in some
+            step = cache.token()
+        cache.release(1)
+        cache.prompts([6], [1])
+        cache.token()
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    assert cache.lens.tolist() == cache.host_lens == [10, 7, 11] and step.positions.tolist() == [8, 14, 9]
+    for b, n in enumerate(cache.host_lens):
+        assert cache.table[b, : -(-n // 4)].tolist() == cache._owned[b][: -(-n // 4)]
+
+
+def test_what_is_sent_without_waiting_is_not_overwritten(cuda_dev):
+    """Steps queued behind a long kernel: each one's pages and lengths arrive as they were when it was made."""
+    cache = PagedKVCache(1, 4, 256, HKV, DIM, cuda_dev, page_size=1)
+    cache.prompts([1, 2, 3, 4])
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    steps = [cache.token() for _ in range(100)]
+    for i, step in enumerate(steps):
+        assert step.positions.tolist() == [1 + i, 2 + i, 3 + i, 4 + i]
+        assert step.slots.tolist() == [cache._owned[b][1 + b + i] for b in range(4)]
