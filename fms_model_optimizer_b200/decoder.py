@@ -94,12 +94,29 @@ def synth_w8a8(n, k, seed, dev, dtype=torch.bfloat16):
     return w8a8_from_float(synth_weight(n, k, seed, dev, dtype), synth_act_scale(k, seed, dev, dtype))
 
 
+def has_own_attention(cfg) -> bool:
+    """Per-head norms or a window: attention runs on this package's kernels instead of the library's."""
+    return bool(cfg.get("qk_norm", False) or cfg.get("window", 0))
+
+
+def attention_mask(cfg) -> dict:
+    return dict(window=cfg.get("window", 0), sinks=cfg.get("sinks", 0))
+
+
+def synth_head_norms(cfg, layer, dev):
+    """Weights of the per-head norms of a layer's queries and keys, (None, None) without ``qk_norm``."""
+    if not cfg.get("qk_norm", False):
+        return None, None
+    g = torch.Generator(device=dev).manual_seed(1000 * layer + 100)
+    return tuple((1 + 0.1 * torch.randn(cfg["head_dim"], generator=g, device=dev)).bfloat16() for _ in range(2))
+
+
 @torch.no_grad()
 def calibrate_act_scales(cfg, dev, ids, layers=None):
     """The SmoothQuant calibration pass for the decoder: one forward of the float (bf16) model on ``ids`` [batch, seq] with
     the per-input-channel absolute maxima of every Linear's input recorded on the device (``ops.col_absmax``, the
     statistic of fms_mo/quant/ptq.py:2586-2596).  The float weights are the seeded ones the quantized decoder is built
-    from; they are generated layer by layer and dropped again.  Returns ``{(layer, name): fp32 [in_features]}``."""
+    from; they are generated layer by layer and dropped again.  ``qk_norm``, ``window`` and ``sinks`` are followed.  Returns ``{(layer, name): fp32 [in_features]}``."""
     B, S = ids.shape
     H, hd = cfg["hidden"], cfg["head_dim"]
     nl = layers if layers is not None else cfg["layers"]
@@ -110,6 +127,8 @@ def calibrate_act_scales(cfg, dev, ids, layers=None):
     cos, sin = ang.cos().contiguous(), ang.sin().contiguous()
     ones = torch.ones(H, device=dev, dtype=torch.bfloat16)
     x = F.embedding(ids, embed).view(B * S, H)
+    positions = torch.arange(S, dtype=torch.int32, device=dev).repeat(B)
+    cu = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=dev)
     scales = {}
     names = list(linear_shapes(cfg).items())
     for li in range(nl):
@@ -117,12 +136,17 @@ def calibrate_act_scales(cfg, dev, ids, layers=None):
         h = F.rms_norm(x, (H,), ones, 1e-5)
         for name in ("q", "k", "v"):
             scales[(li, name)] = ops.col_absmax(h)
-        q = ops.rope_(F.linear(h, w["q"]).view(B * S, cfg["q_heads"], hd), cos, sin, S)
-        k = ops.rope_(F.linear(h, w["k"]).view(B * S, cfg["kv_heads"], hd), cos, sin, S)
+        q, k = F.linear(h, w["q"]).view(B * S, cfg["q_heads"], hd), F.linear(h, w["k"]).view(B * S, cfg["kv_heads"], hd)
         v = F.linear(h, w["v"])
-        a = F.scaled_dot_product_attention(q.view(B, S, -1, hd).transpose(1, 2), k.view(B, S, -1, hd).transpose(1, 2),
-                                           v.view(B, S, -1, hd).transpose(1, 2), is_causal=True, enable_gqa=True)  # fmt: skip
-        a = a.transpose(1, 2).reshape(B * S, -1)
+        if has_own_attention(cfg):
+            q_norm, k_norm = synth_head_norms(cfg, li, dev)
+            q, k = ops.qk_norm_rope(q, k, cos, sin, positions, q_weight=q_norm, k_weight=k_norm, eps=1e-6)
+            a = ops.prompt_attention(q, k, v.view(k.shape), cu, cu, S, **attention_mask(cfg)).view(B * S, -1)
+        else:
+            q, k = ops.rope_(q, cos, sin, S), ops.rope_(k, cos, sin, S)
+            a = F.scaled_dot_product_attention(q.view(B, S, -1, hd).transpose(1, 2), k.view(B, S, -1, hd).transpose(1, 2),
+                                               v.view(B, S, -1, hd).transpose(1, 2), is_causal=True, enable_gqa=True)  # fmt: skip
+            a = a.transpose(1, 2).reshape(B * S, -1)
         scales[(li, "o")] = ops.col_absmax(a)
         x = x + F.linear(a, w["o"])
         h = F.rms_norm(x, (H,), ones, 1e-5)
@@ -173,7 +197,7 @@ class W8A8Decoder:
         nl = layers if layers is not None else cfg["layers"]
         if surface == "modules" and world != 1:
             raise RuntimeError("the module surface runs on one GPU")
-        self.own_attention = bool(cfg.get("qk_norm", False) or cfg.get("window", 0))
+        self.own_attention = has_own_attention(cfg)
         if self.own_attention and (surface != "fused" or world != 1):
             raise RuntimeError("qk_norm and window run on one GPU with the fused surface")
         self.layers = []
@@ -193,11 +217,7 @@ class W8A8Decoder:
                 del w
             lin["ln1"] = torch.ones(H, device=dev, dtype=torch.bfloat16)
             lin["ln2"] = torch.ones(H, device=dev, dtype=torch.bfloat16)
-            lin["q_norm"] = lin["k_norm"] = None
-            if cfg.get("qk_norm", False):
-                g = torch.Generator(device=dev).manual_seed(1000 * li + 100)
-                for name in ("q_norm", "k_norm"):
-                    lin[name] = (1 + 0.1 * torch.randn(cfg["head_dim"], generator=g, device=dev)).bfloat16()
+            lin["q_norm"], lin["k_norm"] = synth_head_norms(cfg, li, dev)
             self.layers.append(lin)
         g = torch.Generator(device=dev).manual_seed(4)
         self.embed = (torch.randn(cfg["vocab"], H, generator=g, device=dev) * 0.02).bfloat16()
@@ -256,9 +276,6 @@ class W8A8Decoder:
     def _rotate(self, lin, q, k, positions, **cache):
         return ops.qk_norm_rope(q, k, self.cos, self.sin, positions, q_weight=lin["q_norm"], k_weight=lin["k_norm"], eps=1e-6, **cache)
 
-    def _mask(self):
-        return dict(window=self.cfg.get("window", 0), sinks=self.cfg.get("sinks", 0))
-
     def _attend_whole(self, B, S):
         """Rotation and attention of B whole sequences of S tokens: (layer, its Linears, q, k, v) -> (q, k, output)."""
         if not self.own_attention:
@@ -273,7 +290,7 @@ class W8A8Decoder:
 
         def attend(li, lin, q, k, v):
             q, k = self._rotate(lin, q, k, positions)
-            a = ops.prompt_attention(q, k, v.view(k.shape), cu, cu, S, **self._mask())
+            a = ops.prompt_attention(q, k, v.view(k.shape), cu, cu, S, **attention_mask(self.cfg))
             return q, k, a.view(B * S, -1)
 
         return attend
@@ -286,9 +303,9 @@ class W8A8Decoder:
             v = v.view(k.shape)
             q, k = self._rotate(lin, q, k, step.positions, v=v, slots=step.slots, want_k=not step.single, **pages)
             if step.single:
-                a = ops.paged_attention(q, block_table=cache.table, lens=cache.lens, **pages, **self._mask())
+                a = ops.paged_attention(q, block_table=cache.table, lens=cache.lens, **pages, **attention_mask(self.cfg))
             else:
-                a = ops.prompt_attention(q, k, v, step.cu, step.cu, step.max_q, **self._mask())
+                a = ops.prompt_attention(q, k, v, step.cu, step.cu, step.max_q, **attention_mask(self.cfg))
             return q, k, a.view(a.shape[0], -1)
 
         return attend
