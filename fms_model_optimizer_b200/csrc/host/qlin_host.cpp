@@ -675,11 +675,15 @@ Tensor qat_linear(const Tensor& x, const Tensor& w, const OptTensor& bias, const
 }
 
 // ------------------------------------------------------------------------------------------------ attention of a generating decoder
-// These calls have no gradient; one that autograd would have to record is refused rather than cut off silently.
+// These calls have no gradient; one that autograd would have to record, or a tangent that it would have to carry on (also under
+// no_grad), is refused rather than cut off silently.
 void refuse_grad(const char* what, std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : tensors)
-    if (t != nullptr && t->defined() && t->requires_grad()) raise(std::string(what) + " has no gradient: call it under torch.no_grad(), or detach its inputs");
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : tensors) {
+    if (t == nullptr || !t->defined()) continue;
+    if ((backward && t->requires_grad()) || (forward && t->_fw_grad(0).defined()))
+      raise(std::string(what) + " has no gradient: call it under torch.no_grad(), or detach its inputs");
+  }
 }
 
 // The stride of a dimension; 0 where a single entry makes it meaningless.
@@ -720,7 +724,7 @@ std::tuple<Tensor, OptTensor> qk_rope(const Tensor& q_in, const Tensor& k_in, co
                                       const OptTensor& slots, const OptTensor& k_scale, const OptTensor& v_scale, bool want_k) {
   const at::Device dev = require_cuda({&q_in, &k_in, &cos, &sin, &positions, ptr_of(q_weight), ptr_of(k_weight), ptr_of(v_in), ptr_of(k_pages), ptr_of(v_pages),
                                        ptr_of(slots), ptr_of(k_scale), ptr_of(v_scale)});
-  refuse_grad("qk_norm_rope", {&q_in, &k_in, ptr_of(q_weight), ptr_of(k_weight), ptr_of(v_in)});
+  refuse_grad("qk_norm_rope", {&q_in, &k_in, &cos, &sin, ptr_of(q_weight), ptr_of(k_weight), ptr_of(v_in), ptr_of(k_pages), ptr_of(v_pages), ptr_of(k_scale), ptr_of(v_scale)});
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k");
   const int64_t t = q.size(0), d = q.size(2);
@@ -805,7 +809,7 @@ Tensor attention_out(const OptTensor& out, const Tensor& q, at::Device dev) {
 Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& lens, const std::optional<double>& scale,
                        int64_t window, int64_t sinks, const OptTensor& k_scale, const OptTensor& v_scale, const OptTensor& out_in) {
   const at::Device dev = require_cuda({&q_in, &k_pages, &v_pages, &block_table, &lens, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
-  refuse_grad("paged_attention", {&q_in, &k_pages, &v_pages});
+  refuse_grad("paged_attention", {&q_in, &k_pages, &v_pages, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor q = head_rows(q_in, "q");
   const int64_t b = q.size(0), d = q.size(2);
@@ -858,7 +862,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
 Tensor prompt_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& cu_q, const Tensor& cu_k, int64_t max_q, const std::optional<double>& scale,
                         int64_t window, int64_t sinks, const OptTensor& out_in) {
   const at::Device dev = require_cuda({&q_in, &k_in, &v_in, &cu_q, &cu_k, ptr_of(out_in)});
-  refuse_grad("prompt_attention", {&q_in, &k_in, &v_in});
+  refuse_grad("prompt_attention", {&q_in, &k_in, &v_in, ptr_of(out_in)});
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k"), v = head_rows(v_in, "v");
   const at::ScalarType type = q.scalar_type();
