@@ -799,10 +799,33 @@ std::tuple<Tensor, OptTensor> qk_rope(const Tensor& q_in, const Tensor& k_in, co
   return {q_out, want_k ? OptTensor(k_out) : std::nullopt};
 }
 
-// `out`: given or fresh, dense and of q's shape and type.
-Tensor attention_out(const OptTensor& out, const Tensor& q, at::Device dev) {
-  if (!out) return empty(q.sizes(), q.scalar_type(), dev);
-  if (out->scalar_type() != q.scalar_type() || out->sizes() != q.sizes() || !out->is_contiguous()) raise("out must be contiguous, with the shape and type of q");
+// The bytes from the first element of a tensor to its last may hold some of those of another.
+bool may_overlap(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto range = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return std::pair(begin, begin + static_cast<uintptr_t>(last + 1) * t.element_size());
+  };
+  const auto [a0, a1] = range(a);
+  const auto [b0, b1] = range(b);
+  return a0 < b1 && b0 < a1;
+}
+
+// Where the kernel writes: the given `out` (dense and of q's shape and type), or a fresh tensor where there is none or where it
+// overlaps an input, since blocks still read while others have written.
+Tensor attention_out(const OptTensor& out, const Tensor& q, at::Device dev, std::initializer_list<const Tensor*> inputs) {
+  if (out && (out->scalar_type() != q.scalar_type() || out->sizes() != q.sizes() || !out->is_contiguous()))
+    raise("out must be contiguous, with the shape and type of q");
+  if (out && std::none_of(inputs.begin(), inputs.end(), [&](const Tensor* t) { return may_overlap(*out, *t); })) return *out;
+  return empty(q.sizes(), q.scalar_type(), dev);
+}
+// What the caller gets: `out` where it was given, filled from the tensor that the kernel wrote.
+Tensor delivered(const OptTensor& out, const Tensor& written) {
+  if (!out || out->data_ptr() == written.data_ptr()) return written;
+  at::NoGradGuard no_grad;
+  out->copy_(written);
   return *out;
 }
 
@@ -821,7 +844,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
     raise("block_table must be int32 [batch, pages of a sequence] with contiguous rows");
   check_index(lens, at::kInt, b, "lens");
   if (b > 0x7fffffff || k_pages.size(0) > 0x7fffffff || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff) raise("batch, pages, window or sinks out of range");
-  const Tensor out = attention_out(out_in, q, dev);
+  const Tensor out = attention_out(out_in, q, dev, {&q, &k_pages, &v_pages});
   qlin_paged_attention_args a = {};
   a.q = data(q);
   a.k_pages = data(k_pages);
@@ -856,7 +879,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
   if (bytes > 0) ws = empty({bytes}, at::kByte, dev);
   a.workspace = data(ws);
   check(qlin_paged_attention(&a, stream_of(dev)), "qlin_paged_attention");
-  return out;
+  return delivered(out_in, out);
 }
 
 Tensor prompt_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& cu_q, const Tensor& cu_k, int64_t max_q, const std::optional<double>& scale,
@@ -874,7 +897,7 @@ Tensor prompt_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_
   if (q.size(0) > 0x7fffff00 || k.size(0) > 0x7fffff00 || max_q < 0 || max_q > q.size(0) || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff)
     raise("tokens, max_q, window or sinks out of range");
   if (q.size(0) > 0 && (cu_q.size(0) < 2 || max_q < 1)) raise("q has rows, but cu_q no sequence or max_q no row");
-  const Tensor out = attention_out(out_in, q, dev);
+  const Tensor out = attention_out(out_in, q, dev, {&q, &k, &v});
   qlin_prompt_attention_args a = {};
   a.q = data(q);
   a.k = data(k);
@@ -901,7 +924,7 @@ Tensor prompt_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_
   a.dtype = dtype_code(type);
   a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2))));
   check(qlin_prompt_attention(&a, stream_of(dev)), "qlin_prompt_attention");
-  return out;
+  return delivered(out_in, out);
 }
 
 }  // namespace

@@ -662,7 +662,7 @@ def paged_attention(
     ``block_table`` int32 ``[batch, pages of a sequence]``, ``lens`` int32 ``[batch]``, both on the device.  ``window`` > 0: only
     the last ``window`` keys and the first ``sinks`` are visible.  ``scale`` defaults to ``head_dim ** -0.5``.  A sequence of
     length 0 gives zeros.  The width of ``block_table`` bounds the lengths and with them how finely the keys are split, so pass
-    no more columns than the longest sequence needs.  No gradient."""
+    no more columns than the longest sequence needs.  ``out``: dense, of q's shape and type; it may be (part of) an input.  No gradient."""
     return _call("paged_attention", 0.0, q.device, L.host().paged_attention, q, k_pages, v_pages, block_table, lens, scale, window, sinks, k_scale, v_scale, out)
 
 
@@ -682,7 +682,7 @@ def prompt_attention(
     """Causal attention of packed prompts (``qlin_prompt_attention``).  Sequence b has the rows ``cu_q[b] : cu_q[b + 1]`` of ``q
     [tokens, q heads, head_dim]`` and ``cu_k[b] : cu_k[b + 1]`` of ``k`` and ``v [keys, kv heads, head_dim]`` (int32 on the device); with n
     queries and m keys, query i stands at position ``i + m - n``.  ``max_q``: the most queries of a sequence.  ``window`` and
-    ``sinks`` as in ``paged_attention``; a query that sees no key gives zeros.  No gradient."""
+    ``sinks`` as in ``paged_attention``; a query that sees no key gives zeros.  ``out`` as in ``paged_attention``.  No gradient."""
     return _call("prompt_attention", 0.0, q.device, L.host().prompt_attention, q, k, v, cu_q, cu_k, max_q, scale, window, sinks, out)
 
 

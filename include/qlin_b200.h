@@ -686,7 +686,7 @@ int qlin_qk_rope(const qlin_qk_rope_args* args, void* stream);
 
 /* qlin_paged_attention -- one new token of every sequence against its keys in the cache, the new token's own key included:
  * sequence b has lens[b] keys and its query stands at position lens[b] - 1.  The keys of a sequence are split over several blocks
- * and joined in order, so results do not depend on timing.  out is dense [batch, q_heads, head_dim].  q_heads is a multiple of
+ * and joined in order, so results do not depend on timing.  out is dense [batch, q_heads, head_dim] and overlaps no input.  q_heads is a multiple of
  * kv_heads; head_dim a multiple of 8 (16 with an e4m3 cache) up to 128.  lens above max_pages * page_size or a page that does not
  * exist write QLIN_ERR_BAD_SHAPE to *status; such a length is cut, such a page read as page 0. */
 typedef struct qlin_paged_attention_args {
@@ -713,7 +713,7 @@ int qlin_paged_attention(const qlin_paged_attention_args* args, void* stream);
 
 /* qlin_prompt_attention -- attention of packed sequences: sequence b has the queries cu_q[b] .. cu_q[b + 1] of q [tokens_q, q_heads,
  * head_dim] and the keys cu_k[b] .. cu_k[b + 1] of k, v [tokens_k, kv_heads, head_dim]; query i of n stands at position i + m - n
- * where m is the number of keys.  out is dense [tokens_q, q_heads, head_dim].  F16 or BF16; q_heads a multiple of kv_heads, at
+ * where m is the number of keys.  out is dense [tokens_q, q_heads, head_dim] and overlaps no input.  F16 or BF16; q_heads a multiple of kv_heads, at
  * most 128 query heads a kv head; head_dim a multiple of 8 up to 128; strides positive.  cu_q and cu_k start at 0, end at tokens_q and tokens_k and
  * do not fall, and no sequence has more than max_q queries; otherwise QLIN_ERR_BAD_SHAPE in *status and rows left unwritten. */
 typedef struct qlin_prompt_attention_args {

@@ -63,3 +63,34 @@ def test_no_gradient_is_cut_off_silently(cuda_dev, which, f8):
                 with pytest.raises(RuntimeError, match="no gradient"):
                     calls(which, **{name: dual})
     ops.check_status(cuda_dev)
+
+
+@pytest.mark.parametrize("lens,dim", [([5000], 128), ([40, 2000, 7], 64)])
+def test_an_output_may_lie_over_an_input(cuda_dev, lens, dim):
+    """Queries, keys or values that the output takes the place of: the result is the one of an output of its own."""
+    g = torch.Generator().manual_seed(32)
+    hq, hkv, page = 16, 1, 16
+    b, per = len(lens), -(-max(lens) // page)
+    q = _randn(g, b, hq, dim).to(cuda_dev)
+    pages = [_randn(g, b * per, hkv, page, dim).to(cuda_dev) for _ in range(2)]
+    table, n = torch.arange(b * per, dtype=torch.int32, device=cuda_dev).view(b, per), torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    want = ops.paged_attention(q, *pages, table, n)
+    own = torch.empty_like(q)
+    assert ops.paged_attention(q, *pages, table, n, out=own) is own and torch.equal(own, want)
+    for over in ("q", "k", "v"):
+        mine, k, v = q.clone(), *(p.clone() for p in pages)
+        out = dict(q=mine, k=k.view(-1)[: q.numel()].view(q.shape), v=v.view(-1)[-q.numel() :].view(q.shape))[over]
+        got = ops.paged_attention(mine, k, v, table, n, out=out)
+        assert got.data_ptr() == out.data_ptr() and torch.equal(got, want), over
+    x = [_randn(g, 2000, 8, dim).to(cuda_dev) for _ in range(3)]
+    cu = torch.tensor([0, 2000], dtype=torch.int32, device=cuda_dev)
+    want = ops.prompt_attention(*x, cu, cu, 2000)
+    for i in range(3):
+        mine = [t.clone() for t in x]
+        assert torch.equal(ops.prompt_attention(*mine, cu, cu, 2000, out=mine[i]), want), i
+    x[2][100, 3, 5] = math.nan  # rows before the 100th are computed again from what they see
+    want = ops.prompt_attention(*x, cu, cu, 2000)
+    assert not want[:100].isnan().any()
+    mine = [t.clone() for t in x]
+    assert torch.equal(ops.prompt_attention(*mine, cu, cu, 2000, out=mine[0])[:100], want[:100])
+    ops.check_status(cuda_dev)
