@@ -756,8 +756,9 @@ std::tuple<Tensor, OptTensor> qk_rope(const Tensor& q_in, const Tensor& k_in, co
     a.v = data(v);
     a.v_token = step(v, 0);
     a.v_head = step(v, 1);
-    a.k_pages = data(*k_pages);
-    a.v_pages = data(*v_pages);
+    // a pool of no pages has no address, but its slots are looked at: none of them is written
+    a.k_pages = k_pages->numel() > 0 ? data(*k_pages) : data(q);
+    a.v_pages = v_pages->numel() > 0 ? data(*v_pages) : data(q);
     a.slots = static_cast<const int64_t*>(data(*slots));
     a.k_scale = static_cast<const float*>(data(ks));
     a.v_scale = static_cast<const float*>(data(vs));

@@ -94,3 +94,18 @@ def test_an_output_may_lie_over_an_input(cuda_dev, lens, dim):
     mine = [t.clone() for t in x]
     assert torch.equal(ops.prompt_attention(*mine, cu, cu, 2000, out=mine[0])[:100], want[:100])
     ops.check_status(cuda_dev)
+
+
+def test_a_cache_without_pages_reports_every_slot(cuda_dev):
+    calls = _Calls(cuda_dev, False)
+    none = torch.empty(0, 2, 8, 64, dtype=torch.bfloat16, device=cuda_dev)
+    ops.check_status(cuda_dev)
+    a = dict(calls.args["rotate"], k_pages=none, v_pages=none)
+    rotate = lambda slots: ops.qk_norm_rope(a["q"], a["k"], a["cos"], a["sin"], calls.i, q_weight=a["q_weight"], k_weight=a["k_weight"], v=a["v"], k_pages=none,  # noqa: E731
+                                            v_pages=none, slots=torch.tensor(slots, device=cuda_dev))  # fmt: skip
+    want = rotate([-1, -1])
+    ops.check_status(cuda_dev)
+    got = rotate([-1, 0])
+    with pytest.raises(RuntimeError, match="status"):
+        ops.check_status(cuda_dev)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
