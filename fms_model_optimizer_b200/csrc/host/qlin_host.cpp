@@ -753,6 +753,9 @@ std::tuple<Tensor, OptTensor> qk_rope(const Tensor& q_in, const Tensor& k_in, co
     vs = f32(v_scale);
     check_cache(*k_pages, *v_pages, k.size(1), d, type, ks, vs);
     check_index(*slots, at::kLong, t, "slots");
+    for (int64_t dim = 0; dim < 3; ++dim)
+      if (k_pages->size(dim) > 1 && k_pages->stride(dim) == 0) raise("places of the cache share memory: it cannot be written");
+    if (k_pages->numel() > 0 && k_pages->data_ptr() == v_pages->data_ptr()) raise("k_pages and v_pages share memory: they cannot be written");
     a.v = data(v);
     a.v_token = step(v, 0);
     a.v_head = step(v, 1);

@@ -109,3 +109,15 @@ def test_a_cache_without_pages_reports_every_slot(cuda_dev):
     with pytest.raises(RuntimeError, match="status"):
         ops.check_status(cuda_dev)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_a_cache_whose_places_share_memory_is_refused(cuda_dev):
+    """Keys and values in the same pages, or pages that are one and the same: what such a cache held would depend on timing."""
+    calls = _Calls(cuda_dev, False)
+    one = torch.zeros(4, 2, 8, 64, dtype=torch.bfloat16, device=cuda_dev)
+    for k, v in ((one, one), (one[:1].expand(4, 2, 8, 64), one[1:2].expand(4, 2, 8, 64)), (one[:, :1].expand(4, 2, 8, 64), one[:, 1:].expand(4, 2, 8, 64))):
+        with pytest.raises(RuntimeError, match="share memory"):
+            calls("rotate", k_pages=k, v_pages=v)
+    calls("token", k_pages=one, v_pages=one)  # reading them is no matter
+    calls("token", k_pages=one[:1].expand(4, 2, 8, 64), v_pages=one[:1].expand(4, 2, 8, 64))
+    assert not one.any()
