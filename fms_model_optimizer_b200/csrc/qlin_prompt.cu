@@ -982,6 +982,20 @@ static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
   return launch_prompt_as<T, DP, false>(tq, tk, tv, p, static_cast<unsigned>(blocks < sm_count() ? blocks : sm_count()), stream);
 }
 
+// The check of the offsets alone, for calls that compute nothing: without sequences, queries of a sequence or keys.
+__global__ void prompt_offsets_kernel(const __grid_constant__ PromptParams p) {
+  bool bad = p.a.batch == 0 || p.a.max_q == 0;  // there are rows, so the offsets cannot cover them
+  if (!bad)
+    for (int b = threadIdx.x; b < p.a.batch; b += blockDim.x) bad |= sequence_of(p, b).bad;
+  if (bad) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
+}
+static int check_offsets(const PromptParams& p, cudaStream_t stream) {
+  if (p.a.status == nullptr) return QLIN_OK;
+  prompt_offsets_kernel<<<1, 256, 0, stream>>>(p);
+  QLIN_CHECK_LAUNCH("qlin_prompt_attention");
+  return QLIN_OK;
+}
+
 }  // namespace qlin
 
 extern "C" int qlin_prompt_attention(const qlin_prompt_attention_args* a, void* stream) {
@@ -992,7 +1006,11 @@ extern "C" int qlin_prompt_attention(const qlin_prompt_attention_args* a, void* 
   if (a->q_heads / a->kv_heads > 128) return fail(QLIN_ERR_UNSUPPORTED, "qlin_prompt_attention: at most 128 query heads share a kv head");
   if (a->dtype != QLIN_DT_F16 && a->dtype != QLIN_DT_BF16) return fail(QLIN_ERR_BAD_DTYPE, "qlin_prompt_attention: q, k and v must be fp16 or bf16");
   if (a->head_dim < 8 || a->head_dim % 8 != 0 || a->head_dim > 128) return fail(QLIN_ERR_BAD_SHAPE, "qlin_prompt_attention: head_dim must be a multiple of 8 up to 128");
-  if (a->batch == 0 || a->tokens_q == 0 || a->max_q == 0) return QLIN_OK;
+  if (a->tokens_q == 0) return QLIN_OK;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  PromptParams p;
+  p.a = *a;
+  if (a->batch == 0 || a->max_q == 0) return check_offsets(p, s);
   if (a->q == nullptr || a->out == nullptr || a->cu_q == nullptr || a->cu_k == nullptr) return fail(QLIN_ERR_NULL, "qlin_prompt_attention: q, out, cu_q or cu_k is NULL");
   if (a->tokens_k > 0 && (a->k == nullptr || a->v == nullptr)) return fail(QLIN_ERR_NULL, "qlin_prompt_attention: k or v is NULL");
   if (a->tokens_q > kMostTokens || a->tokens_k > kMostTokens) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: at most 2^30 tokens");
@@ -1005,8 +1023,6 @@ extern "C" int qlin_prompt_attention(const qlin_prompt_attention_args* a, void* 
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) || a->q_token % 8 != 0 || a->q_head % 8 != 0 || a->k_token % 8 != 0 ||
       a->k_head % 8 != 0 || a->v_token % 8 != 0 || a->v_head % 8 != 0)
     return fail(QLIN_ERR_BAD_ALIGN, "qlin_prompt_attention: every row must start on 16 bytes");
-  PromptParams p;
-  p.a = *a;
   p.group = a->q_heads / a->kv_heads;
   p.cl2 = a->scale * 1.4426950408889634f;
   if (p.a.window > kMostTokens) p.a.window = kMostTokens;  // as far as any sequence reaches, and sums with positions stay in 32 bits
@@ -1015,10 +1031,9 @@ extern "C" int qlin_prompt_attention(const qlin_prompt_attention_args* a, void* 
   p.tq = kRows / p.group;
   p.units = static_cast<int32_t>((static_cast<int64_t>(a->max_q) + 2 * p.tq - 1) / (2 * p.tq));
   if (a->tokens_k == 0) {  // nothing to see: the tensor maps have no memory to describe
-    const cudaError_t e = cudaMemsetAsync(a->out, 0, static_cast<size_t>(a->tokens_q) * a->q_heads * a->head_dim * 2, reinterpret_cast<cudaStream_t>(stream));
-    return e == cudaSuccess ? QLIN_OK : fail(QLIN_ERR_LAUNCH, "qlin_prompt_attention: %s", cudaGetErrorString(e));
+    const cudaError_t e = cudaMemsetAsync(a->out, 0, static_cast<size_t>(a->tokens_q) * a->q_heads * a->head_dim * 2, s);
+    return e == cudaSuccess ? check_offsets(p, s) : fail(QLIN_ERR_LAUNCH, "qlin_prompt_attention: %s", cudaGetErrorString(e));
   }
-  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (a->dtype == QLIN_DT_BF16) return a->head_dim <= 64 ? launch_prompt<__nv_bfloat16, 64>(p, s) : launch_prompt<__nv_bfloat16, 128>(p, s);
   return a->head_dim <= 64 ? launch_prompt<__half, 64>(p, s) : launch_prompt<__half, 128>(p, s);
 }

@@ -121,3 +121,30 @@ def test_a_cache_whose_places_share_memory_is_refused(cuda_dev):
     calls("token", k_pages=one, v_pages=one)  # reading them is no matter
     calls("token", k_pages=one[:1].expand(4, 2, 8, 64), v_pages=one[:1].expand(4, 2, 8, 64))
     assert not one.any()
+
+
+@pytest.mark.parametrize("case", ["no sequences", "no queries a sequence", "keys that are not there", "offsets that fall"])
+def test_offsets_that_do_not_cover_the_queries_are_reported(cuda_dev, case):
+    """... also where there is nothing to compute: the C entry's status word, and outputs that hold no stale value as an answer."""
+    x = torch.ones(4, 2, 64, dtype=torch.bfloat16, device=cuda_dev)
+    out = torch.full_like(x, 3.0)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_dev)
+    none = case in ("keys that are not there", "offsets that fall")
+    cu_q, cu_k = (torch.tensor(c, dtype=torch.int32, device=cuda_dev) for c in (([0, 4, 2] if case == "offsets that fall" else [0, 2, 4]), [0, 3, 3] if "keys" in case else [0, 0, 0]))
+    a = L.PromptAttentionArgs(q=x.data_ptr(), k=x.data_ptr(), v=x.data_ptr(), out=out.data_ptr(), cu_q=cu_q.data_ptr(), cu_k=cu_k.data_ptr(), status=status.data_ptr(),
+                              q_token=128, q_head=64, k_token=128, k_head=64, v_token=128, v_head=64, tokens_q=4, tokens_k=0 if none else 4,
+                              batch=0 if case == "no sequences" else 2, max_q=0 if case == "no queries a sequence" else 2, q_heads=2, kv_heads=2, head_dim=64,
+                              dtype=L.DT_BF16, scale=0.125)  # fmt: skip
+    stream = C.c_void_p(torch.cuda.current_stream(cuda_dev).cuda_stream)
+    assert L.load().qlin_prompt_attention(C.byref(a), stream) == L.OK
+    assert int(status) == L.ERR_BAD_SHAPE
+    if none:  # the call through tensors reports it as well
+        ops.check_status(cuda_dev)
+        ops.prompt_attention(x, x[:0], x[:0], cu_q, cu_k, 2)
+        with pytest.raises(RuntimeError, match="status"):
+            ops.check_status(cuda_dev)
+        good = torch.tensor([0, 2, 4], dtype=torch.int32, device=cuda_dev)
+        assert not ops.prompt_attention(x, x[:0], x[:0], good, torch.zeros_like(good), 2).any()
+        ops.check_status(cuda_dev)
+    else:
+        assert bool((out == 3.0).all())
