@@ -119,6 +119,13 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
+// Four outputs from their sums; zeros where there is no weight at all, whatever the values hold.
+template <bool BF16>
+__device__ __forceinline__ uint2 outputs4(const float (&acc)[4], float sum, float v_scale) {
+  if (sum == 0.0f) return make_uint2(0u, 0u);
+  const float r = v_scale / sum;
+  return make_uint2(pack16<BF16>(acc[0] * r, acc[1] * r), pack16<BF16>(acc[2] * r, acc[3] * r));
+}
 __device__ __forceinline__ float max_of_rows(float v) {  // over the eight lanes that hold one column
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
@@ -400,9 +407,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
   float2* block_ml = reinterpret_cast<float2*>(block_o + C::HEADS * C::OROW);   // [heads]
   const auto store_out = [&](int h, int d, const float (&acc)[4], float sum) {
     constexpr bool bf16 = std::is_same<QT, __nv_bfloat16>::value;
-    const float r = sum == 0.0f ? 0.0f : v_scale / sum;
     QT* out = static_cast<QT*>(p.a.out) + (static_cast<int64_t>(b) * p.a.q_heads + kvh * p.group + head0 + h) * D + d;
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack16<bf16>(acc[0] * r, acc[1] * r), pack16<bf16>(acc[2] * r, acc[3] * r));
+    *reinterpret_cast<uint2*>(out) = outputs4<bf16>(acc, sum, v_scale);
   };
   for (int i = threadIdx.x; i < heads * (DP / 4); i += kPagedThreads) {
     const int h = i / (DP / 4), d = i % (DP / 4) * 4;
@@ -517,9 +523,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
     acc[2] += o.z;
     acc[3] += o.w;
   }
-  const float r = sum == 0.0f ? 0.0f : (f8 ? p.a.v_scale[h / p.group] : 1.0f) / sum;
   constexpr bool bf16 = std::is_same<QT, __nv_bfloat16>::value;
-  *reinterpret_cast<uint2*>(static_cast<QT*>(p.a.out) + row * D + d) = make_uint2(pack16<bf16>(acc[0] * r, acc[1] * r), pack16<bf16>(acc[2] * r, acc[3] * r));
+  *reinterpret_cast<uint2*>(static_cast<QT*>(p.a.out) + row * D + d) = outputs4<bf16>(acc, sum, f8 ? p.a.v_scale[h / p.group] : 1.0f);
 }
 
 // Splits of the keys: blocks for every SM, none with fewer than kMinTiles tiles where the page table is as wide as its longest

@@ -130,7 +130,10 @@ __device__ __noinline__ void attend_row(const PromptParams& p, const Sequence& s
     }
   }
   if (writes) {
-    const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const bool none = sum == 0.0f;  // zeros, whatever the values hold
+    const float r = none ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = none ? 0.0f : acc[e];
     T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(s.q0 + i) * p.a.q_heads + head) * D + lane * 4;
     *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(acc[0] * r, acc[1] * r), pack2<T>(acc[2] * r, acc[3] * r));
   }
@@ -770,7 +773,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         other = ml.x == top ? 1.0f : exp2f(ml.x - top);
         l = l * own + ml.y * other;
       }
-      const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+      const bool none = l == 0.0f;  // no weight anywhere: zeros, whatever the values hold
+      const float scale = none ? 0.0f : 1.0f / l;
       // Rows go through shared memory, 64 outputs at a time, so that eight lanes write the 128 bytes of a row together (a lane for
       // each row touches 32 lines with every store: 8 x 2048 290 us, 282 so).
       T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(u.seq.q0 + token) * p.a.q_heads + head) * p.a.head_dim;
@@ -796,6 +800,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             o[j + 3] = __float_as_uint(__uint_as_float(o[j + 3]) * own + v.w * other);
           }
         }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = none ? 0u : o[j];
 #pragma unroll
         for (int j = 0; j < 32; ++j) again |= __uint_as_float(o[j]) != __uint_as_float(o[j]);
 #pragma unroll

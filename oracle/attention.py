@@ -36,4 +36,5 @@ def attend(q, k, v, pos, window, sinks, scale):
     total = w.sum(-1, keepdim=True)
     w = torch.where(total == 0, 0.0, w / total)
     size = (q.abs() @ k.abs().t()).amax(-1) * scale
-    return (w[:, :, None] * v).sum(1), (w[:, :, None] * v.abs()).sum(1), size
+    none = total == 0  # zeros, whatever the values hold
+    return (w[:, :, None] * v).sum(1).masked_fill(none, 0.0), (w[:, :, None] * v.abs()).sum(1).masked_fill(none, 0.0), size

@@ -148,3 +148,39 @@ def test_offsets_that_do_not_cover_the_queries_are_reported(cuda_dev, case):
         ops.check_status(cuda_dev)
     else:
         assert bool((out == 3.0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_queries_whose_logits_are_all_minus_infinity_give_zeros(cuda_dev, dtype, value):
+    """... whatever the values hold that they see with a weight of zero: in one block, in blocks that join, and in a second launch."""
+    dim = 64
+    minus = lambda *shape: torch.full(shape, -math.inf, dtype=dtype, device=cuda_dev)  # noqa: E731
+    for n, hq, hkv in ((40, 2, 1), (300, 4, 2), (2000, 8, 1)):  # the last shared by two blocks
+        q, k = torch.ones(n, hq, dim, dtype=dtype, device=cuda_dev), torch.ones(n, hkv, dim, dtype=dtype, device=cuda_dev)
+        q[::2] = -math.inf
+        v = torch.zeros(n, hkv, dim, dtype=dtype, device=cuda_dev)
+        v[n // 3 :, :, 5] = value
+        cu = torch.tensor([0, n], dtype=torch.int32, device=cuda_dev)
+        got = ops.prompt_attention(q, k, v, cu, cu, n)
+        assert not got[::2].any(), (n, "rows of minus infinity")
+        assert not got[: n // 3].any() and bool((got[1::2][n // 6 + 1 :, :, 5].isnan() if math.isnan(value) else got[1::2][n // 6 + 1 :, :, 5] == value).all())
+    for lens, page, f8 in (([3], 4, False), ([700, 2, 90], 16, False), ([9000], 64, False), ([500, 0], 16, True), ([9000], 64, True)):
+        if f8 and math.isinf(value):
+            continue  # e4m3 has no infinities
+        per = -(-max(lens) // page)
+        shape = (len(lens) * per, 1, page, dim)
+        k, v = torch.ones(shape, dtype=dtype, device=cuda_dev), torch.zeros(shape, dtype=dtype, device=cuda_dev)
+        v[..., 5] = value
+        one = torch.ones(1, device=cuda_dev) if f8 else None
+        if f8:
+            k, v = k.to(F8), v.to(F8)
+        table = torch.arange(len(lens) * per, dtype=torch.int32, device=cuda_dev).view(len(lens), per)
+        n = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+        q = minus(len(lens), 2, dim)
+        q[:, 1] = 1
+        got = ops.paged_attention(q, k, v, table, n, k_scale=one, v_scale=one)
+        assert not got[:, 0].any(), (lens, f8)
+        seen = got[:, 1, 5][n > 0]
+        assert bool((seen.isnan() if math.isnan(value) else seen == value).all())
+    ops.check_status(cuda_dev)
