@@ -123,6 +123,10 @@ struct PromptCfg {
   static __device__ __forceinline__ uint32_t part_o(int row, int piece) { return static_cast<uint32_t>(row * DP * 4 + ((piece ^ (row & 7)) << 4)); }
   static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(PromptAux));
   static constexpr float SHIFT = std::is_same<T, __half>::value ? 6.0f : 0.0f;
+  // A weight is 2^(x cl2 - r) with r rounded and the product not, so half a unit of r's last place and more is in its exponent, the same for all
+  // keys of a row.  From these references on (logits of 2.9e6 in fp16, 3.7e8 in bf16) that could carry weights out of 16 bits: rows that end with one are
+  // computed again, with the difference taken first.
+  static constexpr float LARGE_REF = std::is_same<T, __half>::value ? 0x1p22f : 0x1p29f;
   static constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
   static constexpr uint32_t IDESC_S = make_idesc(1u, FMT, kRows, kKeys);
   static constexpr uint32_t IDESC_O = make_idesc(1u, FMT, kRows, DP) | (1u << 16);  // V is read with its head dimension contiguous
@@ -355,10 +359,10 @@ struct WarpRows {
 // the queries are the rows of both, the keys the columns of the first.  The order of the head dimensions within a product is free, so each
 // lane loads 16 bytes of a key, and 32 bytes of a value for the columns 16 g + j of the j-th product.  Weights go to 16 bits as in the tiles,
 // but not to zero, so that an infinity that a row sees stays one; keys that only some of the rows see are added in fp32, row by row.
-// Once each output that is NaN as the rows stand is NaN again they stay as they are.
+// Once each output that is NaN as the rows stand is NaN again they stay as they are, unless `rewrite`.
 constexpr int kAgain = 16;
 template <typename T>
-__device__ __forceinline__ void attend_rows(const PromptParams& p, const WarpRows& rows, uint32_t which) {
+__device__ __forceinline__ void attend_rows(const PromptParams& p, const WarpRows& rows, uint32_t which, bool rewrite) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr float kUp = kBf16 ? 0.0f : 12.0f, kLeast = kBf16 ? 0x1p-126f : 0x1p-24f;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, D = p.a.head_dim;
@@ -447,7 +451,7 @@ __device__ __forceinline__ void attend_rows(const PromptParams& p, const WarpRow
         }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2)), top[i]);
-      const float keep = most == top[i] ? 1.0f : exp2f(top[i] - most), ref = (most == -INFINITY ? 0.0f : most) - kUp;
+      const float keep = most == top[i] ? 1.0f : exp2f(top[i] - most), ref = most == -INFINITY ? 0.0f : most;
       top[i] = most;
       sum[i] *= keep;
 #pragma unroll
@@ -455,7 +459,7 @@ __device__ __forceinline__ void attend_rows(const PromptParams& p, const WarpRow
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& y = x[h][2 * i + e];
-          const float w = exp2f(y - ref);
+          const float w = exp2f((y - ref) + kUp);  // the difference first: exact near the maximum, however large that is
           sum[i] += w;
           y = y > -INFINITY ? fmaxf(w, kLeast) : w;
         }
@@ -506,7 +510,7 @@ __device__ __forceinline__ void attend_rows(const PromptParams& p, const WarpRow
         }
       }
     }
-    if (u0 % 128 == 0) {
+    if (u0 % 128 == 0 && !rewrite) {
       uint32_t now[2] = {0, 0};
 #pragma unroll
       for (int j = 0; j < 16; ++j)
@@ -537,8 +541,9 @@ __device__ __forceinline__ void attend_rows(const PromptParams& p, const WarpRow
 // that a row does not see (its tile has them), or sees with a weight that is zero in 16 bits: such a row is computed again from what it
 // sees.  But mostly it sees the NaN, and is right.  The keys that all rows see are gone through once, four columns a lane, from both
 // ends: a NaN or two opposite infinities among the values settle that column of every row, a NaN in a key settles whole rows.
+// `large`: all rows are computed again (see LARGE_REF).
 template <typename T>
-__device__ __forceinline__ void look_again(const PromptParams& p, const WarpRows& rows) {
+__device__ __forceinline__ void look_again(const PromptParams& p, const WarpRows& rows, bool large) {
   const int lane = threadIdx.x & 31, D = p.a.head_dim;
   const Sequence& s = rows.seq;
   const bool holds = lane * 4 < D;
@@ -549,7 +554,19 @@ __device__ __forceinline__ void look_again(const PromptParams& p, const WarpRows
     return nans_of(a.x, a.y, b.x, b.y);
   };
   uint32_t odd = 0, whole = 0, open = 0, found = 0;  // rows with a NaN, rows of nothing else; columns with one, columns whose NaN is seen by all rows
+  const auto attend = [&](uint32_t left) {
+#pragma unroll 1
+    while (left != 0) {
+      uint32_t which = 0;
+      for (int n = 0; n < kAgain && left != 0; ++n) {
+        which |= left & -left;
+        left &= left - 1;
+      }
+      attend_rows<T>(p, rows, which, large);
+    }
+  };
   const int most = min(32, (min(kRows / p.group, s.n - rows.t0)) * p.group - static_cast<int>(threadIdx.x & 96));  // rows that are a query's
+  if (large) odd = most <= 0 ? 0u : 0xffffffffu >> (32 - most);
   uint32_t of_rows[4];  // the lane's four columns of each row, eight rows a word
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -577,7 +594,7 @@ __device__ __forceinline__ void look_again(const PromptParams& p, const WarpRows
   const Seen last = seen_from(p, hi);
   const int first = min(last.first, lo + 1), count = first + max(0, lo + 1 - last.start);
   constexpr int kStep = 16;
-  const int steps = count > 0 ? (count + kStep - 1) / kStep : 0;
+  const int steps = count > 0 && !large ? (count + kStep - 1) / kStep : 0;
   const auto scan = [&](const void* base, int64_t stride, auto take) {  // until `take` says that it has seen enough
 #pragma unroll 1
     for (int n = 0; n < steps; ++n) {
@@ -606,10 +623,10 @@ __device__ __forceinline__ void look_again(const PromptParams& p, const WarpRows
     return !__any_sync(0xffffffffu, (open & ~found) != 0);
   });
   const auto unsettled = [&](int r) { return __any_sync(0xffffffffu, (nans_of_row(r) & ~found) != 0); };
-  uint32_t left = 0;
+  uint32_t left = large ? odd : 0u;
 #pragma unroll 1
-  for (uint32_t rest = odd; rest != 0; rest &= rest - 1) left |= unsettled(__ffs(rest) - 1) ? rest & -rest : 0u;
-  if ((left & whole) != 0) {
+  for (uint32_t rest = large ? 0u : odd; rest != 0; rest &= rest - 1) left |= unsettled(__ffs(rest) - 1) ? rest & -rest : 0u;
+  if (!large && (left & whole) != 0) {
     bool key_nan = false;
     scan(static_cast<const T*>(p.a.k) + s.k0 * p.a.k_token + rows.kvh * p.a.k_head, p.a.k_token, [&](const uint2(&w)[kStep]) {
 #pragma unroll
@@ -619,15 +636,7 @@ __device__ __forceinline__ void look_again(const PromptParams& p, const WarpRows
     });
     if (key_nan) left &= ~whole;
   }
-#pragma unroll 1
-  while (left != 0) {
-    uint32_t which = 0;
-    for (int n = 0; n < kAgain && left != 0; ++n) {
-      which |= left & -left;
-      left &= left - 1;
-    }
-    attend_rows<T>(p, rows, which);
-  }
+  attend(left);
 }
 
 // All units of a block once more, for a warp that met such rows.  Behind everything else: nothing in the block waits for it, however
@@ -635,12 +644,12 @@ __device__ __forceinline__ void look_again(const PromptParams& p, const WarpRows
 // NaN in the first, the 700th, the 2040th value of each sequence: 0.43, 1.1, 1.0 ms, 0.31 without (events around a call); with every
 // such row computed again by itself, in the loop, 101, 92, 17.
 template <typename T, bool SPLIT>
-__device__ __forceinline__ void look_again_at_all(const PromptParams& p) {
+__device__ __forceinline__ void look_again_at_all(const PromptParams& p, bool large) {
   const int i = threadIdx.x >> 7;  // the warp's tile of queries
   Unit u;
 #pragma unroll 1
   for (Units<SPLIT> walk(p); walk.next(p, false, u);)
-    if ((i == 0 || u.second) && u.from == 0) look_again<T>(p, WarpRows{u.seq, u.t0 + i * p.tq, u.kvh});
+    if ((i == 0 || u.second) && u.from == 0) look_again<T>(p, WarpRows{u.seq, u.t0 + i * p.tq, u.kvh}, large);
 }
 
 template <typename T>
@@ -1010,15 +1019,17 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + i * kKeys, o_addr = tmem + lanes + 2 * kKeys + i * DP;
     uint32_t s_uses = 0, o_uses = 0;
-    bool odd = false;  // an output is NaN where it may not be
+    bool odd = false, large = false;  // an output is NaN where it may not be; a reference was too large
     // The outputs of a tile of queries, from its accumulator and sum (with SPLIT, and those of the cluster's other block).
     const auto finish = [&](const Unit& u, float m, float l) {
       const int token = u.t0 + i * p.tq + row_token, head = u.kvh * p.group + row_head;
       const bool row_ok = row_token < p.tq && token < u.seq.n;
       float own = 1.0f, other = 0.0f;  // factors of the two blocks' sums
+      bool far = fabsf(m) >= C::LARGE_REF && m != -INFINITY;
       if constexpr (SPLIT) {
         const float2 ml = ld_cluster_f2(smem_u32(smem) + C::PART_ML + (i * kRows + r) * 8, 1);
         const float top = max3_nan(m, ml.x, ml.x);
+        far |= fabsf(ml.x) >= C::LARGE_REF && ml.x != -INFINITY;
         own = m == top ? 1.0f : exp2f(m - top);
         other = ml.x == top ? 1.0f : exp2f(ml.x - top);
         l = l * own + ml.y * other;
@@ -1076,6 +1087,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       tc_fence_before();  // the next unit's weights are announced behind these reads of the accumulator
       // NaN among the logits that a row sees makes its sum NaN, and with that every output, rightly.  With any other sum:
       odd |= row_ok && again && l == l;
+      large |= row_ok && far;
     };
     Unit u;
     bool mine = false;
@@ -1139,7 +1151,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       if (mine && ok && u.from == 0) finish(u, m, l);
       __syncwarp();
     }
-    if (__any_sync(0xffffffffu, odd && ok)) look_again_at_all<T, SPLIT>(p);
+    large = __any_sync(0xffffffffu, large);
+    if (ok && __any_sync(0xffffffffu, odd || large)) look_again_at_all<T, SPLIT>(p, large);
   }
   if constexpr (SPLIT) {
     __syncwarp();  // the barriers of a cluster are taken by whole warps
