@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
         const float top = fmaxf(m[nt][i], max_of_rows(fmaxf(s[nt][i], s[nt][i + 2])));
         const float keep = top == m[nt][i] ? 1.0f : exp2f(m[nt][i] - top);
         m[nt][i] = top;
-        ref[i] = (top == -INFINITY ? 0.0f : top) - C::SHIFT;
+        ref[i] = top == -INFINITY ? 0.0f : top;
         if (__any_sync(0xffffffffu, keep != 1.0f)) {
           l[nt][i] *= keep;
 #pragma unroll
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[nt][i] = exp2f(s[nt][i] - ref[i & 1]);
+        s[nt][i] = exp2f((s[nt][i] - ref[i & 1]) + C::SHIFT);  // the difference first: exact near the maximum, however large that is
         l[nt][i & 1] += s[nt][i];
       }
       pf[nt][0] = transpose8x8(pack16<C::BF16>(s[nt][0], s[nt][1]));

@@ -33,7 +33,7 @@ def _check(got, q, k, v, scale, first, dtype, what):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("size", [30.0, 1e3, 1e4, 6e4, 1e6, 1e12, 1e18])
 @pytest.mark.parametrize("rising", [False, True])
-@pytest.mark.parametrize("which", ["prompt"])
+@pytest.mark.parametrize("which", ["prompt", "token", "token, e4m3"])
 def test_large_logits(cuda_dev, dtype, size, rising, which):
     if dtype == torch.float16 and size > 65504:
         pytest.skip("not an fp16 number")
