@@ -562,7 +562,7 @@ class W8A8Decoder:
     @torch.no_grad()
     def generate(self, prompts, new_tokens, cache: Optional[PagedKVCache] = None, cache_dtype=torch.bfloat16, page_size=64):
         """Greedy generation: ``new_tokens`` ids [batch, new_tokens] behind each of ``prompts`` (1-D id tensors, lengths as they come).
-        ``cache``: an empty ``PagedKVCache`` for as many sequences; by default one of ``cache_dtype`` (bfloat16, or float8_e4m3fn
+        ``cache``: an empty ``PagedKVCache`` for as many sequences, with room for what they come to; by default one of ``cache_dtype`` (bfloat16, or float8_e4m3fn
         codes) is made.  ``self.last_hidden`` keeps the last step's final hidden states."""
         if self.surface != "fused" or self.world != 1:
             raise RuntimeError("generate runs on one GPU with the fused surface")
@@ -574,8 +574,7 @@ class W8A8Decoder:
             raise RuntimeError(f"{longest} tokens are more than the {self.cos.shape[0]} positions of cfg['seq']")
         if cache is None:
             cache = PagedKVCache(len(self.layers), len(lengths), longest, self.nkv, self.cfg["head_dim"], self.dev, cache_dtype, page_size)
-        if cache.batch != len(lengths) or len(cache.k) != len(self.layers):
-            raise RuntimeError("the cache is for another number of sequences or layers")
+        self._check_cache(cache, lengths, new_tokens)
         ids, step, out = torch.cat([p.reshape(-1) for p in prompts]).to(self.dev), cache.prompts(lengths), []
         while True:
             ids, self.last_hidden = self._drive([self._forward_steps(ids, self._attend_cached(cache, step), step.last)])
@@ -583,6 +582,19 @@ class W8A8Decoder:
             if len(out) == new_tokens:
                 return torch.stack(out, 1)
             step = cache.token()
+
+    def _check_cache(self, cache, lengths, new_tokens):
+        """Refuses a cache that does not fit the model or the whole generation, before anything runs."""
+        if cache.batch != len(lengths) or len(cache.k) != len(self.layers):
+            raise RuntimeError("the cache is for another number of sequences or layers")
+        _, kv_heads, _, head_dim = cache.k[0].shape
+        if (kv_heads, head_dim) != (self.nkv, self.cfg["head_dim"]):
+            raise RuntimeError(f"the cache has {kv_heads} kv heads of {head_dim}, the model {self.nkv} of {self.cfg['head_dim']}")
+        if cache.k[0].dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise RuntimeError("the cache must hold bfloat16 or float8_e4m3fn")
+        if any(cache.host_lens):
+            raise RuntimeError("generate starts with an empty cache: release its sequences first")
+        cache.check([n + new_tokens - 1 for n in lengths])
 
     def _drive(self, gens):
         """Advances the groups round-robin, one segment at a time, each on its own stream."""

@@ -58,13 +58,18 @@ class PagedKVCache:
         """The keyword arguments of layer ``i`` for ``ops.qk_norm_rope`` (and, without the slots, ``ops.paged_attention``)."""
         return dict(k_pages=self.k[i], v_pages=self.v[i], k_scale=self.k_scale[i], v_scale=self.v_scale[i])
 
-    def reserve(self, lengths: Sequence[int]) -> None:
-        """Hands out the pages for sequences of these lengths.  Refused as a whole where the pool does not hold them."""
+    def check(self, lengths: Sequence[int]) -> List[int]:
+        """Refuses lengths that the cache cannot hold; otherwise the pages that every sequence still needs for them."""
         need = [max(0, -(-int(n) // self.page_size) - len(own)) for n, own in zip(lengths, self._owned)]
         if any(n > self.max_len for n in lengths):
             raise RuntimeError(f"a sequence of {max(lengths)} tokens does not fit a cache of {self.max_len}")
         if sum(need) > len(self._free):
             raise RuntimeError(f"the cache is out of pages: {sum(need)} wanted, {len(self._free)} free")
+        return need
+
+    def reserve(self, lengths: Sequence[int]) -> None:
+        """Hands out the pages for sequences of these lengths.  Refused as a whole where the pool does not hold them."""
+        need = self.check(lengths)
         rows, columns, pages = [], [], []
         for b, n in enumerate(need):
             rows += [b] * n

@@ -103,3 +103,29 @@ def test_what_is_sent_without_waiting_is_not_overwritten(cuda_dev):
     for i, step in enumerate(steps):
         assert step.positions.tolist() == [1 + i, 2 + i, 3 + i, 4 + i]
         assert step.slots.tolist() == [cache._owned[b][1 + b + i] for b in range(4)]
+
+
+def test_generate_looks_at_a_given_cache_before_it_runs(cuda_dev):
+    """A cache that cannot take the whole generation is refused before the prompts are computed, and left as it was."""
+    from fms_model_optimizer_b200.decoder import W8A8Decoder
+
+    cfg = dict(layers=1, hidden=256, q_heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=512, rope_theta=10000.0, batch=2, seq=64)
+    model = W8A8Decoder(cfg, cuda_dev)
+    prompts = [torch.arange(n, device=cuda_dev) for n in (5, 9)]
+    make = lambda **kw: PagedKVCache(**{**dict(layers=1, batch=2, max_len=20, kv_heads=2, head_dim=64, dev=cuda_dev, page_size=8), **kw})  # noqa: E731
+    ran = []
+    model._forward_steps, steps = lambda *a: ran.append(1) or steps(*a), model._forward_steps
+    busy = make()
+    busy.prompts([3, 4])
+    for cache, match in ((make(max_len=18), "20"), (make(pages=4), "pages"), (make(kv_heads=4), "heads"), (make(head_dim=128), "heads"), (make(dtype=torch.float16), "bfloat16"),
+                         (make(layers=2), "another number"), (busy, "release")):  # fmt: skip
+        before = list(cache.host_lens), len(cache._free)
+        with pytest.raises(RuntimeError, match=match):
+            model.generate(prompts, 12, cache=cache)
+        assert not ran and (list(cache.host_lens), len(cache._free)) == before
+    cache = make(pages=5)
+    out = model.generate(prompts, 12, cache=cache)
+    assert cache.host_lens == [16, 20] and torch.equal(out, model.generate(prompts, 12))
+    for b in range(2):  # and once more in the same cache
+        cache.release(b)
+    assert torch.equal(out, model.generate(prompts, 12, cache=cache))
