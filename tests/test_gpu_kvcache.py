@@ -129,3 +129,31 @@ def test_generate_looks_at_a_given_cache_before_it_runs(cuda_dev):
     for b in range(2):  # and once more in the same cache
         cache.release(b)
     assert torch.equal(out, model.generate(prompts, 12, cache=cache))
+
+
+def test_a_prompt_alone_and_in_a_batch(cuda_dev):
+    """The last hidden state behind a prompt, and behind five tokens that both runs read: what differs is the order of sums in the
+    attention, split by the number of sequences, and the int8 codes that flip by one with it (two layers under two roundings differ by 4.4 %)."""
+    from fms_model_optimizer_b200.decoder import W8A8Decoder
+
+    cfg = dict(layers=2, hidden=1024, q_heads=8, kv_heads=2, head_dim=128, ffn=2048, vocab=2048, rope_theta=10000.0, batch=3, seq=256)
+    model = W8A8Decoder(cfg, cuda_dev)
+    g = torch.Generator().manual_seed(22)
+    prompts = [torch.randint(0, 2048, (n,), generator=g).to(cuda_dev) for n in (37, 1, 130)]
+
+    def hidden(prompts, tail):
+        cache = PagedKVCache(2, len(prompts), 256, 2, 128, cuda_dev, page_size=16)
+        ids, step = torch.cat(prompts), cache.prompts([p.numel() for p in prompts])
+        out = []
+        for t in [*tail, None]:
+            _, h = model._drive([model._forward_steps(ids, model._attend_cached(cache, step), step.last)])
+            out.append(h.float())
+            if t is not None:
+                ids, step = t.to(cuda_dev), cache.token()
+        return torch.stack(out)
+
+    tail = [torch.randint(0, 2048, (3,), generator=g) for _ in range(5)]
+    batch = hidden(prompts, tail)
+    for b, p in enumerate(prompts):
+        alone = hidden([p], [t[b : b + 1] for t in tail])[:, 0]
+        assert bool(((alone - batch[:, b]).norm(dim=-1) < 0.09 * alone.norm(dim=-1)).all()), b
