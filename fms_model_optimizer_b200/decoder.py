@@ -259,7 +259,7 @@ class W8A8Decoder:
 
     # ------------------------------------------------------------------------------------------------ helpers
     def _note(self, tag, layer, t):
-        if self.trace is not None:
+        if self.trace is not None and t is not None:
             self.trace.append((tag, layer, t.detach().clone()))
 
     def _attention(self, q, k, v, B, S):

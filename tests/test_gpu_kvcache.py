@@ -157,3 +157,16 @@ def test_a_prompt_alone_and_in_a_batch(cuda_dev):
     for b, p in enumerate(prompts):
         alone = hidden([p], [t[b : b + 1] for t in tail])[:, 0]
         assert bool(((alone - batch[:, b]).norm(dim=-1) < 0.09 * alone.norm(dim=-1)).all()), b
+
+
+def test_generation_can_be_traced(cuda_dev):
+    from fms_model_optimizer_b200.decoder import W8A8Decoder
+
+    cfg = dict(layers=2, hidden=256, q_heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=512, rope_theta=10000.0, batch=2, seq=64)
+    model = W8A8Decoder(cfg, cuda_dev)
+    prompts = [torch.arange(n, device=cuda_dev) for n in (5, 9)]
+    want = model.generate(prompts, 3)
+    model.trace = []
+    assert torch.equal(model.generate(prompts, 3), want)
+    rows = [t.shape[0] for tag, li, t in model.trace if tag == "attn" and li == 1]
+    assert rows == [14, 2, 2] and len([1 for tag, li, _ in model.trace if tag == "k_rope" and li == 0]) == 1  # single tokens' keys go to the cache alone
