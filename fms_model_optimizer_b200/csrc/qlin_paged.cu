@@ -335,6 +335,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
       for (int i = 0; i < 4; ++i) {
         s[nt][i] = exp2f((s[nt][i] - ref[i & 1]) + C::SHIFT);  // the difference first: exact near the maximum, however large that is
         l[nt][i & 1] += s[nt][i];
+        // not to zero in fp16, so that an infinite value stays one (e4m3 has none); NaN is in the sum
+        if constexpr (!F8 && !C::BF16) s[nt][i] = fmaxf(s[nt][i], 0x1p-24f);
       }
       pf[nt][0] = transpose8x8(pack16<C::BF16>(s[nt][0], s[nt][1]));
       pf[nt][1] = transpose8x8(pack16<C::BF16>(s[nt][2], s[nt][3]));

@@ -58,3 +58,23 @@ def test_large_logits(cuda_dev, dtype, size, rising, which):
         token = ops.paged_attention(q[-1:], *pages, table, lens, **scales)
         _check(token, q[-1:], *(t[0, 0].float() for t in pages), dim**-0.5, m - 1, dtype, which)
     ops.check_status(cuda_dev)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [20, 700, 9000])
+def test_an_infinite_value_of_small_weight(cuda_dev, dtype, n):
+    """A value of infinity that is seen with a weight of 2^-58, too small for 16 bits: the output is infinite, not 0 * infinity."""
+    g = torch.Generator(device=cuda_dev).manual_seed(42)
+    dim = 64
+    q, k, v = torch.zeros(1, 2, dim, device=cuda_dev), torch.zeros(n, 1, dim, device=cuda_dev), torch.randn(n, 1, dim, generator=g, device=cuda_dev)
+    q[..., 0] = 8  # logits of the first element
+    k[:, :, 0] = torch.rand(n, 1, generator=g, device=cuda_dev)
+    at = n // 3
+    k[at] = 0
+    k[at, :, 0] = -40
+    v[at, :, 3] = torch.inf
+    q, k, v = (t.to(dtype) for t in (q, k, v))
+    cu_q, cu_k = (torch.tensor([0, x], dtype=torch.int32, device=cuda_dev) for x in (1, n))
+    pages = [t.transpose(0, 1)[None].contiguous() for t in (k, v)]
+    for got in (ops.prompt_attention(q, k, v, cu_q, cu_k, 1), ops.paged_attention(q, *pages, torch.zeros(1, 1, dtype=torch.int32, device=cuda_dev), cu_k[1:])):
+        assert bool((got[..., 3] == torch.inf).all()) and int(got.isfinite().sum()) == 2 * (dim - 1)
