@@ -17,9 +17,10 @@
 // order of the 16 head dimensions of a step is permuted, the same way in Q (keys) and in the rows of O^T (values).  A bf16 query
 // meets them as fp16 times a power of two that brings its largest element to 2^13..2^14: no digit of it is lost above 2^-27 of the largest.
 //
-// Measured (device time): 1 x 131072 keys of 8 heads of 128 in bf16 87 us, 6.1 TB/s; 61 x 2050 78.5 us, 6.5 TB/s; 61 x up to 4099 in e4m3
-// 52 us, 5.0 TB/s, where the chain of conversions, products and shuffles of a tile is as long as its loads; 1 x 2048 6.7 us, which is
-// the latency of the length, the page table, the keys and the join behind one another.
+// Measured (device time): 1 x 131072 keys of 8 heads of 128 in bf16 87 us, 6.1 TB/s; 61 x 2050 78 us, 6.5 TB/s; 61 x up to 4099 79 us, 6.6 TB/s,
+// and in e4m3 53 us, 4.9 TB/s, where the chain of conversions, products and shuffles of a tile is as long as its loads; 1 x 2048 6.9 us,
+// which is the latency of the length, the page table, the keys and the join behind one another.  A batch of very unequal lengths takes as long as
+// its longest sequence does in the few blocks that the split of all leaves it: 63 x 500 and one of 100000 1128 us, the bytes 82.
 //
 // Statistics, sums and the join are fp32.  Weights are rounded to the cache's 16-bit type (fp16 with an e4m3 cache) as operands of
 // the product; fp16 weights carry a factor of 2^12, so that weights down to 2^-26 of the largest keep 11 bits.
@@ -36,7 +37,7 @@ namespace qlin {
 constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kTileKeys = 16;
-constexpr int kMinTiles = 4;       // tiles of a block at least, one a warp (1 x 2048 keys 6.7 us; with eight 7.6)
+constexpr int kMinTiles = 4;       // tiles of a block at least, one a warp (with eight 1 x 2048 keys take 0.9 us more)
 
 struct PagedParams {
   qlin_paged_attention_args a;
@@ -129,7 +130,7 @@ struct PagedCfg {
   static constexpr int STAGE = 2 * kTileKeys * RB;     // keys, then values
   // Three stages at least; where they are small, 16 KB a warp, so that a third block fits the SM: its warps cover the latency of the
   // chain from a tile's keys to its outputs (3 x up to 30000 keys in e4m3 32 us, 37 with two).  16-bit rows of 128 run as fast as
-  // memory does with two blocks of three stages (61 x 2050 keys 78.5 us, three blocks of two stages 95).
+  // memory does with two blocks of three stages (61 x 2050 keys 78 us, three blocks of two stages 95).
   static constexpr int RING = STAGE >= 8192 ? 24576 : 16384;
   static constexpr int STAGES = RING / STAGE;
   static constexpr int BLOCKS = NT == 1 && RING == 16384 ? 3 : 2;  // an SM
@@ -519,9 +520,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
 
 // Splits of the keys: blocks for every SM, none with fewer than kMinTiles tiles where the page table is as wide as its longest
 // sequence.  Up to kClusterSplits of them (a power of two) are a cluster of blocks, which joins without a second launch and without
-// a workspace; few heads with long tables take more.  Blocks an SM, device time: 16-bit caches two (1 x 131072 keys 83 us, with
-// three 100, with six 90); e4m3 three, and up to nine where they join in a cluster, which evens out ragged batches (61 x up to 4099
-// keys 59 us unsplit, 52 in pairs, 68 in fours; 3 x up to 30000 keys with two blocks 37, three 32, six 32).
+// a workspace; few heads with long tables take more.  Blocks an SM, device time: 16-bit caches two (1 x 131072 keys 86 us, with
+// three 90, with six 94; 61 x 2050 78, 78, 93; 61 x up to 4099 79, 79, 86; 16 x up to 8000 47, 47, 59); e4m3 three, and up to nine where they
+// join in a cluster, which evens out ragged batches (61 x up to 4099 keys 60 us unsplit, 53 in pairs, 67 in fours; 32 x up to 8000 58 in
+// pairs and in fours, 77 in eights; 3 x up to 30000, which join over the workspace, 37 with two blocks, 32 with three and six).
 constexpr int kClusterSplits = 8;
 struct Splits {
   int32_t n, cluster;

@@ -6,14 +6,15 @@
 // keys.  A tile's rows are 128 / G queries times the G query heads that share the kv head, so grouped heads share each load and a
 // tile spans few positions, which keeps what the mask throws away small.  S = Q K^T on tcgen05 with both operands in shared memory, one
 // thread for each row of 128 logits in tensor memory, the weights back to tensor memory over their logits in 16 bits, O += P V
-// with the weights as the operand from there.  Tensor memory is full: two S of 128 columns, two O of head_dim.  The tiles take turns, one in the softmax
+// with the weights as the operand from there.  At head_dim 128 tensor memory is full: two S of 128 columns, two O of head_dim.  The tiles take turns, one in the softmax
 // while the other is in the tensor core.
 //
 // What bounds it: that chain.  A turn (two tiles against 128 keys) is 2048 cycles of tensor core and 2048 of exponentials (two
-// tiles x 128 a thread x 8 cycles), and takes about 4200: the exponentials of a tile and its products follow one another, and the
-// third pair of buffers that would let a tile's next logits be made meanwhile does not fit.  Measured (device time): 8 x 2048, 32 + 8 heads
-// of 128 in bf16 280 us, 980 TFLOP/s = 0.60 of the measured rate; 1 x 8191 under a window of 2048 with four first keys 243 us,
-// 990; 5 x up to 333 after 77, 12 heads of 64 in fp16 13 us, four turns behind a cold start.  With exponentials, maxima and masks left
+// tiles x 128 a thread x 8 cycles), and takes about 4100: the exponentials of a tile and its products follow one another, and the
+// third pair of buffers that would let a tile's next logits be made meanwhile does not fit (at 64 it would).  The operands that the products
+// read from shared memory and the tiles that arrive there are some 256 KB a turn, about 2048 cycles more beside them.  Measured (device time): 8 x 2048, 32 + 8 heads
+// of 128 in bf16 280 us, 980 TFLOP/s = 0.60 of the measured rate; 1 x 8191 under a window of 2048 with four first keys 242 us,
+// 995; 5 x up to 333 after 77, 12 heads of 64 in fp16 13 us, four turns behind a cold start.  With exponentials, maxima and masks left
 // out the first two would take 252 and 204: what else is in a turn is loads and stores of tensor memory, conversions and hand-overs.
 // Tried and slower, 8 x 2048 in us at the time: a warp for each tile's products 340 against 290 (both tiles fall into step and wait
 // together), the same with the tensor core handed from one to the other 299, all of a tile's weights in one hand-over 307, logits read
@@ -262,7 +263,7 @@ struct Unit {
   bool second;     // the second tile has rows
   // Tiles of the window, then those of the first keys.  Under a window the tile at its edge comes last of the former: a row that sees few
   // keys of its first tile has a low reference, and the next tile would rewrite its accumulator (1 x 8191 under a window of 2048
-  // with four first keys in front: a rewrite for every 13th tile of a warp, 277 us; 243 so).
+  // with four first keys in front: a rewrite for every 13th tile of a warp, 277 us; 242 so).
   __device__ __forceinline__ int key0(int n) const {
     const int t = n * every + from;
     if (t >= win_tiles) return (t - win_tiles) * kKeys;
@@ -270,8 +271,8 @@ struct Unit {
     return (win_tile + (t + 1 == win_tiles ? 0 : t + 1)) * kKeys;
   }
 };
-// The units of a block, every gridDim.x-th one of the list that begins with the last queries of every sequence and head, which see
-// the most keys.  `busy`: units without keys are passed over.  SPLIT: one unit for the two blocks of a cluster, which share out its keys.
+// The units of a block, every gridDim.x-th one of the list that begins with the last queries of the longest prompts, which see the
+// most keys unless others have more in front of them.  `busy`: units without keys are passed over.  SPLIT: one unit for the two blocks of a cluster, which share out its keys.
 template <bool SPLIT>
 struct Units {
   uint32_t id, step, total;
@@ -1234,9 +1235,9 @@ static int launch_prompt(const PromptParams& p, cudaStream_t stream) {
   const int64_t blocks = static_cast<int64_t>(p.units) * p.a.kv_heads * p.a.batch;
   if (blocks > 0x7fffffff) return fail(QLIN_ERR_TOO_LARGE, "qlin_prompt_attention: too many queries, heads and sequences");
   // Units that leave half of the SMs idle are split over two blocks where the longest has kSplitTiles tiles of keys (as far as the host
-  // knows: the earlier keys are taken as evenly spread).  Device time without and with: 1200 queries of 12 heads of 64 (10 tiles) 23.7 and 19.7 us,
-  // 2000 of 8 + 1 heads of 96 35.7 and 30.4, 16 after 2900 of 32 + 8 heads of 128 41.0 and 26.3; 40 after 900 (8 tiles) 20.8 and 22.4.
-  // Four blocks lose more in the join than they save (64 after 2900 of 8 + 2 heads 39 in two, 59 in four).
+  // knows: the earlier keys are taken as evenly spread).  Device time without and with: 1200 queries of 12 heads of 64 (10 tiles) 24.4 and 19.8 us,
+  // 2000 of 8 + 1 heads of 96 36.3 and 30.7, 16 after 2900 of 32 + 8 heads of 128 41.8 and 29.4; 40 after 900 (8 tiles) 21.6 and 22.4.
+  // Four blocks lose more in the join, which one of them does alone, than they save (64 after 2900 of 8 + 2 heads 50 in one, 37 in two, 59 in four).
   int64_t keys = p.a.max_q + (p.a.tokens_k > p.a.tokens_q ? (p.a.tokens_k - p.a.tokens_q) / p.a.batch : 0);
   const int64_t seen = static_cast<int64_t>(p.a.window) + p.a.sinks + 2 * p.tq;
   if (p.a.window > 0 && keys > seen) keys = seen;

@@ -8,7 +8,7 @@
 // chunks that the rotation pairs (or two neighbouring ones behind the rotated part), so the rotation stays inside the lane and
 // only the sum of squares crosses lanes.  Everything is fp32 between the load and the one rounding of each output; the e4m3 code
 // is made from the unrounded value.  Measured (device time): 16384 tokens of 32 + 8 heads of 128 in bf16 with cache 87 us, 5.1 TB/s =
-// 0.78 of the copy rate; 1 token 3.4 us, a position, a row of cos and sin and a launch behind one another.
+// 0.78 of the copy rate; 1 token 3.5 us, a position, a row of cos and sin and a launch behind one another.
 #include <type_traits>
 
 #include <cuda_bf16.h>

@@ -32,7 +32,8 @@ class PagedKVCache:
     def __init__(self, layers: int, batch: int, max_len: int, kv_heads: int, head_dim: int, dev, dtype: torch.dtype = torch.bfloat16, page_size: int = 64,
                  pages: Optional[int] = None):  # fmt: skip
         """``max_len``: the most tokens of a sequence.  ``pages``: size of the pool, by default enough for all sequences at full
-        length.  ``dtype`` float8_e4m3fn holds codes with one fp32 scale per layer and kv head (``k_scale`` / ``v_scale``, 1 at first)."""
+        length.  ``dtype`` float8_e4m3fn holds codes with one fp32 scale per layer and kv head: ``k_scale[layer]`` and ``v_scale[layer]`` are ones until the caller sets them
+        (largest magnitude / 448), before the first token is written."""
         if min(layers, batch, max_len, page_size) < 1:
             raise RuntimeError("layers, batch, max_len and page_size must be positive")
         if dtype not in (torch.bfloat16, torch.float16, torch.float8_e4m3fn):
