@@ -125,7 +125,7 @@ struct PromptCfg {
   static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(PromptAux));
   static constexpr float SHIFT = std::is_same<T, __half>::value ? 6.0f : 0.0f;
   // A weight is 2^(x cl2 - r) with r rounded and the product not, so half a unit of r's last place and more is in its exponent, the same for all
-  // keys of a row.  From these references on (logits of 2.9e6 in fp16, 3.7e8 in bf16) that could carry weights out of 16 bits: rows that end with one are
+  // keys of a row.  From these references on (logits of 2.9e6 in fp16, 3.7e8 in bf16) that could carry weights out of 16 bits: rows that meet one are
   // computed again, with the difference taken first.
   static constexpr float LARGE_REF = std::is_same<T, __half>::value ? 0x1p22f : 0x1p29f;
   static constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
@@ -717,7 +717,8 @@ __device__ __forceinline__ uint32_t columns_under(int n, int from) { return n <=
 // each half is handed to the product when it is there.  The first quarter is made relative to the reference of the tiles before
 // while the maximum is still being looked for, and made again where that has outgrown the reference.
 template <typename T, int DP, bool MASKED>
-__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, float cl2, int hi, int lo, int sinks, bool first, bool live, uint64_t* p_full, float& m, float& l) {
+__device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, float cl2, int hi, int lo, int sinks, bool first, bool live, uint64_t* p_full, float& m, float& l,
+                                             bool& far) {
   using C = PromptCfg<T, DP>;
   uint32_t x[4][32], w[16];
   // column j is seen when j <= hi and (j > lo or j < sinks)
@@ -801,6 +802,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, uint32_t o_addr, f
       }
     }
     m = next;
+    far |= live && fabsf(m) >= C::LARGE_REF && m != -INFINITY;
     sum[0] = sum[1] = 0;
     weigh<T, 0, 16>(x, cl22, reference(), sum, nothing, keep_words);
   }
@@ -1022,15 +1024,14 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     uint32_t s_uses = 0, o_uses = 0;
     bool odd = false, large = false;  // an output is NaN where it may not be; a reference was too large
     // The outputs of a tile of queries, from its accumulator and sum (with SPLIT, and those of the cluster's other block).
-    const auto finish = [&](const Unit& u, float m, float l) {
+    const auto finish = [&](const Unit& u, float m, float l, bool far) {
       const int token = u.t0 + i * p.tq + row_token, head = u.kvh * p.group + row_head;
       const bool row_ok = row_token < p.tq && token < u.seq.n;
       float own = 1.0f, other = 0.0f;  // factors of the two blocks' sums
-      bool far = fabsf(m) >= C::LARGE_REF && m != -INFINITY;
       if constexpr (SPLIT) {
         const float2 ml = ld_cluster_f2(smem_u32(smem) + C::PART_ML + (i * kRows + r) * 8, 1);
         const float top = max3_nan(m, ml.x, ml.x);
-        far |= fabsf(ml.x) >= C::LARGE_REF && ml.x != -INFINITY;
+        far |= ml.x == INFINITY;
         own = m == top ? 1.0f : exp2f(m - top);
         other = ml.x == top ? 1.0f : exp2f(ml.x - top);
         l = l * own + ml.y * other;
@@ -1088,11 +1089,12 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       tc_fence_before();  // the next unit's weights are announced behind these reads of the accumulator
       // NaN among the logits that a row sees makes its sum NaN, and with that every output, rightly.  With any other sum:
       odd |= row_ok && again && l == l;
-      large |= row_ok && far;
+      large |= far;
     };
     Unit u;
     bool mine = false;
     float m, l;
+    bool far = false;  // a reference of this row was too large, if only at first
     for (Units<SPLIT> walk(p); ok && walk.next(p, false, u);) {
       if (i == 1 && !u.second) continue;
       mine = true;
@@ -1102,6 +1104,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       const int tile_lo = u.t0 + i * p.tq + u.shift, tile_hi = tile_lo + p.tq - 1;  // positions of this tile of queries
       m = -INFINITY;
       l = 0.0f;
+      far = false;
       for (int t = 0; t < u.tiles && ok; ++t) {
         ok = uniform_wait(&aux->s_full[i], s_uses & 1, abort_flag);
         if (!ok) break;
@@ -1110,9 +1113,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         const int k0 = u.key0(t);
         const bool full = k0 + kKeys - 1 <= tile_lo && (p.a.window <= 0 || k0 > tile_hi - p.a.window || k0 + kKeys <= p.a.sinks);
         if (full) {
-          softmax_tile<T, DP, false>(s_addr, o_addr, p.cl2, 0, 0, 0, t == 0, row_ok, aux->p_full[i], m, l);
+          softmax_tile<T, DP, false>(s_addr, o_addr, p.cl2, 0, 0, 0, t == 0, row_ok, aux->p_full[i], m, l, far);
         } else {
-          softmax_tile<T, DP, true>(s_addr, o_addr, p.cl2, pos - k0, p.a.window > 0 ? pos - p.a.window - k0 : -1, p.a.sinks - k0, t == 0, row_ok, aux->p_full[i], m, l);
+          softmax_tile<T, DP, true>(s_addr, o_addr, p.cl2, pos - k0, p.a.window > 0 ? pos - p.a.window - k0 : -1, p.a.sinks - k0, t == 0, row_ok, aux->p_full[i], m, l, far);
         }
       }
       if (ok && u.tiles > 0) {
@@ -1122,7 +1125,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       if (!ok) break;
       tc_fence_after();
       if constexpr (!SPLIT) {
-        finish(u, m, l);
+        finish(u, m, l, far);
       } else {
         // the other tile's products may still read what the sums go over
         if (u.second && u.tiles > 0) ok = uniform_wait(&aux->o_full[1 - i], 0, abort_flag);
@@ -1138,7 +1141,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(smem + C::part_o(i * kRows + r, 4 * c + j / 4)) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
-          *reinterpret_cast<float2*>(smem + C::PART_ML + (i * kRows + r) * 8) = make_float2(m, l);
+          *reinterpret_cast<float2*>(smem + C::PART_ML + (i * kRows + r) * 8) = make_float2(far ? INFINITY : m, l);
         }
       }
     }
@@ -1149,7 +1152,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     __syncwarp();
     if constexpr (SPLIT) {
       cluster_arrive_wait();
-      if (mine && ok && u.from == 0) finish(u, m, l);
+      if (mine && ok && u.from == 0) finish(u, m, l, far);
       __syncwarp();
     }
     large = __any_sync(0xffffffffu, large);

@@ -78,3 +78,26 @@ def test_an_infinite_value_of_small_weight(cuda_dev, dtype, n):
     pages = [t.transpose(0, 1)[None].contiguous() for t in (k, v)]
     for got in (ops.prompt_attention(q, k, v, cu_q, cu_k, 1), ops.paged_attention(q, *pages, torch.zeros(1, 1, dtype=torch.int32, device=cuda_dev), cu_k[1:])):
         assert bool((got[..., 3] == torch.inf).all()) and int(got.isfinite().sum()) == 2 * (dim - 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [1e3, 6e4, 1e15])
+@pytest.mark.parametrize("n,m,hq", [(300, 300, 2), (40, 3000, 8), (1500, 1500, 8)])
+def test_keys_far_below_the_others_come_first(cuda_dev, dtype, size, n, m, hq):
+    """Logits of -size^2 for the first keys and ordinary ones behind: those that see an ordinary key are as without the others."""
+    if dtype == torch.float16 and size > 65504:
+        pytest.skip("not an fp16 number")
+    g = torch.Generator(device=cuda_dev).manual_seed(43)
+    dim, low = 64, m - n + 2 * n // 3
+    q, k, v = (torch.randn(rows, h, dim, generator=g, device=cuda_dev).to(dtype) for rows, h in ((n, hq), (m, 1), (m, 1)))
+    q[..., 0] = size
+    k[..., 0] = 0
+    k[:low, :, 0] = -size
+    cu = [torch.tensor([0, x], dtype=torch.int32, device=cuda_dev) for x in (n, m)]
+    got = ops.prompt_attention(q, k, v, *cu, n)
+    keep, part = low - (m - n), n - (low - (m - n))
+    rest = ops.prompt_attention(q[keep:].contiguous(), k[low:].contiguous(), v[low:].contiguous(), *(torch.tensor([0, part], dtype=torch.int32, device=cuda_dev),) * 2, part)
+    assert not got.isnan().any()
+    # two ways of one row, each with weights and output in 16 bits
+    assert float((got[keep:].float() - rest.float()).abs().max()) <= 4 * U[dtype] * float(v.float().abs().max())
+    ops.check_status(cuda_dev)
