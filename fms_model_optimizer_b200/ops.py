@@ -638,8 +638,8 @@ def qk_norm_rope(
     cache, in one pass (``qlin_qk_rope``).  ``q [tokens, q heads, head_dim]``, ``k`` and ``v [tokens, kv heads, head_dim]``;
     ``cos`` / ``sin`` fp32 ``[positions, rotary / 2]`` (``rotary`` <= head_dim, halves rotated as in ``rope_``), ``positions``
     int32 ``[tokens]``.  With ``k_pages`` / ``v_pages [pages, kv heads, page size, head_dim]`` given, token t goes to slot
-    ``slots[t] = page * page size + offset`` (int64, negative: not written), in the model's type or as e4m3 codes of
-    ``x / k_scale[kv head]``.  Returns new ``(q, k)``; ``k`` is None without ``want_k``.  No gradient."""
+    ``slots[t] = page * page size + offset`` (int64, negative: not written; different for different tokens), in the model's type or as e4m3
+    codes of ``x / k_scale[kv head]``.  Returns new ``(q, k)``; ``k`` is None without ``want_k``.  No gradient."""
     return _call("qk_rope", 0.0, q.device, L.host().qk_rope, q, k, cos, sin, positions, q_weight, k_weight, eps, v, k_pages, v_pages, slots, k_scale, v_scale, want_k)
 
 

@@ -643,7 +643,7 @@ int qlin_qat_product(const qlin_qat_args* args, int32_t which, void* stream);
  * page * page_size + offset.  Sequence b keeps its key i in page block_table[b, i / page_size], offset i % page_size.
  *
  * Mask of both attentions: a query at position p sees the keys j <= p with window <= 0 or j > p - window or j < sinks.  A query
- * that sees no key, or whose visible logits are all minus infinity, gives zeros; what is not visible is not part of the result, NaN
+ * that sees no key, or whose visible logits are all minus infinity, gives zeros whatever the values hold; what is not visible is not part of the result, NaN
  * and infinities included.
  * ---------------------------------------------------------------------------------------------- */
 
@@ -653,7 +653,7 @@ int qlin_qat_product(const qlin_qat_args* args, int32_t which, void* stream);
  * in fp32, rounded once; cos / sin are rows positions[t] of [table_rows, r/2] fp32 tables.  q_out and k_out (optional) are dense
  * [tokens, heads, head_dim]; with k_pages given, z of the keys and v go to slot slots[t] of the cache (negative: not written),
  * e4m3 as the code of x * (1 / scale) clamped to +-448.  A position or slot out of range writes QLIN_ERR_BAD_SHAPE to *status;
- * a token with such a position gets NaN in q_out and k_out and stays out of the cache.
+ * a token with such a position gets NaN in q_out and k_out and stays out of the cache.  Tokens have different slots, and slots memory of their own.
  * head_dim and rotary are multiples of 16, head_dim <= 512; rows of every tensor start on 16 bytes. */
 typedef struct qlin_qk_rope_args {
   const void* q;
