@@ -32,29 +32,29 @@ def _shared(name, groups, each, prefix, longest, ragged, q_heads, kv_heads, head
 def listed():
     return [
         # the latest token of one sequence of the benchmark's decoder with five alternatives: a generated token's latency
-        _score("score, 1 x 128256, top 5", 1, 128256, "bf16", 5, 0, 0.0, False),
+        _score("score 1 x 128256 top 5", 1, 128256, "bf16", 5, 0, 0.0, False),
         # a decode batch with twenty alternatives
-        _score("score, 64 x 128256, top 20", 64, 128256, "bf16", 20, 0, 0.0, False),
+        _score("score 64 x 128256 top 20", 64, 128256, "bf16", 20, 0, 0.0, False),
         # two prompts of the benchmark's length scored for their perplexity
-        _score("score, 4096 x 128256", 4096, 128256, "bf16", 0, 0, 0.0, False),
+        _score("score 4096 x 128256", 4096, 128256, "bf16", 0, 0, 0.0, False),
         # a training step's loss: forward and the logits' gradient, some rows padding
-        _score("gradient, 2048 x 128256", 2048, 128256, "bf16", 0, 0, 0.1, True),
+        _score("gradient 2048 x 128256", 2048, 128256, "bf16", 0, 0, 0.1, True),
         # an odd vocabulary in fp32, where a grammar leaves few tokens
-        _score("score, 333 x 50257 fp32, 9 allowed", 333, 50257, "fp32", 20, 9, 0.0, False),
+        _score("score 333 x 50257 fp32 9 allowed", 333, 50257, "fp32", 20, 9, 0.0, False),
         # one token of one request: the latency beside a projection
-        _adapt("adapter, 1 token", 1, 0, 4, 16, 4096, 4096, "bf16", 0.0),
+        _adapt("adapter 1 token", 1, 0, 4, 16, 4096, 4096, "bf16", 0.0),
         # a decode batch of many adapters beside a wide projection
-        _adapt("adapter, 64 tokens of 16", 64, 0, 16, 16, 4096, 14336, "bf16", 0.1),
+        _adapt("adapter 64 tokens of 16", 64, 0, 16, 16, 4096, 14336, "bf16", 0.1),
         # the benchmark's prompts, an adapter each
-        _adapt("adapter, 8 prompts of 2048", 16384, 8, 8, 16, 4096, 4096, "bf16", 0.0),
+        _adapt("adapter 8 prompts of 2048", 16384, 8, 8, 16, 4096, 4096, "bf16", 0.0),
         # prompts of odd lengths beside the down projection, a higher rank
-        _adapt("adapter, 1999 tokens, rank 64", 1999, 5, 3, 64, 14336, 4096, "fp16", 0.2),
+        _adapt("adapter 1999 tokens rank 64", 1999, 5, 3, 64, 14336, 4096, "fp16", 0.2),
         # a few continuations of one prompt
-        _shared("prefix, 4 x (2048 + 128)", 1, 4, 2048, 128, False, 32, 8, 128, "bf16", "bf16", 16, 0, 0),
+        _shared("prefix 4 x (2048 + 128)", 1, 4, 2048, 128, False, 32, 8, 128, "bf16", "bf16", 16, 0, 0),
         # a serving batch behind one long instruction, cache in e4m3, ragged lengths
-        _shared("prefix, 61 x (8200 + 515), e4m3", 1, 61, 8200, 515, True, 32, 8, 128, "bf16", "fp8", 64, 0, 0),
+        _shared("prefix 61 x (8200 + 515) e4m3", 1, 61, 8200, 515, True, 32, 8, 128, "bf16", "fp8", 64, 0, 0),
         # two documents, many questions about each
-        _shared("prefix, 2 of 64 x (32768 + 300)", 2, 64, 32768, 300, True, 32, 8, 128, "bf16", "bf16", 64, 0, 0),
+        _shared("prefix 2 of 64 x (32768 + 300)", 2, 64, 32768, 300, True, 32, 8, 128, "bf16", "bf16", 64, 0, 0),
     ]
 
 
