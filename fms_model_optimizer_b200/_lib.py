@@ -77,6 +77,9 @@ EXPORTED_SYMBOLS = (
     "qlin_paged_attention",
     "qlin_paged_attention_workspace_bytes",
     "qlin_prompt_attention",
+    "qlin_token_logprobs",
+    "qlin_token_logprobs_bwd",
+    "qlin_lora",
 )
 
 
@@ -331,6 +334,22 @@ class PromptAttentionArgs(C.Structure):
     ]  # fmt: skip
 
 
+class TokenLogprobsArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("logits", "tokens", "logprobs", "entropy", "stats", "top_logprobs", "top_ids", "d_logprobs", "d_entropy", "d_logits", "status")),
+        ("ld", C.c_int64),
+        *((n, C.c_int32) for n in ("rows", "vocab", "top", "dtype")),
+    ]  # fmt: skip
+
+
+class LoraArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("x", "a", "b", "y", "rows", "starts", "scale", "status")),
+        *((n, C.c_int64) for n in ("x_row", "y_row", "a_adapter", "a_row", "b_adapter", "b_row")),
+        *((n, C.c_int32) for n in ("tokens", "listed", "adapters", "rank", "width", "out", "dtype")),
+    ]  # fmt: skip
+
+
 _host = None
 
 
@@ -386,6 +405,9 @@ def load() -> C.CDLL:
         ("qlin_qk_rope", QkRopeArgs),
         ("qlin_paged_attention", PagedAttentionArgs),
         ("qlin_prompt_attention", PromptAttentionArgs),
+        ("qlin_token_logprobs", TokenLogprobsArgs),
+        ("qlin_token_logprobs_bwd", TokenLogprobsArgs),
+        ("qlin_lora", LoraArgs),
     ):
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(struct), C.c_void_p]

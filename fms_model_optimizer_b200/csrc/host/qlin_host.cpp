@@ -931,6 +931,128 @@ Tensor prompt_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_
   return delivered(out_in, out);
 }
 
+// ------------------------------------------------------------------------------------------------ many requests at once
+qlin_token_logprobs_args score_args(const Tensor& x, const Tensor& tokens) {
+  qlin_token_logprobs_args a = {};
+  a.logits = data(x);
+  a.tokens = static_cast<const int64_t*>(data(tokens));
+  a.status = static_cast<int32_t*>(status_word(x.device().index()).data_ptr());
+  a.ld = step(x, 0);
+  a.rows = static_cast<int32_t>(x.size(0));
+  a.vocab = static_cast<int32_t>(x.size(1));
+  a.dtype = dtype_code(x.scalar_type());
+  return a;
+}
+// [rows, vocab] with contiguous rows that lie in rising order: a view, or a dense copy.
+Tensor logit_rows(const Tensor& logits) {
+  if (logits.dim() < 1) raise("logits must be [.., vocab]");
+  const Tensor x = logits.dim() == 2 ? logits : logits.reshape({-1, logits.size(-1)});
+  if ((x.size(1) <= 1 || x.stride(1) == 1) && (x.size(0) <= 1 || x.stride(0) >= 0) && !x.is_neg()) return x;
+  return x.resolve_neg().clone(at::MemoryFormat::Contiguous);
+}
+
+// (logprobs, entropy, top_logprobs, top_ids, stats) with the leading dimensions of `tokens`; stats is empty unless wanted.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens_in, int64_t top, bool want_stats) {
+  const at::Device dev = require_cuda({&logits, &tokens_in});
+  if (!is_float(logits.scalar_type())) raise("logits must be float32, float16 or bfloat16");
+  if (tokens_in.scalar_type() != at::kLong || logits.dim() < 1 || tokens_in.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+    raise("tokens must be int64, one for each row of logits");
+  if (logits.size(-1) < 1) raise("logits must have at least one entry a row");
+  if (top < 0 || top > 0x7fffffff || logits.size(-1) > 0x7fffffff || tokens_in.numel() > 0x7fffffff) raise("top, vocab or rows out of range");
+  const c10::cuda::CUDAGuard guard(dev);
+  at::NoGradGuard no_grad;
+  const Tensor x = logit_rows(logits), tokens = tokens_in.contiguous();
+  std::vector<int64_t> wide(tokens.sizes().begin(), tokens.sizes().end());
+  wide.push_back(top);
+  const Tensor logprobs = empty(tokens.sizes(), at::kFloat, dev), entropy = empty(tokens.sizes(), at::kFloat, dev);
+  const Tensor top_logprobs = empty(wide, at::kFloat, dev), top_ids = empty(wide, at::kLong, dev), stats = empty({want_stats ? tokens.numel() : 0, 2}, at::kFloat, dev);
+  qlin_token_logprobs_args a = score_args(x, tokens);
+  a.logprobs = static_cast<float*>(data(logprobs));
+  a.entropy = static_cast<float*>(data(entropy));
+  a.stats = want_stats ? static_cast<float*>(data(stats)) : nullptr;
+  a.top_logprobs = static_cast<float*>(data(top_logprobs));
+  a.top_ids = static_cast<int64_t*>(data(top_ids));
+  a.top = static_cast<int32_t>(top);
+  check(qlin_token_logprobs(&a, stream_of(dev)), "qlin_token_logprobs");
+  return {logprobs, entropy, top_logprobs, top_ids, stats};
+}
+
+Tensor token_logprobs_bwd(const Tensor& logits, const Tensor& tokens_in, const Tensor& entropy, const Tensor& stats, const OptTensor& d_logprobs, const OptTensor& d_entropy) {
+  const at::Device dev = require_cuda({&logits, &tokens_in, &entropy, &stats, ptr_of(d_logprobs), ptr_of(d_entropy)});
+  const c10::cuda::CUDAGuard guard(dev);
+  at::NoGradGuard no_grad;
+  const Tensor x = logit_rows(logits), tokens = tokens_in.contiguous(), dl = f32(d_logprobs), dh = f32(d_entropy);
+  for (const Tensor* t : {&dl, &dh})
+    if (t->defined() && t->numel() != tokens.numel()) raise("the gradients must have one entry for each row of logits");
+  const Tensor out = empty(logits.sizes(), logits.scalar_type(), dev);
+  qlin_token_logprobs_args a = score_args(x, tokens);
+  a.entropy = static_cast<float*>(data(entropy));
+  a.stats = static_cast<float*>(data(stats));
+  a.d_logprobs = static_cast<const float*>(data(dl));
+  a.d_entropy = static_cast<const float*>(data(dh));
+  a.d_logits = data(out);
+  check(qlin_token_logprobs_bwd(&a, stream_of(dev)), "qlin_token_logprobs_bwd");
+  return out;
+}
+
+// Rows (or matrices of rows) of 16-bit numbers that start on 16 bytes: the tensor itself, or a dense copy.
+Tensor aligned_rows(const Tensor& t) {
+  bool fits = t.numel() == 0 || ((t.size(-1) <= 1 || t.stride(-1) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) fits = fits && step(t, d) >= 0 && on16(t, step(t, d));
+  return fits && !t.is_neg() ? t : t.resolve_neg().clone(at::MemoryFormat::Contiguous);
+}
+
+Tensor lora_add(const Tensor& y, const Tensor& x_in, const Tensor& a_in, const Tensor& b_in, const Tensor& rows, const Tensor& starts, const Tensor& scale) {
+  const at::Device dev = require_cuda({&y, &x_in, &a_in, &b_in, &rows, &starts, &scale});
+  refuse_grad("lora_add_", {&y, &x_in, &a_in, &b_in, &scale});
+  const c10::cuda::CUDAGuard guard(dev);
+  const at::ScalarType type = y.scalar_type();
+  if ((type != at::kHalf && type != at::kBFloat16) || x_in.scalar_type() != type || a_in.scalar_type() != type || b_in.scalar_type() != type)
+    raise("y, x, a and b must all be float16 or all bfloat16");
+  if (y.dim() != 2 || x_in.dim() != 2 || x_in.size(0) != y.size(0)) raise("y must be [tokens, out] and x [tokens, width]");
+  if (a_in.dim() != 3 || b_in.dim() != 3 || a_in.size(0) != b_in.size(0) || a_in.size(1) != b_in.size(2) || a_in.size(2) != x_in.size(1) || b_in.size(1) != y.size(1))
+    raise("a must be [adapters, rank, width] and b [adapters, out, rank]");
+  const int64_t n = a_in.size(0), rank = a_in.size(1), width = x_in.size(1), out = y.size(1), tokens = y.size(0);
+  if (std::max({n, rank, width, out, tokens, rows.numel()}) > 0x7fffff00) raise("a dimension is out of range");
+  if (rows.dim() != 1) raise("rows must be a contiguous Int vector");
+  check_index(rows, at::kInt, rows.size(0), "rows");
+  check_index(starts, at::kInt, n + 1, "starts");
+  const Tensor sc = f32(scale);
+  if (sc.numel() != n) raise("scale must have one entry for each adapter");
+  for (int64_t d = 0; d < 2; ++d)
+    if (y.size(d) > 1 && y.stride(d) == 0) raise("rows of y share memory: they cannot be written");
+  for (const Tensor* t : {&x_in, &a_in, &b_in, &sc, &rows, &starts})
+    if (may_overlap(y, *t)) raise("y must not overlap the other tensors");
+  const Tensor x = aligned_rows(x_in), a_ = aligned_rows(a_in), b_ = aligned_rows(b_in), y_ = aligned_rows(y);
+  qlin_lora_args a = {};
+  a.x = data(x);
+  a.a = data(a_);
+  a.b = data(b_);
+  a.y = data(y_);
+  a.rows = static_cast<const int32_t*>(data(rows));
+  a.starts = static_cast<const int32_t*>(data(starts));
+  a.scale = static_cast<const float*>(data(sc));
+  a.status = static_cast<int32_t*>(status_word(dev.index()).data_ptr());
+  a.x_row = step(x, 0);
+  a.y_row = step(y_, 0);
+  a.a_adapter = step(a_, 0);
+  a.a_row = step(a_, 1);
+  a.b_adapter = step(b_, 0);
+  a.b_row = step(b_, 1);
+  a.tokens = static_cast<int32_t>(tokens);
+  a.listed = static_cast<int32_t>(rows.numel());
+  a.adapters = static_cast<int32_t>(n);
+  a.rank = static_cast<int32_t>(rank);
+  a.width = static_cast<int32_t>(width);
+  a.out = static_cast<int32_t>(out);
+  a.dtype = dtype_code(type);
+  check(qlin_lora(&a, stream_of(dev)), "qlin_lora");
+  at::NoGradGuard no_grad;
+  if (!y_.is_same(y)) y.copy_(y_);
+  else if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+  return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_qlin_host, m) {
@@ -949,4 +1071,7 @@ PYBIND11_MODULE(_qlin_host, m) {
   m.def("qk_rope", &qk_rope, rel());
   m.def("paged_attention", &paged_attention, rel());
   m.def("prompt_attention", &prompt_attention, rel());
+  m.def("token_logprobs", &token_logprobs, rel());
+  m.def("token_logprobs_bwd", &token_logprobs_bwd, rel());
+  m.def("lora_add", &lora_add, rel());
 }

@@ -1,0 +1,386 @@
+// qlin_lora: low-rank adapters of many requests added to the output of a projection that they share.
+//
+//   v = x[t] a[i]^T  (rank numbers),   y[t] += scale[i] v b[i]^T       for every row t of adapter i
+//
+// What bounds it: HBM, x and the adapters read once, y read and written once; a row of x against an adapter of rank 16 is 16 operations a byte.
+// One launch does both products.  A tile is 16 or more rows of one adapter, wherever they stand; its block (or cluster of blocks, where tiles are few)
+// shares out the width of x for v and the columns of y afterwards, warp by warp, and joins the parts of v in shared memory in between, in order.
+//
+// Both products are m16n8k16 with the rows as the tile's rows.  Nothing but v goes through shared memory: the order of the terms of a product is free, so a lane
+// loads 16 bytes of a row of x and 16 of a row of a where the instruction wants four pairs of terms, and the columns of y are dealt so that
+// the four n = 8 products of 32 columns leave a lane with 16 bytes of y in a row.  Rows of 128 (tcgen05) would need the operands in shared memory and
+// would not make the loads faster.
+//
+// v goes into the second product as two 16-bit numbers whose sum has 16 (bf16) or 22 (fp16) of its bits; in fp16 a row of v is brought to
+// 1 <= max < 2 first, by a power of two that comes back with the scale, since its sums may leave fp16's range where y does not.
+#include <type_traits>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "qlin_internal.h"
+#include "qlin_ptx.cuh"
+
+namespace qlin {
+
+constexpr int kLoraWarps = 8;
+constexpr int kLoraThreads = kLoraWarps * 32;
+constexpr int kMostCluster = 8;
+
+struct LoraParams {
+  qlin_lora_args a;
+  int32_t cluster;  // blocks of a tile
+};
+
+template <typename T, int R16, int MT>
+struct LoraCfg {
+  static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int RP = 16 * R16;        // the rank, padded
+  static constexpr int ROWS = 16 * MT;
+  static constexpr int PITCH = RP + 4;       // floats of a row of v
+  static constexpr int PITCH16 = RP + 8;     // 16-bit numbers of a row of v
+  static constexpr int STEPS = R16 * MT <= 2 ? 4 : R16 * MT <= 4 ? 2 : 1;  // of 32 terms that a warp has in flight
+  static constexpr int QUADS = RP >= 32 ? RP / 32 : 1;    // 16-byte (8-byte for rank 16) pieces of a row of b a lane holds
+  static constexpr int PARTS = kLoraWarps * ROWS * PITCH * 4;
+  static constexpr int BLOCK_V = PARTS;                    // [rows][PITCH]: the block's, then everybody's
+  static constexpr int V16 = BLOCK_V + ROWS * PITCH * 4;   // [2][rows][PITCH16]
+  static constexpr int UP = V16 + 2 * ROWS * PITCH16 * 2;  // [rows]
+  static constexpr int SMEM = UP + ROWS * 4;
+};
+
+// Adapter and first listed row of a tile; adapter -1: there is no such tile.  Every warp looks for itself.
+struct LoraTile {
+  int adapter, first, count;
+};
+__device__ __forceinline__ LoraTile lora_tile(const LoraParams& p, int tile, int rows, bool report) {
+  const int lane = threadIdx.x & 31;
+  int passed = 0;
+  for (int i0 = 0; i0 < p.a.adapters; i0 += 32) {
+    const int i = i0 + lane;
+    int s0 = 0, n = 0;
+    bool bad = false;
+    if (i < p.a.adapters) {
+      s0 = p.a.starts[i];
+      const int s1 = p.a.starts[i + 1];
+      bad = s0 < 0 || s1 < s0 || s1 > p.a.listed || (i == 0 && s0 != 0);
+      n = bad ? 0 : s1 - s0;
+    }
+    if (report && bad && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
+    const int tiles = (n + rows - 1) / rows;
+    int upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += other;
+    }
+    const int here = __shfl_sync(0xffffffffu, upto, 31);
+    if (tile < passed + here && !report) {
+      const int owner = __ffs(__ballot_sync(0xffffffffu, tile < passed + upto)) - 1;
+      const int within = (tile - passed - (__shfl_sync(0xffffffffu, upto - tiles, owner))) * rows;
+      return LoraTile{i0 + owner, __shfl_sync(0xffffffffu, s0, owner) + within, min(rows, __shfl_sync(0xffffffffu, n, owner) - within)};
+    }
+    passed += here;
+  }
+  return LoraTile{-1, 0, 0};
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack_pair(uint32_t w) {
+  if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+template <typename T, int R16, int MT>
+__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constant__ LoraParams p) {
+  using C = LoraCfg<T, R16, MT>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* parts = reinterpret_cast<float*>(smem);
+  float* block_v = reinterpret_cast<float*>(smem + C::BLOCK_V);
+  T* v16 = reinterpret_cast<T*>(smem + C::V16);
+  float* back = reinterpret_cast<float*>(smem + C::UP);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rank = blockIdx.x % p.cluster;
+  const LoraTile tile = lora_tile(p, blockIdx.x / p.cluster, C::ROWS, false);
+  if (tile.adapter < 0) {  // the whole cluster
+    if (blockIdx.x == 0 && warp == 0) lora_tile(p, 0x7fffffff, C::ROWS, true);
+    return;
+  }
+  const int share = rank * kLoraWarps + warp, shares = p.cluster * kLoraWarps;  // of the width, then of the columns
+
+  // the rows g and g + 8 of each sixteen that this lane loads and stores
+  const T* x_row[2 * MT];
+  T* y_row[2 * MT];
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) {
+    const int at = 8 * i + g;
+    int row = at < tile.count ? p.a.rows[tile.first + at] : -1;
+    if (at < tile.count && (row < 0 || row >= p.a.tokens)) {
+      if (p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
+      row = -1;
+    }
+    x_row[i] = row < 0 ? nullptr : static_cast<const T*>(p.a.x) + row * p.a.x_row;
+    y_row[i] = row < 0 ? nullptr : static_cast<T*>(p.a.y) + row * p.a.y_row;
+  }
+  const uint4 zero4 = make_uint4(0u, 0u, 0u, 0u);
+
+  // ---------------------------------------------------------------- v, this warp's share of the terms
+  float acc[MT][2 * R16][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < 2 * R16; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.0f;
+  {
+    const T* a = static_cast<const T*>(p.a.a) + tile.adapter * p.a.a_adapter;
+    const int steps = (p.a.width + 31) / 32;
+#pragma unroll 1
+    for (int s0 = share; s0 < steps; s0 += shares * C::STEPS) {
+      uint4 xv[C::STEPS][2 * MT], av[C::STEPS][2 * R16];
+#pragma unroll
+      for (int u = 0; u < C::STEPS; ++u) {
+        const int k = (s0 + u * shares) * 32 + 8 * t;
+        const bool in = k < p.a.width;
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) xv[u][i] = in && x_row[i] != nullptr ? __ldg(reinterpret_cast<const uint4*>(x_row[i] + k)) : zero4;
+#pragma unroll
+        for (int j = 0; j < 2 * R16; ++j) av[u][j] = in && 8 * j < p.a.rank ? __ldg(reinterpret_cast<const uint4*>(a + (8 * j + g) * p.a.a_row + k)) : zero4;
+      }
+#pragma unroll
+      for (int u = 0; u < C::STEPS; ++u)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < 2 * R16; ++j) {
+            mma16816<C::BF16>(acc[m][j], xv[u][2 * m].x, xv[u][2 * m + 1].x, xv[u][2 * m].y, xv[u][2 * m + 1].y, av[u][j].x, av[u][j].y);
+            mma16816<C::BF16>(acc[m][j], xv[u][2 * m].z, xv[u][2 * m + 1].z, xv[u][2 * m].w, xv[u][2 * m + 1].w, av[u][j].z, av[u][j].w);
+          }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < 2 * R16; ++j) {
+      float* at = parts + (warp * C::ROWS + 16 * m + g) * C::PITCH + 8 * j + 2 * t;
+      *reinterpret_cast<float2*>(at) = make_float2(acc[m][j][0], acc[m][j][1]);
+      *reinterpret_cast<float2*>(at + 8 * C::PITCH) = make_float2(acc[m][j][2], acc[m][j][3]);
+    }
+
+  // ---------------------------------------------------------------- loads of the second product, 32 columns: the first ones before the join
+  const T* b = static_cast<const T*>(p.a.b) + tile.adapter * p.a.b_adapter;
+  uint4 bv[4][C::QUADS], yv[2 * MT];
+  const auto load_columns = [&](int step) {
+    const int n0 = step * 32;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = n0 + 8 * (g >> 1) + 2 * q + (g & 1);
+#pragma unroll
+      for (int c = 0; c < C::QUADS; ++c) {
+        bv[q][c] = zero4;
+        if constexpr (R16 == 1) {
+          if (n < p.a.out && 4 * t < p.a.rank) {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(b + n * p.a.b_row + 4 * t));
+            bv[q][c].x = w.x;
+            bv[q][c].y = w.y;
+          }
+        } else {
+          if (n < p.a.out && 32 * c + 8 * t < p.a.rank) bv[q][c] = __ldg(reinterpret_cast<const uint4*>(b + n * p.a.b_row + 32 * c + 8 * t));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i)
+      yv[i] = y_row[i] != nullptr && n0 + 8 * t < p.a.out ? *reinterpret_cast<const uint4*>(y_row[i] + n0 + 8 * t) : zero4;
+  };
+  const int columns = (p.a.out + 31) / 32;
+  if (share < columns) load_columns(share);
+
+  // ---------------------------------------------------------------- v of all warps, then of all blocks, in order
+  __syncthreads();
+  for (int i = threadIdx.x; i < C::ROWS * C::RP / 4; i += kLoraThreads) {
+    const int row = i / (C::RP / 4), c = i % (C::RP / 4) * 4;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kLoraWarps; ++w) {
+      const float4 one = *reinterpret_cast<const float4*>(parts + (w * C::ROWS + row) * C::PITCH + c);
+      sum = make_float4(sum.x + one.x, sum.y + one.y, sum.z + one.z, sum.w + one.w);
+    }
+    *reinterpret_cast<float4*>(block_v + row * C::PITCH + c) = sum;
+  }
+  float* v = block_v;
+  if (p.cluster > 1) {
+    cluster_arrive_wait();
+    v = parts;  // the warps' parts are no longer needed
+    const uint32_t base = smem_u32(block_v);
+    for (int i = threadIdx.x; i < C::ROWS * C::RP / 4; i += kLoraThreads) {
+      const int row = i / (C::RP / 4), c = i % (C::RP / 4) * 4;
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int o = 0; o < p.cluster; ++o) {
+        const float4 one = ld_cluster_f4(base + (row * C::PITCH + c) * 4, o);
+        sum = make_float4(sum.x + one.x, sum.y + one.y, sum.z + one.z, sum.w + one.w);
+      }
+      *reinterpret_cast<float4*>(v + row * C::PITCH + c) = sum;
+    }
+    cluster_arrive_wait();  // nobody leaves while its part is read
+  }
+  __syncthreads();
+  const float scale = p.a.scale[tile.adapter];
+  for (int row = warp; row < C::ROWS; row += kLoraWarps) {
+    float up = 1.0f, down = 1.0f;
+    if constexpr (!C::BF16) {
+      float top = 0.0f;
+      for (int c = lane; c < C::RP; c += 32) top = fmaxf(top, fabsf(v[row * C::PITCH + c]));
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+      const int e = static_cast<int>(bits >> 23);
+      if (e > 0 && e < 254) {  // 2^-(e - 127) and its inverse are normal numbers
+        up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+        down = __uint_as_float(static_cast<uint32_t>(e) << 23);
+      }
+    }
+    if (lane == 0) back[row] = down * scale;
+    for (int c = 2 * lane; c < C::RP; c += 64) {
+      const float a0 = v[row * C::PITCH + c] * up, a1 = v[row * C::PITCH + c + 1] * up;
+      const uint32_t hi = pack_pair<C::BF16>(a0, a1);
+      const float2 h = unpack_pair<C::BF16>(hi);
+      // what is infinite or NaN is so in the first part alone
+      const uint32_t lo = pack_pair<C::BF16>(isfinite(h.x) ? a0 - h.x : 0.0f, isfinite(h.y) ? a1 - h.y : 0.0f);
+      *reinterpret_cast<uint32_t*>(v16 + row * C::PITCH16 + c) = hi;
+      *reinterpret_cast<uint32_t*>(v16 + (C::ROWS + row) * C::PITCH16 + c) = lo;
+    }
+  }
+  __syncthreads();
+
+  // ---------------------------------------------------------------- y
+  uint4 vf[2][MT][2][C::QUADS];  // the two parts of the rows g and g + 8
+  float factor[2 * MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = 16 * m + 8 * h + g;
+      factor[2 * m + h] = back[row];
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int c = 0; c < C::QUADS; ++c) {
+          const T* at = v16 + (part * C::ROWS + row) * C::PITCH16;
+          if constexpr (R16 == 1) {
+            const uint2 w = *reinterpret_cast<const uint2*>(at + 4 * t);
+            vf[part][m][h][c] = make_uint4(w.x, w.y, 0u, 0u);
+          } else {
+            vf[part][m][h][c] = *reinterpret_cast<const uint4*>(at + 32 * c + 8 * t);
+          }
+        }
+    }
+#pragma unroll 1
+  for (int step = share; step < columns; step += shares) {
+    float o[MT][4][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        o[m][q][0] = o[m][q][1] = o[m][q][2] = o[m][q][3] = 0.0f;
+#pragma unroll
+        for (int part = 1; part >= 0; --part)  // the small part first
+#pragma unroll
+          for (int c = 0; c < C::QUADS; ++c) {
+            const uint4 &r0 = vf[part][m][0][c], &r1 = vf[part][m][1][c];
+            mma16816<C::BF16>(o[m][q], r0.x, r1.x, r0.y, r1.y, bv[q][c].x, bv[q][c].y);
+            if constexpr (R16 > 1) mma16816<C::BF16>(o[m][q], r0.z, r1.z, r0.w, r1.w, bv[q][c].z, bv[q][c].w);
+          }
+      }
+    const int n = step * 32 + 8 * t;
+    uint4 w[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const uint32_t old[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
+      uint32_t sum[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 y = unpack_pair<C::BF16>(old[q]);
+        const float* more = &o[i / 2][q][2 * (i & 1)];
+        sum[q] = pack_pair<C::BF16>(fmaf(more[0], factor[i], y.x), fmaf(more[1], factor[i], y.y));
+      }
+      w[i] = make_uint4(sum[0], sum[1], sum[2], sum[3]);
+    }
+    if (step + shares < columns) load_columns(step + shares);
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i)
+      if (y_row[i] != nullptr && n < p.a.out) *reinterpret_cast<uint4*>(y_row[i] + n) = w[i];
+  }
+  if (blockIdx.x == 0 && warp == 0) lora_tile(p, 0x7fffffff, C::ROWS, true);
+}
+
+template <typename T, int R16, int MT>
+static int launch_lora(LoraParams p, cudaStream_t stream) {
+  using C = LoraCfg<T, R16, MT>;
+  const auto kernel = lora_kernel<T, R16, MT>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return fail(QLIN_ERR_DEVICE, "device ordinal %d out of range", dev);
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return fail(QLIN_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    configured[dev] = true;
+  }
+  // every adapter has at most one tile that is not full, every tile a row
+  const int64_t most = static_cast<int64_t>(p.a.listed) / C::ROWS + p.a.adapters;
+  const int64_t tiles = most < p.a.listed ? most : p.a.listed;
+  p.cluster = 1;
+  while (p.cluster < kMostCluster && tiles * p.cluster < sm_count()) p.cluster *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * p.cluster, 1, 1);
+  cfg.blockDim = dim3(kLoraThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(p.cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(QLIN_ERR_LAUNCH, "qlin_lora: %s", cudaGetErrorString(e));
+  }
+  return QLIN_OK;
+}
+template <typename T>
+static int pick_lora(const LoraParams& p, cudaStream_t s) {
+  const bool many = p.a.listed > 16 * 2 * sm_count();  // enough tiles of 32 rows for every SM
+  if (p.a.rank <= 16) return many ? launch_lora<T, 1, 2>(p, s) : launch_lora<T, 1, 1>(p, s);
+  if (p.a.rank <= 32) return many ? launch_lora<T, 2, 2>(p, s) : launch_lora<T, 2, 1>(p, s);
+  if (p.a.rank <= 64) return many ? launch_lora<T, 4, 2>(p, s) : launch_lora<T, 4, 1>(p, s);
+  return launch_lora<T, 8, 1>(p, s);
+}
+
+}  // namespace qlin
+
+extern "C" int qlin_lora(const qlin_lora_args* a, void* stream) {
+  using namespace qlin;
+  if (a == nullptr) return fail(QLIN_ERR_NULL, "qlin_lora: args is NULL");
+  if (a->tokens < 0 || a->listed < 0 || a->adapters < 0 || a->width < 0 || a->out < 0 || a->rank < 1) return fail(QLIN_ERR_BAD_SHAPE, "qlin_lora: a dimension is negative");
+  if (a->rank > 128 || a->rank % 8 != 0 || a->width % 8 != 0 || a->out % 8 != 0)
+    return fail(QLIN_ERR_BAD_SHAPE, "qlin_lora: width, out and rank must be multiples of 8, rank at most 128");
+  if (a->listed > (1 << 27)) return fail(QLIN_ERR_TOO_LARGE, "qlin_lora: at most 2^27 rows");
+  if (a->dtype != QLIN_DT_F16 && a->dtype != QLIN_DT_BF16) return fail(QLIN_ERR_BAD_DTYPE, "qlin_lora: x, a, b and y must be fp16 or bf16");
+  if (a->listed == 0 || a->adapters == 0 || a->out == 0 || a->width == 0) return QLIN_OK;
+  if (a->x == nullptr || a->y == nullptr || a->a == nullptr || a->b == nullptr || a->rows == nullptr || a->starts == nullptr || a->scale == nullptr)
+    return fail(QLIN_ERR_NULL, "qlin_lora: x, y, a, b, rows, starts or scale is NULL");
+  if (!aligned16(a->x) || !aligned16(a->y) || !aligned16(a->a) || !aligned16(a->b) || a->x_row % 8 != 0 || a->y_row % 8 != 0 || a->a_adapter % 8 != 0 ||
+      a->a_row % 8 != 0 || a->b_adapter % 8 != 0 || a->b_row % 8 != 0)
+    return fail(QLIN_ERR_BAD_ALIGN, "qlin_lora: every row of x, y, a and b must start on 16 bytes");
+  const LoraParams p{*a, 1};
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return a->dtype == QLIN_DT_BF16 ? pick_lora<__nv_bfloat16>(p, s) : pick_lora<__half>(p, s);
+}

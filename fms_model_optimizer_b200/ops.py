@@ -687,6 +687,65 @@ def prompt_attention(
 
 
 # --------------------------------------------------------------------------------------------------
+# Many requests answered at once: what the head says about given tokens, low-rank adapters
+# --------------------------------------------------------------------------------------------------
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top):
+        logprobs, entropy, top_logprobs, top_ids, stats = _call("token_logprobs", float(logits.numel() * logits.element_size()), logits.device, L.host().token_logprobs,
+                                                                logits, tokens, int(top), True)  # fmt: skip
+        ctx.save_for_backward(logits, tokens, entropy, stats)
+        ctx.mark_non_differentiable(top_logprobs, top_ids)
+        ctx.set_materialize_grads(False)
+        return logprobs, entropy, top_logprobs, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_logprobs, d_entropy, _top_logprobs, _top_ids):
+        if d_logprobs is None and d_entropy is None:
+            return None, None, None
+        logits, tokens, entropy, stats = ctx.saved_tensors
+        work = 2.0 * logits.numel() * logits.element_size()
+        return _call("token_logprobs_bwd", work, logits.device, L.host().token_logprobs_bwd, logits, tokens, entropy, stats, d_logprobs, d_entropy), None, None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """What a model's head says about given tokens, in one pass over the logits (``qlin_token_logprobs``): ``(logprobs, entropy, top_logprobs,
+    top_ids)``.  ``logits [.., vocab]`` fp32, fp16 or bf16 of any alignment, ``tokens [..]`` int64; ``logprobs`` and ``entropy`` are fp32
+    ``[..]``, ``top_logprobs`` (fp32) and ``top_ids`` (int64) ``[.., top]`` the ``top`` <= 32 most likely tokens in falling order, equal ones by
+    rising id.  A negative token (padding, such as -100) gives a log probability of 0; one of ``vocab`` or more does too and is
+    reported by ``check_status``.  Logits of minus infinity have no weight; a row of nothing else, or with NaN or plus infinity, gives NaN, and NaN counts
+    as the largest logit.
+
+    ``logprobs`` and ``entropy`` have a gradient (once differentiable, of the logits' type, ``qlin_token_logprobs_bwd``):
+    ``-logprobs.sum() / count`` is the loss of a language model.  A row whose incoming gradients are zero gets zeros."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TokenLogprobs.apply(logits, tokens, top)
+    return _call("token_logprobs", float(logits.numel() * logits.element_size()), logits.device, L.host().token_logprobs, logits, tokens, int(top), False)[:4]
+
+
+def lora_groups(which: torch.Tensor, adapters: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The rows of each adapter for ``lora_add_``, from the adapter of each row (``which [rows]``, integers; anything outside ``0 .. adapters - 1`` has none):
+    ``(rows, starts)``, int32, rows ``rows[starts[i] : starts[i + 1]]`` belong to adapter i, in rising order.  Made once a step, for all projections of
+    all layers; nothing is read back to the host."""
+    if which.dim() != 1 or which.is_floating_point() or adapters < 0:
+        raise RuntimeError("which must be a vector of integers, adapters must not be negative")
+    order = torch.where((which < 0) | (which >= adapters), adapters, which).sort(stable=True)
+    starts = torch.searchsorted(order.values, torch.arange(adapters + 1, device=which.device, dtype=order.values.dtype))
+    return order.indices.to(torch.int32), starts.to(torch.int32)
+
+
+def lora_add_(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, rows: torch.Tensor, starts: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """``y[t] += scale[i] * (x[t] @ a[i].T) @ b[i].T`` in place for the rows t of each adapter i (``qlin_lora``): low-rank adapters of many requests beside a projection
+    that they share.  ``y [tokens, out]`` the projection's output, ``x [tokens, width]`` its input, ``a [adapters, rank, width]``, ``b [adapters,
+    out, rank]``, all fp16 or all bf16, ``width``, ``out`` and ``rank`` <= 128 multiples of 8 (a lower rank is padded with zeros); ``rows`` and
+    ``starts`` as ``lora_groups`` gives them, each row at most once; ``scale`` fp32 ``[adapters]``.  Sums are fp32, y is rounded once; rows that no adapter has keep their
+    bytes.  Returns y.  No gradient."""
+    work = 2.0 * rows.numel() * a.shape[1] * (x.shape[-1] + y.shape[-1]) if a.dim() == 3 else 0.0
+    return _call("lora", work, y.device, L.host().lora_add, y, x, a, b, rows, starts, scale)
+
+
+# --------------------------------------------------------------------------------------------------
 # Calibration statistics
 # --------------------------------------------------------------------------------------------------
 def col_absmax(x: torch.Tensor, running: Optional[torch.Tensor] = None) -> torch.Tensor:

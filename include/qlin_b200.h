@@ -732,6 +732,63 @@ typedef struct qlin_prompt_attention_args {
 
 int qlin_prompt_attention(const qlin_prompt_attention_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Many requests answered at once beside the quantized Linears: what a decoder's head says about given tokens, low-rank adapters of many
+ * requests on one projection, and attention of sequences that share a prefix.  No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* qlin_token_logprobs -- of each row x of logits [rows, vocab] with m = max x and S = sum exp(x - m):
+ *   logprobs = x[token] - m - log S,   entropy = log S - sum exp(x - m) (x - m) / S,
+ *   top_ids, top_logprobs = the `top` largest in falling order, equal ones by rising id (NaN counts as the largest)
+ * in fp32.  Logits of minus infinity have no weight; a row that holds NaN, plus infinity or nothing but minus infinity has NaN sums.  A
+ * negative token gives a log probability of 0; one of vocab or more does too and writes QLIN_ERR_BAD_SHAPE to *status.  stats (optional) keeps
+ * m (0 where it is minus infinity) and log S of each row for qlin_token_logprobs_bwd.  top <= 32 and <= vocab <= 2^20; rows of logits need the alignment of their type
+ * only.  Outputs overlap no input.
+ *
+ * qlin_token_logprobs_bwd -- d_logits[j] = d_logprobs ([j = token] - p_j) - d_entropy p_j (log p_j + entropy), dense, in the type of the logits,
+ * from the entropy and stats of the forward pass.  d_logprobs and d_entropy are each optional (NULL: zeros); a row whose token is negative or
+ * out of range has no d_logprobs, and one whose two gradients are zero gets zeros. */
+typedef struct qlin_token_logprobs_args {
+  const void* logits;        /* [rows, vocab], ld elements apart */
+  const int64_t* tokens;     /* [rows] */
+  float* logprobs;           /* [rows]; forward */
+  float* entropy;            /* [rows]; written forward, read backward */
+  float* stats;              /* [rows, 2]; optional forward */
+  float* top_logprobs;       /* [rows, top]; forward */
+  int64_t* top_ids;          /* [rows, top]; forward */
+  const float* d_logprobs;   /* [rows]; backward */
+  const float* d_entropy;    /* [rows]; backward */
+  void* d_logits;            /* [rows, vocab] dense; backward */
+  int32_t* status;           /* optional device status word, written only on failure */
+  int64_t ld;
+  int32_t rows, vocab, top;
+  int32_t dtype;             /* qlin_dtype of logits and d_logits: F32, F16 or BF16 */
+} qlin_token_logprobs_args;
+
+int qlin_token_logprobs(const qlin_token_logprobs_args* args, void* stream);
+int qlin_token_logprobs_bwd(const qlin_token_logprobs_args* args, void* stream);
+
+/* qlin_lora -- y[t] += scale[i] (x[t] a[i]^T) b[i]^T in place for the rows t of adapter i, which are rows[starts[i]] .. rows[starts[i + 1] - 1]; rows of y
+ * that are not listed keep their bytes, and a row is listed once at most.  x [tokens, width], y [tokens, out], a [adapters, rank, width], b [adapters, out, rank], all
+ * F16 or all BF16; sums in fp32, y rounded once.  width, out and rank are multiples of 8, rank <= 128; rows of x, y, a and b start on 16 bytes;
+ * x, a and b overlap y nowhere.  starts that do not rise from 0 to at most `listed`, or a row that does not exist, write QLIN_ERR_BAD_SHAPE to
+ * *status; such adapters and rows are passed over. */
+typedef struct qlin_lora_args {
+  const void* x;
+  const void* a;
+  const void* b;
+  void* y;
+  const int32_t* rows;   /* [listed] */
+  const int32_t* starts; /* [adapters + 1] */
+  const float* scale;    /* [adapters] */
+  int32_t* status;       /* optional device status word, written only on failure */
+  int64_t x_row, y_row, a_adapter, a_row, b_adapter, b_row; /* strides in elements */
+  int32_t tokens, listed, adapters, rank, width, out;
+  int32_t dtype;
+} qlin_lora_args;
+
+int qlin_lora(const qlin_lora_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
