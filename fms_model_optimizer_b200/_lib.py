@@ -80,6 +80,8 @@ EXPORTED_SYMBOLS = (
     "qlin_token_logprobs",
     "qlin_token_logprobs_bwd",
     "qlin_lora",
+    "qlin_prefix_attention",
+    "qlin_prefix_attention_workspace_bytes",
 )
 
 
@@ -342,6 +344,16 @@ class TokenLogprobsArgs(C.Structure):
     ]  # fmt: skip
 
 
+class PrefixAttentionArgs(C.Structure):
+    _fields_ = [
+        ("own", PagedAttentionArgs),
+        *((n, C.c_void_p) for n in ("prefix_table", "prefix_lens", "groups")),
+        ("prefix_stride", C.c_int64),
+        ("num_groups", C.c_int32),
+        ("max_prefix_pages", C.c_int32),
+    ]
+
+
 class LoraArgs(C.Structure):
     _fields_ = [
         *((n, C.c_void_p) for n in ("x", "a", "b", "y", "rows", "starts", "scale", "status")),
@@ -408,6 +420,7 @@ def load() -> C.CDLL:
         ("qlin_token_logprobs", TokenLogprobsArgs),
         ("qlin_token_logprobs_bwd", TokenLogprobsArgs),
         ("qlin_lora", LoraArgs),
+        ("qlin_prefix_attention", PrefixAttentionArgs),
     ):
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(struct), C.c_void_p]
@@ -431,6 +444,8 @@ def load() -> C.CDLL:
     lib.qlin_tensor_fq_workspace_bytes.restype = C.c_int64
     lib.qlin_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedAttentionArgs)]
     lib.qlin_paged_attention_workspace_bytes.restype = C.c_int64
+    lib.qlin_prefix_attention_workspace_bytes.argtypes = [C.POINTER(PrefixAttentionArgs)]
+    lib.qlin_prefix_attention_workspace_bytes.restype = C.c_int64
     _lib = lib
     return lib
 

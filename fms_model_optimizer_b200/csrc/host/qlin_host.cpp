@@ -833,22 +833,18 @@ Tensor delivered(const OptTensor& out, const Tensor& written) {
   return *out;
 }
 
-Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& lens, const std::optional<double>& scale,
-                       int64_t window, int64_t sinks, const OptTensor& k_scale, const OptTensor& v_scale, const OptTensor& out_in) {
-  const at::Device dev = require_cuda({&q_in, &k_pages, &v_pages, &block_table, &lens, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
-  refuse_grad("paged_attention", {&q_in, &k_pages, &v_pages, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
-  const c10::cuda::CUDAGuard guard(dev);
-  const Tensor q = head_rows(q_in, "q");
+// Checks and argument block of attention over pages; q is what head_rows gave, ks and vs the scales in fp32.
+qlin_paged_attention_args paged_args(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& lens, const std::optional<double>& scale,
+                                     int64_t window, int64_t sinks, const Tensor& ks, const Tensor& vs) {
+  const at::Device dev = q.device();
   const int64_t b = q.size(0), d = q.size(2);
   if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) raise("q must be float16 or bfloat16");
   if (k_pages.dim() != 4) raise("k_pages and v_pages must both be [pages, kv heads, page size, head_dim]");
-  const Tensor ks = f32(k_scale), vs = f32(v_scale);
   check_cache(k_pages, v_pages, k_pages.size(1), d, q.scalar_type(), ks, vs);
   if (block_table.scalar_type() != at::kInt || block_table.dim() != 2 || block_table.size(0) != b || (block_table.size(1) > 1 && block_table.stride(1) != 1))
     raise("block_table must be int32 [batch, pages of a sequence] with contiguous rows");
   check_index(lens, at::kInt, b, "lens");
   if (b > 0x7fffffff || k_pages.size(0) > 0x7fffffff || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff) raise("batch, pages, window or sinks out of range");
-  const Tensor out = attention_out(out_in, q, dev, {&q, &k_pages, &v_pages});
   qlin_paged_attention_args a = {};
   a.q = data(q);
   a.k_pages = data(k_pages);
@@ -857,7 +853,6 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
   a.lens = static_cast<const int32_t*>(data(lens));
   a.k_scale = static_cast<const float*>(data(ks));
   a.v_scale = static_cast<const float*>(data(vs));
-  a.out = data(out);
   a.status = static_cast<int32_t*>(status_word(dev.index()).data_ptr());
   a.q_batch = step(q, 0);
   a.q_head = step(q, 1);
@@ -877,12 +872,56 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
   a.dtype = dtype_code(q.scalar_type());
   a.cache_dtype = dtype_code(k_pages.scalar_type());
   a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d)));
+  return a;
+}
+
+Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& lens, const std::optional<double>& scale,
+                       int64_t window, int64_t sinks, const OptTensor& k_scale, const OptTensor& v_scale, const OptTensor& out_in) {
+  const at::Device dev = require_cuda({&q_in, &k_pages, &v_pages, &block_table, &lens, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
+  refuse_grad("paged_attention", {&q_in, &k_pages, &v_pages, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor q = head_rows(q_in, "q"), ks = f32(k_scale), vs = f32(v_scale);
+  qlin_paged_attention_args a = paged_args(q, k_pages, v_pages, block_table, lens, scale, window, sinks, ks, vs);
+  const Tensor out = attention_out(out_in, q, dev, {&q, &k_pages, &v_pages});
+  a.out = data(out);
   const int64_t bytes = qlin_paged_attention_workspace_bytes(&a);
   if (bytes < 0) check(static_cast<int>(bytes), "qlin_paged_attention");
   Tensor ws;
   if (bytes > 0) ws = empty({bytes}, at::kByte, dev);
   a.workspace = data(ws);
   check(qlin_paged_attention(&a, stream_of(dev)), "qlin_paged_attention");
+  return delivered(out_in, out);
+}
+
+Tensor prefix_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& prefix_table, const Tensor& prefix_lens, const Tensor& groups,
+                        const Tensor& block_table, const Tensor& lens, const std::optional<double>& scale, int64_t window, int64_t sinks, const OptTensor& k_scale,
+                        const OptTensor& v_scale, const OptTensor& out_in) {
+  const at::Device dev = require_cuda({&q_in, &k_pages, &v_pages, &prefix_table, &prefix_lens, &groups, &block_table, &lens, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
+  refuse_grad("prefix_attention", {&q_in, &k_pages, &v_pages, ptr_of(k_scale), ptr_of(v_scale), ptr_of(out_in)});
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor q = head_rows(q_in, "q"), ks = f32(k_scale), vs = f32(v_scale);
+  qlin_prefix_attention_args a = {};
+  a.own = paged_args(q, k_pages, v_pages, block_table, lens, scale, window, sinks, ks, vs);
+  if (prefix_table.scalar_type() != at::kInt || prefix_table.dim() != 2 || (prefix_table.size(1) > 1 && prefix_table.stride(1) != 1))
+    raise("prefix_table must be int32 [groups, pages of a prefix] with contiguous rows");
+  const int64_t n = prefix_table.size(0);
+  if (n > 0x7ffffffe || prefix_table.size(1) > 0x7fffffff) raise("prefix_table is out of range");
+  check_index(prefix_lens, at::kInt, n, "prefix_lens");
+  check_index(groups, at::kInt, n + 1, "groups");
+  const Tensor out = attention_out(out_in, q, dev, {&q, &k_pages, &v_pages});
+  a.own.out = data(out);
+  a.prefix_table = static_cast<const int32_t*>(data(prefix_table));
+  a.prefix_lens = static_cast<const int32_t*>(data(prefix_lens));
+  a.groups = static_cast<const int32_t*>(data(groups));
+  a.prefix_stride = step(prefix_table, 0);
+  a.num_groups = static_cast<int32_t>(n);
+  a.max_prefix_pages = static_cast<int32_t>(prefix_table.size(1));
+  const int64_t bytes = qlin_prefix_attention_workspace_bytes(&a);
+  if (bytes < 0) check(static_cast<int>(bytes), "qlin_prefix_attention");
+  Tensor ws;
+  if (bytes > 0) ws = empty({bytes}, at::kByte, dev);
+  a.own.workspace = data(ws);
+  check(qlin_prefix_attention(&a, stream_of(dev)), "qlin_prefix_attention");
   return delivered(out_in, out);
 }
 
@@ -1070,6 +1109,7 @@ PYBIND11_MODULE(_qlin_host, m) {
   m.def("qat_linear", &qat_linear, rel());
   m.def("qk_rope", &qk_rope, rel());
   m.def("paged_attention", &paged_attention, rel());
+  m.def("prefix_attention", &prefix_attention, rel());
   m.def("prompt_attention", &prompt_attention, rel());
   m.def("token_logprobs", &token_logprobs, rel());
   m.def("token_logprobs_bwd", &token_logprobs_bwd, rel());

@@ -1,0 +1,121 @@
+// qlin_prefix_attention: one new token of every sequence against its keys in a paged cache, where groups of sequences share the first of them.
+//
+// The softmax of a row splits into any parts of its keys, each with its own maximum and sums.  Here the keys of the prefix that all sequences of a group
+// see are one part: the queries of all of them are the columns of the products (eight or sixteen a block), and each key is loaded once for these.
+// What else a sequence sees, its own keys, and those of the prefix that its window or length sets apart from the others', is the part that
+// qlin_paged_attention's kernel reads, whose blocks then take in the sums over the prefix.  No row of a product is masked that way: what a sequence does not see
+// is not loaded beside its query, NaN and infinities included.
+//
+// What bounds it: HBM, each key of a prefix once and each own key once, while a group has few rows; then the products.  The launch for the own keys begins while the one
+// for the prefixes ends, and waits for its sums only when it joins them.
+#include "qlin_paged.cuh"
+
+namespace qlin {
+
+struct PrefixPlan {
+  Splits own;
+  int32_t units, splits, columns;  // of the launch for the prefixes: blocks of columns of all kv heads, splits of the keys, columns of a block
+  int64_t own_floats, shared_floats;  // of the workspace
+};
+static PrefixPlan plan_prefix(const qlin_prefix_attention_args& a) {
+  PrefixPlan plan = {};
+  const int group = a.own.q_heads / a.own.kv_heads;
+  // the tables' widths say how many keys of their own sequences may have
+  qlin_paged_attention_args own = a.own;
+  own.max_pages = a.own.max_pages > a.max_prefix_pages ? a.own.max_pages - a.max_prefix_pages + 1 : 1;
+  plan.own = choose_splits(own, (group + heads_per_block(group) - 1) / heads_per_block(group));
+  const int64_t rows = static_cast<int64_t>(a.own.batch) * a.own.q_heads;
+  if (plan.own.n > 1 && !plan.own.cluster) plan.own_floats = rows * plan.own.n * (a.own.head_dim + 2);
+  const int64_t keys = static_cast<int64_t>(a.max_prefix_pages) * a.own.page_size;
+  if (keys > 0 && a.own.num_pages > 0) {
+    const int64_t per_head = rows / a.own.kv_heads;
+    plan.columns = per_head > 8 * static_cast<int64_t>(a.num_groups) ? 16 : 8;
+    const int64_t blocks = per_head / plan.columns + a.num_groups;  // a group has one block that is not full at most
+    plan.units = static_cast<int32_t>(blocks * a.own.kv_heads);
+    const int64_t most = (keys + kSharedStep - 1) / kSharedStep, want = (2 * sm_count() + plan.units - 1) / plan.units;
+    plan.splits = static_cast<int32_t>(want < most ? want : most);
+    plan.shared_floats = rows * plan.splits * (a.own.head_dim + 2);
+  }
+  return plan;
+}
+
+static int check_prefix(const qlin_prefix_attention_args* a) {
+  if (a == nullptr) return fail(QLIN_ERR_NULL, "qlin_prefix_attention: args is NULL");
+  const int rc = check_paged(&a->own, "qlin_prefix_attention");
+  if (rc != QLIN_OK) return rc;
+  if (a->num_groups < 0 || a->max_prefix_pages < 0 || (a->own.batch > 0 && a->num_groups < 1))
+    return fail(QLIN_ERR_BAD_SHAPE, "qlin_prefix_attention: at least one group is wanted, and no negative width");
+  if (a->num_groups > (1 << 20)) return fail(QLIN_ERR_TOO_LARGE, "qlin_prefix_attention: at most 2^20 groups");
+  if (static_cast<int64_t>(a->max_prefix_pages) * a->own.page_size > (1 << 30)) return fail(QLIN_ERR_TOO_LARGE, "qlin_prefix_attention: at most 2^30 keys a prefix");
+  return QLIN_OK;
+}
+
+template <typename QT, bool F8, int DP>
+static int launch_prefix(const PagedParams& p, const PrefixPlan& plan, cudaStream_t s) {
+  if (p.pre.blocks > 0) {
+    const int rc = plan.columns == 16 ? launch_paged<QT, F8, DP, 2, kShared>(p, s) : launch_paged<QT, F8, DP, 1, kShared>(p, s);
+    if (rc != QLIN_OK) return rc;
+  }
+  return heads_per_block(p.group) == 16 ? launch_paged<QT, F8, DP, 2, kOwn>(p, s) : launch_paged<QT, F8, DP, 1, kOwn>(p, s);
+}
+template <typename QT, bool F8>
+static int pick_prefix(const PagedParams& p, const PrefixPlan& plan, cudaStream_t s) {
+  return p.a.head_dim <= 64 ? launch_prefix<QT, F8, 64>(p, plan, s) : launch_prefix<QT, F8, 128>(p, plan, s);
+}
+
+}  // namespace qlin
+
+extern "C" int64_t qlin_prefix_attention_workspace_bytes(const qlin_prefix_attention_args* a) {
+  using namespace qlin;
+  const int rc = check_prefix(a);
+  if (rc != QLIN_OK) return rc;
+  if (a->own.batch == 0) return 0;
+  const PrefixPlan plan = plan_prefix(*a);
+  return (plan.own_floats + plan.shared_floats) * 4;
+}
+
+extern "C" int qlin_prefix_attention(const qlin_prefix_attention_args* a, void* stream) {
+  using namespace qlin;
+  int rc = check_prefix(a);
+  if (rc != QLIN_OK) return rc;
+  if (a->own.batch == 0) return QLIN_OK;
+  rc = check_paged_pointers(&a->own, "qlin_prefix_attention");
+  if (rc != QLIN_OK) return rc;
+  if (a->groups == nullptr || a->prefix_lens == nullptr || (a->max_prefix_pages > 0 && (a->prefix_table == nullptr || (a->own.num_pages > 0 && (a->own.k_pages == nullptr || a->own.v_pages == nullptr)))))
+    return fail(QLIN_ERR_NULL, "qlin_prefix_attention: groups, prefix_lens, prefix_table, k_pages or v_pages is NULL");
+  const PrefixPlan plan = plan_prefix(*a);
+  PagedParams p = {};
+  p.a = a->own;
+  p.group = a->own.q_heads / a->own.kv_heads;
+  p.head_blocks = (p.group + heads_per_block(p.group) - 1) / heads_per_block(p.group);
+  p.splits = plan.own.n;
+  p.cluster = plan.own.cluster;
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (a->own.page_size == 1 << i) p.page_shift = i;
+  const int64_t rows = static_cast<int64_t>(a->own.batch) * a->own.q_heads;
+  if (plan.own_floats + plan.shared_floats > 0) {
+    if (a->own.workspace == nullptr) return fail(QLIN_ERR_NULL, "qlin_prefix_attention: workspace is NULL");
+    if (!aligned16(a->own.workspace)) return fail(QLIN_ERR_BAD_ALIGN, "qlin_prefix_attention: workspace must start on 16 bytes");
+  }
+  // outputs first, then maxima and sums: the former stay on 16 bytes
+  float* at = static_cast<float*>(a->own.workspace);
+  p.pre.part_o = at;
+  p.part_o = at + rows * plan.splits * a->own.head_dim;
+  const bool parts = plan.own_floats > 0;
+  float* ml = p.part_o + (parts ? rows * plan.own.n * a->own.head_dim : 0);
+  p.pre.part_ml = reinterpret_cast<float2*>(ml);
+  p.part_ml = reinterpret_cast<float2*>(ml + rows * plan.splits * 2);
+  p.pre.table = a->prefix_table;
+  p.pre.lens = a->prefix_lens;
+  p.pre.groups = a->groups;
+  p.pre.table_stride = a->prefix_stride;
+  p.pre.count = a->num_groups;
+  p.pre.max_pages = a->max_prefix_pages;
+  p.pre.splits = plan.splits > 0 ? plan.splits : 1;
+  p.pre.blocks = plan.units * plan.splits;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool f8 = a->own.cache_dtype == QLIN_DT_F8E4M3;
+  if (a->own.dtype == QLIN_DT_BF16) return f8 ? pick_prefix<__nv_bfloat16, true>(p, plan, s) : pick_prefix<__nv_bfloat16, false>(p, plan, s);
+  return f8 ? pick_prefix<__half, true>(p, plan, s) : pick_prefix<__half, false>(p, plan, s);
+}

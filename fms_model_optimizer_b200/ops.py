@@ -666,6 +666,33 @@ def paged_attention(
     return _call("paged_attention", 0.0, q.device, L.host().paged_attention, q, k_pages, v_pages, block_table, lens, scale, window, sinks, k_scale, v_scale, out)
 
 
+def prefix_attention(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    prefix_table: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    groups: torch.Tensor,
+    block_table: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    scale: Optional[float] = None,
+    window: int = 0,
+    sinks: int = 0,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``paged_attention`` for groups of sequences that share their first tokens, whose keys are read once for a group (``qlin_prefix_attention``).
+    Sequences ``groups[g] : groups[g + 1]`` (int32 ``[groups + 1]``, rising from 0 to the batch) find their keys ``i < prefix_lens[g]`` in page
+    ``prefix_table[g, i // page size]`` and the others in ``block_table[b, i // page size]``, whose entries in front of them are not read; ``lens``
+    count the prefix in.  A group of one sequence, or a prefix of length 0, is fine.  ``prefix_table`` int32 ``[groups, pages of a prefix]``,
+    ``prefix_lens`` int32 ``[groups]``, everything else as in ``paged_attention``.  As there, the widths of the tables should be no more than the longest need.
+    No gradient."""
+    return _call("prefix_attention", 0.0, q.device, L.host().prefix_attention, q, k_pages, v_pages, prefix_table, prefix_lens, groups, block_table, lens, scale, window, sinks,
+                 k_scale, v_scale, out)  # fmt: skip
+
+
 def prompt_attention(
     q: torch.Tensor,
     k: torch.Tensor,

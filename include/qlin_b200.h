@@ -789,6 +789,25 @@ typedef struct qlin_lora_args {
 
 int qlin_lora(const qlin_lora_args* args, void* stream);
 
+/* qlin_prefix_attention -- qlin_paged_attention where groups of sequences share their first tokens: sequences groups[g] .. groups[g + 1] - 1 find their
+ * keys i < prefix_lens[g] in page prefix_table[g, i / page_size] and the others, as ever, in page block_table[b, i / page_size], offset i % page_size of either.
+ * lens, positions, window and sinks count from the first token of the prefix; lens[b] may be 0 (zeros) or fall short of the prefix.  The keys of a
+ * prefix that all its sequences see are read once for the group.  groups rises from 0 to batch; otherwise, and for prefix_lens below 0 or above
+ * max_prefix_pages * page_size, QLIN_ERR_BAD_SHAPE in *status and unspecified outputs.  The widths of the tables bound how finely keys are split: a
+ * sequence's own keys are expected not to pass max_pages - max_prefix_pages + 1 pages by much.  Entries of block_table in front of a sequence's own
+ * first key are not read. */
+typedef struct qlin_prefix_attention_args {
+  qlin_paged_attention_args own; /* workspace: qlin_prefix_attention_workspace_bytes */
+  const int32_t* prefix_table;   /* [num_groups, max_prefix_pages], row stride prefix_stride */
+  const int32_t* prefix_lens;    /* [num_groups] */
+  const int32_t* groups;         /* [num_groups + 1] */
+  int64_t prefix_stride;
+  int32_t num_groups, max_prefix_pages;
+} qlin_prefix_attention_args;
+
+int64_t qlin_prefix_attention_workspace_bytes(const qlin_prefix_attention_args* args);
+int qlin_prefix_attention(const qlin_prefix_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,7 +13,7 @@ from fms_model_optimizer_b200 import _lib as L
 from fms_model_optimizer_b200 import ops
 
 HEADER = Path(__file__).resolve().parent.parent / "include" / "qlin_b200.h"
-STRUCTS = (("qlin_token_logprobs_args", L.TokenLogprobsArgs), ("qlin_lora_args", L.LoraArgs))
+STRUCTS = (("qlin_token_logprobs_args", L.TokenLogprobsArgs), ("qlin_lora_args", L.LoraArgs), ("qlin_prefix_attention_args", L.PrefixAttentionArgs))
 
 
 @pytest.mark.parametrize("name,cls", STRUCTS)
@@ -72,6 +72,27 @@ def test_refusals_of_the_adapters():
     assert rc(tokens=-1) == L.ERR_BAD_SHAPE and rc(rank=0) == L.ERR_BAD_SHAPE and rc(rank=12) == L.ERR_BAD_SHAPE and rc(rank=136) == L.ERR_BAD_SHAPE
     assert rc(width=60) == L.ERR_BAD_SHAPE and rc(out=4) == L.ERR_BAD_SHAPE and rc(listed=(1 << 27) + 1) == L.ERR_TOO_LARGE
     assert rc(dtype=L.DT_F32) == L.ERR_BAD_DTYPE and rc(y=base + 8) == L.ERR_BAD_ALIGN and rc(b_row=20) == L.ERR_BAD_ALIGN
+
+
+def test_refusals_of_the_attention_behind_a_prefix():
+    lib = L.load()
+    buf, base = _base()
+    own = dict(q=base, k_pages=base, v_pages=base, block_table=base, lens=base, out=base, workspace=base, q_batch=64, q_head=64, page_stride=64, head_stride=64,
+               slot_stride=64, table_stride=1, batch=1, q_heads=2, kv_heads=1, head_dim=64, page_size=1, num_pages=1, max_pages=1, dtype=L.DT_BF16,
+               cache_dtype=L.DT_BF16, scale=0.125)  # fmt: skip
+    good = dict(prefix_table=base, prefix_lens=base, groups=base, prefix_stride=1, num_groups=1, max_prefix_pages=1)
+
+    def rc(kw={}, **own_kw):
+        return lib.qlin_prefix_attention(C.byref(L.PrefixAttentionArgs(own=L.PagedAttentionArgs(**{**own, **own_kw}), **{**good, **kw})), None)
+
+    assert lib.qlin_prefix_attention(None, None) == L.ERR_NULL and rc(batch=0) == L.OK
+    assert rc(q=None) == L.ERR_NULL and rc(dict(groups=None)) == L.ERR_NULL and rc(dict(prefix_table=None)) == L.ERR_NULL and rc(workspace=None) == L.ERR_NULL
+    assert rc(dict(num_groups=0)) == L.ERR_BAD_SHAPE and rc(dict(max_prefix_pages=-1)) == L.ERR_BAD_SHAPE and rc(dict(num_groups=(1 << 20) + 1)) == L.ERR_TOO_LARGE
+    assert rc(dict(max_prefix_pages=1 << 20), page_size=1 << 11) == L.ERR_TOO_LARGE
+    assert rc(q_heads=3, kv_heads=2) == L.ERR_BAD_SHAPE and rc(head_dim=60) == L.ERR_BAD_SHAPE and rc(dtype=L.DT_F32) == L.ERR_BAD_DTYPE
+    assert rc(k_pages=base + 8) == L.ERR_BAD_ALIGN and rc(workspace=base + 4) == L.ERR_BAD_ALIGN
+    a = L.PrefixAttentionArgs(own=L.PagedAttentionArgs(**{**own, "head_dim": 60}), **good)
+    assert lib.qlin_prefix_attention_workspace_bytes(C.byref(a)) == L.ERR_BAD_SHAPE
 
 
 def test_no_cpu_path():
