@@ -108,6 +108,17 @@ __device__ __forceinline__ int shared_splits(const SharedPrefix& pre, const Comm
   const int n = c.to - c.from, per = keys_per_split(n, pre.splits);
   return (n + per - 1) / per;
 }
+// The kv head, the group and the block of `columns` of its rows of a unit; false: there is no such unit.
+__device__ __forceinline__ bool shared_unit(const PagedParams& p, int unit, int columns, int& kvh, int& g, int& block) {
+  kvh = unit % p.a.kv_heads;
+  block = unit / p.a.kv_heads;
+  for (g = 0; g < p.pre.count; ++g) {
+    const int rows = max(0, min(p.pre.groups[g + 1], p.a.batch) - max(p.pre.groups[g], 0)) * p.group, blocks = (rows + columns - 1) / columns;
+    if (block < blocks) return true;
+    block -= blocks;
+  }
+  return false;
+}
 // What is left to a sequence: its first keys and those of its window before the common ones, then what follows these.
 struct Rest {
   int sinks, start, mid, after, n;
@@ -244,14 +255,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
   Common common{0, 0, 0, 0, 0};
   if constexpr (MODE == kShared) {
     if (blockIdx.x == 0) check_groups(p);
-    kvh = unit % p.a.kv_heads;
-    int left = unit / p.a.kv_heads, g_ = 0;
-    for (; g_ < p.pre.count; ++g_) {
-      const int rows = max(0, min(p.pre.groups[g_ + 1], p.a.batch) - max(p.pre.groups[g_], 0)) * p.group, blocks = (rows + C::HEADS - 1) / C::HEADS;
-      if (left < blocks) break;
-      left -= blocks;
-    }
-    if (g_ == p.pre.count) return;
+    int g_, left;
+    if (!shared_unit(p, unit, C::HEADS, kvh, g_, left)) return;
     common = common_keys(p, g_, threadIdx.x == 0);
     b = g_;
     head0 = left * C::HEADS;
@@ -777,4 +782,8 @@ static int launch_paged(const PagedParams& p, cudaStream_t stream) {
   }
   return QLIN_OK;
 }
+
+// The prefix's part on tcgen05, tiles of 128 rows (qlin_prefix_tc.cu): two tiles a block where `pair`, otherwise one tile and two splits.
+int launch_prefix_tc(const PagedParams& p, bool pair, cudaStream_t stream);
+
 }  // namespace qlin

@@ -12,9 +12,14 @@
 
 namespace qlin {
 
+// Rows of a group (its sequences times the query heads of a kv head) from which on the tensor cores' 128-row tiles take the prefix, and above which a
+// block has two of them.
+constexpr int kRowsTensor = 32, kRowsPair = 128;
+
 struct PrefixPlan {
   Splits own;
-  int32_t units, splits, columns;  // of the launch for the prefixes: blocks of columns of all kv heads, splits of the keys, columns of a block
+  int32_t units, splits, columns;  // of the launch for the prefixes: blocks of columns of all kv heads at most, splits of the keys, columns of a block
+  int32_t blocks;                  // of that launch
   int64_t own_floats, shared_floats;  // of the workspace
 };
 static PrefixPlan plan_prefix(const qlin_prefix_attention_args& a) {
@@ -28,12 +33,25 @@ static PrefixPlan plan_prefix(const qlin_prefix_attention_args& a) {
   if (plan.own.n > 1 && !plan.own.cluster) plan.own_floats = rows * plan.own.n * (a.own.head_dim + 2);
   const int64_t keys = static_cast<int64_t>(a.max_prefix_pages) * a.own.page_size;
   if (keys > 0 && a.own.num_pages > 0) {
-    const int64_t per_head = rows / a.own.kv_heads;
-    plan.columns = per_head > 8 * static_cast<int64_t>(a.num_groups) ? 16 : 8;
+    const int64_t per_head = rows / a.own.kv_heads, each = (per_head + a.num_groups - 1) / a.num_groups;  // rows of a kv head, and of a group on average
+    plan.columns = each > kRowsPair ? 256 : each >= kRowsTensor ? 128 : each > 8 ? 16 : 8;
     const int64_t blocks = per_head / plan.columns + a.num_groups;  // a group has one block that is not full at most
+    if (blocks * a.own.kv_heads > (1 << 24)) return plan;
     plan.units = static_cast<int32_t>(blocks * a.own.kv_heads);
-    const int64_t most = (keys + kSharedStep - 1) / kSharedStep, want = (2 * sm_count() + plan.units - 1) / plan.units;
-    plan.splits = static_cast<int32_t>(want < most ? want : most);
+    const int64_t expected = a.num_groups * ((each + plan.columns - 1) / plan.columns) * a.own.kv_heads, most = (keys + kSharedStep - 1) / kSharedStep;
+    if (plan.columns >= 128) {
+      // one block an SM, none with fewer than four tiles of keys for each of its streams; 128 rows take two splits at once
+      const int streams = plan.columns == 128 ? 2 : 1;
+      int64_t each_unit = sm_count() / expected;
+      if (each_unit > most / (4 * streams)) each_unit = most / (4 * streams);
+      if (each_unit < 1) each_unit = 1;
+      plan.splits = static_cast<int32_t>(each_unit * streams);
+      plan.blocks = plan.units * static_cast<int32_t>(each_unit);
+    } else {
+      const int64_t want = (2 * sm_count() + expected - 1) / expected;
+      plan.splits = static_cast<int32_t>(want < most ? want : most);
+      plan.blocks = plan.units * plan.splits;
+    }
     plan.shared_floats = rows * plan.splits * (a.own.head_dim + 2);
   }
   return plan;
@@ -53,7 +71,7 @@ static int check_prefix(const qlin_prefix_attention_args* a) {
 template <typename QT, bool F8, int DP>
 static int launch_prefix(const PagedParams& p, const PrefixPlan& plan, cudaStream_t s) {
   if (p.pre.blocks > 0) {
-    const int rc = plan.columns == 16 ? launch_paged<QT, F8, DP, 2, kShared>(p, s) : launch_paged<QT, F8, DP, 1, kShared>(p, s);
+    const int rc = plan.columns >= 128 ? launch_prefix_tc(p, plan.columns == 256, s) : plan.columns == 16 ? launch_paged<QT, F8, DP, 2, kShared>(p, s) : launch_paged<QT, F8, DP, 1, kShared>(p, s);
     if (rc != QLIN_OK) return rc;
   }
   return heads_per_block(p.group) == 16 ? launch_paged<QT, F8, DP, 2, kOwn>(p, s) : launch_paged<QT, F8, DP, 1, kOwn>(p, s);
@@ -84,6 +102,7 @@ extern "C" int qlin_prefix_attention(const qlin_prefix_attention_args* a, void* 
   if (a->groups == nullptr || a->prefix_lens == nullptr || (a->max_prefix_pages > 0 && (a->prefix_table == nullptr || (a->own.num_pages > 0 && (a->own.k_pages == nullptr || a->own.v_pages == nullptr)))))
     return fail(QLIN_ERR_NULL, "qlin_prefix_attention: groups, prefix_lens, prefix_table, k_pages or v_pages is NULL");
   const PrefixPlan plan = plan_prefix(*a);
+  if (a->max_prefix_pages > 0 && a->own.num_pages > 0 && plan.blocks < 1) return fail(QLIN_ERR_TOO_LARGE, "qlin_prefix_attention: too many rows and groups");
   PagedParams p = {};
   p.a = a->own;
   p.group = a->own.q_heads / a->own.kv_heads;
@@ -113,7 +132,7 @@ extern "C" int qlin_prefix_attention(const qlin_prefix_attention_args* a, void* 
   p.pre.count = a->num_groups;
   p.pre.max_pages = a->max_prefix_pages;
   p.pre.splits = plan.splits > 0 ? plan.splits : 1;
-  p.pre.blocks = plan.units * plan.splits;
+  p.pre.blocks = plan.blocks;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool f8 = a->own.cache_dtype == QLIN_DT_F8E4M3;
   if (a->own.dtype == QLIN_DT_BF16) return f8 ? pick_prefix<__nv_bfloat16, true>(p, plan, s) : pick_prefix<__nv_bfloat16, false>(p, plan, s);
