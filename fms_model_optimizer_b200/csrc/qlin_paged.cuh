@@ -76,27 +76,28 @@ __device__ __forceinline__ void check_groups(const PagedParams& p) {
   for (int g = threadIdx.x; g < p.pre.count; g += blockDim.x) bad |= p.pre.groups[g] > p.pre.groups[g + 1];
   if (bad && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
 }
-__device__ __forceinline__ Common common_keys(const PagedParams& p, int g, bool report) {  // by a whole warp
-  const int g0 = p.pre.groups[g], g1 = p.pre.groups[g + 1];
+__device__ __forceinline__ Common common_keys(const PagedParams& p, int g, int g0, int g1, bool report) {  // by a whole warp
+  const int given = p.pre.lens[g];  // beside the lengths, before anything waits for it
   const bool rises = g0 >= 0 && g0 <= g1 && g1 <= p.a.batch;
-  Common c{rises ? g0 : 0, rises ? g1 - g0 : 0, p.pre.lens[g], 0, 0};
   const int64_t most = p.a.num_pages > 0 ? static_cast<int64_t>(p.pre.max_pages) * p.a.page_size : 0;
-  if (c.prefix < 0 || c.prefix > most) {
-    if (report && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
-    c.prefix = c.prefix < 0 ? 0 : static_cast<int>(most);
-  }
-  int from = 0, to = 0x7fffffff;
+  const int64_t wide = p.a.num_pages > 0 ? static_cast<int64_t>(p.a.max_pages) * p.a.page_size : 0;
+  Common c{rises ? g0 : 0, rises ? g1 - g0 : 0, 0, 0, 0};
+  int longest = 0, shortest = 0x7fffffff;  // of the lengths as they are given
   for (int i = threadIdx.x & 31; i < c.sequences; i += 32) {
-    const int len = sequence_length(p, c.first + i, false, c.prefix);
+    const int len = p.a.lens[c.first + i];
     if (len > 0) {
-      from = max(from, p.a.window > 0 && len > p.a.window ? len - p.a.window : 0);
-      to = min(to, len);
+      longest = max(longest, len);
+      shortest = min(shortest, len);
     }
   }
-  from = __reduce_max_sync(0xffffffffu, from);
-  to = __reduce_min_sync(0xffffffffu, to);
-  if (to == 0x7fffffff) to = 0;
-  to = min(to, c.prefix);
+  c.prefix = given < 0 ? 0 : given > most ? static_cast<int>(most) : given;
+  if (report && c.prefix != given && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  shortest = __reduce_min_sync(0xffffffffu, shortest);
+  if (longest == 0) return c;
+  const int cut = static_cast<int>(wide > c.prefix ? wide : c.prefix);  // lengths above it are cut there
+  longest = min(longest, cut);
+  const int from = p.a.window > 0 && longest > p.a.window ? longest - p.a.window : 0, to = min(min(shortest, cut), c.prefix);
   c.from = from < to ? from : 0;
   c.to = from < to ? to : 0;
   return c;
@@ -133,37 +134,55 @@ __device__ __forceinline__ Rest rest_of(const Visible& v, const Common& c, int l
   }
   return r;
 }
-// The group of a sequence; -1 where the groups do not say.
-__device__ __forceinline__ int group_of(const SharedPrefix& pre, int b) {
-  int lo = 0, hi = pre.count;  // groups[lo] <= b < groups[hi], if they rise from 0
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (pre.groups[mid] <= b) lo = mid;
-    else hi = mid;
+// The group of a sequence and its bounds, by a whole warp: 32 bounds a look.  g is -1 where the groups do not say.
+struct Group {
+  int g, first, end;
+};
+__device__ __forceinline__ Group group_of(const SharedPrefix& pre, int b) {
+  const int lane = threadIdx.x & 31;
+  for (int base = 0; base < pre.count; base += 31) {
+    const int at = min(base + lane, pre.count), bound = pre.groups[at];
+    const uint32_t under = __ballot_sync(0xffffffffu, bound <= b && base + lane < pre.count);
+    const int i = under == 0 ? 0 : 31 - __clz(under);
+    const int first = __shfl_sync(0xffffffffu, bound, i), end = __shfl_sync(0xffffffffu, bound, min(i + 1, 31));
+    if (under != 0 && i < 31 && first <= b && b < end) return Group{base + i, first, end};
   }
-  return pre.groups[lo] <= b && b < pre.groups[lo + 1] ? lo : -1;
+  return Group{-1, 0, 0};
 }
-// The sums over the prefix join those of a sequence's own keys, which carry a factor of 2^shift, split by split in order.
+// The sums over the prefix join those of a sequence's own keys, which carry a factor of 2^shift, split by split in order; eight are read at a time.
 __device__ __forceinline__ void join_prefix(const PagedParams& p, int64_t row, int d, int used, float shift, float& top, float& sum, float (&acc)[4]) {
   const float2* ml = p.pre.part_ml + row * p.pre.splits;
   const float* o = p.pre.part_o + row * p.pre.splits * p.a.head_dim + d;
-  float most = top;
-  for (int s = 0; s < used; ++s) most = fmaxf(most, ml[s].x);
-  const float keep = top == most ? 1.0f : exp2f(top - most);
-  top = most;
-  sum *= keep;
+#pragma unroll 1
+  for (int s0 = 0; s0 < used; s0 += 8) {
+    float2 one[8];
+    float4 v[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i] *= keep;
-#pragma unroll 4
-  for (int s = 0; s < used; ++s) {
-    const float2 one = ml[s];
-    const float4 v = *reinterpret_cast<const float4*>(o + static_cast<int64_t>(s) * p.a.head_dim);
-    const float f = (one.x == most ? 1.0f : exp2f(one.x - most)) * shift;
-    sum += one.y * f;
-    acc[0] += v.x * f;
-    acc[1] += v.y * f;
-    acc[2] += v.z * f;
-    acc[3] += v.w * f;
+    for (int i = 0; i < 8; ++i) {
+      one[i] = make_float2(-INFINITY, 0.0f);
+      if (s0 + i < used) {
+        one[i] = __ldcg(ml + s0 + i);
+        v[i] = __ldcg(reinterpret_cast<const float4*>(o + static_cast<int64_t>(s0 + i) * p.a.head_dim));
+      }
+    }
+    float most = top;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, one[i].x);
+    const float keep = top == most ? 1.0f : exp2f(top - most);
+    top = most;
+    sum *= keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= keep;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (s0 + i < used) {
+        const float f = (one[i].x == most ? 1.0f : exp2f(one[i].x - most)) * shift;
+        sum += one[i].y * f;
+        acc[0] += v[i].x * f;
+        acc[1] += v[i].y * f;
+        acc[2] += v[i].z * f;
+        acc[3] += v[i].w * f;
+      }
   }
 }
 
@@ -257,7 +276,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
     if (blockIdx.x == 0) check_groups(p);
     int g_, left;
     if (!shared_unit(p, unit, C::HEADS, kvh, g_, left)) return;
-    common = common_keys(p, g_, threadIdx.x == 0);
+    common = common_keys(p, g_, p.pre.groups[g_], p.pre.groups[g_ + 1], threadIdx.x == 0);
     b = g_;
     head0 = left * C::HEADS;
     heads = min(C::HEADS, common.sequences * p.group - head0);
@@ -276,8 +295,9 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
   int len = 0, group = 0;
   if constexpr (MODE == kSingle) len = sequence_length(p, b, threadIdx.x == 0);
   if constexpr (MODE == kOwn) {
-    group = group_of(p.pre, b);
-    if (group >= 0) common = common_keys(p, group, false);
+    const Group of = group_of(p.pre, b);
+    group = of.g;
+    if (group >= 0) common = common_keys(p, group, of.first, of.end, false);
     else if (threadIdx.x == 0 && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
     len = sequence_length(p, b, threadIdx.x == 0, common.prefix);
   }
@@ -621,8 +641,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane * 4, D = p.a.head_dim;
   Common common{0, 0, 0, 0, 0};
   if constexpr (MODE == kOwn) {
-    const int group = group_of(p.pre, b);
-    if (group >= 0) common = common_keys(p, group, false);
+    const Group of = group_of(p.pre, b);
+    if (of.g >= 0) common = common_keys(p, of.g, of.first, of.end, false);
   }
   const int len = sequence_length(p, b, false, common.prefix);
   const Visible all = visible_keys(len, p.a.window, p.a.sinks);

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   const int part = blockIdx.x % block_splits;
   int kvh, g, unit;
   if (!shared_unit(p, blockIdx.x / block_splits, C::Q_TILES * kRows, kvh, g, unit)) return;
-  const Common common = common_keys(p, g, threadIdx.x == 0);
+  const Common common = common_keys(p, g, p.pre.groups[g], p.pre.groups[g + 1], threadIdx.x == 0);
   const int keys = common.to - common.from, per = keys_per_split(keys, splits);
   const int rows = common.sequences * p.group - unit * C::Q_TILES * kRows;  // from the block's first one on
   // of each stream: its split, the first of its keys, their number; and the tiles of both
@@ -166,6 +166,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   if (warp == kSharedMmaWarp) {
     tmem_alloc(&aux->tmem_base, 512);
     tmem_relinquish();
+  }
+  if (!F8 && p.a.head_dim < DP) {  // head dimensions past the end are zeros in every stage, and stay so
+    for (int i = threadIdx.x; i < C::STAGES * C::TILE_BYTES / 16; i += kSharedThreads) reinterpret_cast<uint4*>(smem + C::KV_OFFSET)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async();
   }
   tc_fence_before();
   __syncthreads();
@@ -208,35 +212,57 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
         if (++turn == kSharedLoadWarps) turn = 0;
         if (!mine) return;
         const int begin = begin_of(i), count = count_of(i);
-        const auto look_up = [&](int j) {  // where row 32 j + lane begins, in bytes; -1: no key
-          const int at = t * kKeys + 32 * j + lane;
-          if (j > 3 || at >= count) return static_cast<int64_t>(-1);
-          const int key = begin + at, pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.a.page_size;
-          int page = table[pg];
-          if (page < 0 || page >= p.a.num_pages) {
-            bad_page = true;
-            page = 0;
-          }
-          return (page * p.a.page_stride + (key - pg * p.a.page_size) * p.a.slot_stride + head_off) * C::ES;
+        // the pages of the rows 32 j + lane are on their way while the stage is waited for (read one after the other they cost 5000 cycles a tile)
+        const auto place = [&](int j, int& offset) {
+          const int key = min(begin + t * kKeys + 32 * j + lane, begin + count - 1), pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.a.page_size;
+          offset = key - pg * p.a.page_size;
+          return pg;
         };
-        int64_t next = look_up(0);
-        if (pending >= 0 && !__all_sync(0xffffffffu, mbar_try_wait(&aux->kv_empty[stage], parity))) finish_pending();
+        int o0, o1, o2, o3;
+        const int p0 = table[place(0, o0)], p1 = table[place(1, o1)], p2 = table[place(2, o2)], p3 = table[place(3, o3)];
+        if (pending >= 0 && !__all_sync(0xffffffffu, mbar_test_wait(&aux->kv_empty[stage], parity))) finish_pending();
         ok = uniform_wait(&aux->kv_empty[stage], parity, abort_flag);
         if (!ok) return;
         const uint8_t* base = static_cast<const uint8_t*>(kv ? p.a.v_pages : p.a.k_pages);
         const uint32_t dst = smem_u32(smem) + C::KV_OFFSET + stage * C::TILE_BYTES;
+        const auto address = [&](int j) {  // in bytes; -1: no key
+          int page = j < 2 ? (j == 0 ? p0 : p1) : (j == 2 ? p2 : p3);
+          const int offset = j < 2 ? (j == 0 ? o0 : o1) : (j == 2 ? o2 : o3);
+          if (t * kKeys + 32 * j + lane >= count) return static_cast<int64_t>(-1);
+          if (page < 0 || page >= p.a.num_pages) {
+            bad_page = true;
+            page = 0;
+          }
+          return (page * p.a.page_stride + offset * p.a.slot_stride + head_off) * C::ES;
+        };
         if constexpr (!F8) {
-#pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            const int64_t off = next;
-            next = look_up(j + 1);
+          // Eight addresses, then eight copies: with each copy right behind its own address, and with a size that may be zero, a copy takes 117 cycles and the
+          // loads are what the rest waits for (2 x 64 sequences behind 32768 keys 190 us).  Rows that are not there are written as zeros, which only the last tile has.
+          const bool whole = (t + 1) * kKeys <= count;
+          const uint32_t x = static_cast<uint32_t>((lc & 7) ^ lrow) << 4, to = dst + (lc >> 3) * kChunkBytes + lrow * 128;
+          const auto copy_rows = [&](int j, bool all) {
+            const int64_t off = address(j);
 #pragma unroll
-            for (int n = 0; n < 32 / AT_ONCE; ++n) {
-              const int row = n * AT_ONCE + lrow;
-              const int64_t at = __shfl_sync(0xffffffffu, off, row);
-              const uint32_t bytes = piece_real && at >= 0 ? 16u : 0u;
-              cp_async16(dst + tile_piece(32 * j + row, lc), bytes ? base + at + lc * 16 : base, bytes);
+            for (int n0 = 0; n0 < 32 / AT_ONCE; n0 += 8) {
+              int64_t at[8];
+#pragma unroll
+              for (int n = 0; n < 8; ++n) at[n] = __shfl_sync(0xffffffffu, off, (n0 + n) * AT_ONCE + lrow);
+              if (piece_real) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                  const uint32_t place = to + (32 * j + (n0 + n) * AT_ONCE) * 128 + (x ^ static_cast<uint32_t>((((n0 + n) * AT_ONCE) & 7) << 4));
+                  if (all || at[n] >= 0) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place), "l"(base + at[n] + lc * 16) : "memory");
+                  else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(place), "r"(0u) : "memory");
+                }
+              }
             }
+          };
+          if (whole) {
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) copy_rows(j, true);
+          } else {
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) copy_rows(j, false);
           }
           asm volatile("cp.async.commit_group;" ::: "memory");
           if (pending >= 0) {
@@ -248,12 +274,14 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
           constexpr int BATCH = 32 / AT_ONCE < 8 ? 32 / AT_ONCE : 8;  // pieces that a lane has in flight
 #pragma unroll 1
           for (int j = 0; j < 4; ++j) {
-            const int64_t off = next;
-            next = look_up(j + 1);
+            const int64_t off = address(j);
             uint4 v[BATCH];
+            int64_t from[BATCH];
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) from[n] = __shfl_sync(0xffffffffu, off, n * AT_ONCE + lrow);
 #pragma unroll
             for (int n = 0; n < BATCH; ++n) {
-              const int64_t at = __shfl_sync(0xffffffffu, off, n * AT_ONCE + lrow);
+              const int64_t at = from[n];
               v[n] = piece_real && at >= 0 ? __ldg(reinterpret_cast<const uint4*>(base + at + lc * 16)) : make_uint4(0u, 0u, 0u, 0u);
             }
 #pragma unroll
