@@ -27,6 +27,7 @@ constexpr int kPieceLoads = 8;       // 16-byte loads of a piece
 constexpr int kMostTop = 32;
 constexpr int kMostParts = 8;        // blocks that share a row
 constexpr int kCandidates = 1024;
+constexpr int kHits = 512;
 constexpr int kMostVocab = 1 << 20;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -138,49 +139,88 @@ __device__ __forceinline__ void orders_of(const uint4& v, uint32_t (&o)[16 / siz
 }
 
 // Shared memory of a block: what the threads and pieces found, and the elements that may be among the top ones.
+constexpr int kGroups = kScoreThreads / 4;
 struct ScoreShared {
   Sums warp[kScoreWarps], block;
-  uint32_t best[kScoreThreads];
+  uint4 best[kGroups / 4];  // of four threads each
   uint64_t candidate[kCandidates];
   uint64_t chosen[kMostTop];
+  uint32_t hit[kHits];  // pieces that are looked at again: piece * threads + thread
   uint32_t threshold;
-  int found, scan[kScoreWarps];
+  int found, hits, scan[kScoreWarps];
 };
 
-// Elements of this block's share from `least` on, as many as there are places for; returns how many there are.
+// Elements of this block's share from `least` on, as many as there are places for; returns how many there are.  The pieces that reach it are listed first and
+// then read by whole warps, a word a lane; -1, and nothing read, where they are too many to list.
 template <typename T>
 __device__ __forceinline__ int gather(const Row<T>& row, ScoreShared& sh, const uint32_t* piece_best, int pieces, int first, int last, int edges, uint32_t least) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __syncthreads();
-  if (tid == 0) sh.found = 0;
+  if (tid == 0) sh.found = sh.hits = 0;
   __syncthreads();
+  for (int p = 0; p < pieces; ++p)
+    if (piece_best[p * kScoreThreads + tid] >= least) {
+      const int at = atomicAdd(&sh.hits, 1);
+      if (at < kHits) sh.hit[at] = static_cast<uint32_t>(p * kScoreThreads + tid);
+    }
   const auto offer = [&](uint32_t order, int id) {
     if (order < least) return;
     const int at = atomicAdd(&sh.found, 1);
     if (at < kCandidates) sh.candidate[at] = ranked(order, static_cast<uint32_t>(id));
   };
-#pragma unroll 1
-  for (int p = 0; p < pieces; ++p) {
-    if (piece_best[p * kScoreThreads + tid] < least) continue;
-    uint4 v[kPieceLoads];
-#pragma unroll
-    for (int u = 0; u < kPieceLoads; ++u) {
-      const int i = first + (p * kPieceLoads + u) * kScoreThreads + tid;
-      if (i < last) v[u] = row.vector(i);
-    }
-#pragma unroll
-    for (int u = 0; u < kPieceLoads; ++u) {
-      const int i = first + (p * kPieceLoads + u) * kScoreThreads + tid;
-      if (i >= last) break;
-      uint32_t o[Row<T>::PER];
-      orders_of<T>(v[u], o);
-#pragma unroll
-      for (int e = 0; e < Row<T>::PER; ++e) offer(o[e], row.id(i) + e);
-    }
-  }
   if (tid < edges) offer(order_of(to_float(row.x[row.edge_id(tid)])), row.edge_id(tid));
   __syncthreads();
+  const int hits = sh.hits;
+  if (hits > kHits) return -1;
+  constexpr int AHEAD = 4;
+  for (int h0 = warp * AHEAD; h0 < hits; h0 += kScoreWarps * AHEAD) {
+    uint32_t word[AHEAD];
+    int id[AHEAD];
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {  // lane: load lane / 4 of the piece, word lane % 4 of it
+      const uint32_t hit = h0 + e < hits ? sh.hit[h0 + e] : 0u;
+      const int i = first + (static_cast<int>(hit / kScoreThreads) * kPieceLoads + (lane >> 2)) * kScoreThreads + static_cast<int>(hit % kScoreThreads);
+      id[e] = h0 + e < hits && i < last ? row.id(i) + (lane & 3) * static_cast<int>(4 / sizeof(T)) : -1;
+      word[e] = id[e] >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(row.x + id[e])) : 0u;
+    }
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      if (id[e] < 0) continue;
+      if constexpr (std::is_same<T, float>::value) {
+        offer(order_of(__uint_as_float(word[e])), id[e]);
+      } else {
+        const float2 f = word_pair<T>(word[e]);
+        offer(order_of(f.x), id[e]);
+        offer(order_of(f.y), id[e] + 1);
+      }
+    }
+  }
+  __syncthreads();
   return sh.found;
+}
+// After a call of gather that found too much: a value that at least `want` elements reach, from the listed pieces' maxima (n < 0) or the elements that found a
+// place.  The least of these at first, which is the answer for rows of few values; then the `want`-th largest.
+__device__ __forceinline__ uint32_t raised(ScoreShared& sh, const uint32_t* piece_best, int n, int want, bool again) {
+  const int tid = threadIdx.x, all = n < 0 ? kHits : kCandidates;
+  const auto value = [&](int i) { return n < 0 ? piece_best[sh.hit[i]] : static_cast<uint32_t>(sh.candidate[i] >> 32); };
+  __syncthreads();
+  if (!again) {
+    uint32_t low = 0xffffffffu;
+    for (int i = tid; i < all; i += kScoreThreads) low = min(low, value(i));
+    low = __reduce_min_sync(0xffffffffu, low);
+    if ((tid & 31) == 0) sh.scan[tid >> 5] = static_cast<int>(low);
+    __syncthreads();
+    for (int w = 0; w < kScoreWarps; ++w) low = min(low, static_cast<uint32_t>(sh.scan[w]));
+    return low;
+  }
+  for (int i = tid; i < all; i += kScoreThreads) {
+    const uint32_t mine = value(i);
+    int above = 0;
+    for (int j = 0; j < all; ++j) above += value(j) > mine || (value(j) == mine && j < i) ? 1 : 0;
+    if (above == want - 1) sh.threshold = mine;
+  }
+  __syncthreads();
+  return sh.threshold;
 }
 // The `want` first of n candidates, in order, to `to`; returns how many there are.
 __device__ __forceinline__ int rank_candidates(ScoreShared& sh, int n, int want, uint64_t* to) {
@@ -331,7 +371,13 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const __grid_const
   for (int o = 16; o > 0; o >>= 1)
     mine = joined(mine, Sums{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o)});
   if (lane == 0) sh.warp[warp] = mine;
-  if constexpr (TOP) sh.best[tid] = pieces > 0 && first + tid < last ? order_of(body) : 0u;
+  if constexpr (TOP) {
+    uint32_t best = pieces > 0 && first + tid < last ? order_of(body) : 0u;
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
+    // the group takes the place of the last bits: no two are equal, and the threshold is not above the true one
+    if ((lane & 3) == 0) reinterpret_cast<uint32_t*>(sh.best)[tid >> 2] = (best & ~static_cast<uint32_t>(kGroups - 1)) | static_cast<uint32_t>(tid >> 2);
+  }
   __syncthreads();
   if (tid == 0) {
     Sums all = sh.warp[0];
@@ -344,27 +390,27 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const __grid_const
   int have = 0;
   if constexpr (TOP) {
     const int want = p.a.top;
-    {
-      const uint32_t best = sh.best[tid];
+    if (tid < kGroups) {
+      const uint32_t best = reinterpret_cast<const uint32_t*>(sh.best)[tid];
       int above = 0;
-#pragma unroll 8
-      for (int j = 0; j < kScoreThreads; ++j) above += sh.best[j] > best || (sh.best[j] == best && j < tid) ? 1 : 0;
-      if (above == want - 1) sh.threshold = best;  // 0 where fewer threads have elements: all of these are looked at
+#pragma unroll
+      for (int j = 0; j < kGroups / 4; ++j) {
+        const uint4 o = sh.best[j];
+        above += (o.x > best ? 1 : 0) + (o.y > best ? 1 : 0) + (o.z > best ? 1 : 0) + (o.w > best ? 1 : 0);
+      }
+      if (above == want - 1) sh.threshold = best & ~static_cast<uint32_t>(kGroups - 1);  // 0 where fewer groups have elements: all of these are looked at
     }
     __syncthreads();
     uint32_t least = max(sh.threshold, 1u);
     int n = gather<T>(row, sh, piece_best, pieces, first, last, edges, least);
-    if (n <= kCandidates) {
+    if (n >= 0 && n <= kCandidates) {
       have = rank_candidates(sh, n, want, sh.chosen);
     } else {
-      // more elements than places, by many equal ones or by their order: first those above the threshold, then, in order, those at it.
-      // If the former are too many too, the threshold becomes the k-th largest of those that found a place.
-      while (true) {
+      // More than there are places for, by many equal elements or by their order.  The threshold rises to one that enough elements reach; what lies above it is wanted, and of
+      // what lies at it, in order, as many as are left.  If the former is too much as well, once more.
+      for (bool again = false; n < 0 || n > kCandidates; again = true) {
+        least = raised(sh, piece_best, n, want, again);
         n = least == 0xffffffffu ? 0 : gather<T>(row, sh, piece_best, pieces, first, last, edges, least + 1);
-        if (n <= kCandidates) break;
-        rank_candidates(sh, kCandidates, want, sh.chosen);
-        least = static_cast<uint32_t>(sh.chosen[want - 1] >> 32);
-        __syncthreads();
       }
       have = rank_candidates(sh, n, want, sh.chosen);
       if (have < want) have = take_ties<T>(row, sh, first, last, edges, least, have, want);
@@ -430,8 +476,11 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const __grid_const
 }
 
 // ------------------------------------------------------------------------------------------------ the gradient
-constexpr int kGradLoads = 4;  // 16-byte pieces of a thread
+constexpr int kGradLoads = 4;  // 16-byte pieces of a thread in flight
+constexpr int kGradSteps = 4;  // times that many
 
+// A block takes kGradSteps times 16 KB of a row and has the next loads under way while it works on the last ones (2048 x 128256, with the forward
+// pass: one step a block 300 us).
 template <typename T>
 __global__ void __launch_bounds__(kScoreThreads) score_grad_kernel(const __grid_constant__ ScoreParams p) {
   constexpr int PER = 16 / sizeof(T);
@@ -454,38 +503,43 @@ __global__ void __launch_bounds__(kScoreThreads) score_grad_kernel(const __grid_
   };
   const Row<T> row(reinterpret_cast<const T*>(out), vocab);  // pieces by where the gradient lies
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  uint4 v[kGradLoads];
+  const auto vector_of = [&](int step, int u) { return ((part * kGradSteps + step) * kGradLoads + u) * kScoreThreads + static_cast<int>(threadIdx.x); };
+  const auto load = [&](int step, uint4 (&v)[kGradLoads]) {
 #pragma unroll
-  for (int u = 0; u < kGradLoads; ++u) {
-    const int i = (part * kGradLoads + u) * kScoreThreads + threadIdx.x;
-    if (i >= row.vectors || none) continue;
-    const T* at = x + row.id(i);
-    if (same) {
-      v[u] = __ldg(reinterpret_cast<const uint4*>(at));
-    } else {
-      T e[PER];
+    for (int u = 0; u < kGradLoads; ++u) {
+      const int i = vector_of(step, u);
+      if (i >= row.vectors || none) continue;
+      const T* at = x + row.id(i);
+      if (same) {
+        v[u] = __ldg(reinterpret_cast<const uint4*>(at));
+      } else {
+        T e[PER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) e[j] = at[j];
-      memcpy(&v[u], e, 16);
+        for (int j = 0; j < PER; ++j) e[j] = at[j];
+        memcpy(&v[u], e, 16);
+      }
     }
-  }
+  };
+  uint4 v[2][kGradLoads];
+  load(0, v[0]);
 #pragma unroll
-  for (int u = 0; u < kGradLoads; ++u) {
-    const int i = (part * kGradLoads + u) * kScoreThreads + threadIdx.x;
-    if (i >= row.vectors) continue;
-    const int id = row.id(i);
-    T e[PER];
-    if (none) {
+  for (int step = 0; step < kGradSteps; ++step) {
+    if (step + 1 < kGradSteps) load(step + 1, v[(step + 1) & 1]);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) e[j] = from_float<T>(0.0f);
-    } else {
-      memcpy(e, &v[u], 16);
+    for (int u = 0; u < kGradLoads; ++u) {
+      const int i = vector_of(step, u);
+      if (i >= row.vectors) continue;
+      const int id = row.id(i);
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (!none) {
+        T e[PER];
+        memcpy(e, &v[step & 1][u], 16);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) e[j] = from_float<T>(gradient(to_float(e[j]), id + j));
+        for (int j = 0; j < PER; ++j) e[j] = from_float<T>(gradient(to_float(e[j]), id + j));
+        memcpy(&w, e, 16);
+      }
+      reinterpret_cast<uint4*>(out + row.head)[i] = w;
     }
-    uint4 w;
-    memcpy(&w, e, 16);
-    reinterpret_cast<uint4*>(out + row.head)[i] = w;
   }
   if (part == 0 && static_cast<int>(threadIdx.x) < row.head + row.tail) {
     const int id = row.edge_id(threadIdx.x);
@@ -552,7 +606,7 @@ static int launch_score(ScoreParams p, cudaStream_t stream) {
 template <typename T>
 static int launch_score_grad(ScoreParams p, cudaStream_t stream) {
   const int vectors = p.a.vocab / (16 / static_cast<int>(sizeof(T)));
-  p.parts = vectors / (kGradLoads * kScoreThreads) + 1;
+  p.parts = vectors / (kGradSteps * kGradLoads * kScoreThreads) + 1;
   const int64_t blocks = static_cast<int64_t>(p.a.rows) * p.parts;
   if (blocks > 0x7fffffff) return fail(QLIN_ERR_TOO_LARGE, "qlin_token_logprobs_bwd: too many rows");
   score_grad_kernel<T><<<static_cast<unsigned>(blocks), kScoreThreads, 0, stream>>>(p);

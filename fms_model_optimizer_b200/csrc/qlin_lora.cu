@@ -6,10 +6,10 @@
 // One launch does both products.  A tile is 16 or more rows of one adapter, wherever they stand; its block (or cluster of blocks, where tiles are few)
 // shares out the width of x for v and the columns of y afterwards, warp by warp, and joins the parts of v in shared memory in between, in order.
 //
-// Both products are m16n8k16 with the rows as the tile's rows.  Nothing but v goes through shared memory: the order of the terms of a product is free, so a lane
-// loads 16 bytes of a row of x and 16 of a row of a where the instruction wants four pairs of terms, and the columns of y are dealt so that
-// the four n = 8 products of 32 columns leave a lane with 16 bytes of y in a row.  Rows of 128 (tcgen05) would need the operands in shared memory and
-// would not make the loads faster.
+// Both products are m16n8k16 with the rows as the tile's rows.  No lane needs what another one loads, but for v: the order of the terms of a product is free, so a lane
+// takes 16 bytes of a row of x and 16 of a row of a where the instruction wants four pairs of terms, and the columns of y are dealt so that
+// the four n = 8 products of 32 columns leave a lane with 16 bytes of y in a row.  Asynchronous copies bring them to places of the lane's own in shared memory, several
+// steps ahead; a lane waits for its own copies only.  Rows of 128 (tcgen05) would not make the loads faster.
 //
 // v goes into the second product as two 16-bit numbers whose sum has 16 (bf16) or 22 (fp16) of its bits; in fp16 a row of v is brought to
 // 1 <= max < 2 first, by a power of two that comes back with the scale, since its sums may leave fp16's range where y does not.
@@ -39,13 +39,25 @@ struct LoraCfg {
   static constexpr int ROWS = 16 * MT;
   static constexpr int PITCH = RP + 4;       // floats of a row of v
   static constexpr int PITCH16 = RP + 8;     // 16-bit numbers of a row of v
-  static constexpr int STEPS = R16 * MT <= 2 ? 4 : R16 * MT <= 4 ? 2 : 1;  // of 32 terms that a warp has in flight
-  static constexpr int QUADS = RP >= 32 ? RP / 32 : 1;    // 16-byte (8-byte for rank 16) pieces of a row of b a lane holds
-  static constexpr int PARTS = kLoraWarps * ROWS * PITCH * 4;
-  static constexpr int BLOCK_V = PARTS;                    // [rows][PITCH]: the block's, then everybody's
-  static constexpr int V16 = BLOCK_V + ROWS * PITCH * 4;   // [2][rows][PITCH16]
-  static constexpr int UP = V16 + 2 * ROWS * PITCH16 * 2;  // [rows]
-  static constexpr int SMEM = UP + ROWS * 4;
+  static constexpr int QUADS = RP >= 32 ? RP / 32 : 1;  // 16-byte (8-byte for rank 16) pieces of a row of b a lane has
+  static constexpr bool HOLD = R16 * MT <= 8;           // v stays in registers while the columns go by
+  // A stage of a warp: 32 terms of the tile's rows of x and of the rows of a, or 32 columns of y and the rows of b behind them.  Stages for two blocks
+  // an SM, or for one where they are large.
+  static constexpr int B_BYTES = R16 == 1 ? 4 * 256 : 4 * QUADS * 512;
+  static constexpr int FIRST = (2 * MT + 2 * R16) * 512, SECOND = 2 * MT * 512 + B_BYTES;
+  static constexpr int STAGE = FIRST > SECOND ? FIRST : SECOND;
+  static constexpr int BLOCKS = STAGE <= 4096 ? 2 : 1;
+  static constexpr int STAGES = STAGE <= 2048 ? 6 : STAGE <= 4096 ? 3 : STAGE <= 6144 ? 4 : STAGE <= 8192 ? 3 : 2;
+  static constexpr int RING = kLoraWarps * STAGES * STAGE;
+  static constexpr int PARTS = RING;                       // [warps][rows][PITCH], in the room of the stages where those are not needed yet
+  static constexpr int PART_BYTES = kLoraWarps * ROWS * PITCH * 4;
+  static constexpr bool APART = RING + PART_BYTES + ROWS * PITCH * 4 + 4 * ROWS * PITCH16 + ROWS * 4 <= (BLOCKS == 2 ? 114 : 226) * 1024;
+  static constexpr int BLOCK_V = APART ? PARTS + PART_BYTES : PART_BYTES;  // [rows][PITCH]: the block's, then everybody's
+  static constexpr int V_END = BLOCK_V + ROWS * PITCH * 4;
+  static constexpr int V16 = APART || V_END > RING ? V_END : RING;  // [2][rows][PITCH16]
+  static constexpr int BACK = V16 + 2 * ROWS * PITCH16 * 2;  // [rows]
+  static constexpr int SMEM = BACK + ROWS * 4;
+  static_assert(SMEM <= (BLOCKS == 2 ? 114 : 227) * 1024, "fits");
 };
 
 // Adapter and first listed row of a tile; adapter -1: there is no such tile.  Every warp looks for itself.
@@ -101,13 +113,13 @@ __device__ __forceinline__ float2 unpack_pair(uint32_t w) {
 }
 
 template <typename T, int R16, int MT>
-__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __launch_bounds__(kLoraThreads, (LoraCfg<T, R16, MT>::BLOCKS)) lora_kernel(const __grid_constant__ LoraParams p) {
   using C = LoraCfg<T, R16, MT>;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* parts = reinterpret_cast<float*>(smem);
+  float* parts = reinterpret_cast<float*>(smem + (C::APART ? C::PARTS : 0));
   float* block_v = reinterpret_cast<float*>(smem + C::BLOCK_V);
   T* v16 = reinterpret_cast<T*>(smem + C::V16);
-  float* back = reinterpret_cast<float*>(smem + C::UP);
+  float* back = reinterpret_cast<float*>(smem + C::BACK);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % p.cluster;
   const LoraTile tile = lora_tile(p, blockIdx.x / p.cluster, C::ROWS, false);
@@ -131,7 +143,60 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     x_row[i] = row < 0 ? nullptr : static_cast<const T*>(p.a.x) + row * p.a.x_row;
     y_row[i] = row < 0 ? nullptr : static_cast<T*>(p.a.y) + row * p.a.y_row;
   }
-  const uint4 zero4 = make_uint4(0u, 0u, 0u, 0u);
+  // ---------------------------------------------------------------- copies: this warp's steps of 32 terms, then its steps of 32 columns
+  const T* a = static_cast<const T*>(p.a.a) + tile.adapter * p.a.a_adapter;
+  const T* b = static_cast<const T*>(p.a.b) + tile.adapter * p.a.b_adapter;
+  const int terms = (p.a.width + 31) / 32, columns = (p.a.out + 31) / 32;
+  const int terms_each = (terms + shares - 1) / shares, columns_each = (columns + shares - 1) / shares;
+  const int term0 = share * terms_each, column0 = share * columns_each;
+  const int n1 = max(0, min(terms_each, terms - term0)), n2 = max(0, min(columns_each, columns - column0));
+  const uint32_t ring = smem_u32(smem) + warp * C::STAGES * C::STAGE + lane * 16;
+  const auto copy = [&](uint32_t to, const void* from, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(real ? from : p.a.x), "r"(real ? 16 : 0) : "memory");
+  };
+  const auto copy_terms = [&](int i, uint32_t to) {
+    const int k = (term0 + i) * 32 + 8 * t;
+    const bool in = k < p.a.width;
+#pragma unroll
+    for (int j = 0; j < 2 * MT; ++j) copy(to + j * 512, x_row[j] + k, in && x_row[j] != nullptr);
+#pragma unroll
+    for (int j = 0; j < 2 * R16; ++j) copy(to + (2 * MT + j) * 512, a + (8 * j + g) * p.a.a_row + k, in && 8 * j < p.a.rank);
+  };
+  const auto copy_columns = [&](int i, uint32_t to) {
+    const int n0 = (column0 + i) * 32;
+#pragma unroll
+    for (int j = 0; j < 2 * MT; ++j) copy(to + j * 512, y_row[j] + n0 + 8 * t, y_row[j] != nullptr && n0 + 8 * t < p.a.out);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = n0 + 8 * (g >> 1) + 2 * q + (g & 1);
+      if constexpr (R16 == 1) {
+        const bool real = n < p.a.out && 4 * t < p.a.rank;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to - lane * 8 + 2 * MT * 512 + q * 256), "l"(real ? static_cast<const void*>(b + n * p.a.b_row + 4 * t) : p.a.x),
+                     "r"(real ? 8 : 0)
+                     : "memory");
+      } else {
+#pragma unroll
+        for (int c = 0; c < C::QUADS; ++c) copy(to + (2 * MT + q * C::QUADS + c) * 512, b + n * p.a.b_row + 32 * c + 8 * t, n < p.a.out && 32 * c + 8 * t < p.a.rank);
+      }
+    }
+  };
+  const auto stage_of = [&](int i) { return ring + static_cast<uint32_t>(i % C::STAGES) * C::STAGE; };
+  // The i-th copies of the warp.  Where the warps' parts of v lie over the stages, those of the columns begin behind the join.
+  const int first_total = C::APART ? n1 + n2 : n1;
+  const auto issue = [&](int i, int total) {
+    if (i < total) {
+      if (i < n1) copy_terms(i, stage_of(i));
+      else copy_columns(i - n1, stage_of(i));
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const auto held = [&](uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+  };
+#pragma unroll 1
+  for (int i = 0; i < C::STAGES - 1; ++i) issue(i, first_total);
 
   // ---------------------------------------------------------------- v, this warp's share of the terms
   float acc[MT][2 * R16][4];
@@ -139,69 +204,36 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int j = 0; j < 2 * R16; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.0f;
-  {
-    const T* a = static_cast<const T*>(p.a.a) + tile.adapter * p.a.a_adapter;
-    const int steps = (p.a.width + 31) / 32;
 #pragma unroll 1
-    for (int s0 = share; s0 < steps; s0 += shares * C::STEPS) {
-      uint4 xv[C::STEPS][2 * MT], av[C::STEPS][2 * R16];
+  for (int i = 0; i < n1; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
+    const uint32_t at = stage_of(i);
+    uint4 xv[2 * MT];
 #pragma unroll
-      for (int u = 0; u < C::STEPS; ++u) {
-        const int k = (s0 + u * shares) * 32 + 8 * t;
-        const bool in = k < p.a.width;
+    for (int j = 0; j < 2 * MT; ++j) xv[j] = held(at + j * 512);
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) xv[u][i] = in && x_row[i] != nullptr ? __ldg(reinterpret_cast<const uint4*>(x_row[i] + k)) : zero4;
+    for (int j = 0; j < 2 * R16; ++j) {
+      const uint4 av = held(at + (2 * MT + j) * 512);
 #pragma unroll
-        for (int j = 0; j < 2 * R16; ++j) av[u][j] = in && 8 * j < p.a.rank ? __ldg(reinterpret_cast<const uint4*>(a + (8 * j + g) * p.a.a_row + k)) : zero4;
+      for (int m = 0; m < MT; ++m) {
+        mma16816<C::BF16>(acc[m][j], xv[2 * m].x, xv[2 * m + 1].x, xv[2 * m].y, xv[2 * m + 1].y, av.x, av.y);
+        mma16816<C::BF16>(acc[m][j], xv[2 * m].z, xv[2 * m + 1].z, xv[2 * m].w, xv[2 * m + 1].w, av.z, av.w);
       }
-#pragma unroll
-      for (int u = 0; u < C::STEPS; ++u)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int j = 0; j < 2 * R16; ++j) {
-            mma16816<C::BF16>(acc[m][j], xv[u][2 * m].x, xv[u][2 * m + 1].x, xv[u][2 * m].y, xv[u][2 * m + 1].y, av[u][j].x, av[u][j].y);
-            mma16816<C::BF16>(acc[m][j], xv[u][2 * m].z, xv[u][2 * m + 1].z, xv[u][2 * m].w, xv[u][2 * m + 1].w, av[u][j].z, av[u][j].w);
-          }
     }
+    issue(i + C::STAGES - 1, first_total);  // over the step before this one, which has been read
+  }
+  if constexpr (!C::APART) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int j = 0; j < 2 * R16; ++j) {
-      float* at = parts + (warp * C::ROWS + 16 * m + g) * C::PITCH + 8 * j + 2 * t;
-      *reinterpret_cast<float2*>(at) = make_float2(acc[m][j][0], acc[m][j][1]);
-      *reinterpret_cast<float2*>(at + 8 * C::PITCH) = make_float2(acc[m][j][2], acc[m][j][3]);
+      float* to = parts + (warp * C::ROWS + 16 * m + g) * C::PITCH + 8 * j + 2 * t;
+      *reinterpret_cast<float2*>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
+      *reinterpret_cast<float2*>(to + 8 * C::PITCH) = make_float2(acc[m][j][2], acc[m][j][3]);
     }
-
-  // ---------------------------------------------------------------- loads of the second product, 32 columns: the first ones before the join
-  const T* b = static_cast<const T*>(p.a.b) + tile.adapter * p.a.b_adapter;
-  uint4 bv[4][C::QUADS], yv[2 * MT];
-  const auto load_columns = [&](int step) {
-    const int n0 = step * 32;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int n = n0 + 8 * (g >> 1) + 2 * q + (g & 1);
-#pragma unroll
-      for (int c = 0; c < C::QUADS; ++c) {
-        bv[q][c] = zero4;
-        if constexpr (R16 == 1) {
-          if (n < p.a.out && 4 * t < p.a.rank) {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(b + n * p.a.b_row + 4 * t));
-            bv[q][c].x = w.x;
-            bv[q][c].y = w.y;
-          }
-        } else {
-          if (n < p.a.out && 32 * c + 8 * t < p.a.rank) bv[q][c] = __ldg(reinterpret_cast<const uint4*>(b + n * p.a.b_row + 32 * c + 8 * t));
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i)
-      yv[i] = y_row[i] != nullptr && n0 + 8 * t < p.a.out ? *reinterpret_cast<const uint4*>(y_row[i] + n0 + 8 * t) : zero4;
-  };
-  const int columns = (p.a.out + 31) / 32;
-  if (share < columns) load_columns(share);
 
   // ---------------------------------------------------------------- v of all warps, then of all blocks, in order
   __syncthreads();
@@ -222,14 +254,15 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     const uint32_t base = smem_u32(block_v);
     for (int i = threadIdx.x; i < C::ROWS * C::RP / 4; i += kLoraThreads) {
       const int row = i / (C::RP / 4), c = i % (C::RP / 4) * 4;
-      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int o = 0; o < p.cluster; ++o) {
-        const float4 one = ld_cluster_f4(base + (row * C::PITCH + c) * 4, o);
-        sum = make_float4(sum.x + one.x, sum.y + one.y, sum.z + one.z, sum.w + one.w);
-      }
+      float4 one[kMostCluster];
+#pragma unroll
+      for (int o = 0; o < kMostCluster; ++o) one[o] = o < p.cluster ? ld_cluster_f4(base + (row * C::PITCH + c) * 4, o) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float4 sum = one[0];
+#pragma unroll
+      for (int o = 1; o < kMostCluster; ++o) sum = make_float4(sum.x + one[o].x, sum.y + one[o].y, sum.z + one[o].z, sum.w + one[o].w);
       *reinterpret_cast<float4*>(v + row * C::PITCH + c) = sum;
     }
-    cluster_arrive_wait();  // nobody leaves while its part is read
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
   __syncthreads();
   const float scale = p.a.scale[tile.adapter];
@@ -259,64 +292,101 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
   __syncthreads();
 
   // ---------------------------------------------------------------- y
-  uint4 vf[2][MT][2][C::QUADS];  // the two parts of the rows g and g + 8
   float factor[2 * MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int i = 0; i < 2 * MT; ++i) factor[i] = back[8 * i + g];
+  const auto part_of_v = [&](int part, int m, int h, int c) {  // of row g or g + 8 of the sixteen
+    const T* at = v16 + (part * C::ROWS + 16 * m + 8 * h + g) * C::PITCH16;
+    if constexpr (R16 == 1) {
+      const uint2 w = *reinterpret_cast<const uint2*>(at + 4 * t);
+      return make_uint4(w.x, w.y, 0u, 0u);
+    } else {
+      return *reinterpret_cast<const uint4*>(at + 32 * c + 8 * t);
+    }
+  };
+  uint4 vf[C::HOLD ? 2 : 1][C::HOLD ? MT : 1][2][C::QUADS];
+  if constexpr (C::HOLD) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = 16 * m + 8 * h + g;
-      factor[2 * m + h] = back[row];
+    for (int part = 0; part < 2; ++part)
 #pragma unroll
-      for (int part = 0; part < 2; ++part)
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < C::QUADS; ++c) vf[part][m][h][c] = part_of_v(part, m, h, c);
+  }
+  const auto leave = [&]() {  // nobody leaves, or copies over its part of v, while that is read
+    if (p.cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  };
+  if constexpr (!C::APART) {
+    leave();
+    __syncthreads();  // v has been read
+#pragma unroll 1
+    for (int i = 0; i < C::STAGES - 1; ++i) issue(n1 + i, n1 + n2);
+  }
+#pragma unroll 1
+  for (int i = n1; i < n1 + n2; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
+    const uint32_t at = stage_of(i);
+    uint4 bv[4][C::QUADS];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int c = 0; c < C::QUADS; ++c) {
+        if constexpr (R16 == 1) {
+          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(bv[q][c].x), "=r"(bv[q][c].y) : "r"(at - lane * 8 + 2 * MT * 512 + q * 256) : "memory");
+        } else {
+          bv[q][c] = held(at + (2 * MT + q * C::QUADS + c) * 512);
+        }
+      }
+    const int n = (column0 + i - n1) * 32 + 8 * t;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float o[4][4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q][0] = o[q][1] = o[q][2] = o[q][3] = 0.0f;
+#pragma unroll
+      for (int part = 1; part >= 0; --part)  // the small part first
 #pragma unroll
         for (int c = 0; c < C::QUADS; ++c) {
-          const T* at = v16 + (part * C::ROWS + row) * C::PITCH16;
-          if constexpr (R16 == 1) {
-            const uint2 w = *reinterpret_cast<const uint2*>(at + 4 * t);
-            vf[part][m][h][c] = make_uint4(w.x, w.y, 0u, 0u);
-          } else {
-            vf[part][m][h][c] = *reinterpret_cast<const uint4*>(at + 32 * c + 8 * t);
+          const uint4 r0 = C::HOLD ? vf[part % (C::HOLD ? 2 : 1)][m % (C::HOLD ? MT : 1)][0][c] : part_of_v(part, m, 0, c);
+          const uint4 r1 = C::HOLD ? vf[part % (C::HOLD ? 2 : 1)][m % (C::HOLD ? MT : 1)][1][c] : part_of_v(part, m, 1, c);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            mma16816<C::BF16>(o[q], r0.x, r1.x, r0.y, r1.y, bv[q][c].x, bv[q][c].y);
+            if constexpr (R16 > 1) mma16816<C::BF16>(o[q], r0.z, r1.z, r0.w, r1.w, bv[q][c].z, bv[q][c].w);
           }
         }
-    }
-#pragma unroll 1
-  for (int step = share; step < columns; step += shares) {
-    float o[MT][4][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int h = 0; h < 2; ++h) {
+        const uint4 y4 = held(at + (2 * m + h) * 512);
+        const uint32_t old[4] = {y4.x, y4.y, y4.z, y4.w};
+        uint32_t sum[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        o[m][q][0] = o[m][q][1] = o[m][q][2] = o[m][q][3] = 0.0f;
-#pragma unroll
-        for (int part = 1; part >= 0; --part)  // the small part first
-#pragma unroll
-          for (int c = 0; c < C::QUADS; ++c) {
-            const uint4 &r0 = vf[part][m][0][c], &r1 = vf[part][m][1][c];
-            mma16816<C::BF16>(o[m][q], r0.x, r1.x, r0.y, r1.y, bv[q][c].x, bv[q][c].y);
-            if constexpr (R16 > 1) mma16816<C::BF16>(o[m][q], r0.z, r1.z, r0.w, r1.w, bv[q][c].z, bv[q][c].w);
-          }
+        for (int q = 0; q < 4; ++q) {
+          const float2 y = unpack_pair<C::BF16>(old[q]);
+          sum[q] = pack_pair<C::BF16>(fmaf(o[q][2 * h], factor[2 * m + h], y.x), fmaf(o[q][2 * h + 1], factor[2 * m + h], y.y));
+        }
+        if (y_row[2 * m + h] != nullptr && n < p.a.out) *reinterpret_cast<uint4*>(y_row[2 * m + h] + n) = make_uint4(sum[0], sum[1], sum[2], sum[3]);
       }
-    const int n = step * 32 + 8 * t;
-    uint4 w[2 * MT];
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      const uint32_t old[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
-      uint32_t sum[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 y = unpack_pair<C::BF16>(old[q]);
-        const float* more = &o[i / 2][q][2 * (i & 1)];
-        sum[q] = pack_pair<C::BF16>(fmaf(more[0], factor[i], y.x), fmaf(more[1], factor[i], y.y));
-      }
-      w[i] = make_uint4(sum[0], sum[1], sum[2], sum[3]);
     }
-    if (step + shares < columns) load_columns(step + shares);
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i)
-      if (y_row[i] != nullptr && n < p.a.out) *reinterpret_cast<uint4*>(y_row[i] + n) = w[i];
+    issue(i + C::STAGES - 1, n1 + n2);
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (C::APART) leave();
   if (blockIdx.x == 0 && warp == 0) lora_tile(p, 0x7fffffff, C::ROWS, true);
+}
+
+// Sixteens of rows of a tile: as many as an adapter has rows for on average, and no more than leave a cluster of blocks for every eighth SM.
+static int64_t tiles_at_most(const qlin_lora_args& a, int rows) {
+  // every adapter has at most one tile that is not full, every tile a row
+  const int64_t most = static_cast<int64_t>(a.listed) / rows + a.adapters;
+  return most < a.listed ? most : a.listed;
+}
+static int sixteens(const qlin_lora_args& a, int most) {
+  int mt = 1;
+  while (mt < most && a.listed / a.adapters >= 32 * mt && tiles_at_most(a, 32 * mt) * kMostCluster >= sm_count()) mt *= 2;
+  return mt;
 }
 
 template <typename T, int R16, int MT>
@@ -332,11 +402,9 @@ static int launch_lora(LoraParams p, cudaStream_t stream) {
     if (e != cudaSuccess) return fail(QLIN_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     configured[dev] = true;
   }
-  // every adapter has at most one tile that is not full, every tile a row
-  const int64_t most = static_cast<int64_t>(p.a.listed) / C::ROWS + p.a.adapters;
-  const int64_t tiles = most < p.a.listed ? most : p.a.listed;
-  p.cluster = 1;
-  while (p.cluster < kMostCluster && tiles * p.cluster < sm_count()) p.cluster *= 2;
+  const int64_t tiles = tiles_at_most(p.a, C::ROWS);
+  p.cluster = 1;  // as many blocks a tile as are resident at once: a second wave costs more than they save (1999 rows of rank 64 36 us in fours, 74 in eights)
+  while (p.cluster < kMostCluster && tiles * p.cluster * 2 <= static_cast<int64_t>(C::BLOCKS) * sm_count()) p.cluster *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles) * p.cluster, 1, 1);
   cfg.blockDim = dim3(kLoraThreads, 1, 1);
@@ -355,13 +423,21 @@ static int launch_lora(LoraParams p, cudaStream_t stream) {
   }
   return QLIN_OK;
 }
+template <typename T, int R16, int MOST>
+static int pick_rows(const LoraParams& p, cudaStream_t s) {
+  const int mt = sixteens(p.a, MOST);
+  if constexpr (MOST >= 4) {
+    if (mt == 4) return launch_lora<T, R16, 4>(p, s);
+  }
+  if (mt == 2) return launch_lora<T, R16, 2>(p, s);
+  return launch_lora<T, R16, 1>(p, s);
+}
 template <typename T>
 static int pick_lora(const LoraParams& p, cudaStream_t s) {
-  const bool many = p.a.listed > 16 * 2 * sm_count();  // enough tiles of 32 rows for every SM
-  if (p.a.rank <= 16) return many ? launch_lora<T, 1, 2>(p, s) : launch_lora<T, 1, 1>(p, s);
-  if (p.a.rank <= 32) return many ? launch_lora<T, 2, 2>(p, s) : launch_lora<T, 2, 1>(p, s);
-  if (p.a.rank <= 64) return many ? launch_lora<T, 4, 2>(p, s) : launch_lora<T, 4, 1>(p, s);
-  return launch_lora<T, 8, 1>(p, s);
+  if (p.a.rank <= 16) return pick_rows<T, 1, 2>(p, s);
+  if (p.a.rank <= 32) return pick_rows<T, 2, 2>(p, s);
+  if (p.a.rank <= 64) return pick_rows<T, 4, 4>(p, s);
+  return pick_rows<T, 8, 2>(p, s);
 }
 
 }  // namespace qlin
