@@ -54,6 +54,23 @@ __device__ __forceinline__ float2 word_pair(uint32_t w) {  // the two 16-bit ele
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
+template <typename T>
+__device__ __forceinline__ uint4 packed(const float (&e)[16 / sizeof(T)]) {  // 16 bytes of the type, rounded to nearest
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (std::is_same<T, float>::value) {
+      w[j] = __float_as_uint(e[j]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(e[2 * j], e[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(e[2 * j], e[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 // The larger of two, NaN if one is NaN.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -62,11 +79,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 template <typename T>
 __device__ __forceinline__ uint32_t max_words(uint32_t a, uint32_t b) {
-  if constexpr (std::is_same<T, float>::value) return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
-  uint32_t r;
-  if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+  if constexpr (std::is_same<T, float>::value) {
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+  } else {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
 }
 template <typename T>
 __device__ __forceinline__ uint32_t lowest_word() {  // minus infinity, twice in 16 bits
@@ -476,11 +496,9 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const __grid_const
 }
 
 // ------------------------------------------------------------------------------------------------ the gradient
-constexpr int kGradLoads = 4;  // 16-byte pieces of a thread in flight
-constexpr int kGradSteps = 4;  // times that many
+// 16-byte pieces of a thread.  Blocks that go over four times as much with the next loads under way are slower: 2048 x 128256, forward and backward, 311 us, 263 so.
+constexpr int kGradLoads = 4;
 
-// A block takes kGradSteps times 16 KB of a row and has the next loads under way while it works on the last ones (2048 x 128256, with the forward
-// pass: one step a block 300 us).
 template <typename T>
 __global__ void __launch_bounds__(kScoreThreads) score_grad_kernel(const __grid_constant__ ScoreParams p) {
   constexpr int PER = 16 / sizeof(T);
@@ -494,56 +512,69 @@ __global__ void __launch_bounds__(kScoreThreads) score_grad_kernel(const __grid_
   const float dl = known && p.a.d_logprobs != nullptr ? p.a.d_logprobs[r] : 0.0f, dh = p.a.d_entropy != nullptr ? p.a.d_entropy[r] : 0.0f;
   const float ref = p.a.stats[2 * r], log_s = p.a.stats[2 * r + 1], entropy = p.a.entropy[r];
   const bool none = dl == 0.0f && dh == 0.0f;
-  const auto gradient = [&](float v, int id) {
-    const float log_p = (v - ref) - log_s;
-    const float prob = exp2_ftz(log_p * kLog2e);
-    float g = -prob * dl;
-    if (dh != 0.0f) g -= prob * dh * (fmaxf(log_p, -1e30f) + entropy);  // no probability, no entropy: 0 times a finite number
-    return id == token ? g + dl : g;
+  // p (a + b log p) for two logits, with the [j = t] term left out; where there is no probability log p is finite: 0 times a finite number
+  const float a = -fmaf(dh, entropy, dl), b = -dh;
+  const uint64_t minus_ref = pair64(-ref, -ref), minus_log_s = pair64(-log_s, -log_s), log2e = pair64(kLog2e, kLog2e), a2 = pair64(a, a), b2 = pair64(b, b);
+  const auto gradient = [&](float& u, float& w) {
+    float lu, lw, eu, ew;
+    unpair64(add2(add2(pair64(u, w), minus_ref), minus_log_s), lu, lw);
+    const uint64_t log_p = pair64(fmaxf(lu, -1e30f), fmaxf(lw, -1e30f));
+    unpair64(mul2(pair64(lu, lw), log2e), eu, ew);
+    unpair64(mul2(pair64(exp2_ftz(eu), exp2_ftz(ew)), fma2(log_p, b2, a2)), u, w);
   };
   const Row<T> row(reinterpret_cast<const T*>(out), vocab);  // pieces by where the gradient lies
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  const auto vector_of = [&](int step, int u) { return ((part * kGradSteps + step) * kGradLoads + u) * kScoreThreads + static_cast<int>(threadIdx.x); };
-  const auto load = [&](int step, uint4 (&v)[kGradLoads]) {
+  const auto vector_of = [&](int u) { return (part * kGradLoads + u) * kScoreThreads + static_cast<int>(threadIdx.x); };
+  uint4 v[kGradLoads];
 #pragma unroll
-    for (int u = 0; u < kGradLoads; ++u) {
-      const int i = vector_of(step, u);
-      if (i >= row.vectors || none) continue;
-      const T* at = x + row.id(i);
-      if (same) {
-        v[u] = __ldg(reinterpret_cast<const uint4*>(at));
-      } else {
-        T e[PER];
+  for (int u = 0; u < kGradLoads; ++u) {
+    const int i = vector_of(u);
+    if (i >= row.vectors || none) continue;
+    const T* at = x + row.id(i);
+    if (same) {
+      v[u] = __ldg(reinterpret_cast<const uint4*>(at));
+    } else {
+      float e[PER];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) e[j] = at[j];
-        memcpy(&v[u], e, 16);
-      }
+      for (int j = 0; j < PER; ++j) e[j] = to_float(at[j]);
+      v[u] = packed<T>(e);
     }
-  };
-  uint4 v[2][kGradLoads];
-  load(0, v[0]);
+  }
 #pragma unroll
-  for (int step = 0; step < kGradSteps; ++step) {
-    if (step + 1 < kGradSteps) load(step + 1, v[(step + 1) & 1]);
+  for (int u = 0; u < kGradLoads; ++u) {
+    const int i = vector_of(u);
+    if (i >= row.vectors) continue;
+    const int id = row.id(i);
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (!none) {
+      const uint32_t in[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      float e[PER];
 #pragma unroll
-    for (int u = 0; u < kGradLoads; ++u) {
-      const int i = vector_of(step, u);
-      if (i >= row.vectors) continue;
-      const int id = row.id(i);
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (!none) {
-        T e[PER];
-        memcpy(e, &v[step & 1][u], 16);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) e[j] = from_float<T>(gradient(to_float(e[j]), id + j));
-        memcpy(&w, e, 16);
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (std::is_same<T, float>::value) {
+          e[j] = __uint_as_float(in[j]);
+        } else {
+          const float2 f = word_pair<T>(in[j]);
+          e[2 * j] = f.x;
+          e[2 * j + 1] = f.y;
+        }
       }
-      reinterpret_cast<uint4*>(out + row.head)[i] = w;
+#pragma unroll
+      for (int j = 0; j < PER; j += 2) gradient(e[j], e[j + 1]);
+      if (token >= id && token < id + PER) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (token == id + j) e[j] += dl;
+      }
+      w = packed<T>(e);
     }
+    reinterpret_cast<uint4*>(out + row.head)[i] = w;
   }
   if (part == 0 && static_cast<int>(threadIdx.x) < row.head + row.tail) {
     const int id = row.edge_id(threadIdx.x);
-    out[id] = from_float<T>(none ? 0.0f : gradient(to_float(x[id]), id));
+    float e = to_float(x[id]), twice = e;
+    gradient(e, twice);
+    out[id] = from_float<T>(none ? 0.0f : id == token ? e + dl : e);
   }
 }
 
@@ -606,7 +637,7 @@ static int launch_score(ScoreParams p, cudaStream_t stream) {
 template <typename T>
 static int launch_score_grad(ScoreParams p, cudaStream_t stream) {
   const int vectors = p.a.vocab / (16 / static_cast<int>(sizeof(T)));
-  p.parts = vectors / (kGradSteps * kGradLoads * kScoreThreads) + 1;
+  p.parts = vectors / (kGradLoads * kScoreThreads) + 1;
   const int64_t blocks = static_cast<int64_t>(p.a.rows) * p.parts;
   if (blocks > 0x7fffffff) return fail(QLIN_ERR_TOO_LARGE, "qlin_token_logprobs_bwd: too many rows");
   score_grad_kernel<T><<<static_cast<unsigned>(blocks), kScoreThreads, 0, stream>>>(p);

@@ -11,7 +11,9 @@ SwiGLU are plumbing; the seven Linears of every layer run ``QLinearINT8Deploy``'
   norms and activations as PyTorch ops.  One GPU only.
 * ``generate``: greedy generation on one GPU with the fused surface.  A prompt's keys and values go into a paged cache on their way out
   of the rotation, later tokens attend over it (``kvcache.PagedKVCache``, ``ops.qk_norm_rope``, ``ops.prompt_attention``,
-  ``ops.paged_attention``).  ``cfg`` may ask for per-head norms of queries and keys (``qk_norm``) and a sliding window with first
+  ``ops.paged_attention``); prompts may share a prefix, which is computed, kept and read once for all (``ops.prefix_attention``), requests may each have a
+  low-rank adapter beside the quantized Linears (``adapters.LoraAdapters``), and the answers come with log probabilities if wanted (``ops.token_logprobs``).  ``score`` says how likely
+  given prompts are.  ``cfg`` may ask for per-head norms of queries and keys (``qk_norm``) and a sliding window with first
   tokens that stay visible (``window``, ``sinks``); ``forward`` follows them too.
 * sharded (``world > 1``): weights split column-parallel (q, k, v, gate, up) and row-parallel (o, down) following the
   reference's tables (fms_mo/aiu_addons/i8i8/i8i8_aiu_linear.py:304-389), one process per GPU.  ``exchange`` picks how
@@ -28,7 +30,7 @@ SwiGLU are plumbing; the seven Linears of every layer run ``QLinearINT8Deploy``'
 
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import List, NamedTuple, Optional, Sequence
 
 import torch
 import torch.distributed as dist
@@ -36,6 +38,7 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from . import ops, tp
+from .adapters import LoraAdapters, LoraStep
 from .kvcache import PagedKVCache, Step
 
 LLAMA3_8B = dict(layers=32, hidden=4096, q_heads=32, kv_heads=8, head_dim=128, ffn=14336, vocab=128256, rope_theta=500000.0,
@@ -159,6 +162,25 @@ def calibrate_act_scales(cfg, dev, ids, layers=None):
     return scales
 
 
+class Generated(NamedTuple):
+    """Generated ids and what the model said about them, [batch, new tokens] and, of the alternatives, [batch, new tokens, top]."""
+
+    ids: torch.Tensor
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_ids: torch.Tensor
+
+
+class Scored(NamedTuple):
+    """What the model says about each token of a prompt but the first, given those in front of it: [n - 1] and, of the alternatives, [n - 1, top]."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_ids: torch.Tensor
+
+
 class _Group:
     """Exchange buffers of one group of sequences (see W8A8Decoder.enable_token_split)."""
 
@@ -268,9 +290,12 @@ class W8A8Decoder:
                                            v.view(B, S, self.nkv, hd).transpose(1, 2), is_causal=True, enable_gqa=True)  # fmt: skip
         return a.transpose(1, 2).reshape(B * S, self.nq * hd)
 
-    def _head(self, last):
-        """(next-token ids, the normalised hidden state they were computed from) for the last token of every sequence."""
-        return (last @ self.lm_head.t()).argmax(-1), last
+    def _head(self, last, top=None):
+        """(next-token ids, the normalised hidden state they were computed from) for the last token of every sequence, and with ``top`` what
+        ``ops.token_logprobs`` says about these ids and ``top`` alternatives."""
+        logits = last @ self.lm_head.t()
+        ids = logits.argmax(-1)
+        return (ids, last) if top is None else (ids, last, *ops.token_logprobs(logits, ids, top=top))
 
     # ------------------------------------------------------------------------------------------------ one GPU / NCCL
     def _rotate(self, lin, q, k, positions, **cache):
@@ -302,19 +327,23 @@ class W8A8Decoder:
             pages = cache.layer(li)
             v = v.view(k.shape)
             q, k = self._rotate(lin, q, k, step.positions, v=v, slots=step.slots, want_k=not step.single, **pages)
-            if step.single:
+            if step.single and cache.prefix:
+                a = ops.prefix_attention(q, block_table=cache.table, lens=cache.lens, **cache.shared(), **pages, **attention_mask(self.cfg))
+            elif step.single:
                 a = ops.paged_attention(q, block_table=cache.table, lens=cache.lens, **pages, **attention_mask(self.cfg))
             else:
-                a = ops.prompt_attention(q, k, v, step.cu, step.cu, step.max_q, **attention_mask(self.cfg))
+                keys, values, cu_k = (k, v, step.cu) if step.keys is None else (k[step.keys], v[step.keys], step.cu_k)
+                a = ops.prompt_attention(q, keys, values, step.cu, cu_k, step.max_q, **attention_mask(self.cfg))
             return q, k, a.view(a.shape[0], -1)
 
         return attend
 
-    def _forward_steps(self, ids, attend=None, last=None):
+    def _forward_steps(self, ids, attend=None, last=None, lora: Optional[LoraStep] = None, head=None):
         """The forward pass of one group of sequences as a generator: it yields after every row-parallel Linear
         (whose all-reduce, if any, has just been queued), so that a driver can advance another group on another
         stream meanwhile.  Returns the next-token ids through StopIteration.  ``ids`` [batch, seq], or with ``attend`` (what
-        ``_attend_cached`` returns) [tokens] packed, ``last`` the rows that reach the head."""
+        ``_attend_cached`` returns) [tokens] packed, ``last`` the rows that reach the head.  ``lora``: the adapters of the rows.  ``head``: what is made
+        of the rows' final hidden states, by default ``_head``."""
         cfg = self.cfg
         if attend is None:
             B, S = ids.shape
@@ -325,14 +354,16 @@ class W8A8Decoder:
         x = F.embedding(ids, self.embed).view(B * S, -1)
         pending = None  # output of the last row-parallel Linear, added to the stream by the next fused kernel
         tr = self.trace is not None
+        want_h = tr or lora is not None
+        add = lora.add_ if lora is not None else lambda li, name, y, x: y
         for li, lin in enumerate(self.layers):
             # (x += pending) -> RMSNorm -> per-token int8 codes for q, k, v: one pass over the stream
-            cs, ss, xs, h = ops.block_quant(x, prologue=L.BLOCK_NORM, r=pending, norm_w=lin["ln1"], store_sum=True, want_h=tr,
+            cs, ss, xs, h = ops.block_quant(x, prologue=L.BLOCK_NORM, r=pending, norm_w=lin["ln1"], store_sum=True, want_h=want_h,
                                             smooth_rcps=[lin["q"].smooth_rcp, lin["k"].smooth_rcp, lin["v"].smooth_rcp])  # fmt: skip
             x = xs if xs is not None else x
-            q = lin["q"](None, (cs[0], ss[0]), bf)
-            k = lin["k"](None, (cs[1], ss[1]), bf)
-            v = lin["v"](None, (cs[2], ss[2]), bf)
+            q = add(li, "q", lin["q"](None, (cs[0], ss[0]), bf), h)
+            k = add(li, "k", lin["k"](None, (cs[1], ss[1]), bf), h)
+            v = add(li, "v", lin["v"](None, (cs[2], ss[2]), bf), h)
             if tr:
                 for tag, t in (("x_attn_in", x), ("h_attn", h), ("q", q), ("k", k), ("v", v)):
                     self._note(tag, li, t)
@@ -342,18 +373,20 @@ class W8A8Decoder:
             del cs, ss
             q, k, a = attend(li, lin, q.view(B * S, self.nq, hd), k.view(B * S, self.nkv, hd), v)
             qa = lin["o"].quantise_fused(a)
-            pending = lin["o"](None, qa, bf)
+            pending = add(li, "o", lin["o"](None, qa, bf), a)
             if tr:
                 for tag, t in (("q_rope", q), ("k_rope", k), ("attn", a), ("codes_o", qa[0]), ("scale_o", qa[1]), ("o", pending)):
                     self._note(tag, li, t)
             yield
-            cs, ss, x, h = ops.block_quant(x, prologue=L.BLOCK_NORM, r=pending, norm_w=lin["ln2"], store_sum=True, want_h=tr,
+            cs, ss, x, h = ops.block_quant(x, prologue=L.BLOCK_NORM, r=pending, norm_w=lin["ln2"], store_sum=True, want_h=want_h,
                                            smooth_rcps=[lin["gate"].smooth_rcp, lin["up"].smooth_rcp])  # fmt: skip
-            g = lin["gate"](None, (cs[0], ss[0]), bf)
-            u = lin["up"](None, (cs[1], ss[1]), bf)
-            keep = [] if tr else None
+            g = add(li, "gate", lin["gate"](None, (cs[0], ss[0]), bf), h)
+            u = add(li, "up", lin["up"](None, (cs[1], ss[1]), bf), h)
+            keep = [] if want_h else None
             qd = lin["down"].quantise_fused(g, L.BLOCK_SILU_MUL, u, keep_h=keep)
             pending = lin["down"](None, qd, bf)
+            if lora is not None:
+                add(li, "down", pending, keep[0])
             if tr:
                 for tag, t in (("x_mlp_in", x), ("h_mlp", h), ("gate", g), ("up", u), ("codes_gate", cs[0]), ("scale_gate", ss[0]),
                                ("codes_up", cs[1]), ("scale_up", ss[1]), ("h_down", keep[0]), ("codes_down", qd[0]), ("scale_down", qd[1]),
@@ -368,7 +401,7 @@ class W8A8Decoder:
             x_last, p_last = x[last], pending[last]
         _, _, x_last, h = ops.block_quant(x_last, prologue=L.BLOCK_NORM, r=p_last, norm_w=self.norm, store_sum=True, smooth_rcps=[], want_h=True)
         self._note("x_final_last", len(self.layers), x_last)
-        return self._head(h)
+        return (head or self._head)(h)
 
     def _forward_steps_modules(self, ids):
         """The same decoder through the module surface: RMSNorm, SiLU*up and the residual adds as PyTorch ops, every
@@ -560,30 +593,83 @@ class W8A8Decoder:
         return out
 
     @torch.no_grad()
-    def generate(self, prompts, new_tokens, cache: Optional[PagedKVCache] = None, cache_dtype=torch.bfloat16, page_size=64):
+    def generate(self, prompts, new_tokens, cache: Optional[PagedKVCache] = None, cache_dtype=torch.bfloat16, page_size=64, prefix: Optional[torch.Tensor] = None,
+                 adapters: Optional[LoraAdapters] = None, which: Optional[Sequence[int]] = None, logprobs: Optional[int] = None):  # fmt: skip
         """Greedy generation: ``new_tokens`` ids [batch, new_tokens] behind each of ``prompts`` (1-D id tensors, lengths as they come).
         ``cache``: an empty ``PagedKVCache`` for as many sequences, with room for what they come to; by default one of ``cache_dtype`` (bfloat16, or float8_e4m3fn
-        codes) is made.  ``self.last_hidden`` keeps the last step's final hidden states."""
+        codes) is made.  ``prefix``: ids that stand in front of every prompt; their keys are computed, kept and read once for all of them.  ``adapters`` and ``which``: the adapter
+        of each prompt, -1 for none; the prefix has none.  ``logprobs``: a number of alternatives (0 for none): the answer is then a ``Generated``.  ``self.last_hidden`` keeps the
+        last step's final hidden states."""
         if self.surface != "fused" or self.world != 1:
             raise RuntimeError("generate runs on one GPU with the fused surface")
         lengths = [int(p.numel()) for p in prompts]
         if not lengths or min(lengths) < 1 or new_tokens < 1:
             raise RuntimeError("generate takes prompts of at least one token and produces at least one")
-        longest = max(lengths) + new_tokens - 1  # the last id is produced, not read
+        shared = 0 if prefix is None else int(prefix.numel())
+        if prefix is not None and shared < 1:
+            raise RuntimeError("a prefix has at least one token")
+        if (adapters is None) != (which is None):
+            raise RuntimeError("adapters and the adapter of each prompt belong together")
+        longest = shared + max(lengths) + new_tokens - 1  # the last id is produced, not read
         if longest > self.cos.shape[0]:
             raise RuntimeError(f"{longest} tokens are more than the {self.cos.shape[0]} positions of cfg['seq']")
+        rows = adapters.which(which, lengths, self.dev, shared) if adapters is not None else None
         if cache is None:
             cache = PagedKVCache(len(self.layers), len(lengths), longest, self.nkv, self.cfg["head_dim"], self.dev, cache_dtype, page_size)
-        self._check_cache(cache, lengths, new_tokens)
-        ids, step, out = torch.cat([p.reshape(-1) for p in prompts]).to(self.dev), cache.prompts(lengths), []
+        self._check_cache(cache, lengths, new_tokens, shared)
+        ids = torch.cat([p.reshape(-1) for p in ([] if prefix is None else [prefix]) + list(prompts)]).to(self.dev)
+        if prefix is None:
+            step = cache.prompts(lengths)
+        else:
+            first = cache.share(shared)
+            step = cache.behind(first, cache.prompts(lengths))
+        lora = adapters.step(rows) if adapters is not None else None
+        out = []
         while True:
-            ids, self.last_hidden = self._drive([self._forward_steps(ids, self._attend_cached(cache, step), step.last)])
-            out.append(ids)
+            ids, self.last_hidden, *said = self._drive([self._forward_steps(ids, self._attend_cached(cache, step), step.last, lora, lambda h: self._head(h, logprobs))])
+            out.append((ids, *said))
             if len(out) == new_tokens:
-                return torch.stack(out, 1)
+                every = [torch.stack(t, 1) for t in zip(*out)]
+                return every[0] if logprobs is None else Generated(*every)
             step = cache.token()
+            if adapters is not None and len(out) == 1:  # from now on a row for every sequence
+                lora = adapters.step(adapters.which(which, [1] * len(lengths), self.dev))
 
-    def _check_cache(self, cache, lengths, new_tokens):
+    @torch.no_grad()
+    def score(self, prompts, top: int = 0, adapters: Optional[LoraAdapters] = None, which: Optional[Sequence[int]] = None) -> List[Scored]:
+        """How likely the model holds the tokens of each of ``prompts`` (1-D id tensors of at least two tokens), each given those in front of it, with its ``top`` alternatives: a
+        ``Scored`` for each.  ``torch.cat([s.logprobs for s in ...]).mean().neg().exp()`` is the perplexity (what fms_mo/dq.py:290-293 evaluates).  ``adapters`` and ``which`` as in ``generate``."""
+        if self.surface != "fused" or self.world != 1:
+            raise RuntimeError("score runs on one GPU with the fused surface")
+        lengths = [int(p.numel()) for p in prompts]
+        if not lengths or min(lengths) < 2:
+            raise RuntimeError("score takes prompts of at least two tokens")
+        if max(lengths) > self.cos.shape[0]:
+            raise RuntimeError(f"{max(lengths)} tokens are more than the {self.cos.shape[0]} positions of cfg['seq']")
+        if (adapters is None) != (which is None):
+            raise RuntimeError("adapters and the adapter of each prompt belong together")
+        lora = adapters.step(adapters.which(which, lengths, self.dev)) if adapters is not None else None
+        ids = torch.cat([p.reshape(-1) for p in prompts]).to(self.dev)
+        n = torch.tensor(lengths)
+        ends = n.cumsum(0)
+        positions = (torch.arange(int(ends[-1])) - torch.repeat_interleave(ends - n, n)).to(self.dev, torch.int32)
+        cu = torch.cat([torch.zeros(1, dtype=torch.int64), ends]).to(self.dev, torch.int32)
+        asked = (positions > 0).nonzero()[:, 0] - 1  # the rows in front of a token that is asked about
+
+        def attend(li, lin, q, k, v):
+            q, k = self._rotate(lin, q, k, positions)
+            a = ops.prompt_attention(q, k, v.view(k.shape), cu, cu, max(lengths), **attention_mask(self.cfg))
+            return q, k, a.view(a.shape[0], -1)
+
+        def head(h):
+            part = max(1, (1 << 28) // self.lm_head.shape[0])  # rows whose logits are half a gigabyte
+            said = [ops.token_logprobs(h[i : i + part] @ self.lm_head.t(), ids[asked[i : i + part] + 1], top=top) for i in range(0, h.shape[0], part)]
+            return tuple(torch.cat(t) for t in zip(*said))
+
+        said = self._drive([self._forward_steps(ids, attend, asked, lora, head)])
+        return [Scored(*t) for t in zip(*(x.split([m - 1 for m in lengths]) for x in said))]
+
+    def _check_cache(self, cache, lengths, new_tokens, shared=0):
         """Refuses a cache that does not fit the model or the whole generation, before anything runs."""
         if cache.batch != len(lengths) or len(cache.k) != len(self.layers):
             raise RuntimeError("the cache is for another number of sequences or layers")
@@ -592,9 +678,9 @@ class W8A8Decoder:
             raise RuntimeError(f"the cache has {kv_heads} kv heads of {head_dim}, the model {self.nkv} of {self.cfg['head_dim']}")
         if cache.k[0].dtype not in (torch.bfloat16, torch.float8_e4m3fn):
             raise RuntimeError("the cache must hold bfloat16 or float8_e4m3fn")
-        if any(cache.host_lens):
-            raise RuntimeError("generate starts with an empty cache: release its sequences first")
-        cache.check([n + new_tokens - 1 for n in lengths])
+        if any(cache.host_lens) or cache.prefix:
+            raise RuntimeError("generate starts with an empty cache: release its sequences, and what they share, first")
+        cache.check([shared + n + new_tokens - 1 for n in lengths], shared or None)
 
     def _drive(self, gens):
         """Advances the groups round-robin, one segment at a time, each on its own stream."""

@@ -1,6 +1,8 @@
 """A paged key-value cache for a decoder that generates: the pool of pages, the page table and the lengths that
 ``ops.qk_norm_rope`` writes with and ``ops.paged_attention`` reads with.
 
+Sequences may share their first tokens (``share``): these have pages of their own, which ``ops.prefix_attention`` reads once for all sequences.
+
 Every layer has its own pool ``[pages, kv heads, page size, head_dim]`` of keys and of values; all layers share one page table
 ``[batch, pages of a sequence]`` and one length for each sequence.  Pages are handed out as sequences grow and come back with
 ``release``; a released place stays out of the steps until ``prompts`` fills it again.  Tables, lengths, positions and slots live on
@@ -26,6 +28,8 @@ class Step:
     single: bool  # a row for every sequence of the cache, one new token for those that run
     cu: Optional[torch.Tensor] = None  # int32 [sequences + 1], prompts only
     max_q: int = 1
+    keys: Optional[torch.Tensor] = None  # int64: the rows whose keys every sequence sees, one sequence behind the other; None: its own
+    cu_k: Optional[torch.Tensor] = None  # int32 [sequences + 1], of `keys`
 
 
 class PagedKVCache:
@@ -54,27 +58,75 @@ class PagedKVCache:
         self._runs_dev = torch.ones(batch, dtype=torch.int32, device=dev)
         self._owned: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(pages - 1, -1, -1))
+        self.prefix = 0  # tokens that all sequences share
+        self._prefix_pages: List[int] = []
+        self.prefix_table = self.prefix_lens = self.groups = None
 
     def layer(self, i: int) -> dict:
         """The keyword arguments of layer ``i`` for ``ops.qk_norm_rope`` (and, without the slots, ``ops.paged_attention``)."""
         return dict(k_pages=self.k[i], v_pages=self.v[i], k_scale=self.k_scale[i], v_scale=self.v_scale[i])
 
-    def check(self, lengths: Sequence[int]) -> List[int]:
-        """Refuses lengths that the cache cannot hold; otherwise the pages that every sequence still needs for them."""
-        need = [max(0, -(-int(n) // self.page_size) - len(own)) for n, own in zip(lengths, self._owned)]
+    def shared(self) -> dict:
+        """The arguments of the shared prefix for ``ops.prefix_attention``."""
+        return dict(prefix_table=self.prefix_table, prefix_lens=self.prefix_lens, groups=self.groups)
+
+    def check(self, lengths: Sequence[int], prefix: Optional[int] = None) -> List[int]:
+        """Refuses lengths that the cache cannot hold; otherwise the pages that every sequence still needs for them.  ``prefix``: as if so many tokens were still
+        to be shared."""
+        common = -(-prefix // self.page_size) if prefix is not None else 0
+        first = (self.prefix if prefix is None else prefix) // self.page_size  # the page that a sequence's own tokens begin in
+        need = [max(0, -(-int(n) // self.page_size) - first - len(own)) for n, own in zip(lengths, self._owned)]
         if any(n > self.max_len for n in lengths):
             raise RuntimeError(f"a sequence of {max(lengths)} tokens does not fit a cache of {self.max_len}")
-        if sum(need) > len(self._free):
-            raise RuntimeError(f"the cache is out of pages: {sum(need)} wanted, {len(self._free)} free")
+        if sum(need) + common > len(self._free):
+            raise RuntimeError(f"the cache is out of pages: {sum(need) + common} wanted, {len(self._free)} free")
         return need
+
+    def share(self, tokens: int) -> Step:
+        """Room for ``tokens`` >= 1 first tokens that all sequences have in common, in an empty cache: the step that writes them.  Every sequence's length counts them
+        from then on, and ``prompts`` places its tokens behind them."""
+        if self.prefix or any(self.host_lens):
+            raise RuntimeError("a prefix goes into an empty cache: release its sequences, and unshare, first")
+        if not 1 <= tokens <= self.max_len:
+            raise RuntimeError(f"a prefix of {tokens} tokens does not fit a cache of {self.max_len}")
+        self.check([0] * self.batch, tokens)
+        self.prefix = tokens
+        self._prefix_pages = [self._free.pop() for _ in range(-(-tokens // self.page_size))]
+        positions, pages, lens, groups, last = self._send(range(tokens), self._prefix_pages, [tokens], [0, self.batch], [tokens - 1])
+        self.prefix_table, self.prefix_lens, self.groups = pages.to(torch.int32)[None], lens.to(torch.int32), groups.to(torch.int32)
+        slots = pages[positions // self.page_size] * self.page_size + positions % self.page_size
+        cu = torch.cat([positions[:1], lens]).to(torch.int32)
+        return Step(positions.to(torch.int32), slots, last, False, cu, tokens)
+
+    def unshare(self) -> None:
+        """The shared tokens are over: their pages go back to the pool.  All sequences have been released."""
+        if any(self.host_lens):
+            raise RuntimeError("sequences still have the shared tokens: release them first")
+        self._free += reversed(self._prefix_pages)
+        self.prefix, self._prefix_pages = 0, []
+        self.prefix_table = self.prefix_lens = self.groups = None
+
+    def behind(self, shared: Step, step: Step) -> Step:
+        """The step of ``share`` and that of the prompts behind it as one: the shared tokens, then the prompts, whose queries see the former's keys and their own."""
+        n = self.prefix
+        own = step.cu.diff().long()
+        cu_k = torch.cat([step.cu[:1], (step.cu[1:] + n * torch.arange(1, own.numel() + 1, device=self.dev, dtype=torch.int32))])
+        key = torch.arange(step.positions.numel() + n * own.numel(), device=self.dev)
+        of = torch.searchsorted(cu_k[1:].contiguous(), key.to(torch.int32), right=True)  # the sequence of each key
+        within = key - cu_k[of]
+        keys = torch.where(within < n, within, n + step.cu[of] + within - n)
+        first = torch.arange(n, device=self.dev)
+        return Step(torch.cat([shared.positions, step.positions]), torch.cat([shared.slots, step.slots]), step.last + n, False, torch.cat([shared.cu, step.cu[1:] + n]),
+                    max(shared.max_q, step.max_q), torch.cat([first, keys]), torch.cat([shared.cu, cu_k[1:] + n]))  # fmt: skip
 
     def reserve(self, lengths: Sequence[int]) -> None:
         """Hands out the pages for sequences of these lengths.  Refused as a whole where the pool does not hold them."""
         need = self.check(lengths)
+        first = self.prefix // self.page_size
         rows, columns, pages = [], [], []
         for b, n in enumerate(need):
             rows += [b] * n
-            columns += range(len(self._owned[b]), len(self._owned[b]) + n)
+            columns += range(first + len(self._owned[b]), first + len(self._owned[b]) + n)
             self._owned[b] += [self._free.pop() for _ in range(n)]
             pages += self._owned[b][len(self._owned[b]) - n :]
         if rows:
@@ -104,7 +156,7 @@ class PagedKVCache:
         return page * self.page_size + positions % self.page_size
 
     def prompts(self, lengths: Sequence[int], which: Optional[Sequence[int]] = None) -> Step:
-        """Room for prompts of ``lengths[i]`` >= 1 tokens in the empty sequences ``which[i]``, by default in all of them.  From then on
+        """Room for prompts of ``lengths[i]`` >= 1 tokens (behind the shared ones, if there are any) in the empty sequences ``which[i]``, by default in all of them.  From then on
         ``token`` goes on with these and with those that have tokens already; other empty ones wait for a prompt of their own."""
         which = list(range(self.batch)) if which is None else [int(b) for b in which]
         if len(lengths) != len(which) or not which or min(lengths) < 1:
@@ -113,7 +165,7 @@ class PagedKVCache:
             raise RuntimeError(f"prompts go to different sequences of the {self.batch}")
         if any(self.host_lens[b] for b in which):
             raise RuntimeError("prompts start empty sequences: release them first")
-        new = dict(zip(which, (int(n) for n in lengths)))
+        new = dict(zip(which, (self.prefix + int(n) for n in lengths)))
         self.reserve([new.get(b, 0) for b in range(self.batch)])
         n, rows = torch.tensor(lengths), torch.tensor(which)
         cu = torch.zeros(len(which) + 1, dtype=torch.int64)
@@ -121,7 +173,7 @@ class PagedKVCache:
         of = torch.repeat_interleave(torch.arange(len(which)), n)
         self.host_lens = [new.get(b, have) for b, have in enumerate(self.host_lens)]
         self._runs = [have > 0 for have in self.host_lens]
-        positions, of, last, cu, lens, runs = self._send(torch.arange(int(cu[-1])) - cu[of], rows[of], cu[1:] - 1, cu, self.host_lens, self._runs)
+        positions, of, last, cu, lens, runs = self._send(torch.arange(int(cu[-1])) - cu[of] + self.prefix, rows[of], cu[1:] - 1, cu, self.host_lens, self._runs)
         self.lens.copy_(lens)
         self._runs_dev.copy_(runs)
         return Step(positions.to(torch.int32), self._slots(of, positions), last, False, cu.to(torch.int32), int(n.max()))

@@ -109,7 +109,7 @@ class W8A8Linear:
         (``ops.block_quant``); a row-parallel shard takes two passes around the MAX all-reduce of the scales.
         ``exchange`` (a ``ScaleExchange``) replaces that all-reduce: the first pass stores this shard's scales into slot
         ``rank`` on every GPU, and after the barrier the second pass takes the maximum over the slots itself.
-        ``keep_h``: a list that receives the bf16 row the Linear sees (``prologue(x2, r)``), for tests."""
+        ``keep_h``: a list that receives the bf16 row the Linear sees (``prologue(x2, r)``), for adapters beside the Linear and for tests."""
         rcp = [self.smooth_rcp]
         want_h = keep_h is not None
         if exchange is not None:

@@ -55,3 +55,55 @@ def test_places_that_never_had_a_prompt_wait_for_one():
     # a whole empty cache can start from its first token, as before
     cache = _cache()
     assert cache.token().positions.tolist() == [0, 0] and cache.lens.tolist() == [1, 1]
+
+
+def test_a_shared_prefix_has_pages_of_its_own():
+    cache = _cache(batch=3, max_len=40, page_size=8, pages=9)
+    first = cache.share(19)  # three pages, the last one with room that nobody else's keys go into
+    assert first.positions.tolist() == list(range(19)) and first.cu.tolist() == [0, 19] and first.last.tolist() == [18] and first.max_q == 19 and not first.single
+    assert first.slots.tolist() == [int(cache.prefix_table[0, i // 8]) * 8 + i % 8 for i in range(19)]
+    assert cache.prefix_lens.tolist() == [19] and cache.groups.tolist() == [0, 3]
+    step = cache.prompts([4, 9, 1])
+    assert cache.host_lens == [23, 28, 20] == cache.lens.tolist()
+    assert step.positions.tolist() == [*range(19, 23), *range(19, 28), 19]
+    assert step.slots.tolist() == [int(cache.table[b, i // 8]) * 8 + i % 8 for b, n in ((0, 4), (1, 9), (2, 1)) for i in range(19, 19 + n)]
+    used = {s // 8 for s in first.slots.tolist()}
+    assert len(used) == 3 and not used & {s // 8 for s in step.slots.tolist()} and len(set(step.slots.tolist())) == 14
+    both = cache.behind(first, step)
+    assert both.positions.tolist() == [*range(19), *range(19, 23), *range(19, 28), 19] and both.cu.tolist() == [0, 19, 23, 32, 33]
+    assert both.cu_k.tolist() == [0, 19, 42, 70, 90] and both.last.tolist() == [22, 31, 32] and both.max_q == 19
+    assert both.keys.tolist() == [*range(19), *range(19), *range(19, 23), *range(19), *range(23, 32), *range(19), 32]
+    assert both.slots.tolist() == first.slots.tolist() + step.slots.tolist()
+    one = cache.token()
+    assert one.positions.tolist() == [23, 28, 20] and cache.lens.tolist() == [24, 29, 21]
+    # 3 + 1 + 2 + 1 pages of nine: two are left, and the lengths count the prefix
+    cache.reserve([32, 29, 32])
+    with pytest.raises(RuntimeError, match="out of pages"):
+        cache.reserve([33, 29, 32])
+    with pytest.raises(RuntimeError, match="does not fit"):
+        cache.check([41, 1, 1])
+    with pytest.raises(RuntimeError, match="release"):
+        cache.unshare()
+    with pytest.raises(RuntimeError, match="empty cache"):
+        cache.share(1)
+    cache.release(1)
+    step = cache.prompts([2], [1])
+    assert step.positions.tolist() == [19, 20] and cache.host_lens == [24, 21, 21]
+    for b in range(3):
+        cache.release(b)
+    cache.unshare()
+    assert cache.prefix == 0 and len(cache._free) == 9 and cache.prompts([40, 1, 8]).positions.tolist()[:2] == [0, 1]
+
+
+def test_a_shared_prefix_that_does_not_fit_is_refused():
+    cache = _cache(batch=2, max_len=40, page_size=8, pages=4)
+    for bad in (0, 41, 33):
+        with pytest.raises(RuntimeError, match="fit|out of pages"):
+            cache.share(bad)
+    assert cache.prefix == 0 and len(cache._free) == 4
+    cache.check([20, 20], 16)  # two pages together, one each
+    with pytest.raises(RuntimeError, match="out of pages"):
+        cache.check([20, 20], 17)
+    cache.prompts([1, 1])
+    with pytest.raises(RuntimeError, match="empty cache"):
+        cache.share(4)
