@@ -26,6 +26,7 @@ struct SharedPrefix {
   int64_t table_stride;
   int32_t count, max_pages, splits;
   int32_t blocks;         // of the launch
+  int32_t align;          // a power of two: the keys that are read for a group begin and end at multiples of it
   float* part_o;          // [batch * q_heads, splits, head_dim]
   float2* part_ml;        // [batch * q_heads, splits]: maximum and sum
 };
@@ -97,7 +98,8 @@ __device__ __forceinline__ Common common_keys(const PagedParams& p, int g, int g
   if (longest == 0) return c;
   const int cut = static_cast<int>(wide > c.prefix ? wide : c.prefix);  // lengths above it are cut there
   longest = min(longest, cut);
-  const int from = p.a.window > 0 && longest > p.a.window ? longest - p.a.window : 0, to = min(min(shortest, cut), c.prefix);
+  const int first = p.a.window > 0 && longest > p.a.window ? longest - p.a.window : 0, past = p.pre.align - 1;
+  const int from = (first + past) & ~past, to = min(min(shortest, cut), c.prefix) & ~past;
   c.from = from < to ? from : 0;
   c.to = from < to ? to : 0;
   return c;
@@ -804,6 +806,8 @@ static int launch_paged(const PagedParams& p, cudaStream_t stream) {
 }
 
 // The prefix's part on tcgen05, tiles of 128 rows (qlin_prefix_tc.cu): two tiles a block where `pair`, otherwise one tile and two splits.
+// Only where prefix_box says how many keys of a page a copy takes, which `align` then is.
 int launch_prefix_tc(const PagedParams& p, bool pair, cudaStream_t stream);
+int prefix_box(const qlin_paged_attention_args& a);
 
 }  // namespace qlin

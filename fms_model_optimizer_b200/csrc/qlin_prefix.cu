@@ -20,10 +20,12 @@ struct PrefixPlan {
   Splits own;
   int32_t units, splits, columns;  // of the launch for the prefixes: blocks of columns of all kv heads at most, splits of the keys, columns of a block
   int32_t blocks;                  // of that launch
+  int32_t align;                   // see SharedPrefix
   int64_t own_floats, shared_floats;  // of the workspace
 };
 static PrefixPlan plan_prefix(const qlin_prefix_attention_args& a) {
   PrefixPlan plan = {};
+  plan.align = 1;
   const int group = a.own.q_heads / a.own.kv_heads;
   // the tables' widths say how many keys of their own sequences may have
   qlin_paged_attention_args own = a.own;
@@ -34,7 +36,9 @@ static PrefixPlan plan_prefix(const qlin_prefix_attention_args& a) {
   const int64_t keys = static_cast<int64_t>(a.max_prefix_pages) * a.own.page_size;
   if (keys > 0 && a.own.num_pages > 0) {
     const int64_t per_head = rows / a.own.kv_heads, each = (per_head + a.num_groups - 1) / a.num_groups;  // rows of a kv head, and of a group on average
-    plan.columns = each > kRowsPair ? 256 : each >= kRowsTensor ? 128 : each > 8 ? 16 : 8;
+    const int box = prefix_box(a.own);
+    plan.columns = box == 0 || each < kRowsTensor ? (each > 8 ? 16 : 8) : each > kRowsPair ? 256 : 128;
+    if (plan.columns >= 128) plan.align = box;
     const int64_t blocks = per_head / plan.columns + a.num_groups;  // a group has one block that is not full at most
     if (blocks * a.own.kv_heads > (1 << 24)) return plan;
     plan.units = static_cast<int32_t>(blocks * a.own.kv_heads);
@@ -133,6 +137,7 @@ extern "C" int qlin_prefix_attention(const qlin_prefix_attention_args* a, void* 
   p.pre.max_pages = a->max_prefix_pages;
   p.pre.splits = plan.splits > 0 ? plan.splits : 1;
   p.pre.blocks = plan.blocks;
+  p.pre.align = plan.align;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool f8 = a->own.cache_dtype == QLIN_DT_F8E4M3;
   if (a->own.dtype == QLIN_DT_BF16) return f8 ? pick_prefix<__nv_bfloat16, true>(p, plan, s) : pick_prefix<__nv_bfloat16, false>(p, plan, s);

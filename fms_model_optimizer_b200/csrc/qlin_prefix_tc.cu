@@ -7,24 +7,29 @@
 // weights as the operand from there.  Two streams of tiles take turns, one in the softmax while the other is in the tensor core: two tiles of rows that share each tile of keys and
 // values, or, where a group has no more than 128 rows, one tile of rows against two splits of the keys.
 //
-// Pages may have any size and stride and end anywhere in a tile, and the cache may hold e4m3 codes, so no tensor map describes it: three warps find the rows through
-// the page table and bring them to the 128-byte swizzle by 16-byte asynchronous copies, a tile of keys or values a warp, or through registers where
-// codes become fp16 on the way.  A bf16 query meets codes as fp16 times a power of two that brings its largest element to 2^13..2^14.
+// Keys and values come by TMA, a box of up to 32 keys of a page at a time, found through the page table; pages whose size has no factor of 8, and strides that no tensor map
+// describes, are left to the kernel of the attention over pages.  The keys that are read here begin and end at multiples of the box, so that no box holds a key that
+// somebody does not see; the few beside them are the sequences' own.  e4m3 codes land beside the tiles and two warps make fp16 of them on the way there; a bf16 query
+// meets these as fp16 times a power of two that brings its largest element to 2^13..2^14.  (Through the threads' registers and 16-byte asynchronous copies, which take
+// pages of any size, the loads were what the rest waited for: 2 x 64 sequences behind 32768 keys 127 us.)
 //
 // Logits enter the exponent as their difference from the reference, so that it is exact near the maximum however large they are.
+#include <cuda.h>
+
 #include "qlin_attend.cuh"
 #include "qlin_paged.cuh"
 
 namespace qlin {
 
-constexpr int kSharedSoftmaxWarps = 8, kSharedLoadWarps = 3;
-constexpr int kSharedMmaWarp = kSharedSoftmaxWarps + kSharedLoadWarps;
+constexpr int kSharedSoftmaxWarps = 8, kSharedLoadWarp = kSharedSoftmaxWarps, kSharedWidenWarp = kSharedLoadWarp + 1, kSharedWidenWarps = 2;
+constexpr int kSharedMmaWarp = kSharedWidenWarp + kSharedWidenWarps;
+constexpr int kMostBox = 32;  // keys of a copy
 constexpr int kSharedThreads = (kSharedMmaWarp + 1) * 32;
 // As in the attention of prompts: 168 registers a thread at first (64,512 in all), 216 for the softmax once the others are down to 72.
 constexpr int kSharedSoftmaxRegs = 216, kSharedOtherRegs = 72;
 
 struct SharedAux {
-  uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], p_full[2][2], o_full[2], drain;
+  uint64_t q_full[2], kv_full[8], kv_empty[8], raw_full[8], raw_empty[8], s_full[2], p_full[2][2], o_full[2], drain;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -37,9 +42,11 @@ struct SharedCfg {
   static constexpr int CHUNKS = DP / 64;
   static constexpr int TILE_BYTES = CHUNKS * kChunkBytes;
   static constexpr int Q_TILES = PAIR ? 2 : 1;
-  static constexpr int STAGES = DP == 128 ? (PAIR ? 5 : 6) : 8;
+  static constexpr int STAGES = F8 ? (DP == 128 ? (PAIR ? 3 : 4) : 6) : DP == 128 ? (PAIR ? 5 : 6) : 8;
+  static constexpr int RAW_BYTES = kKeys * DP, RAW = F8 ? (DP == 128 ? 4 : 6) : 0;  // tiles of codes
   static constexpr int KV_OFFSET = Q_TILES * TILE_BYTES;
-  static constexpr int AUX_OFFSET = KV_OFFSET + STAGES * TILE_BYTES;
+  static constexpr int RAW_OFFSET = KV_OFFSET + STAGES * TILE_BYTES;
+  static constexpr int AUX_OFFSET = RAW_OFFSET + RAW * RAW_BYTES;
   static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(SharedAux));
   static constexpr float SHIFT = HALF ? 6.0f : 0.0f;
   static constexpr uint32_t FMT = HALF ? 0u : 1u;
@@ -118,8 +125,16 @@ __device__ __forceinline__ void shared_softmax(uint32_t s_addr, uint32_t o_addr,
   l += a + b;
 }
 
+// A box of keys of one page, [keys][64 elements or a row of codes].
+__device__ __forceinline__ void box_load(uint32_t bar, uint32_t dst, const void* tmap, int32_t x, int32_t slot, int32_t head, int32_t page) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%3, %4, %5, %6}], [%0];" ::"r"(bar), "r"(dst),
+               "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(slot), "r"(head), "r"(page)
+               : "memory");
+}
+
 template <typename QT, bool F8, int DP, bool PAIR>
-__global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                                                                    const __grid_constant__ PagedParams p) {
   using C = SharedCfg<QT, F8, DP, PAIR>;
   using T = typename C::T;
   extern __shared__ __align__(1024) uint8_t shared_tiles[];
@@ -148,9 +163,11 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   if (rows <= 0 || tiles0 == 0) return;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::STAGES; ++i) {
+    for (int i = 0; i < 8; ++i) {
       mbar_init(&aux->kv_full[i], 1);
       mbar_init(&aux->kv_empty[i], 1);
+      mbar_init(&aux->raw_full[i], 1);
+      mbar_init(&aux->raw_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&aux->q_full[i], kRows);
@@ -167,10 +184,6 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
     tmem_alloc(&aux->tmem_base, 512);
     tmem_relinquish();
   }
-  if (!F8 && p.a.head_dim < DP) {  // head dimensions past the end are zeros in every stage, and stay so
-    for (int i = threadIdx.x; i < C::STAGES * C::TILE_BYTES / 16; i += kSharedThreads) reinterpret_cast<uint4*>(smem + C::KV_OFFSET)[i] = make_uint4(0u, 0u, 0u, 0u);
-    fence_proxy_async();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -179,151 +192,115 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
 
   if (warp >= kSharedSoftmaxWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSharedOtherRegs));
-    if (warp < kSharedMmaWarp) {
-      // ------------------------------------------------------------------ loads, in the order in which the products take them
-      constexpr int CH = DP * C::ES / 16;  // 16-byte pieces of a row in the cache
-      constexpr int AT_ONCE = 32 / CH;     // rows that a warp's instruction copies
-      const int lrow = lane / CH, lc = lane % CH;
-      const bool piece_real = lc * 16 < p.a.head_dim * C::ES;
+    // The tiles in the order in which the products take them: `tile(stream, values, t)` until it says no.
+    const auto every_tile = [&](auto tile) {
+      if constexpr (PAIR) {
+        for (int t = 0; t < tiles0; ++t)
+          if (!tile(0, false, t) || !tile(0, true, t)) return;
+      } else {
+        if (!tile(0, false, 0) || (tiles1 > 0 && !tile(1, false, 0))) return;
+        for (int t = 0; t < tiles0; ++t)
+          for (int i = 0; i < 2; ++i) {
+            const int mine = i ? tiles1 : tiles0;
+            if (t < mine && !tile(i, true, t)) return;
+            if (t + 1 < mine && !tile(i, false, t + 1)) return;
+          }
+      }
+    };
+    if (warp == kSharedLoadWarp) {
+      // ------------------------------------------------------------------ loads: lane i brings the i-th box of a tile
+      constexpr int RING = F8 ? C::RAW : C::STAGES, BYTES = F8 ? C::RAW_BYTES : C::TILE_BYTES;
+      constexpr int CHUNKS = F8 ? 1 : C::CHUNKS, ROW = F8 ? DP : 128;  // pieces of a row, bytes of one
+      uint64_t* const full = F8 ? aux->raw_full : aux->kv_full;
+      uint64_t* const empty = F8 ? aux->raw_empty : aux->kv_empty;
+      const uint32_t ring = smem_u32(smem) + (F8 ? C::RAW_OFFSET : C::KV_OFFSET);
       const int32_t* table = p.pre.table + g * p.pre.table_stride;
-      const int64_t head_off = kvh * p.a.head_stride;
+      const int box = p.pre.align;
       bool bad_page = false;
       uint32_t s = 0, ph = 1;
-      int turn = 0, pending = -1;
-      const auto hand_over = [&](int stage) {  // what all lanes wrote is there for the tensor core
-        fence_proxy_async();
+      int issued = 0;
+      every_tile([&](int i, bool values, int t) {
+        const int key = begin_of(i) + t * kKeys + lane * box, left = min(count_of(i) - t * kKeys, kKeys);  // a multiple of the box
+        const bool mine = lane * box < left;
+        const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.a.page_size;
+        int page = mine ? table[pg] : 0;
+        ok = uniform_wait(&empty[s], ph, abort_flag);
+        if (!ok) return false;
+        if (page < 0 || page >= p.a.num_pages) {
+          bad_page = true;
+          page = 0;
+        }
+        const uint32_t dst = ring + s * BYTES;
+        if (left < kKeys) {  // rows behind the last key are zeros: what lay there before meets weights of zero, but may be infinite
+          for (int at = left * ROW / 16 + lane; at < kKeys * ROW / 16; at += 32)
+            for (int c = 0; c < CHUNKS; ++c) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + c * kChunkBytes + at * 16), "r"(0u) : "memory");
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>(left * ROW * CHUNKS));
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->kv_full[stage]);
-      };
-      const auto finish_pending = [&]() {
-        if (pending < 0) return;
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        hand_over(pending);
-        pending = -1;
-      };
-      const auto load = [&](int i, int kv, int t) {
-        if (!ok) return;
-        const uint32_t stage = s, parity = ph;
-        if (++s == C::STAGES) {
+        if (mine)
+          for (int c = 0; c < CHUNKS; ++c)
+            box_load(smem_u32(&full[s]), dst + c * kChunkBytes + lane * box * ROW, values ? &tmap_v : &tmap_k, c * 64, key - pg * p.a.page_size, kvh, page);
+        __syncwarp();
+        ++issued;
+        if (++s == RING) {
           s = 0;
           ph ^= 1u;
         }
-        const bool mine = turn == warp - kSharedSoftmaxWarps;
-        if (++turn == kSharedLoadWarps) turn = 0;
-        if (!mine) return;
-        const int begin = begin_of(i), count = count_of(i);
-        // the pages of the rows 32 j + lane are on their way while the stage is waited for (read one after the other they cost 5000 cycles a tile)
-        const auto place = [&](int j, int& offset) {
-          const int key = min(begin + t * kKeys + 32 * j + lane, begin + count - 1), pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.a.page_size;
-          offset = key - pg * p.a.page_size;
-          return pg;
-        };
-        int o0, o1, o2, o3;
-        const int p0 = table[place(0, o0)], p1 = table[place(1, o1)], p2 = table[place(2, o2)], p3 = table[place(3, o3)];
-        if (pending >= 0 && !__all_sync(0xffffffffu, mbar_test_wait(&aux->kv_empty[stage], parity))) finish_pending();
-        ok = uniform_wait(&aux->kv_empty[stage], parity, abort_flag);
-        if (!ok) return;
-        const uint8_t* base = static_cast<const uint8_t*>(kv ? p.a.v_pages : p.a.k_pages);
-        const uint32_t dst = smem_u32(smem) + C::KV_OFFSET + stage * C::TILE_BYTES;
-        const auto address = [&](int j) {  // in bytes; -1: no key
-          int page = j < 2 ? (j == 0 ? p0 : p1) : (j == 2 ? p2 : p3);
-          const int offset = j < 2 ? (j == 0 ? o0 : o1) : (j == 2 ? o2 : o3);
-          if (t * kKeys + 32 * j + lane >= count) return static_cast<int64_t>(-1);
-          if (page < 0 || page >= p.a.num_pages) {
-            bad_page = true;
-            page = 0;
-          }
-          return (page * p.a.page_stride + offset * p.a.slot_stride + head_off) * C::ES;
-        };
-        if constexpr (!F8) {
-          // Eight addresses, then eight copies: with each copy right behind its own address, and with a size that may be zero, a copy takes 117 cycles and the
-          // loads are what the rest waits for (2 x 64 sequences behind 32768 keys 190 us).  Rows that are not there are written as zeros, which only the last tile has.
-          const bool whole = (t + 1) * kKeys <= count;
-          const uint32_t x = static_cast<uint32_t>((lc & 7) ^ lrow) << 4, to = dst + (lc >> 3) * kChunkBytes + lrow * 128;
-          const auto copy_rows = [&](int j, bool all) {
-            const int64_t off = address(j);
-#pragma unroll
-            for (int n0 = 0; n0 < 32 / AT_ONCE; n0 += 8) {
-              int64_t at[8];
-#pragma unroll
-              for (int n = 0; n < 8; ++n) at[n] = __shfl_sync(0xffffffffu, off, (n0 + n) * AT_ONCE + lrow);
-              if (piece_real) {
-#pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                  const uint32_t place = to + (32 * j + (n0 + n) * AT_ONCE) * 128 + (x ^ static_cast<uint32_t>((((n0 + n) * AT_ONCE) & 7) << 4));
-                  if (all || at[n] >= 0) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place), "l"(base + at[n] + lc * 16) : "memory");
-                  else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(place), "r"(0u) : "memory");
-                }
-              }
-            }
-          };
-          if (whole) {
-#pragma unroll 1
-            for (int j = 0; j < 4; ++j) copy_rows(j, true);
-          } else {
-#pragma unroll 1
-            for (int j = 0; j < 4; ++j) copy_rows(j, false);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          if (pending >= 0) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            hand_over(pending);
-          }
-          pending = static_cast<int>(stage);
-        } else {
-          constexpr int BATCH = 32 / AT_ONCE < 8 ? 32 / AT_ONCE : 8;  // pieces that a lane has in flight
-#pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            const int64_t off = address(j);
-            uint4 v[BATCH];
-            int64_t from[BATCH];
-#pragma unroll
-            for (int n = 0; n < BATCH; ++n) from[n] = __shfl_sync(0xffffffffu, off, n * AT_ONCE + lrow);
-#pragma unroll
-            for (int n = 0; n < BATCH; ++n) {
-              const int64_t at = from[n];
-              v[n] = piece_real && at >= 0 ? __ldg(reinterpret_cast<const uint4*>(base + at + lc * 16)) : make_uint4(0u, 0u, 0u, 0u);
-            }
-#pragma unroll
-            for (int n = 0; n < BATCH; ++n) {
-              const int row = 32 * j + n * AT_ONCE + lrow;
-              // lanes of the second 64 dimensions write their halves in the other order: eight lanes meet all banks
-              const bool swap = lc >= 4;
-              const uint32_t x = swap ? v[n].z : v[n].x, y = swap ? v[n].w : v[n].y, z = swap ? v[n].x : v[n].z, w = swap ? v[n].y : v[n].w;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + tile_piece(row, 2 * lc + (swap ? 1 : 0))), "r"(widen_lo(x)), "r"(widen_hi(x)),
-                           "r"(widen_lo(y)), "r"(widen_hi(y))
-                           : "memory");
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + tile_piece(row, 2 * lc + (swap ? 0 : 1))), "r"(widen_lo(z)), "r"(widen_hi(z)),
-                           "r"(widen_lo(w)), "r"(widen_hi(w))
-                           : "memory");
-            }
-          }
-          hand_over(static_cast<int>(stage));
+        return true;
+      });
+      if (!ok) {  // copies in flight land before the block retires
+        if (lane == 0) {
+          timed_out = !*abort_flag;
+          *abort_flag = 1;
         }
-      };
-      if constexpr (PAIR) {
-        for (int t = 0; t < tiles0 && ok; ++t) {
-          load(0, 0, t);
-          load(0, 1, t);
-        }
-      } else {
-        load(0, 0, 0);
-        if (tiles1 > 0) load(1, 0, 0);
-        for (int t = 0; t < tiles0 && ok; ++t)
-          for (int i = 0; i < 2; ++i) {
-            const int mine = i ? tiles1 : tiles0;
-            if (t < mine) load(i, 1, t);
-            if (t + 1 < mine) load(i, 0, t + 1);
-          }
+        for (int n = max(0, issued - RING); n < issued; ++n) mbar_wait_drain(&full[n % RING], (n / RING) & 1);
       }
-      if (ok) finish_pending();
-      if (!ok && lane == 0) {
-        timed_out = !*abort_flag;
-        *abort_flag = 1;
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");  // copies in flight land before the block retires
       if (bad_page && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
       __syncwarp();
+    } else if (warp < kSharedMmaWarp) {
+      // ------------------------------------------------------------------ codes to fp16, every other tile
+      if constexpr (F8) {
+        constexpr int CH = DP / 16, AT_ONCE = 32 / CH;  // 16-byte pieces of a row of codes, rows that a warp's instruction takes
+        const int lrow = lane / CH, lc = lane % CH;
+        // lanes of the second 64 dimensions write their halves in the other order: eight lanes meet all banks
+        const bool swap = lc >= 4;
+        int n = 0;
+        every_tile([&](int, bool, int) {
+          const int turn = n++;
+          if (turn % kSharedWidenWarps != warp - kSharedWidenWarp) return true;
+          const int r = turn % C::RAW, s = turn % C::STAGES;
+          ok = uniform_wait(&aux->raw_full[r], (turn / C::RAW) & 1, abort_flag, &aux->kv_empty[s], ((turn / C::STAGES) & 1) ^ 1);
+          if (!ok) return false;
+          const uint32_t from = smem_u32(smem) + C::RAW_OFFSET + r * C::RAW_BYTES, dst = smem_u32(smem) + C::KV_OFFSET + s * C::TILE_BYTES;
+#pragma unroll 4
+          for (int k = 0; k < kKeys / AT_ONCE; ++k) {
+            const int row = k * AT_ONCE + lrow;
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from + piece<DP>(row, lc)) : "memory");
+            const uint32_t x = swap ? v.z : v.x, y = swap ? v.w : v.y, z = swap ? v.x : v.z, w = swap ? v.y : v.w;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + tile_piece(row, 2 * lc + (swap ? 1 : 0))), "r"(widen_lo(x)), "r"(widen_hi(x)), "r"(widen_lo(y)),
+                         "r"(widen_hi(y))
+                         : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + tile_piece(row, 2 * lc + (swap ? 0 : 1))), "r"(widen_lo(z)), "r"(widen_hi(z)), "r"(widen_lo(w)),
+                         "r"(widen_hi(w))
+                         : "memory");
+          }
+          fence_proxy_async();  // what all lanes wrote is there for the tensor core, and what they read may be written over
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&aux->kv_full[s]);
+            mbar_arrive(&aux->raw_empty[r]);
+          }
+          return true;
+        });
+        if (!ok && lane == 0) {
+          timed_out = !*abort_flag;
+          *abort_flag = 1;
+        }
+        __syncwarp();
+      }
     } else {
       // ------------------------------------------------------------------ products
       const uint32_t base = (smem_u32(smem) & 0x3FFFFu) >> 4, d0 = uniform(tmem);
@@ -523,6 +500,34 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   }
 }
 
+// The keys of a page that one copy takes: a power of two that divides the page, so that a box lies in one page; 0 where there is none of 8 or the strides are no tensor map's.
+int prefix_box(const qlin_paged_attention_args& a) {
+  int box = a.page_size & -a.page_size;
+  if (box > kMostBox) box = kMostBox;
+  const int64_t size = a.cache_dtype == QLIN_DT_F8E4M3 ? 1 : 2, most = int64_t{1} << 38;
+  const auto fits = [&](int64_t stride, int64_t n) { return n <= 1 || (stride > 0 && stride * size < most); };
+  return box >= 8 && fits(a.slot_stride, a.page_size) && fits(a.head_stride, a.kv_heads) && fits(a.page_stride, a.num_pages) && tensor_map_encoder() != nullptr ? box : 0;
+}
+// [pages, kv heads, slots, head_dim] read in boxes of `box` keys of one head; head dimensions past the end are zeros.
+static int page_map(CUtensorMap* tm, const void* base, const qlin_paged_attention_args& a, int box) {
+  using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                          CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  const Fn enc = reinterpret_cast<Fn>(tensor_map_encoder());
+  const bool f8 = a.cache_dtype == QLIN_DT_F8E4M3;
+  const int64_t size = f8 ? 1 : 2, row = (a.head_dim * size + 15) / 16 * 16;  // stands in for the stride of a dimension with one entry
+  const int width = f8 ? (a.head_dim <= 64 ? 64 : 128) : 64;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.num_pages)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.page_size > 1 ? a.slot_stride * size : row), static_cast<cuuint64_t>(a.kv_heads > 1 ? a.head_stride * size : row),
+                           static_cast<cuuint64_t>(a.num_pages > 1 ? a.page_stride * size : row)};
+  cuuint32_t boxes[4] = {static_cast<cuuint32_t>(width), static_cast<cuuint32_t>(box), 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(tm, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : a.dtype == QLIN_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                         const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         width * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(QLIN_ERR_BAD_ALIGN, "qlin_prefix_attention: cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+  return QLIN_OK;
+}
+
 template <typename QT, bool F8, int DP, bool PAIR>
 static int launch_shared(const PagedParams& p, cudaStream_t stream) {
   using C = SharedCfg<QT, F8, DP, PAIR>;
@@ -538,11 +543,15 @@ static int launch_shared(const PagedParams& p, cudaStream_t stream) {
     const cudaError_t f = cudaFuncGetAttributes(&attr, kernel);
     if (f != cudaSuccess) return fail(QLIN_ERR_LAUNCH, "cudaFuncGetAttributes: %s", cudaGetErrorString(f));
     // what the softmax warps ask for must be there, or they would wait for it for good
-    if (attr.numRegs * kSharedThreads < 32 * (kSharedSoftmaxWarps * kSharedSoftmaxRegs + (kSharedLoadWarps + 1) * kSharedOtherRegs))
+    if (attr.numRegs * kSharedThreads < 32 * (kSharedSoftmaxWarps * kSharedSoftmaxRegs + 4 * kSharedOtherRegs))
       return fail(QLIN_ERR_LAUNCH, "qlin_prefix_attention: built with %d registers a thread, too few for its split", attr.numRegs);
     configured[dev] = true;
   }
-  shared_kernel<QT, F8, DP, PAIR><<<static_cast<unsigned>(p.pre.blocks), kSharedThreads, C::SMEM_BYTES, stream>>>(p);
+  CUtensorMap tk, tv;
+  int rc = page_map(&tk, p.a.k_pages, p.a, p.pre.align);
+  if (rc == QLIN_OK) rc = page_map(&tv, p.a.v_pages, p.a, p.pre.align);
+  if (rc != QLIN_OK) return rc;
+  shared_kernel<QT, F8, DP, PAIR><<<static_cast<unsigned>(p.pre.blocks), kSharedThreads, C::SMEM_BYTES, stream>>>(tk, tv, p);
   QLIN_CHECK_LAUNCH("qlin_prefix_attention");
   return QLIN_OK;
 }
