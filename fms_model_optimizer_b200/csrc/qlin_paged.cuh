@@ -262,7 +262,9 @@ __device__ __forceinline__ uint32_t piece(int row, int c) {
   return static_cast<uint32_t>(row * RB + ((RB >= 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4));
 }
 
-template <typename QT, bool F8, int DP, int NT, PagedMode MODE>
+// WARPS: of a unit, a kv head of a sequence (up to 8 or 16 query heads of it).  Fewer than the block's four where there are more units than blocks fit the SMs at once: a block
+// then has two or four units, and each unit fewer warps to join.
+template <typename QT, bool F8, int DP, int NT, PagedMode MODE, int WARPS>
 __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOCKS)) paged_kernel(const __grid_constant__ PagedParams p) {
   using C = PagedCfg<QT, F8, DP, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -270,8 +272,10 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int splits = MODE == kShared ? p.pre.splits : p.splits;
-  const int split = blockIdx.x % splits;
-  const int unit = blockIdx.x / splits;
+  const int split = WARPS == kPagedWarps ? blockIdx.x % splits : 0, sub = warp % WARPS;
+  const int units = p.a.batch * p.a.kv_heads * p.head_blocks, given = WARPS == kPagedWarps ? blockIdx.x / splits : blockIdx.x * (kPagedWarps / WARPS) + warp / WARPS;
+  const bool idle = WARPS != kPagedWarps && given >= units;
+  const int unit = idle ? units - 1 : given;
   int b, kvh, head0, heads;  // head0: first query head of the block within the kv head's, kShared: first of the group's rows
   Common common{0, 0, 0, 0, 0};
   if constexpr (MODE == kShared) {
@@ -300,8 +304,9 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
     const Group of = group_of(p.pre, b);
     group = of.g;
     if (group >= 0) common = common_keys(p, group, of.first, of.end, false);
-    else if (threadIdx.x == 0 && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
-    len = sequence_length(p, b, threadIdx.x == 0, common.prefix);
+    else if (lane == 0 && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
+    len = sequence_length(p, b, lane == 0, common.prefix);
+    if (idle) len = 0;
   }
   const auto vis = [&]() {
     if constexpr (MODE == kShared) return Visible{0, common.from, common.to - common.from};
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
     if constexpr (MODE == kOwn) griddep_wait();
     return;
   }
-  const int first = split * per + warp, last = min(tiles, (split + 1) * per);
+  const int first = split * per + sub, last = min(tiles, (split + 1) * per);
 
   // ---------------------------------------------------------------- loads
   const int32_t* table = MODE == kShared ? p.pre.table + b * p.pre.table_stride : p.a.block_table + static_cast<int64_t>(b) * p.a.table_stride;
@@ -366,11 +371,11 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
   {
     Place ahead[C::STAGES - 1];  // all of them are read together
 #pragma unroll
-    for (int s = 0; s < C::STAGES - 1; ++s) ahead[s] = look_up(first + s * kPagedWarps);
+    for (int s = 0; s < C::STAGES - 1; ++s) ahead[s] = look_up(first + s * WARPS);
 #pragma unroll
-    for (int s = 0; s < C::STAGES - 1; ++s) load_tile(first + s * kPagedWarps, s, ahead[s]);
+    for (int s = 0; s < C::STAGES - 1; ++s) load_tile(first + s * WARPS, s, ahead[s]);
   }
-  Place place = look_up(first + (C::STAGES - 1) * kPagedWarps);
+  Place place = look_up(first + (C::STAGES - 1) * WARPS);
 
   // ---------------------------------------------------------------- queries, as columns g of the product's second operand
   uint32_t qf[DP / 16][NT][2];
@@ -429,11 +434,11 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
   int stage = 0, stage_in = C::STAGES - 1;
   const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;   // ldmatrix: rows, then pieces
   const int vrow = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;   // ldmatrix.trans of 16-bit values: pieces, then rows
-  for (int tile = first; tile < last; tile += kPagedWarps) {
+  for (int tile = first; tile < last; tile += WARPS) {
     asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
     __syncwarp();
-    load_tile(tile + (C::STAGES - 1) * kPagedWarps, stage_in, place);  // into the stage of the tile before this one
-    place = look_up(tile + C::STAGES * kPagedWarps);
+    load_tile(tile + (C::STAGES - 1) * WARPS, stage_in, place);  // into the stage of the tile before this one
+    place = look_up(tile + C::STAGES * WARPS);
     const uint32_t ks = ring + stage * C::STAGE, vs = ks + kTileKeys * C::RB;
     float s[NT][4];
 #pragma unroll
@@ -559,14 +564,15 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
     if constexpr (MODE == kOwn) join_prefix(p, static_cast<int64_t>(b) * p.a.q_heads + head_of(h), d, pre_used, C::BF16 ? 1.0f : 4096.0f, top, sum, acc);
   };
   if constexpr (MODE == kOwn) griddep_wait();  // the sums over the prefix are there
-  for (int i = threadIdx.x; i < heads * (DP / 4); i += kPagedThreads) {
+  const int warp0 = warp - sub;  // the unit's first
+  for (int i = sub * 32 + lane; i < heads * (DP / 4); i += WARPS * 32) {
     const int h = i / (DP / 4), d = i % (DP / 4) * 4;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, warp_ml[w * C::HEADS + h].x);
+    for (int w = warp0; w < warp0 + WARPS; ++w) top = fmaxf(top, warp_ml[w * C::HEADS + h].x);
     float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) {
+    for (int w = warp0; w < warp0 + WARPS; ++w) {
       const float2 ml = warp_ml[w * C::HEADS + h];
       const float f = ml.x == top ? 1.0f : exp2f(ml.x - top);
       sum += ml.y * f;
@@ -576,7 +582,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
       acc[2] += v.z * f;
       acc[3] += v.w * f;
     }
-    if (d >= D) continue;
+    if (d >= D || idle) continue;
     if constexpr (MODE == kShared) {
       constexpr float down = C::BF16 ? 1.0f : 1.0f / 4096.0f;  // without the factor that fp16 weights carry
       const int64_t row = (static_cast<int64_t>(sequence_of(h)) * p.a.q_heads + head_of(h)) * splits + split;
@@ -748,10 +754,10 @@ inline int check_paged_pointers(const qlin_paged_attention_args* a, const char* 
   return QLIN_OK;
 }
 
-template <typename QT, bool F8, int DP, int NT, PagedMode MODE>
+template <typename QT, bool F8, int DP, int NT, PagedMode MODE, int WARPS = kPagedWarps>
 static int launch_paged(const PagedParams& p, cudaStream_t stream) {
   using C = PagedCfg<QT, F8, DP, NT>;
-  const auto kernel = paged_kernel<QT, F8, DP, NT, MODE>;
+  const auto kernel = paged_kernel<QT, F8, DP, NT, MODE, WARPS>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -762,7 +768,8 @@ static int launch_paged(const PagedParams& p, cudaStream_t stream) {
     configured[dev] = true;
   }
   const bool shared = MODE == kShared, cluster = !shared && p.cluster;
-  const unsigned blocks = shared ? static_cast<unsigned>(p.pre.blocks) : static_cast<unsigned>(p.a.batch) * p.a.kv_heads * p.head_blocks * p.splits;
+  constexpr unsigned units_of_block = kPagedWarps / WARPS;
+  const unsigned blocks = shared ? static_cast<unsigned>(p.pre.blocks) : (static_cast<unsigned>(p.a.batch) * p.a.kv_heads * p.head_blocks * p.splits + units_of_block - 1) / units_of_block;
   cudaLaunchConfig_t main = {};
   main.gridDim = dim3(blocks, 1, 1);
   main.blockDim = dim3(kPagedThreads, 1, 1);

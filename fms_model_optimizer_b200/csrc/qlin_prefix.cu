@@ -15,12 +15,14 @@ namespace qlin {
 // Rows of a group (its sequences times the query heads of a kv head) from which on the tensor cores' 128-row tiles take the prefix, and above which a
 // block has two of them.
 constexpr int kRowsTensor = 32, kRowsPair = 128;
+constexpr int kLongOwn = 2048;  // keys of its own that a sequence may have for fewer warps than four
 
 struct PrefixPlan {
   Splits own;
   int32_t units, splits, columns;  // of the launch for the prefixes: blocks of columns of all kv heads at most, splits of the keys, columns of a block
   int32_t blocks;                  // of that launch
   int32_t align;                   // see SharedPrefix
+  int32_t warps;                   // of a sequence's kv head in the launch for its own keys
   int64_t own_floats, shared_floats;  // of the workspace
 };
 static PrefixPlan plan_prefix(const qlin_prefix_attention_args& a) {
@@ -30,7 +32,14 @@ static PrefixPlan plan_prefix(const qlin_prefix_attention_args& a) {
   // the tables' widths say how many keys of their own sequences may have
   qlin_paged_attention_args own = a.own;
   own.max_pages = a.own.max_pages > a.max_prefix_pages ? a.own.max_pages - a.max_prefix_pages + 1 : 1;
-  plan.own = choose_splits(own, (group + heads_per_block(group) - 1) / heads_per_block(group));
+  const int head_blocks = (group + heads_per_block(group) - 1) / heads_per_block(group);
+  plan.own = choose_splits(own, head_blocks);
+  // Warps that are all resident at once, if the keys are few enough for that to count: a block of four for each kv head of 128 sequences comes in three or four
+  // waves, each of them the latency of the lookups, the keys and the join.
+  const bool f8 = a.own.cache_dtype == QLIN_DT_F8E4M3;
+  const int64_t units = static_cast<int64_t>(a.own.batch) * a.own.kv_heads * head_blocks, slots = static_cast<int64_t>(f8 && group <= 8 ? 3 : 2) * kPagedWarps * sm_count();
+  plan.warps = units * 4 <= slots || static_cast<int64_t>(own.max_pages) * own.page_size > kLongOwn ? 4 : units * 2 <= slots ? 2 : 1;
+  if (plan.warps < 4) plan.own = Splits{1, 0};
   const int64_t rows = static_cast<int64_t>(a.own.batch) * a.own.q_heads;
   if (plan.own.n > 1 && !plan.own.cluster) plan.own_floats = rows * plan.own.n * (a.own.head_dim + 2);
   const int64_t keys = static_cast<int64_t>(a.max_prefix_pages) * a.own.page_size;
@@ -72,13 +81,19 @@ static int check_prefix(const qlin_prefix_attention_args* a) {
   return QLIN_OK;
 }
 
+template <typename QT, bool F8, int DP, int NT>
+static int launch_own(const PagedParams& p, int warps, cudaStream_t s) {
+  if (warps == 1) return launch_paged<QT, F8, DP, NT, kOwn, 1>(p, s);
+  if (warps == 2) return launch_paged<QT, F8, DP, NT, kOwn, 2>(p, s);
+  return launch_paged<QT, F8, DP, NT, kOwn>(p, s);
+}
 template <typename QT, bool F8, int DP>
 static int launch_prefix(const PagedParams& p, const PrefixPlan& plan, cudaStream_t s) {
   if (p.pre.blocks > 0) {
     const int rc = plan.columns >= 128 ? launch_prefix_tc(p, plan.columns == 256, s) : plan.columns == 16 ? launch_paged<QT, F8, DP, 2, kShared>(p, s) : launch_paged<QT, F8, DP, 1, kShared>(p, s);
     if (rc != QLIN_OK) return rc;
   }
-  return heads_per_block(p.group) == 16 ? launch_paged<QT, F8, DP, 2, kOwn>(p, s) : launch_paged<QT, F8, DP, 1, kOwn>(p, s);
+  return heads_per_block(p.group) == 16 ? launch_own<QT, F8, DP, 2>(p, plan.warps, s) : launch_own<QT, F8, DP, 1>(p, plan.warps, s);
 }
 template <typename QT, bool F8>
 static int pick_prefix(const PagedParams& p, const PrefixPlan& plan, cudaStream_t s) {
