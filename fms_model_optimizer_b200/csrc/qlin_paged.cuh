@@ -151,40 +151,50 @@ __device__ __forceinline__ Group group_of(const SharedPrefix& pre, int b) {
   }
   return Group{-1, 0, 0};
 }
-// The sums over the prefix join those of a sequence's own keys, which carry a factor of 2^shift, split by split in order; eight are read at a time.
+// The sums over the prefix join those of a sequence's own keys, which carry a factor of `shift`, sixteen splits at a time in order.  Sixteen lanes that have outputs of one head
+// (d: the first of four) share the work on maxima and sums, a split each: done by every lane for itself, with the library's exponential, a turn took 4000 cycles.
+constexpr int kJoinAtOnce = 16;
+__device__ __forceinline__ float exp2_or_zero(float x) {  // 2 ulp
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ void join_prefix(const PagedParams& p, int64_t row, int d, int used, float shift, float& top, float& sum, float (&acc)[4]) {
+  const int lane = threadIdx.x & 31, base = lane & 16;
+  const uint32_t group = 0xffffu << base;
   const float2* ml = p.pre.part_ml + row * p.pre.splits;
-  const float* o = p.pre.part_o + row * p.pre.splits * p.a.head_dim + d;
+  const float* o = p.pre.part_o + row * p.pre.splits * p.a.head_dim + min(d, p.a.head_dim - 4);
 #pragma unroll 1
-  for (int s0 = 0; s0 < used; s0 += 8) {
-    float2 one[8];
-    float4 v[8];
+  for (int s0 = 0; s0 < used; s0 += kJoinAtOnce) {
+    const int mine = s0 + (lane & 15);
+    float4 v[kJoinAtOnce];
+    float2 one = __ldcg(ml + min(mine, used - 1));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      one[i] = make_float2(-INFINITY, 0.0f);
-      if (s0 + i < used) {
-        one[i] = __ldcg(ml + s0 + i);
-        v[i] = __ldcg(reinterpret_cast<const float4*>(o + static_cast<int64_t>(s0 + i) * p.a.head_dim));
-      }
-    }
-    float most = top;
+    for (int i = 0; i < kJoinAtOnce; ++i)  // past the last one it is read again: loads behind branches would wait for one another
+      v[i] = __ldcg(reinterpret_cast<const float4*>(o + static_cast<int64_t>(min(s0 + i, used - 1)) * p.a.head_dim));
+    if (mine >= used) one = make_float2(-INFINITY, 0.0f);
+    float most = one.x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = fmaxf(most, one[i].x);
-    const float keep = top == most ? 1.0f : exp2f(top - most);
+    for (int w = 1; w < kJoinAtOnce; w <<= 1) most = fmaxf(most, __shfl_xor_sync(group, most, w));
+    most = fmaxf(most, top);
+    const float ref = most == -INFINITY ? 0.0f : most, keep = exp2_or_zero(top - ref), f = exp2_or_zero(one.x - ref) * shift;
+    float total = one.y * f;
+#pragma unroll
+    for (int w = 1; w < kJoinAtOnce; w <<= 1) total += __shfl_xor_sync(group, total, w);
     top = most;
-    sum *= keep;
+    sum = fmaf(sum, keep, total);
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] *= keep;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (s0 + i < used) {
-        const float f = (one[i].x == most ? 1.0f : exp2f(one[i].x - most)) * shift;
-        sum += one[i].y * f;
-        acc[0] += v[i].x * f;
-        acc[1] += v[i].y * f;
-        acc[2] += v[i].z * f;
-        acc[3] += v[i].w * f;
+    for (int i = 0; i < kJoinAtOnce; ++i) {
+      const float fi = __shfl_sync(group, f, base + i);
+      if (s0 + i < used) {  // not 0 times what is read again
+        acc[0] = fmaf(v[i].x, fi, acc[0]);
+        acc[1] = fmaf(v[i].y, fi, acc[1]);
+        acc[2] = fmaf(v[i].z, fi, acc[2]);
+        acc[3] = fmaf(v[i].w, fi, acc[3]);
       }
+    }
   }
 }
 
@@ -236,7 +246,7 @@ __device__ __forceinline__ float max_of_rows(float v) {  // over the eight lanes
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
 
-template <typename QT, bool F8, int DP, int NT>
+template <typename QT, bool F8, int DP, int NT, bool OWN = false>
 struct PagedCfg {
   static constexpr bool BF16 = std::is_same<QT, __nv_bfloat16>::value && !F8;  // type of the products
   static constexpr int ES = F8 ? 1 : 2;
@@ -246,7 +256,8 @@ struct PagedCfg {
   // Three stages at least; where they are small, 16 KB a warp, so that a third block fits the SM: its warps cover the latency of the
   // chain from a tile's keys to its outputs (3 x up to 30000 keys in e4m3 32 us, 37 with two).  16-bit rows of 128 run as fast as
   // memory does with two blocks of three stages (61 x 2050 keys 78 us, three blocks of two stages 95).
-  static constexpr int RING = STAGE >= 8192 ? 24576 : 16384;
+  // A sequence's own keys behind a prefix are few: three blocks of two stages there.
+  static constexpr int RING = STAGE >= 8192 && !OWN ? 24576 : 16384;
   static constexpr int STAGES = RING / STAGE;
   static constexpr int BLOCKS = NT == 1 && RING == 16384 ? 3 : 2;  // an SM
   static constexpr int LOADS = kTileKeys * CH / 32;    // pieces of K a lane copies, and as many of V
@@ -265,8 +276,8 @@ __device__ __forceinline__ uint32_t piece(int row, int c) {
 // WARPS: of a unit, a kv head of a sequence (up to 8 or 16 query heads of it).  Fewer than the block's four where there are more units than blocks fit the SMs at once: a block
 // then has two or four units, and each unit fewer warps to join.
 template <typename QT, bool F8, int DP, int NT, PagedMode MODE, int WARPS>
-__global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOCKS)) paged_kernel(const __grid_constant__ PagedParams p) {
-  using C = PagedCfg<QT, F8, DP, NT>;
+__global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT, MODE == kOwn>::BLOCKS)) paged_kernel(const __grid_constant__ PagedParams p) {
+  using C = PagedCfg<QT, F8, DP, NT, MODE == kOwn>;
   extern __shared__ __align__(128) uint8_t smem[];
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -582,7 +593,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
       acc[2] += v.z * f;
       acc[3] += v.w * f;
     }
-    if (d >= D || idle) continue;
+    if ((MODE != kOwn && d >= D) || idle) continue;
+    const bool real = d < D;  // the lanes of a head stay together until the sums over the prefix have joined
     if constexpr (MODE == kShared) {
       constexpr float down = C::BF16 ? 1.0f : 1.0f / 4096.0f;  // without the factor that fp16 weights carry
       const int64_t row = (static_cast<int64_t>(sequence_of(h)) * p.a.q_heads + head_of(h)) * splits + split;
@@ -592,12 +604,13 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
     }
     const int64_t row = static_cast<int64_t>(b) * p.a.q_heads + kvh * p.group + head0 + h;
     if (p.cluster) {
+      if (!real) continue;
       *reinterpret_cast<float4*>(block_o + h * C::OROW + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (d == 0) block_ml[h] = make_float2(top, sum);
     } else if (used == 1) {
       with_prefix(h, d, acc, sum, top);
-      store_out(h, d, acc, sum);
-    } else {
+      if (real) store_out(h, d, acc, sum);
+    } else if (real) {
       *reinterpret_cast<float4*>(p.part_o + (row * p.splits + split) * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (d == 0) p.part_ml[row * p.splits + split] = make_float2(top, sum);
     }
@@ -608,7 +621,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
     const uint32_t o_base = smem_u32(block_o), ml_base = smem_u32(block_ml);
     for (int i = static_cast<int>(cluster_cta_rank()) * kPagedThreads + threadIdx.x; i < heads * (DP / 4); i += p.splits * kPagedThreads) {
       const int h = i / (DP / 4), d = i % (DP / 4) * 4;
-      if (d >= D) continue;
+      if (MODE != kOwn && d >= D) continue;
       float2 ml[8];
       float4 v[8];
       float top = -INFINITY;
@@ -631,7 +644,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT>::BLOC
           acc[3] += v[r].w * f;
         }
       with_prefix(h, d, acc, sum, top);
-      store_out(h, d, acc, sum);
+      if (d < D) store_out(h, d, acc, sum);
     }
     cluster_arrive_wait();  // nobody leaves while its sums are read
   }
@@ -684,7 +697,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
   warp_o[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   if (lane == 0) warp_sum[warp] = sum;
   __syncthreads();
-  if (warp != 0 || d >= D) return;
+  if (warp != 0 || (MODE != kOwn && d >= D)) return;
 #pragma unroll
   for (int w = 1; w < kJoinWarps; ++w) {
     sum += warp_sum[w];
@@ -696,7 +709,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
   }
   constexpr bool bf16 = std::is_same<QT, __nv_bfloat16>::value;
   if constexpr (MODE == kOwn) join_prefix(p, row, d, len > 0 ? shared_splits(p.pre, common) : 0, bf16 && !f8 ? 1.0f : 4096.0f, top, sum, acc);
-  *reinterpret_cast<uint2*>(static_cast<QT*>(p.a.out) + row * D + d) = outputs4<bf16>(acc, sum, f8 ? p.a.v_scale[h / p.group] : 1.0f);
+  if (d < D) *reinterpret_cast<uint2*>(static_cast<QT*>(p.a.out) + row * D + d) = outputs4<bf16>(acc, sum, f8 ? p.a.v_scale[h / p.group] : 1.0f);
 }
 
 // Splits of the keys: blocks for every SM, none with fewer than kMinTiles tiles where the page table is as wide as its longest
@@ -756,7 +769,7 @@ inline int check_paged_pointers(const qlin_paged_attention_args* a, const char* 
 
 template <typename QT, bool F8, int DP, int NT, PagedMode MODE, int WARPS = kPagedWarps>
 static int launch_paged(const PagedParams& p, cudaStream_t stream) {
-  using C = PagedCfg<QT, F8, DP, NT>;
+  using C = PagedCfg<QT, F8, DP, NT, MODE == kOwn>;
   const auto kernel = paged_kernel<QT, F8, DP, NT, MODE, WARPS>;
   static bool configured[64] = {};
   int dev = 0;

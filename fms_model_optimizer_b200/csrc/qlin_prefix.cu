@@ -14,7 +14,8 @@ namespace qlin {
 
 // Rows of a group (its sequences times the query heads of a kv head) from which on the tensor cores' 128-row tiles take the prefix, and above which a
 // block has two of them.
-constexpr int kRowsTensor = 32, kRowsPair = 128;
+// Measured with 128 keys of their own, mma.sync and tcgen05 in us: 8 sequences (32 rows) behind 8192 in bf16 24.4 and 22.4, in e4m3 25.1 and 26.6; 16 (64 rows) 42 and 34, 42 and 37.
+constexpr int kRowsTensor = 32, kRowsTensorE4m3 = 48, kRowsPair = 128;
 constexpr int kLongOwn = 2048;  // keys of its own that a sequence may have for fewer warps than four
 
 struct PrefixPlan {
@@ -34,29 +35,28 @@ static PrefixPlan plan_prefix(const qlin_prefix_attention_args& a) {
   own.max_pages = a.own.max_pages > a.max_prefix_pages ? a.own.max_pages - a.max_prefix_pages + 1 : 1;
   const int head_blocks = (group + heads_per_block(group) - 1) / heads_per_block(group);
   plan.own = choose_splits(own, head_blocks);
-  // Warps that are all resident at once, if the keys are few enough for that to count: a block of four for each kv head of 128 sequences comes in three or four
-  // waves, each of them the latency of the lookups, the keys and the join.
+  // Warps that are resident at once, or nearly, if the keys are few enough for that to count: a second wave of blocks costs the latency of the lookups, the keys and the join again.
   const bool f8 = a.own.cache_dtype == QLIN_DT_F8E4M3;
-  const int64_t units = static_cast<int64_t>(a.own.batch) * a.own.kv_heads * head_blocks, slots = static_cast<int64_t>(f8 && group <= 8 ? 3 : 2) * kPagedWarps * sm_count();
-  plan.warps = units * 4 <= slots || static_cast<int64_t>(own.max_pages) * own.page_size > kLongOwn ? 4 : units * 2 <= slots ? 2 : 1;
-  if (plan.warps < 4) plan.own = Splits{1, 0};
+  const int64_t units = static_cast<int64_t>(a.own.batch) * a.own.kv_heads * head_blocks, slots = static_cast<int64_t>(group <= 8 ? 3 : 2) * kPagedWarps * sm_count(), nearly = slots + slots / 4;
+  plan.warps = units * 4 <= nearly || static_cast<int64_t>(own.max_pages) * own.page_size > kLongOwn ? 4 : units * 2 <= nearly ? 2 : 1;
+  if (plan.warps < 4 || (plan.own.cluster && units * 4 * plan.own.n > nearly)) plan.own = Splits{1, 0};
   const int64_t rows = static_cast<int64_t>(a.own.batch) * a.own.q_heads;
   if (plan.own.n > 1 && !plan.own.cluster) plan.own_floats = rows * plan.own.n * (a.own.head_dim + 2);
   const int64_t keys = static_cast<int64_t>(a.max_prefix_pages) * a.own.page_size;
   if (keys > 0 && a.own.num_pages > 0) {
     const int64_t per_head = rows / a.own.kv_heads, each = (per_head + a.num_groups - 1) / a.num_groups;  // rows of a kv head, and of a group on average
     const int box = prefix_box(a.own);
-    plan.columns = box == 0 || each < kRowsTensor ? (each > 8 ? 16 : 8) : each > kRowsPair ? 256 : 128;
+    plan.columns = box == 0 || each < (f8 ? kRowsTensorE4m3 : kRowsTensor) ? (each > 8 ? 16 : 8) : each > kRowsPair ? 256 : 128;
     if (plan.columns >= 128) plan.align = box;
     const int64_t blocks = per_head / plan.columns + a.num_groups;  // a group has one block that is not full at most
     if (blocks * a.own.kv_heads > (1 << 24)) return plan;
     plan.units = static_cast<int32_t>(blocks * a.own.kv_heads);
     const int64_t expected = a.num_groups * ((each + plan.columns - 1) / plan.columns) * a.own.kv_heads, most = (keys + kSharedStep - 1) / kSharedStep;
     if (plan.columns >= 128) {
-      // one block an SM, none with fewer than four tiles of keys for each of its streams; 128 rows take two splits at once
+      // one block an SM, none with fewer than two tiles of keys for each of its streams (16 sequences behind 2048 keys 24.2 us, with four 30.5); 128 rows take two splits at once
       const int streams = plan.columns == 128 ? 2 : 1;
       int64_t each_unit = sm_count() / expected;
-      if (each_unit > most / (4 * streams)) each_unit = most / (4 * streams);
+      if (each_unit > most / (2 * streams)) each_unit = most / (2 * streams);
       if (each_unit < 1) each_unit = 1;
       plan.splits = static_cast<int32_t>(each_unit * streams);
       plan.blocks = plan.units * static_cast<int32_t>(each_unit);
