@@ -42,11 +42,13 @@ struct SharedCfg {
   static constexpr int CHUNKS = DP / 64;
   static constexpr int TILE_BYTES = CHUNKS * kChunkBytes;
   static constexpr int Q_TILES = PAIR ? 2 : 1;
-  static constexpr int STAGES = F8 ? (DP == 128 ? (PAIR ? 3 : 4) : 6) : DP == 128 ? (PAIR ? 5 : 6) : 8;
+  static constexpr int STAGES = F8 ? (DP == 128 ? 3 : 6) : DP == 128 ? 5 : 8;
   static constexpr int RAW_BYTES = kKeys * DP, RAW = F8 ? (DP == 128 ? 4 : 6) : 0;  // tiles of codes
   static constexpr int KV_OFFSET = Q_TILES * TILE_BYTES;
   static constexpr int RAW_OFFSET = KV_OFFSET + STAGES * TILE_BYTES;
-  static constexpr int AUX_OFFSET = RAW_OFFSET + RAW * RAW_BYTES;
+  // 32 rows of 32 outputs for each softmax warp: over the queries of the warp's own tile, which are no longer needed, or where the streams share these, beside the tiles
+  static constexpr int OUT_OFFSET = PAIR ? 0 : RAW_OFFSET + RAW * RAW_BYTES, OUT_BYTES = 4096;
+  static constexpr int AUX_OFFSET = RAW_OFFSET + RAW * RAW_BYTES + (PAIR ? 0 : kSharedSoftmaxWarps * OUT_BYTES);
   static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(SharedAux));
   static constexpr float SHIFT = HALF ? 6.0f : 0.0f;
   static constexpr uint32_t FMT = HALF ? 0u : 1u;
@@ -470,18 +472,26 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
         tc_fence_after();
         constexpr float down = C::HALF ? 1.0f / 64.0f : 1.0f;  // without the factor that fp16 weights carry
         if (live) p.pre.part_ml[out_row] = make_float2(m * cl2, l * down);
-        float* out = p.pre.part_o + out_row * D;
-#pragma unroll
+        // Rows go through shared memory, 32 outputs at a time, so that eight lanes write 128 bytes of a row together.
+        const uint64_t to = live ? reinterpret_cast<uint64_t>(p.pre.part_o + out_row * D) : 0;
+        uint8_t* stage = smem + C::OUT_OFFSET + (PAIR ? i * C::TILE_BYTES + (warp & 3) * C::OUT_BYTES : warp * C::OUT_BYTES);
+#pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
-          if (live) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              if (32 * c + j < D)
-                *reinterpret_cast<float4*>(out + 32 * c + j) =
-                    make_float4(__uint_as_float(o[j]) * down, __uint_as_float(o[j + 1]) * down, __uint_as_float(o[j + 2]) * down, __uint_as_float(o[j + 3]) * down);
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(__uint_as_float(o[4 * j]) * down, __uint_as_float(o[4 * j + 1]) * down,
+                                                                                                  __uint_as_float(o[4 * j + 2]) * down, __uint_as_float(o[4 * j + 3]) * down);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int from = 4 * k + (lane >> 3), j = lane & 7;
+            const uint64_t row_to = __shfl_sync(0xffffffffu, to, from);
+            const float4 v = *reinterpret_cast<const float4*>(stage + from * 128 + ((j ^ (from & 7)) << 4));
+            if (row_to != 0 && 32 * c + 4 * j < D) *reinterpret_cast<float4*>(reinterpret_cast<float*>(row_to) + 32 * c + 4 * j) = v;
           }
+          __syncwarp();
         }
       }
       if (!ok && lane == 0) {
