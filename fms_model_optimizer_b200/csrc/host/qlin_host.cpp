@@ -16,6 +16,7 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -993,6 +994,7 @@ Tensor logit_rows(const Tensor& logits) {
 // (logprobs, entropy, top_logprobs, top_ids, stats) with the leading dimensions of `tokens`; stats is empty unless wanted.
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens_in, int64_t top, bool want_stats) {
   const at::Device dev = require_cuda({&logits, &tokens_in});
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && logits._fw_grad(0).defined()) raise("token_logprobs has no forward-mode gradient");
   if (!is_float(logits.scalar_type())) raise("logits must be float32, float16 or bfloat16");
   if (tokens_in.scalar_type() != at::kLong || logits.dim() < 1 || tokens_in.sizes() != logits.sizes().slice(0, logits.dim() - 1))
     raise("tokens must be int64, one for each row of logits");
@@ -1033,6 +1035,29 @@ Tensor token_logprobs_bwd(const Tensor& logits, const Tensor& tokens_in, const T
   check(qlin_token_logprobs_bwd(&a, stream_of(dev)), "qlin_token_logprobs_bwd");
   return out;
 }
+
+// The same with a gradient of logprobs and entropy, once differentiable.  In Python the step from a small batch's loss to its gradient took 85 us, whatever the GPU did.
+struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+  static std::vector<Tensor> forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top) {
+    const auto [logprobs, entropy, top_logprobs, top_ids, stats] = token_logprobs(logits, tokens, top, true);
+    ctx->save_for_backward({logits, tokens, entropy, stats});
+    ctx->mark_non_differentiable({top_logprobs, top_ids});
+    ctx->set_materialize_grads(false);
+    return {logprobs, entropy, top_logprobs, top_ids};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
+    const torch::autograd::variable_list saved = ctx->get_saved_variables();
+    const auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+    Tensor out = token_logprobs_bwd(saved[0], saved[1], saved[2], saved[3], given(grads[0]), given(grads[1]));
+    if (at::GradMode::is_enabled()) {
+      const auto refuse = std::make_shared<torch::autograd::DelayedError>("token_logprobs can be differentiated once", 1);
+      out = (*refuse)({out.requires_grad_(true)})[0];
+    }
+    return {out, Tensor(), Tensor()};
+  }
+};
+std::vector<Tensor> token_logprobs_grad(const Tensor& logits, const Tensor& tokens, int64_t top) { return TokenLogprobs::apply(logits, tokens, top); }
 
 // Rows (or matrices of rows) of 16-bit numbers that start on 16 bytes: the tensor itself, or a dense copy.
 Tensor aligned_rows(const Tensor& t) {
@@ -1112,6 +1137,6 @@ PYBIND11_MODULE(_qlin_host, m) {
   m.def("prefix_attention", &prefix_attention, rel());
   m.def("prompt_attention", &prompt_attention, rel());
   m.def("token_logprobs", &token_logprobs, rel());
-  m.def("token_logprobs_bwd", &token_logprobs_bwd, rel());
+  m.def("token_logprobs_grad", &token_logprobs_grad, rel());
   m.def("lora_add", &lora_add, rel());
 }

@@ -716,26 +716,6 @@ def prompt_attention(
 # --------------------------------------------------------------------------------------------------
 # Many requests answered at once: what the head says about given tokens, low-rank adapters
 # --------------------------------------------------------------------------------------------------
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top):
-        logprobs, entropy, top_logprobs, top_ids, stats = _call("token_logprobs", float(logits.numel() * logits.element_size()), logits.device, L.host().token_logprobs,
-                                                                logits, tokens, int(top), True)  # fmt: skip
-        ctx.save_for_backward(logits, tokens, entropy, stats)
-        ctx.mark_non_differentiable(top_logprobs, top_ids)
-        ctx.set_materialize_grads(False)
-        return logprobs, entropy, top_logprobs, top_ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_logprobs, d_entropy, _top_logprobs, _top_ids):
-        if d_logprobs is None and d_entropy is None:
-            return None, None, None
-        logits, tokens, entropy, stats = ctx.saved_tensors
-        work = 2.0 * logits.numel() * logits.element_size()
-        return _call("token_logprobs_bwd", work, logits.device, L.host().token_logprobs_bwd, logits, tokens, entropy, stats, d_logprobs, d_entropy), None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """What a model's head says about given tokens, in one pass over the logits (``qlin_token_logprobs``): ``(logprobs, entropy, top_logprobs,
     top_ids)``.  ``logits [.., vocab]`` fp32, fp16 or bf16 of any alignment, ``tokens [..]`` int64; ``logprobs`` and ``entropy`` are fp32
@@ -746,9 +726,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
 
     ``logprobs`` and ``entropy`` have a gradient (once differentiable, of the logits' type, ``qlin_token_logprobs_bwd``):
     ``-logprobs.sum() / count`` is the loss of a language model.  A row whose incoming gradients are zero gets zeros."""
+    nbytes = float(logits.numel() * logits.element_size())
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _TokenLogprobs.apply(logits, tokens, top)
-    return _call("token_logprobs", float(logits.numel() * logits.element_size()), logits.device, L.host().token_logprobs, logits, tokens, int(top), False)[:4]
+        return tuple(_call("token_logprobs", nbytes, logits.device, L.host().token_logprobs_grad, logits, tokens, int(top)))
+    return _call("token_logprobs", nbytes, logits.device, L.host().token_logprobs, logits, tokens, int(top), False)[:4]
 
 
 def lora_groups(which: torch.Tensor, adapters: int) -> Tuple[torch.Tensor, torch.Tensor]:
