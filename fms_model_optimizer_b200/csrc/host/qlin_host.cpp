@@ -1085,17 +1085,18 @@ Tensor lora_add(const Tensor& y, const Tensor& x_in, const Tensor& a_in, const T
   if (sc.numel() != n) raise("scale must have one entry for each adapter");
   for (int64_t d = 0; d < 2; ++d)
     if (y.size(d) > 1 && y.stride(d) == 0) raise("rows of y share memory: they cannot be written");
-  for (const Tensor* t : {&x_in, &a_in, &b_in, &sc, &rows, &starts})
-    if (may_overlap(y, *t)) raise("y must not overlap the other tensors");
-  const Tensor x = aligned_rows(x_in), a_ = aligned_rows(a_in), b_ = aligned_rows(b_in), y_ = aligned_rows(y);
+  // what shares memory with y is read from a copy: other blocks have written some of it by the time it is read
+  const auto apart = [&](const Tensor& t) { return may_overlap(y, t) ? t.clone(at::MemoryFormat::Contiguous) : t; };
+  const Tensor x = aligned_rows(apart(x_in)), a_ = aligned_rows(apart(a_in)), b_ = aligned_rows(apart(b_in)), y_ = aligned_rows(y);
+  const Tensor rows_ = apart(rows), starts_ = apart(starts), sc_ = apart(sc);
   qlin_lora_args a = {};
   a.x = data(x);
   a.a = data(a_);
   a.b = data(b_);
   a.y = data(y_);
-  a.rows = static_cast<const int32_t*>(data(rows));
-  a.starts = static_cast<const int32_t*>(data(starts));
-  a.scale = static_cast<const float*>(data(sc));
+  a.rows = static_cast<const int32_t*>(data(rows_));
+  a.starts = static_cast<const int32_t*>(data(starts_));
+  a.scale = static_cast<const float*>(data(sc_));
   a.status = static_cast<int32_t*>(status_word(dev.index()).data_ptr());
   a.x_row = step(x, 0);
   a.y_row = step(y_, 0);

@@ -111,14 +111,31 @@ __device__ __forceinline__ int shared_splits(const SharedPrefix& pre, const Comm
   const int n = c.to - c.from, per = keys_per_split(n, pre.splits);
   return (n + per - 1) / per;
 }
-// The kv head, the group and the block of `columns` of its rows of a unit; false: there is no such unit.
+// The kv head, the group and the block of `columns` of its rows of a unit, by a whole warp, 32 groups a look; false: there is no such unit.
 __device__ __forceinline__ bool shared_unit(const PagedParams& p, int unit, int columns, int& kvh, int& g, int& block) {
+  const int lane = threadIdx.x & 31;
   kvh = unit % p.a.kv_heads;
-  block = unit / p.a.kv_heads;
-  for (g = 0; g < p.pre.count; ++g) {
-    const int rows = max(0, min(p.pre.groups[g + 1], p.a.batch) - max(p.pre.groups[g], 0)) * p.group, blocks = (rows + columns - 1) / columns;
-    if (block < blocks) return true;
-    block -= blocks;
+  int left = unit / p.a.kv_heads;
+  for (int base = 0; base < p.pre.count; base += 32) {
+    int blocks = 0;
+    if (base + lane < p.pre.count) {
+      const int rows = max(0, min(p.pre.groups[base + lane + 1], p.a.batch) - max(p.pre.groups[base + lane], 0)) * p.group;
+      blocks = (rows + columns - 1) / columns;
+    }
+    int upto = blocks;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += other;
+    }
+    const int here = __shfl_sync(0xffffffffu, upto, 31);
+    if (left < here) {
+      const int owner = __ffs(__ballot_sync(0xffffffffu, left < upto)) - 1;
+      g = base + owner;
+      block = left - __shfl_sync(0xffffffffu, upto - blocks, owner);
+      return true;
+    }
+    left -= here;
   }
   return false;
 }

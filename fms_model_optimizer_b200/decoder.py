@@ -610,6 +610,8 @@ class W8A8Decoder:
             raise RuntimeError("a prefix has at least one token")
         if (adapters is None) != (which is None):
             raise RuntimeError("adapters and the adapter of each prompt belong together")
+        if logprobs is not None and not 0 <= logprobs <= min(32, self.cfg["vocab"]):
+            raise RuntimeError("logprobs is a number of top alternatives, up to 32")
         longest = shared + max(lengths) + new_tokens - 1  # the last id is produced, not read
         if longest > self.cos.shape[0]:
             raise RuntimeError(f"{longest} tokens are more than the {self.cos.shape[0]} positions of cfg['seq']")
@@ -617,7 +619,7 @@ class W8A8Decoder:
         if cache is None:
             cache = PagedKVCache(len(self.layers), len(lengths), longest, self.nkv, self.cfg["head_dim"], self.dev, cache_dtype, page_size)
         self._check_cache(cache, lengths, new_tokens, shared)
-        ids = torch.cat([p.reshape(-1) for p in ([] if prefix is None else [prefix]) + list(prompts)]).to(self.dev)
+        ids = torch.cat([p.reshape(-1) for p in ([] if prefix is None else [prefix.to(prompts[0].device)]) + list(prompts)]).to(self.dev)
         if prefix is None:
             step = cache.prompts(lengths)
         else:

@@ -285,3 +285,46 @@ def test_offsets_beyond_32_bits(cuda_dev):
             for kk, vv, t in ((k, v, at.tolist()), (*small, [0, 1, 2, 3, 4]))]  # fmt: skip
     ops.check_status(cuda_dev)
     assert torch.equal(*both)
+
+
+@pytest.mark.parametrize("dim,f8", [(8, False), (40, False), (80, False), (112, False), (16, True), (48, True), (80, True), (112, True)])
+@pytest.mark.parametrize("sequences", [20, 50])
+def test_head_dimensions(cuda_dev, dim, f8, sequences):
+    """Head dimensions that fill no tile, with as many rows as one tile of 128 has, and two; what lies between the heads in memory is NaN."""
+    c = Case(15, cuda_dev, [(333, [340 + (7 * i) % 60 for i in range(sequences)])], 4, 1, dim, 16, torch.bfloat16, f8)
+    args = c.args()
+    for i in (1, 2):
+        wide = torch.full((*args[i].shape[:3], dim + 16), math.nan, device=cuda_dev).to(args[i].dtype)
+        wide[..., :dim] = args[i]
+        args[i] = wide[..., :dim]
+    c.check(ops.prefix_attention(*args, **c.scales()))
+    ops.check_status(cuda_dev)
+
+
+def test_many_groups(cuda_dev):
+    """More groups than a warp looks at in one go, some without sequences, and sequences of no prefix among them."""
+    groups = [((i * 13) % 50, [(i * 13) % 50 + 1 + (i + j) % 9 for j in range(i % 4)]) for i in range(150)]
+    c = Case(16, cuda_dev, groups, 4, 2, 64, 16, torch.bfloat16)
+    c.check(ops.prefix_attention(*c.args()))
+    ops.check_status(cuda_dev)
+    big = [(300, [310 + i for i in range(33)])] + [(20, [25])] * 40 + [(200, [201 + i for i in range(40)])]
+    c = Case(17, cuda_dev, big, 8, 1, 64, 16, torch.float16)
+    c.check(ops.prefix_attention(*c.args()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sequences", [3, 20, 70])
+@pytest.mark.parametrize("at", [100, 705])
+def test_an_infinite_value_of_small_weight(cuda_dev, dtype, sequences, at):
+    """A value of infinity that is seen with a weight of 2^-58, too small for fp16, in the prefix or among a sequence's own keys: the output is infinite, not 0 * infinity."""
+    c = Case(18, cuda_dev, [(700, [720] * sequences)], 4, 1, 64, 16, dtype)
+    c.q[:], c.k[~c.k.isnan()] = 0.0, 0.0
+    c.q[..., 0] = 8
+    page, offset = c.place(0, at)
+    c.k[page, 0, offset, 0] = -40
+    c.v[page, 0, offset, 3] = math.inf
+    got = ops.prefix_attention(*c.args()).cpu()
+    sees = torch.arange(sequences) >= (0 if at < 700 else sequences)
+    sees[0] = True
+    assert bool((got[sees][..., 3] == math.inf).all()) and bool(got[~sees].isfinite().all())
+    assert bool(got[..., [d for d in range(64) if d != 3]].isfinite().all())

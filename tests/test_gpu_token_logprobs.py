@@ -45,7 +45,7 @@ def _logits(g, rows, vocab, dtype, std=3.0):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 7, 7), (3, 33, 5), (2, 1000, 32), (5, 50257, 20), (2, 128256, 5), (300, 2053, 8), (1, 262145, 32), (700, 512, 0),
-                                            (9, 4096, 1), (2, 300001, 0), (160, 8191, 31)])  # fmt: skip
+                                            (9, 4096, 1), (2, 300001, 0), (160, 8191, 31), (1, 1 << 20, 32), (150, 1 << 17, 9)])  # fmt: skip
 def test_against_64_bits(cuda_dev, dtype, rows, vocab, top):
     g = torch.Generator().manual_seed(rows * 31 + vocab)
     x = _logits(g, rows, vocab, dtype)
