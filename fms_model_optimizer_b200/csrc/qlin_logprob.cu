@@ -5,12 +5,17 @@
 //
 // What bounds it: HBM, the logits once (the gradient: once more, and its own bytes).  A thread keeps its own m, S and T over pieces of
 // eight 16-byte loads and moves m once a piece at most; they are joined in the block and, where rows are few, in a cluster of blocks that share
-// a row.  An element costs one exponential and about four packed operations, half of what would bound 16-bit logits.
+// a row.  An element costs one exponential and four or five other operations, which 16-bit logits just leave time for.
 //
-// The top alternatives come out of the same pass.  The k-th largest of the threads' maxima is at most the k-th largest element, and for
-// elements in no special order nearly as large (256 threads, k = 20: 20.8 elements expected above it); each piece's maximum stays in shared
-// memory, so only the few pieces that reach that threshold are read again, from L2.  What they hold above it is ordered by counting for
+// The top alternatives come out of the same pass.  The k-th largest of the maxima of the block's 64 groups of threads is at most the k-th largest element, and for
+// elements in no special order nearly as large (k = 20: 24 elements expected above it); each piece's maximum stays in shared
+// memory, so only the few pieces that reach that threshold are listed and read again, from L2, by whole warps.  What they hold above it is ordered by counting for
 // each element how many are larger.  Elements are ordered by value, then by the lower id, so results do not depend on timing.
+//
+// Measured (device time, bf16): 4096 x 128256 165 us, 6.4 TB/s, 0.97 of the copy rate, with the exponentials' unit busy for 77 % of it; 2048 x 128256 forward and backward 261 us,
+// 6.0 TB/s; 64 x 128256 with 20 alternatives 11 us and one row with five 8 us, which are the latency of the row, its sums, the pieces and the cluster behind one another; 333 x 50257 in
+// fp32 with all but nine logits minus infinity 18 us.  Tried and no faster, 4096 x 128256: every fourth or eighth pair of exponentials by a polynomial on the FMA pipe 179 and 167 us (the
+// instructions are what there is no room for), pieces without the guard for minus infinity, which are done again where they held one, 170.
 #include <type_traits>
 
 #include <cuda_bf16.h>

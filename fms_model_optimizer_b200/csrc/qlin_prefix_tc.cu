@@ -13,6 +13,9 @@
 // meets these as fp16 times a power of two that brings its largest element to 2^13..2^14.  (Through the threads' registers and 16-byte asynchronous copies, which take
 // pages of any size, the loads were what the rest waited for: 2 x 64 sequences behind 32768 keys 127 us.)
 //
+// What bounds it: the chain of products and exponentials, 3450 cycles for two tiles of rows against a tile of keys where the tensor core needs 2048 and so do the exponentials (2 x 64 sequences
+// behind 32768 keys 72 us, the tensor pipe busy for half of it); short prefixes by the start and the end of a block, some 12 us.
+//
 // Logits enter the exponent as their difference from the reference, so that it is exact near the maximum however large they are.
 #include <cuda.h>
 
