@@ -329,9 +329,11 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedCfg<QT, F8, DP, NT, MODE 
   int len = 0, group = 0;
   if constexpr (MODE == kSingle) len = sequence_length(p, b, threadIdx.x == 0);
   if constexpr (MODE == kOwn) {
+    const bool alone = p.pre.blocks == 0;  // no launch for the prefixes, which would have reported
+    if (alone && blockIdx.x == 0) check_groups(p);
     const Group of = group_of(p.pre, b);
     group = of.g;
-    if (group >= 0) common = common_keys(p, group, of.first, of.end, false);
+    if (group >= 0) common = common_keys(p, group, of.first, of.end, alone && lane == 0);
     else if (lane == 0 && p.a.status != nullptr) atomicExch(p.a.status, static_cast<int32_t>(QLIN_ERR_BAD_SHAPE));
     len = sequence_length(p, b, lane == 0, common.prefix);
     if (idle) len = 0;

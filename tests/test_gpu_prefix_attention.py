@@ -225,6 +225,21 @@ def test_bad_values_are_reported(cuda_dev):
                 ops.check_status(cuda_dev)
 
 
+def test_bad_values_without_pages_of_a_prefix_are_reported(cuda_dev):
+    """No launch for prefixes: the other one looks at the groups and lengths."""
+    c = Case(10, cuda_dev, [(0, [20, 40]), (0, [31])], 8, 2, 64, 16, torch.bfloat16)
+    good = c.args()
+    good[3] = good[3][:, :0]
+    c.check(ops.prefix_attention(*good))
+    ops.check_status(cuda_dev)
+    for at, value in ((4, [0, 5]), (4, [-1, 0]), (5, [0, 1, 2]), (5, [0, 3, 2]), (5, [1, 2, 3])):
+        args = list(good)
+        args[at] = torch.tensor(value, dtype=torch.int32, device=cuda_dev)
+        ops.prefix_attention(*args)
+        with pytest.raises(RuntimeError, match="status"):
+            ops.check_status(cuda_dev)
+
+
 def test_refusals(cuda_dev):
     c = Case(11, cuda_dev, [(100, [101, 140]), (30, [31])], 8, 2, 64, 16, torch.bfloat16)
     good = c.args()
