@@ -32,10 +32,13 @@ class LoraAdapters:
                 self.a[li, name] = torch.zeros(adapters, padded, width, dtype=dtype, device=dev)
                 self.b[li, name] = torch.zeros(adapters, out, padded, dtype=dtype, device=dev)
 
+    @torch.no_grad()
     def load(self, adapter: int, layer: int, name: str, a: torch.Tensor, b: torch.Tensor) -> None:
         """The weights of one adapter for one Linear: ``a [r, in]``, ``b [out, r]`` with ``r`` up to the pool's rank."""
+        if not 0 <= adapter < self.adapters or (layer, name) not in self.a:
+            raise RuntimeError(f"there is no adapter {adapter} for {name} in layer {layer}")
         pool_a, pool_b = self.a[layer, name][adapter], self.b[layer, name][adapter]
-        r = a.shape[0]
+        r = a.shape[0] if a.dim() == 2 else 0
         if a.dim() != 2 or b.dim() != 2 or r > self.rank or a.shape[1] != pool_a.shape[1] or tuple(b.shape) != (pool_b.shape[0], r):
             raise RuntimeError(f"an adapter of {name} has weights [r, {pool_a.shape[1]}] and [{pool_b.shape[0]}, r], r up to {self.rank}")
         for pool, new in ((pool_a[:r], a), (pool_b[:, :r], b)):

@@ -738,6 +738,8 @@ def lora_groups(which: torch.Tensor, adapters: int) -> Tuple[torch.Tensor, torch
     all layers; nothing is read back to the host."""
     if which.dim() != 1 or which.is_floating_point() or adapters < 0:
         raise RuntimeError("which must be a vector of integers, adapters must not be negative")
+    if which.dtype != torch.int32:  # narrower ones need not hold `adapters`
+        which = which.long()
     order = torch.where((which < 0) | (which >= adapters), adapters, which).sort(stable=True)
     starts = torch.searchsorted(order.values, torch.arange(adapters + 1, device=which.device, dtype=order.values.dtype))
     return order.indices.to(torch.int32), starts.to(torch.int32)

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from fms_model_optimizer_b200 import ops
 from fms_model_optimizer_b200.adapters import LoraAdapters
 
 SHAPES = dict(q=(64, 32), down=(32, 96))
@@ -38,3 +39,22 @@ def test_rows_of_a_step():
     for bad in (([3, 0], [1, 1]), ([-2, 0], [1, 1]), ([0], [1, 1])):
         with pytest.raises(RuntimeError, match="every prompt"):
             pool.which(*bad, "cpu")
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_rows_of_adapters_from_integers_of_any_width(dtype):
+    rows, starts = ops.lora_groups(torch.tensor([1, 0, 127, 1], dtype=dtype), 300)
+    assert rows.tolist() == [1, 0, 3, 2]
+    assert starts.tolist() == [0, 1] + [3] * 126 + [4] * 173
+
+
+def test_the_pool_takes_trained_weights_without_their_graph_and_names_what_it_lacks():
+    pool = LoraAdapters({"q": (16, 8)}, 1, 2, 8, "cpu")
+    a, b = torch.nn.Parameter(torch.ones(8, 8)), torch.nn.Parameter(torch.ones(16, 8))
+    pool.load(1, 0, "q", a, b)
+    assert not pool.a[0, "q"].requires_grad and not pool.b[0, "q"].requires_grad
+    for adapter, layer, name in ((-1, 0, "q"), (2, 0, "q"), (0, 1, "q"), (0, 0, "k")):
+        with pytest.raises(RuntimeError, match="there is no adapter"):
+            pool.load(adapter, layer, name, a, b)
+    with pytest.raises(RuntimeError, match="has weights"):
+        pool.load(0, 0, "q", torch.tensor(1.0), b)
