@@ -84,7 +84,9 @@ __device__ __forceinline__ void shared_softmax(uint32_t s_addr, uint32_t o_addr,
   for (int n = 0; n < 15; ++n) top.step(x, n);
   const float most = top.result();
   // The reference follows the maximum only when that has outgrown it by 2^kSlack.  NaN or an infinity among the logits makes it NaN, and with it the row.
-  const bool grow = !(most <= m + slack) || (m == -INFINITY && most > -INFINITY);
+  // The difference, which is exact for numbers this near each other, is compared: m + slack rounds to a whole place of a large m, up to twice the slack, and 2^(2 kSlack + SHIFT) is
+  // no fp16 number.
+  const bool grow = m == -INFINITY ? !(most <= m) : !(most - m <= slack);
   if (first || __any_sync(0xffffffffu, grow)) {
     const float next = !grow ? m : (most == INFINITY ? __int_as_float(0x7fc00000) : most);
     if (!first) {

@@ -343,3 +343,33 @@ def test_an_infinite_value_of_small_weight(cuda_dev, dtype, sequences, at):
     sees[0] = True
     assert bool((got[sees][..., 3] == math.inf).all()) and bool(got[~sees].isfinite().all())
     assert bool(got[..., [d for d in range(64) if d != 3]].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype,f8", [(torch.bfloat16, False), (torch.float16, False), (torch.float16, True), (torch.bfloat16, True)])
+@pytest.mark.parametrize("sequences", [3, 70])
+def test_large_logits_a_few_units_apart(cuda_dev, dtype, f8, sequences):
+    """Logits whose last place is worth more than the weights' reference may lag behind: every other 128 keys lie 8 above the rest.  Products, sums and differences of logits are exact, so
+    the weights are as near as any (2^-20 for their exponents), whatever the logits' size."""
+    n, dim = 1024, 64
+    c = Case(19, cuda_dev, [(n, [n + 10] * sequences)], 16, 1, dim, 64, dtype, f8)
+    high = (torch.arange(n + 10) // 128 % 2 == 1) & (torch.arange(n + 10) < n)
+    common, step, q = (256.0, 2.0, (32768.0, 32768.0, 1.0)) if f8 else (16384.0, 8.0, (32768.0, 0.0, 8.0))
+    k = torch.zeros(c.k.shape)
+    for b in range(sequences):
+        for j in range(n if b else 0, n + 10):
+            page, offset = c.place(b, j)
+            k[page, 0, offset, :2], k[page, 0, offset, 2] = common, step * float(high[j])
+    c.k = k.to(c.k.dtype)
+    c.q[:] = 0.0
+    c.q[..., :3] = torch.tensor(q)
+    if f8:
+        c.ks[:] = 32.0
+    got = ops.prefix_attention(*c.args(), **c.scales()).cpu().double()
+    p = torch.softmax(torch.where(high, 8.0, 0.0).double(), 0)
+    wt = torch.float16 if f8 else dtype
+    for b in range(sequences):
+        at = [c.place(b, j) for j in range(n + 10)]
+        v = torch.stack([c.v[page, 0, offset].double() for page, offset in at]) * (c.vs[0].double() if f8 else 1.0)
+        want, weighted = p @ v, p @ v.abs()
+        tol = (2 * U[wt] + 2.0**-20) * weighted + U[dtype] * want.abs() + (n + 10) * 2.0**-30 * v.abs().max() + 2.0**-25
+        assert bool(((got[b] - want).abs() <= tol).all()), (b, got[b].isfinite().all(), float((got[b] - want).abs().max()))
