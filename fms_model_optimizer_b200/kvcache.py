@@ -83,14 +83,16 @@ class PagedKVCache:
         return need
 
     def share(self, tokens: int) -> Step:
-        """Room for ``tokens`` >= 1 first tokens that all sequences have in common, in an empty cache: the step that writes them.  Every sequence's length counts them
-        from then on, and ``prompts`` places its tokens behind them."""
+        """Room for ``tokens`` >= 1 first tokens that all sequences have in common, in an empty cache: the step that writes them.  From then on ``prompts`` places a sequence's
+        tokens behind them and its length counts them in; until then a sequence has length 0, and ``token`` passes it over."""
         if self.prefix or any(self.host_lens):
             raise RuntimeError("a prefix goes into an empty cache: release its sequences, and unshare, first")
         if not 1 <= tokens <= self.max_len:
             raise RuntimeError(f"a prefix of {tokens} tokens does not fit a cache of {self.max_len}")
         self.check([0] * self.batch, tokens)
         self.prefix = tokens
+        self._runs = [False] * self.batch
+        self._runs_dev.zero_()
         self._prefix_pages = [self._free.pop() for _ in range(-(-tokens // self.page_size))]
         positions, pages, lens, groups, last = self._send(range(tokens), self._prefix_pages, [tokens], [0, self.batch], [tokens - 1])
         self.prefix_table, self.prefix_lens, self.groups = pages.to(torch.int32)[None], lens.to(torch.int32), groups.to(torch.int32)
@@ -99,7 +101,7 @@ class PagedKVCache:
         return Step(positions.to(torch.int32), slots, last, False, cu, tokens)
 
     def unshare(self) -> None:
-        """The shared tokens are over: their pages go back to the pool.  All sequences have been released."""
+        """The shared tokens are over: their pages go back to the pool.  All sequences have been released, and wait for prompts."""
         if any(self.host_lens):
             raise RuntimeError("sequences still have the shared tokens: release them first")
         self._free += reversed(self._prefix_pages)

@@ -107,3 +107,22 @@ def test_a_shared_prefix_that_does_not_fit_is_refused():
     cache.prompts([1, 1])
     with pytest.raises(RuntimeError, match="empty cache"):
         cache.share(4)
+
+
+def test_places_wait_for_a_prompt_behind_the_shared_tokens():
+    """Nobody runs between `share` and `prompts`: a step then writes nothing, and least of all over the shared keys."""
+    cache = _cache(batch=2, max_len=40, page_size=4)
+    first = cache.share(10)
+    for _ in range(2):
+        step = cache.token()
+        assert step.slots.tolist() == [-1, -1] and cache.host_lens == [0, 0] == cache.lens.tolist() and cache._owned == [[], []]
+    step = cache.prompts([2], [1])
+    assert step.positions.tolist() == [10, 11] and cache.host_lens == [0, 12] == cache.lens.tolist()
+    assert not {s // 4 for s in first.slots.tolist()} & {s // 4 for s in step.slots.tolist()}
+    step = cache.token()
+    assert step.positions.tolist() == [0, 12] and int(step.slots[0]) == -1 and int(step.slots[1]) == int(cache.table[1, 3]) * 4
+    assert cache.host_lens == [0, 13] == cache.lens.tolist()
+    cache.release(1)
+    cache.unshare()
+    # as after `release`: places wait for a prompt without shared tokens too
+    assert cache.token().slots.tolist() == [-1, -1] and cache.prompts([3, 1]).positions.tolist() == [0, 1, 2, 0]
