@@ -85,7 +85,7 @@ class PagedKVCache:
     def share(self, tokens: int) -> Step:
         """Room for ``tokens`` >= 1 first tokens that all sequences have in common, in an empty cache: the step that writes them.  From then on ``prompts`` places a sequence's
         tokens behind them and its length counts them in; until then a sequence has length 0, and ``token`` passes it over."""
-        if self.prefix or any(self.host_lens):
+        if self.prefix or any(self.host_lens) or any(self._owned):
             raise RuntimeError("a prefix goes into an empty cache: release its sequences, and unshare, first")
         if not 1 <= tokens <= self.max_len:
             raise RuntimeError(f"a prefix of {tokens} tokens does not fit a cache of {self.max_len}")
@@ -102,8 +102,8 @@ class PagedKVCache:
 
     def unshare(self) -> None:
         """The shared tokens are over: their pages go back to the pool.  All sequences have been released, and wait for prompts."""
-        if any(self.host_lens):
-            raise RuntimeError("sequences still have the shared tokens: release them first")
+        if any(self.host_lens) or any(self._owned):
+            raise RuntimeError("sequences still have the shared tokens, or pages behind them: release them first")
         self._free += reversed(self._prefix_pages)
         self.prefix, self._prefix_pages = 0, []
         self.prefix_table = self.prefix_lens = self.groups = None

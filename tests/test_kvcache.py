@@ -126,3 +126,25 @@ def test_places_wait_for_a_prompt_behind_the_shared_tokens():
     cache.unshare()
     # as after `release`: places wait for a prompt without shared tokens too
     assert cache.token().slots.tolist() == [-1, -1] and cache.prompts([3, 1]).positions.tolist() == [0, 1, 2, 0]
+
+
+def test_pages_handed_out_ahead_are_where_they_were_meant():
+    """`reserve` before `share`, or between `share` and `unshare`, hands out pages for other columns of the table than those that the tokens would then be looked for in."""
+    cache = _cache(batch=2, max_len=40, page_size=8)
+    cache.reserve([16, 9])
+    with pytest.raises(RuntimeError, match="empty cache"):
+        cache.share(19)
+    for b in range(2):
+        cache.release(b)
+    cache.share(19)
+    cache.reserve([30, 0])
+    assert cache.prompts([11, 5]).slots.tolist() == [int(cache.table[b, i // 8]) * 8 + i % 8 for b, n in ((0, 11), (1, 5)) for i in range(19, 19 + n)]
+    for b in range(2):
+        cache.release(b)
+    cache.reserve([30, 30])
+    with pytest.raises(RuntimeError, match="release"):
+        cache.unshare()
+    for b in range(2):
+        cache.release(b)
+    cache.unshare()
+    assert len(cache._free) == 10
