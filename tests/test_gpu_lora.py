@@ -237,3 +237,35 @@ def test_inputs_that_share_memory_with_the_output(cuda_dev):
     assert torch.equal(both[:, :128].cpu(), x)
     same = y.to(cuda_dev)
     _near(ops.lora_add_(same, same, da, db, rows, starts, ds).cpu(), y, y, a, b, which, scale)
+
+
+def _same_extremes(got, want):
+    """NaN, infinities and their signs where 64 bits have them."""
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()) and torch.equal(got[want.isinf()].double(), want[want.isinf()])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,adapters,rank", [(30, 2, 8), (30, 2, 16), (5000, 2, 16), (30, 2, 32), (30, 2, 64), (5000, 2, 64), (30, 2, 128)])
+def test_infinite_weights_reach_y_as_they_are(cuda_dev, dtype, tokens, adapters, rank):
+    """Infinities and NaN in b: v times an infinity is one, whatever v's parts are, and outputs beside it stay as near as ever."""
+    y, x, a, b, which, scale = _inputs(17, tokens, adapters, rank, 136, 72, dtype, 0.0)
+    inf, clean = float("inf"), b.clone()
+    b[0, 5, 3], b[1, 6, 0], b[1, 9, 2], b[1, 9, 7], b[0, 11, 1] = inf, -inf, inf, -inf, float("nan")
+    got, want = _run(cuda_dev, y, x, a, b, which, scale), OR.lora(y, x, a, b, which, scale)[0]
+    assert int(want.isinf().sum()) > tokens / 2
+    _same_extremes(got, want)
+    got[~want.isfinite()] = 0.0
+    keep = want.isfinite()
+    plain = _run(cuda_dev, y, x, a, clean, which, scale)
+    assert torch.equal(got[keep], plain[keep])
+
+
+def test_an_infinite_weight_meets_a_small_v(cuda_dev):
+    """v in fp16 that is 2^-28 of the row's largest, below the last place of both its parts, is not zero where an infinity meets it."""
+    y, x, a, b, which, scale = _inputs(18, 40, 2, 16, 136, 72, torch.float16, 0.0)
+    a, b = a * 64, b / 64
+    a[:, 3] = a[:, 3].sign() * 2.0**-24
+    b[0, 5, 3], b[1, 6, 3] = float("inf"), float("-inf")
+    v = OR.lora(y, x, a, b, which, scale)[1]
+    assert all(bool((v[i][:, 3].abs() < 2.0**-25 * v[i].abs().amax(-1)).all()) and bool((v[i][:, 3] != 0).all()) for i in v)
+    _same_extremes(_run(cuda_dev, y, x, a, b, which, scale), OR.lora(y, x, a, b, which, scale)[0])
