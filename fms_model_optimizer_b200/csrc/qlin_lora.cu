@@ -283,7 +283,10 @@ __global__ void __launch_bounds__(kLoraThreads, (LoraCfg<T, R16, MT>::BLOCKS)) l
     float up = 1.0f, down = 1.0f;
     if constexpr (!C::BF16) {
       float top = 0.0f;
-      for (int c = lane; c < C::RP; c += 32) top = fmaxf(top, fabsf(v[row * C::PITCH + c]));
+      for (int c = lane; c < C::RP; c += 32) {
+        const float one = fabsf(v[row * C::PITCH + c]);
+        top = one < INFINITY ? fmaxf(top, one) : top;  // an infinity needs no room, those beside it do
+      }
       const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
       const int e = static_cast<int>(bits >> 23);
       if (e > 0 && e < 254) {  // 2^-(e - 127) and its inverse are normal numbers

@@ -269,3 +269,14 @@ def test_an_infinite_weight_meets_a_small_v(cuda_dev):
     v = OR.lora(y, x, a, b, which, scale)[1]
     assert all(bool((v[i][:, 3].abs() < 2.0**-25 * v[i].abs().amax(-1)).all()) and bool((v[i][:, 3] != 0).all()) for i in v)
     _same_extremes(_run(cuda_dev, y, x, a, b, which, scale), OR.lora(y, x, a, b, which, scale)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_an_infinite_sum_beside_large_ones(cuda_dev, dtype):
+    """One infinite number of v leaves the others as they are, outside fp16 too: y is that infinity, not the difference of two."""
+    y, x, a, b, which, scale = _inputs(19, 40, 2, 16, 136, 72, dtype, 0.0)
+    x, a, b = x * 2.0**9, a * 2.0**12, (b * 2.0**-12).abs() * torch.randn(b.shape, generator=torch.Generator().manual_seed(20)).sign().to(dtype)
+    a[0, 3, 7], a[1, 9, 0] = float("inf"), float("-inf")
+    want, v, _, _ = OR.lora(y, x, a, b, which, scale)
+    assert all(float(v[i][v[i].isfinite()].abs().max()) > 65504 for i in v)
+    _same_extremes(_run(cuda_dev, y, x, a, b, which, scale), want)
