@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <numeric>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -1059,6 +1060,14 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
 };
 std::vector<Tensor> token_logprobs_grad(const Tensor& logits, const Tensor& tokens, int64_t top) { return TokenLogprobs::apply(logits, tokens, top); }
 
+// Two elements of a matrix lie in one place: i rows on and j columns back, or the other way around, for the least i and j that do.
+bool overlaps_itself(const Tensor& t) {
+  const int64_t rows = t.size(0), columns = t.size(1), down = step(t, 0), right = step(t, 1);
+  if (rows == 0 || columns == 0) return false;
+  if (down == 0 || right == 0) return (rows > 1 && down == 0) || (columns > 1 && right == 0);
+  const int64_t g = std::gcd(down, right);
+  return right / g < rows && down / g < columns;
+}
 // Rows (or matrices of rows) of 16-bit numbers that start on 16 bytes: the tensor itself, or a dense copy.
 Tensor aligned_rows(const Tensor& t) {
   bool fits = t.numel() == 0 || ((t.size(-1) <= 1 || t.stride(-1) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
@@ -1083,8 +1092,7 @@ Tensor lora_add(const Tensor& y, const Tensor& x_in, const Tensor& a_in, const T
   check_index(starts, at::kInt, n + 1, "starts");
   const Tensor sc = f32(scale);
   if (sc.numel() != n) raise("scale must have one entry for each adapter");
-  for (int64_t d = 0; d < 2; ++d)
-    if (y.size(d) > 1 && y.stride(d) == 0) raise("rows of y share memory: they cannot be written");
+  if (overlaps_itself(y)) raise("rows of y share memory: they cannot be written");
   // what shares memory with y is read from a copy: other blocks have written some of it by the time it is read
   const auto apart = [&](const Tensor& t) { return may_overlap(y, t) ? t.clone(at::MemoryFormat::Contiguous) : t; };
   const Tensor x = aligned_rows(apart(x_in)), a_ = aligned_rows(apart(a_in)), b_ = aligned_rows(apart(b_in)), y_ = aligned_rows(y);

@@ -750,7 +750,7 @@ def lora_add_(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor
     that they share.  ``y [tokens, out]`` the projection's output, ``x [tokens, width]`` its input, ``a [adapters, rank, width]``, ``b [adapters,
     out, rank]``, all fp16 or all bf16, ``width``, ``out`` and ``rank`` <= 128 multiples of 8 (a lower rank is padded with zeros); ``rows`` and
     ``starts`` as ``lora_groups`` gives them, each row at most once; ``scale`` fp32 ``[adapters]``.  Sums are fp32, y is rounded once; rows that no adapter has keep their
-    bytes.  What shares memory with y is read as it was before the call.  Returns y.  No gradient."""
+    bytes.  What shares memory with y is read as it was before the call; a y whose own rows share some is refused.  Returns y.  No gradient."""
     work = 2.0 * rows.numel() * a.shape[1] * (x.shape[-1] + y.shape[-1]) if a.dim() == 3 else 0.0
     return _call("lora", work, y.device, L.host().lora_add, y, x, a, b, rows, starts, scale)
 

@@ -280,3 +280,19 @@ def test_an_infinite_sum_beside_large_ones(cuda_dev, dtype):
     want, v, _, _ = OR.lora(y, x, a, b, which, scale)
     assert all(float(v[i][v[i].isfinite()].abs().max()) > 65504 for i in v)
     _same_extremes(_run(cuda_dev, y, x, a, b, which, scale), want)
+
+
+def test_rows_of_y_that_overlap_are_refused(cuda_dev):
+    """Blocks that write the same bytes would leave what comes last; rows that only lie between one another are fine."""
+    y, x, a, b, which, scale = _inputs(21, 20, 2, 16, 64, 64, torch.bfloat16, 0.0)
+    rows, starts = ops.lora_groups(which.to(cuda_dev), 2)
+    rest = [t.to(cuda_dev) for t in (x, a, b)]
+    room = torch.zeros(20 * 256, dtype=torch.bfloat16, device=cuda_dev)
+    for strides in ((32, 1), (0, 1), (64, 0), (8, 8), (1, 1), (4, 6), (63, 1)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            ops.lora_add_(room.as_strided((20, 64), strides), *rest, rows, starts, scale.to(cuda_dev))
+    assert int(room.count_nonzero()) == 0
+    for strides in ((64, 1), (1, 20), (2, 41), (192, 3), (3, 64)):
+        at = room.as_strided((20, 64), strides)
+        at.copy_(y)
+        _near(ops.lora_add_(at, *rest, rows, starts, scale.to(cuda_dev)).cpu(), y, x, a, b, which, scale)
