@@ -53,7 +53,9 @@ struct SharedCfg {
   static constexpr int OUT_OFFSET = PAIR ? 0 : RAW_OFFSET + RAW * RAW_BYTES, OUT_BYTES = 4096;
   static constexpr int AUX_OFFSET = RAW_OFFSET + RAW * RAW_BYTES + (PAIR ? 0 : kSharedSoftmaxWarps * OUT_BYTES);
   static constexpr int SMEM_BYTES = AUX_OFFSET + static_cast<int>(sizeof(SharedAux));
-  static constexpr float SHIFT = HALF ? 6.0f : 0.0f;
+  // The reference may lie SLACK (in powers of two) below the maximum, and fp16 weights carry a factor of 2^SHIFT: they stay below 2^16, lose bits under 2^-26 of the largest only, and the
+  // least of them, which a weight is kept at for the sake of infinite values, is 2^-36 of it, as in the attention over pages.
+  static constexpr float SHIFT = HALF ? 12.0f : 0.0f, SLACK = HALF ? 3.875f : kSlack;
   static constexpr uint32_t FMT = HALF ? 0u : 1u;
   static constexpr uint32_t IDESC_S = make_idesc(1u, FMT, kRows, kKeys);
   static constexpr uint32_t IDESC_O = make_idesc(1u, FMT, kRows, DP) | (1u << 16);  // V is read with its head dimension contiguous
@@ -83,8 +85,8 @@ __device__ __forceinline__ void shared_softmax(uint32_t s_addr, uint32_t o_addr,
 #pragma unroll
   for (int n = 0; n < 15; ++n) top.step(x, n);
   const float most = top.result();
-  // The reference follows the maximum only when that has outgrown it by 2^kSlack.  NaN or an infinity among the logits makes it NaN, and with it the row.
-  // The difference, which is exact for numbers this near each other, is compared: m + slack rounds to a whole place of a large m, up to twice the slack, and 2^(2 kSlack + SHIFT) is
+  // The reference follows the maximum only when that has outgrown it by 2^SLACK.  NaN or an infinity among the logits makes it NaN, and with it the row.
+  // The difference, which is exact for numbers this near each other, is compared: m + slack rounds to a whole place of a large m, up to twice the slack, and 2^(2 SLACK + SHIFT) is
   // no fp16 number.
   const bool grow = m == -INFINITY ? !(most <= m) : !(most - m <= slack);
   if (first || __any_sync(0xffffffffu, grow)) {
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
           mbar_arrive(&aux->q_full[i]);
         }
       }
-      const float slack = kSlack / cl2;
+      const float slack = C::SLACK / cl2;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t s_addr = tmem + lanes + i * kKeys, o_addr = tmem + lanes + 2 * kKeys + i * DP;
       float m = -INFINITY, l = 0.0f;
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
       if (ok) ok = uniform_wait(&aux->o_full[i], 0, abort_flag);
       if (ok) {
         tc_fence_after();
-        constexpr float down = C::HALF ? 1.0f / 64.0f : 1.0f;  // without the factor that fp16 weights carry
+        constexpr float down = C::HALF ? 1.0f / 4096.0f : 1.0f;  // without the factor that fp16 weights carry
         if (live) p.pre.part_ml[out_row] = make_float2(m * cl2, l * down);
         // Rows go through shared memory, 32 outputs at a time, so that eight lanes write 128 bytes of a row together.
         const uint64_t to = live ? reinterpret_cast<uint64_t>(p.pre.part_o + out_row * D) : 0;

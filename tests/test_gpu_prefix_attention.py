@@ -373,3 +373,26 @@ def test_large_logits_a_few_units_apart(cuda_dev, dtype, f8, sequences):
         want, weighted = p @ v, p @ v.abs()
         tol = (2 * U[wt] + 2.0**-20) * weighted + U[dtype] * want.abs() + (n + 10) * 2.0**-30 * v.abs().max() + 2.0**-25
         assert bool(((got[b] - want).abs() <= tol).all()), (b, got[b].isfinite().all(), float((got[b] - want).abs().max()))
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sequences", [8, 48, 136])
+def test_many_keys_of_no_weight(cuda_dev, dtype, f8, sequences):
+    """A key with all of the weight and a value of zero, and 2^17 with 2^-58 of it and values of one: no output comes of these.  An fp16 weight that is kept from zero, so that an
+    infinite value stays one, adds 2^-36 of the largest at most."""
+    heads, dim, page, n = 80, 16 if f8 else 8, 64, 1 << 17
+    k, v = (torch.zeros(n // page + 1, heads, page, dim, device=cuda_dev) for _ in range(2))
+    k[..., 0], v[:] = -8.0, 1.0
+    k[0, :, 0, 0], v[0, :, 0] = 0.0, 0.0
+    q = torch.zeros(sequences, heads, dim, dtype=dtype, device=cuda_dev)
+    q[..., 0] = 58 / 8 * math.log(2) / dim**-0.5
+    ct = F8 if f8 else dtype
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda_dev)  # noqa: E731
+    table = torch.arange(n // page, dtype=torch.int32, device=cuda_dev)
+    own = torch.zeros(sequences, n // page + 1, dtype=torch.int32, device=cuda_dev)
+    own[:, -1] = n // page
+    scales = dict(k_scale=torch.ones(heads, device=cuda_dev), v_scale=torch.ones(heads, device=cuda_dev)) if f8 else {}
+    got = ops.prefix_attention(q, k.to(ct), v.to(ct), table[None], i32(n), i32(0, sequences), own, i32(*[n + 3] * sequences), **scales)
+    ops.check_status(cuda_dev)
+    assert float(got.abs().max()) <= (n + 3) * 2.0**-36 + 2.0**-25
