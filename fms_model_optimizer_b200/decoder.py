@@ -172,6 +172,9 @@ class Generated(NamedTuple):
     top_ids: torch.Tensor
 
 
+SCORE_LOGITS = 1 << 28  # logits that `score` holds at a time: half a gigabyte
+
+
 class Scored(NamedTuple):
     """What the model says about each token of a prompt but the first, given those in front of it: [n - 1] and, of the alternatives, [n - 1, top]."""
 
@@ -664,7 +667,7 @@ class W8A8Decoder:
             return q, k, a.view(a.shape[0], -1)
 
         def head(h):
-            part = max(1, (1 << 28) // self.lm_head.shape[0])  # rows whose logits are half a gigabyte
+            part = max(1, SCORE_LOGITS // self.lm_head.shape[0])
             said = [ops.token_logprobs(h[i : i + part] @ self.lm_head.t(), ids[asked[i : i + part] + 1], top=top) for i in range(0, h.shape[0], part)]
             return tuple(torch.cat(t) for t in zip(*said))
 

@@ -9,7 +9,7 @@ kept to 2^-16 and its sums to 2^-12 of the sum of magnitudes.  Log probabilities
 import pytest
 import torch
 
-from fms_model_optimizer_b200 import ops
+from fms_model_optimizer_b200 import decoder, ops
 from fms_model_optimizer_b200.adapters import LoraAdapters
 from fms_model_optimizer_b200.decoder import Generated, W8A8Decoder, linear_shapes
 from fms_model_optimizer_b200.kvcache import PagedKVCache
@@ -229,3 +229,30 @@ def test_refusals(cuda_dev, model):
     for bad in (lambda: model.score([]), lambda: model.score([prefix[:1]]), lambda: model.score([prefix], adapters=pool), lambda: model.score([torch.cat([prefix] * 26)])):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("rows", [1, 7, 32])
+def test_scores_in_parts(cuda_dev, model, monkeypatch, rows):
+    """The head's logits a few rows at a time, whose bounds fall inside prompts: each part with its own tokens, and the answers in one piece."""
+    prompts = _ids(cuda_dev, 20, 2, 33)
+    whole, calls, real = model.score(prompts, top=3), [], ops.token_logprobs
+
+    def noted(logits, tokens, *, top=0):
+        calls.append((logits.clone(), tokens.clone()))
+        return real(logits, tokens, top=top)
+
+    monkeypatch.setattr(ops, "token_logprobs", noted)
+    monkeypatch.setattr(decoder, "SCORE_LOGITS", rows * CFG["vocab"] + 5)
+    parts = model.score(prompts, top=3)
+    assert [c[0].shape[0] for c in calls] == [min(rows, 52 - i) for i in range(0, 52, rows)]
+    logits, tokens = (torch.cat(t) for t in zip(*calls))
+    assert torch.equal(tokens, torch.cat([p[1:] for p in prompts]))
+    want = OR.score(logits.cpu(), tokens.cpu(), 3)
+    at = 0
+    for p, s, w in zip(prompts, parts, whole):
+        here = slice(at, at := at + p.numel() - 1)
+        assert all(x.shape == y.shape for x, y in zip(s, w))
+        assert float((s.logprobs.cpu() - want["logprobs"][here]).abs().max()) < 2.0**-16 and float((s.entropy.cpu() - want["entropy"][here]).abs().max()) < 2.0**-14
+        assert torch.equal(s.top_ids.cpu(), want["top_ids"][here]) and float((s.top_logprobs.cpu() - want["top_logprobs"][here]).abs().max()) < 2.0**-16
+        # two products of one row, each rounded to bf16, of the token and of the largest
+        assert float((s.logprobs - w.logprobs).abs().max()) <= 4 * 2.0**-8 * float(logits.abs().max())
