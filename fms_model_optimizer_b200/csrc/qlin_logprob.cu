@@ -13,8 +13,8 @@
 // each element how many are larger.  Elements are ordered by value, then by the lower id, so results do not depend on timing.
 //
 // Measured (device time, bf16): 4096 x 128256 165 us, 6.4 TB/s, 0.97 of the copy rate, with the exponentials' unit busy for 77 % of it; 2048 x 128256 forward and backward 261 us,
-// 6.0 TB/s; 64 x 128256 with 20 alternatives 11 us and one row with five 8 us, which are the latency of the row, its sums, the pieces and the cluster behind one another; 333 x 50257 in
-// fp32 with all but nine logits minus infinity 18 us.  Tried and no faster, 4096 x 128256: every fourth or eighth pair of exponentials by a polynomial on the FMA pipe 179 and 167 us (the
+// 6.0 TB/s (188 and 276 a call in a long run, whose clock falls); 64 x 128256 with 20 alternatives 11 us and one row with five 8 us (12 a call, on the host), which are the latency of the row, its sums, the pieces and the cluster behind one another; 333 x 50257 in
+// fp32 with all but nine logits minus infinity 21 us (18 where L2 holds them).  Tried and no faster, 4096 x 128256: every fourth or eighth pair of exponentials by a polynomial on the FMA pipe 179 and 167 us (the
 // instructions are what there is no room for), pieces without the guard for minus infinity, which are done again where they held one, 170.
 #include <type_traits>
 

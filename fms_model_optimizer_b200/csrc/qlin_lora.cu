@@ -12,8 +12,8 @@
 // steps ahead; a lane waits for its own copies only.  Rows of 128 (tcgen05) would not make the loads faster.
 //
 // Measured (device time): 8 prompts of 2048 rows, rank 16, 4096 -> 4096 in bf16 80 us, 5.0 TB/s, 0.77 of the copy rate (registers instead of the copies 86, a tile of 16 rows 104 and
-// of 64 82); 1999 rows of rank 64, 14336 -> 4096 in fp16 36 us, 2.2 TB/s: 112 blocks of 64 rows that go through 1.2 MB each, a step's copies and products behind one another; 64 rows of 16
-// adapters, rank 16, 4096 -> 14336 10 us; one row 5.6: the latency of starts, rows, x, the join of v in the cluster, and y behind one another.
+// of 64 82); 1999 rows of rank 64, 14336 -> 4096 in fp16 32 to 36 us, 2.2 TB/s: 112 blocks of 64 rows that go through 1.2 MB each, a step's copies and products behind one another; 1999 rows of
+// rank 128, 4096 -> 4096 in bf16 45 us; 64 rows of 16 adapters, rank 16, 4096 -> 14336 9 us; one row 5.9: the latency of starts, rows, x, the join of v in the cluster, and y behind one another.
 //
 // v goes into the second product as two 16-bit numbers whose sum has 16 (bf16) or 22 (fp16) of its bits; in fp16 a row of v is brought to
 // 1 <= max < 2 first, by a power of two that comes back with the scale, since its sums may leave fp16's range where y does not.

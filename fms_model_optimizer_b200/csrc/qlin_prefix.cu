@@ -1,17 +1,23 @@
 // qlin_prefix_attention: one new token of every sequence against its keys in a paged cache, where groups of sequences share the first of them.
 //
 // The softmax of a row splits into any parts of its keys, each with its own maximum and sums.  Here the keys of the prefix that all sequences of a group
-// see are one part: the queries of all of them are the columns of the products (eight or sixteen a block), and each key is loaded once for these.
+// see are one part: the queries of all of them are the columns of the products (eight or sixteen a block, or a tile or two of 128), and each key is loaded once for these.
 // What else a sequence sees, its own keys, and those of the prefix that its window or length sets apart from the others', is the part that
 // qlin_paged_attention's kernel reads, whose blocks then take in the sums over the prefix.  No row of a product is masked that way: what a sequence does not see
 // is not loaded beside its query, NaN and infinities included.
 //
-// What bounds it: HBM, each key of a prefix once and each own key once, while a group has few rows; then the products, which groups of 32 rows and more (48 with e4m3) have on tcgen05
+// What bounds it: HBM, each key of a prefix once for a block's columns and each own key once, while a group has few rows; then the products, which groups of 32 rows and more (48 with e4m3) have on tcgen05
 // (qlin_prefix_tc.cu).  The launch for the own keys begins while the one for the prefixes ends, and waits for its sums only when it joins them.
 //
 // Measured (device time, 32 + 8 heads of 128): 2 x 64 sequences behind 32768 keys with up to 300 of their own in bf16 86 us, 774 TFLOP/s, 0.47 of the burst rate (72 for the prefixes, the
-// own keys 15 behind them); 61 behind 8200 with up to 515 in e4m3 36 us (23 and 13); 4 behind 2048 with 128 in bf16 12.8 us, two launches of 8 that overlap; 16 behind 8192 with 128
-// 30 us, where the attention over pages reads the prefix 16 times in 63.
+// own keys 15 behind them; 103 a call in a long run, whose clock falls); 61 behind 8200 with up to 515 in e4m3 39 us (40 a call); 4 behind 2048 with 128 in bf16 12.9 us, two launches of 8
+// that overlap (14.4 a call).
+// Beside the attention over pages, which reads the prefix for each sequence: 16 behind 8192 with 128 30 us, 64 there; 32 behind 2048 25.5 and 37.5, 16 22.7 and 24.7, 8 15.8 and 18.9, 4
+// 13.2 and 13.8; but 4 behind 512 with 50 11.6 and 7.2, and 16 16.0 and 14.5: a prefix of a few hundred keys, which L2 holds, does not pay for its launch.
+//
+// The host knows neither the groups' sizes nor the prefixes' lengths, which lie on the device; the rules below go by averages and by the tables' widths.  So 64 sequences behind 32768 keys with
+// 100 of their own take 55 us, with 8 single requests in the same call 161 and with 63 of them 455 (838 over pages): the average says few rows and few splits.  And 15 sequences behind
+// 8192 keys with a 16th of 100 take 82 us (63 over pages), since what all of them see ends there and the rest is left to each, unsplit.
 #include "qlin_paged.cuh"
 
 namespace qlin {

@@ -11,7 +11,7 @@
 // describes, are left to the kernel of the attention over pages.  The keys that are read here begin and end at multiples of the box, so that no box holds a key that
 // somebody does not see; the few beside them are the sequences' own.  e4m3 codes land beside the tiles and two warps make fp16 of them on the way there; a bf16 query
 // meets these as fp16 times a power of two that brings its largest element to 2^13..2^14.  (Through the threads' registers and 16-byte asynchronous copies, which take
-// pages of any size, the loads were what the rest waited for: 2 x 64 sequences behind 32768 keys 127 us.)
+// pages of any size, the loads were what the rest waited for: with them 2 x 64 sequences behind 32768 keys took the whole operator 127 us at best, the first boxes by TMA 101.)
 //
 // What bounds it: the chain of products and exponentials, 3450 cycles for two tiles of rows against a tile of keys where the tensor core needs 2048 and so do the exponentials (2 x 64 sequences
 // behind 32768 keys 72 us, the tensor pipe busy for half of it); short prefixes by the start and the end of a block, some 12 us.

@@ -683,12 +683,12 @@ def prefix_attention(
     v_scale: Optional[torch.Tensor] = None,
     out: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """``paged_attention`` for groups of sequences that share their first tokens, whose keys are read once for a group (``qlin_prefix_attention``).
+    """``paged_attention`` for groups of sequences that share their first tokens, whose keys are read once for many rows of a group (``qlin_prefix_attention``).
     Sequences ``groups[g] : groups[g + 1]`` (int32 ``[groups + 1]``, rising from 0 to the batch) find their keys ``i < prefix_lens[g]`` in page
     ``prefix_table[g, i // page size]`` and the others in ``block_table[b, i // page size]``, whose entries in front of them are not read; ``lens``
     count the prefix in.  A group of one sequence, or a prefix of length 0, is fine.  ``prefix_table`` int32 ``[groups, pages of a prefix]``,
-    ``prefix_lens`` int32 ``[groups]``, everything else as in ``paged_attention``.  As there, the widths of the tables should be no more than the longest need.
-    No gradient."""
+    ``prefix_lens`` int32 ``[groups]``, everything else as in ``paged_attention``.  As there, the widths of the tables should be no more than the longest need;
+    and how many rows share a key goes by the groups' average rows, so a large group is better called apart from many small ones.  No gradient."""
     return _call("prefix_attention", 0.0, q.device, L.host().prefix_attention, q, k_pages, v_pages, prefix_table, prefix_lens, groups, block_table, lens, scale, window, sinks,
                  k_scale, v_scale, out)  # fmt: skip
 

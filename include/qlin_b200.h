@@ -771,7 +771,8 @@ int qlin_token_logprobs_bwd(const qlin_token_logprobs_args* args, void* stream);
 /* qlin_lora -- y[t] += scale[i] (x[t] a[i]^T) b[i]^T in place for the rows t of adapter i, which are rows[starts[i]] .. rows[starts[i + 1] - 1]; rows of y
  * that are not listed keep their bytes, and a row is listed once at most.  x [tokens, width], y [tokens, out], a [adapters, rank, width], b [adapters, out, rank], all
  * F16 or all BF16; sums in fp32, y rounded once.  width, out and rank are multiples of 8, rank <= 128; rows of x, y, a and b start on 16 bytes;
- * x, a and b overlap y nowhere.  starts that do not rise from 0 to at most `listed`, or a row that does not exist, write QLIN_ERR_BAD_SHAPE to
+ * x, a and b overlap y nowhere, nor rows of y one another.  Infinities and NaN reach
+ * what they reach by the formula.  starts that do not rise from 0 to at most `listed`, or a row that does not exist, write QLIN_ERR_BAD_SHAPE to
  * *status; such adapters and rows are passed over. */
 typedef struct qlin_lora_args {
   const void* x;
@@ -792,10 +793,12 @@ int qlin_lora(const qlin_lora_args* args, void* stream);
 /* qlin_prefix_attention -- qlin_paged_attention where groups of sequences share their first tokens: sequences groups[g] .. groups[g + 1] - 1 find their
  * keys i < prefix_lens[g] in page prefix_table[g, i / page_size] and the others, as ever, in page block_table[b, i / page_size], offset i % page_size of either.
  * lens, positions, window and sinks count from the first token of the prefix; lens[b] may be 0 (zeros) or fall short of the prefix.  The keys of a
- * prefix that all its sequences see are read once for the group.  groups rises from 0 to batch; otherwise, and for prefix_lens below 0 or above
- * max_prefix_pages * page_size, QLIN_ERR_BAD_SHAPE in *status and unspecified outputs.  The widths of the tables bound how finely keys are split: a
- * sequence's own keys are expected not to pass max_pages - max_prefix_pages + 1 pages by much.  Entries of block_table in front of a sequence's own
- * first key are not read. */
+ * prefix that all its sequences see are read once for 8, 16, 128 or 256 rows of the group (its sequences times the query heads of a kv head).  groups rises from 0 to batch;
+ * otherwise, and for prefix_lens below 0 or above max_prefix_pages * page_size, QLIN_ERR_BAD_SHAPE in *status and unspecified outputs.  Entries of block_table in front of a
+ * sequence's own first key are not read.
+ * The time (not the result) goes by more: the groups' average rows (batch / num_groups, groups without sequences or prefix counted in) say how many rows share a key, so a large group
+ * is better called apart from many small ones; the widths of the tables bound how finely keys are split, so a sequence's own keys are expected not to pass
+ * max_pages - max_prefix_pages + 1 pages by much; and a sequence that is shorter than the prefix, or a window, leaves the group only what all of it sees. */
 typedef struct qlin_prefix_attention_args {
   qlin_paged_attention_args own; /* workspace: qlin_prefix_attention_workspace_bytes */
   const int32_t* prefix_table;   /* [num_groups, max_prefix_pages], row stride prefix_stride */
